@@ -42,6 +42,11 @@ SIGNATURES = {
                                     _vp, _vp]),
     "dh_cross_entropy_bwd": (_i32, [_vp, _i64, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _f32, _i32, _vp, _i64,
                                     _vp]),
+    "dh_distill_workspace_bytes": (_sz, [_i64, _i64]),
+    "dh_distill_fwd": (_i32, [_vp, _i64, _vp, _i32, _vp, _i32, _vp, _vp, _i64, _i64, _i32, _i64, _i64, _f32, _f32, _i32, _vp, _i64, _vp,
+                              _sz, _vp]),
+    "dh_distill_bwd": (_i32, [_vp, _i64, _vp, _i32, _vp, _i32, _vp, _vp, _i64, _vp, _i64, _i64, _i32, _i64, _i64, _f32, _f32, _i32, _vp,
+                              _i64, _vp]),
     "dh_embedding_fwd": (_i32, [_vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp, _vp]),
     "dh_embedding_bwd": (_i32, [_vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp, _i32, _vp]),
     "dh_masked_mean_fwd": (_i32, [_vp, _vp, _i64, _f32, _vp, _vp]),
@@ -59,6 +64,7 @@ SIGNATURES = {
     "dh_gelu": (_i32, [_vp, _vp, _i64, _i32, _vp]),
     "dh_bias_mask_add": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i32, _vp]),
     "dh_rope": (_i32, [_vp] * 6 + [_i64, _i32, _i32, _i32, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _vp]),
+    "dh_rotary": (_i32, [_vp] * 6 + [_i32, _i64] + [_i32] * 4 + [_i64] * 9 + [_i32, _i32, _f32, _i32, _vp]),
     "dh_attn_fwd": (_i32, [_vp] * 7 + [_i32] * 6 + [_i64] * 4 + [_f32, _i32, _i32, _vp]),
     "dh_attn_fwd_total": (_i32, [_vp] * 7 + [_i32] * 5 + [_i64] + [_i32] * 3 + [_i64] * 4 + [_f32, _i32, _i32, _vp]),
     "dh_attn_fwd_state": (_i32, [_vp] * 8 + [_i32] * 5 + [_i64] + [_i32] * 3 + [_i64] * 4 + [_f32, _i32, _i32, _vp]),
@@ -78,6 +84,9 @@ SIGNATURES = {
     "dh_attn_merge": (_i32, [_vp, _vp, _vp, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp]),
     "dh_moe_route_topk": (_i32, [_vp, _vp, _vp, _i64, _i32, _i32, _vp]),
     "dh_moe_route_lanes": (_i32, [_i64, _i32, _i32]),
+    "dh_balance_loss_workspace_bytes": (_sz, [_i64, _i32]),
+    "dh_balance_loss_fwd": (_i32, [_vp] * 3 + [_i64, _i32, _i32, _f32, _f32] + [_vp] * 6 + [_sz, _vp]),
+    "dh_moe_route_bwd": (_i32, [_vp] * 9 + [_i64, _i32, _i32, _f32, _f32, _vp, _vp]),
     "dh_moe_sort_workspace_bytes": (_sz, [_i64, _i32]),
     "dh_moe_sort": (_i32, [_vp] * 6 + [_sz, _i64, _i32, _vp]),
     "dh_moe_sort_static_max_assign": (_i64, []),

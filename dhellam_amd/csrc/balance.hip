@@ -1,0 +1,357 @@
+// The router's training side: losses that keep the experts in balance, counts, and the gradient of the logits.
+//
+//   p_t = softmax(logits_t),  lse_t = log sum exp(logits_t),  N = tokens that count
+//   counts_e = choices of expert e,  P_e = sum_t p_te           (over the tokens that count)
+//   balance = a E / (k N^2) sum_e counts_e P_e,   z = b / N sum_t lse_t^2
+//   d balance / d logit_te = a E / (k N^2) p_te (counts_e - sum_f counts_f p_tf),   d z / d logit_te = 2 b / N lse_t p_te
+//   and through the gates, g = softmax of the chosen logits:  d logit of choice j = g_j (dg_j - sum_i g_i dg_i)
+//
+// A token's row of up to 64 logits is held by L lanes of 4 each: 16-byte loads, exchanges over L lanes only.  Sums over tokens
+// stay in registers, then LDS, then one partial sum a workgroup that a second launch adds in order: no atomics on
+// floats, the same result every time.
+#include "common.h"
+
+namespace dh {
+namespace {
+
+constexpr int BAL_MAX_E = 64, BAL_MAX_K = 8, BAL_MAX_BLOCKS = 512;
+
+struct BalancePartial {
+  float prob[BAL_MAX_E];
+  int32_t counts[BAL_MAX_E];
+  float z;
+  int32_t n;
+};
+
+// The four logits of a lane, -inf past the last expert.
+__device__ __forceinline__ void load_row(const float *logits, int64_t t, int e0, int E, bool vec, float x[4]) {
+  const float *row = logits + t * E;
+  if (vec) {
+    float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    if (e0 < E) v = *reinterpret_cast<const float4 *>(row + e0);
+    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = e0 + i < E ? row[e0 + i] : -INFINITY;
+  }
+}
+
+template <int L> __device__ __forceinline__ float lanes_max(float v) {
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  return v;
+}
+template <int L> __device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// Totals in LDS -> the outputs, by the first wavefront.
+__device__ __forceinline__ void balance_finish(const float *prob, const int *counts, float z, int n, int E, int K, float a, float b,
+                                               float *losses, int32_t *counts_out, float *prob_out, int32_t *tokens_out) {
+  const int e = threadIdx.x;
+  if (e >= 64) return;
+  const float p = e < E ? prob[e] : 0.f;
+  const int c = e < E ? counts[e] : 0;
+  const float inv = n > 0 ? 1.f / (float)n : 0.f;
+  const float s = wave_sum(n > 0 ? ((float)c * inv) * (p * inv) : 0.f);
+  if (e < E) {
+    counts_out[e] = c;
+    prob_out[e] = p;
+  }
+  if (e == 0) {
+    losses[0] = a * (float)E / (float)K * s;
+    losses[1] = n > 0 ? b * z * inv : 0.f;
+    tokens_out[0] = n;
+  }
+}
+
+template <int L, int BT>
+__global__ void __launch_bounds__(BT)
+balance_fwd_kernel(const float *__restrict__ logits, const int32_t *__restrict__ idx, const uint8_t *__restrict__ mask, int64_t tokens,
+                   int E, int K, float a, float b, float *__restrict__ lse_out, BalancePartial *__restrict__ partials,
+                   float *__restrict__ losses, int32_t *__restrict__ counts_out, float *__restrict__ prob_out,
+                   int32_t *__restrict__ tokens_out, bool vec) {
+  constexpr int WAVES = BT / 64, TPB = BT / L;
+  __shared__ int cnt[WAVES][BAL_MAX_E];
+  __shared__ float prob[WAVES][BAL_MAX_E];
+  __shared__ float red_z[WAVES];
+  __shared__ int red_n[WAVES];
+  const int tid = threadIdx.x, w = tid >> 6, l = tid % L, e0 = 4 * l;
+  cnt[w][tid & 63] = 0;
+  prob[w][tid & 63] = 0.f;
+  __syncthreads();
+  float acc[4] = {0.f, 0.f, 0.f, 0.f}, z = 0.f;
+  int n = 0;
+  for (int64_t t0 = (int64_t)blockIdx.x * TPB; t0 < tokens; t0 += (int64_t)gridDim.x * TPB) {
+    const int64_t t = t0 + tid / L;
+    const bool in = t < tokens;
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    bool on = in;
+    if (in) {
+      load_row(logits, t, e0, E, vec, x);
+      if (mask) on = mask[t] != 0;
+      if (on)
+        for (int j = l; j < K; j += L) {
+          const int e = idx[t * K + j];
+          if ((unsigned)e < (unsigned)E) atomicAdd(&cnt[w][e], 1);      // (whole numbers: any order)
+        }
+    }
+    const float m = lanes_max<L>(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+    float ex[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ex[i] = expf(x[i] - m);
+    const float s = lanes_sum<L>((ex[0] + ex[1]) + (ex[2] + ex[3]));
+    const float lse = m + logf(s), inv = 1.f / s;
+    if (in && l == 0) lse_out[t] = lse;
+    if (on) {                                       // (a masked row may hold anything)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] += ex[i] * inv;
+      if (l == 0) {
+        z += lse * lse;
+        n += 1;
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 32; o >= L; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] += __shfl_xor(acc[i], o, 64);
+  z = wave_sum(z);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+  if ((tid & 63) < L)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) prob[w][e0 + i] = acc[i];
+  if ((tid & 63) == 0) {
+    red_z[w] = z;
+    red_n[w] = n;
+  }
+  __syncthreads();
+  if (tid < 64) {
+    float p = 0.f;
+    int c = 0;
+    z = 0.f;
+    n = 0;
+    for (int i = 0; i < WAVES; ++i) {
+      p += prob[i][tid];
+      c += cnt[i][tid];
+      z += red_z[i];
+      n += red_n[i];
+    }
+    if (partials) {
+      BalancePartial &out = partials[blockIdx.x];
+      out.prob[tid] = p;
+      out.counts[tid] = c;
+      if (tid == 0) {
+        out.z = z;
+        out.n = n;
+      }
+    } else {
+      prob[0][tid] = p;
+      cnt[0][tid] = c;
+      __builtin_amdgcn_wave_barrier();
+      balance_finish(prob[0], cnt[0], z, n, E, K, a, b, losses, counts_out, prob_out, tokens_out);
+    }
+  }
+}
+
+// The workgroups' sums, added in their order: 16 wavefronts take every 16th, a lane an expert.
+__global__ void __launch_bounds__(1024)
+balance_join_kernel(const BalancePartial *__restrict__ partials, int blocks, int E, int K, float a, float b, float *__restrict__ losses,
+                    int32_t *__restrict__ counts_out, float *__restrict__ prob_out, int32_t *__restrict__ tokens_out) {
+  __shared__ float prob[16][64];
+  __shared__ int cnt[16][64];
+  __shared__ float red_z[16];
+  __shared__ int red_n[16];
+  const int e = threadIdx.x & 63, w = threadIdx.x >> 6;
+  float p = 0.f, z = 0.f;
+  int c = 0, n = 0;
+  for (int i = w; i < blocks; i += 16) {
+    p += partials[i].prob[e];
+    c += partials[i].counts[e];
+  }
+  for (int i = w + 16 * e; i < blocks; i += 16 * 64) {
+    z += partials[i].z;
+    n += partials[i].n;
+  }
+  z = wave_sum(z);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+  prob[w][e] = p;
+  cnt[w][e] = c;
+  if (e == 0) {
+    red_z[w] = z;
+    red_n[w] = n;
+  }
+  __syncthreads();
+  if (w == 0) {
+    p = 0.f, z = 0.f;
+    c = 0, n = 0;
+    for (int i = 0; i < 16; ++i) {
+      p += prob[i][e];
+      c += cnt[i][e];
+      z += red_z[i];
+      n += red_n[i];
+    }
+    prob[0][e] = p;
+    cnt[0][e] = c;
+    __builtin_amdgcn_wave_barrier();
+    balance_finish(prob[0], cnt[0], z, n, E, K, a, b, losses, counts_out, prob_out, tokens_out);
+  }
+}
+
+template <int L>
+__global__ void __launch_bounds__(256)
+route_bwd_kernel(const float *__restrict__ logits, const int32_t *__restrict__ idx, const float *__restrict__ gates,
+                 const float *__restrict__ dgates, const uint8_t *__restrict__ mask, const float *__restrict__ lse,
+                 const int32_t *__restrict__ counts, const int32_t *__restrict__ n_tokens, const float *__restrict__ dlosses,
+                 int64_t tokens, int E, int K, float a, float b, float *__restrict__ dlogits, bool vec) {
+  constexpr int TPB = 256 / L, S = (BAL_MAX_K + L - 1) / L;       // choices a lane holds
+  const int tid = threadIdx.x, l = tid % L, e0 = 4 * l, first = (tid & 63) - l;
+  float ca = 0.f, cb = 0.f, c[4] = {0.f, 0.f, 0.f, 0.f};
+  if (lse) {
+    const int n = n_tokens[0];
+    const float inv = n > 0 ? 1.f / (float)n : 0.f;
+    ca = a * (float)E / (float)K * inv * (dlosses ? dlosses[0] : 1.f);
+    cb = 2.f * b * inv * (dlosses ? dlosses[1] : 1.f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (e0 + i < E) c[i] = (float)counts[e0 + i] * inv;
+  }
+  for (int64_t t0 = (int64_t)blockIdx.x * TPB; t0 < tokens; t0 += (int64_t)gridDim.x * TPB) {
+    const int64_t t = t0 + tid / L;
+    const bool in = t < tokens;
+    float d[4] = {0.f, 0.f, 0.f, 0.f};
+    if (lse) {
+      float x[4] = {0.f, 0.f, 0.f, 0.f}, p[4], z = 0.f;
+      bool on = in;
+      if (in) {
+        load_row(logits, t, e0, E, vec, x);
+        z = lse[t];
+        if (mask) on = mask[t] != 0;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = expf(x[i] - z);
+      const float mean = lanes_sum<L>((c[0] * p[0] + c[1] * p[1]) + (c[2] * p[2] + c[3] * p[3]));
+      if (on)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[i] = p[i] * (ca * (c[i] - mean) + cb * z);
+    }
+    if (dgates) {
+      int e[S];
+      float g[S], v[S], sum = 0.f;
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        const int j = l + s * L;
+        e[s] = -1;
+        g[s] = v[s] = 0.f;
+        if (in && j < K) {
+          e[s] = idx[t * K + j];
+          g[s] = gates[t * K + j];
+          v[s] = dgates[t * K + j];
+        }
+        sum += g[s] * v[s];
+      }
+      sum = lanes_sum<L>(sum);
+#pragma unroll
+      for (int s = 0; s < S; ++s) v[s] = g[s] * (v[s] - sum);
+#pragma unroll
+      for (int j = 0; j < BAL_MAX_K; ++j)
+        if (j < K) {
+          const int to = __shfl(e[j / L], first + j % L, 64) - e0;
+          const float val = __shfl(v[j / L], first + j % L, 64);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (to == i) d[i] += val;
+        }
+    }
+    if (in) {
+      float *row = dlogits + t * E;
+      if (vec) {
+        if (e0 < E) *reinterpret_cast<float4 *>(row + e0) = make_float4(d[0], d[1], d[2], d[3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (e0 + i < E) row[e0 + i] = d[i];
+      }
+    }
+  }
+}
+
+int lanes_of(int E) { return E <= 4 ? 1 : E <= 8 ? 2 : E <= 16 ? 4 : E <= 32 ? 8 : 16; }
+
+constexpr int BAL_ONE_BT = 1024;      // threads of the only workgroup of a small call
+bool balance_one(int64_t tokens, int E) { return tokens * lanes_of(E) <= 4 * BAL_ONE_BT; }
+
+#define BAL_LANES(E, ...)                                  \
+  switch (lanes_of(E)) {                                   \
+    case 1: { constexpr int L = 1; __VA_ARGS__; } break;   \
+    case 2: { constexpr int L = 2; __VA_ARGS__; } break;   \
+    case 4: { constexpr int L = 4; __VA_ARGS__; } break;   \
+    case 8: { constexpr int L = 8; __VA_ARGS__; } break;   \
+    default: { constexpr int L = 16; __VA_ARGS__; }        \
+  }
+
+}  // namespace
+}  // namespace dh
+
+using namespace dh;
+
+extern "C" size_t dh_balance_loss_workspace_bytes(int64_t tokens, int experts) {
+  if (tokens <= 0 || experts < 1 || experts > BAL_MAX_E || balance_one(tokens, experts)) return 0;
+  return BAL_MAX_BLOCKS * sizeof(BalancePartial);
+}
+
+extern "C" int dh_balance_loss_fwd(const float *logits, const int32_t *topk_idx, const uint8_t *mask, int64_t tokens, int experts,
+                                   int k, float balance_coef, float z_coef, float *losses, int32_t *counts, float *prob_sum,
+                                   int32_t *n_tokens, float *lse, void *workspace, size_t workspace_bytes, void *stream) {
+  DH_CHECK(tokens >= 0 && tokens < (1ll << 31) / BAL_MAX_K, "tokens=%lld", (long long)tokens);
+  DH_CHECK(experts >= 1 && experts <= BAL_MAX_E, "experts=%d must be in [1, %d]", experts, BAL_MAX_E);
+  DH_CHECK(k >= 1 && k <= BAL_MAX_K && k <= experts, "k=%d must be in [1, min(%d, experts)]", k, BAL_MAX_K);
+  DH_CHECK(losses && counts && prob_sum && n_tokens && (tokens == 0 || (logits && topk_idx && lse)), "null pointer");
+  const size_t need = dh_balance_loss_workspace_bytes(tokens, experts);
+  DH_CHECK(need == 0 || (workspace && workspace_bytes >= need), "workspace of %zu bytes, %zu are needed", workspace_bytes, need);
+  const bool vec = experts % 4 == 0 && aligned16(logits);
+  const hipStream_t st = (hipStream_t)stream;
+  BAL_LANES(experts, {
+    if (need == 0) {
+      hipLaunchKernelGGL((balance_fwd_kernel<L, BAL_ONE_BT>), dim3(1), dim3(BAL_ONE_BT), 0, st, logits, topk_idx, mask, tokens, experts,
+                         k, balance_coef, z_coef, lse, nullptr, losses, counts, prob_sum, n_tokens, vec);
+    } else {
+      int64_t blocks = cdiv(tokens * L, 256);
+      if (blocks > BAL_MAX_BLOCKS) blocks = BAL_MAX_BLOCKS;
+      hipLaunchKernelGGL((balance_fwd_kernel<L, 256>), dim3((unsigned)blocks), dim3(256), 0, st, logits, topk_idx, mask, tokens, experts,
+                         k, balance_coef, z_coef, lse, (BalancePartial *)workspace, losses, counts, prob_sum, n_tokens, vec);
+      hipLaunchKernelGGL(balance_join_kernel, dim3(1), dim3(1024), 0, st, (const BalancePartial *)workspace, (int)blocks, experts, k,
+                         balance_coef, z_coef, losses, counts, prob_sum, n_tokens);
+    }
+  });
+  DH_LAUNCH_CHECK();
+  return DH_OK;
+}
+
+extern "C" int dh_moe_route_bwd(const float *logits, const int32_t *topk_idx, const float *gates, const float *dgates,
+                                const uint8_t *mask, const float *lse, const int32_t *counts, const int32_t *n_tokens,
+                                const float *dlosses, int64_t tokens, int experts, int k, float balance_coef, float z_coef,
+                                float *dlogits, void *stream) {
+  DH_CHECK(tokens >= 0 && tokens < (1ll << 31) / BAL_MAX_K, "tokens=%lld", (long long)tokens);
+  DH_CHECK(experts >= 1 && experts <= BAL_MAX_E, "experts=%d must be in [1, %d]", experts, BAL_MAX_E);
+  DH_CHECK(k >= 1 && k <= BAL_MAX_K && k <= experts, "k=%d must be in [1, min(%d, experts)]", k, BAL_MAX_K);
+  if (tokens == 0) return DH_OK;
+  DH_CHECK(topk_idx && dlogits, "null pointer");
+  DH_CHECK(!dgates || gates, "dgates without gates");
+  DH_CHECK(!lse || (logits && counts && n_tokens), "the losses' gradient needs the logits, counts and n_tokens");
+  DH_CHECK(dgates || lse, "neither dgates nor the losses' statistics: there is no gradient");
+  const bool vec = experts % 4 == 0 && aligned16(logits) && aligned16(dlogits);
+  const hipStream_t st = (hipStream_t)stream;
+  BAL_LANES(experts, {
+    int64_t blocks = cdiv(tokens * L, 256);
+    if (blocks > 4096) blocks = 4096;
+    hipLaunchKernelGGL((route_bwd_kernel<L>), dim3((unsigned)blocks), dim3(256), 0, st, logits, topk_idx, gates, dgates, mask, lse,
+                       counts, n_tokens, dlosses, tokens, experts, k, balance_coef, z_coef, dlogits, vec);
+  });
+  DH_LAUNCH_CHECK();
+  return DH_OK;
+}

@@ -96,6 +96,27 @@ class On {
   hipStream_t raw_;
 };
 
+// All tensors on one GPU, which is made the current one, and on its current stream or the given one (of that GPU): for operators
+// that allocate workspaces, so no raw handles, whose stream the allocator does not know.
+class OnGpu {
+ public:
+  OnGpu(std::initializer_list<const Tensor *> ts, const OptStream &stream) {
+    const auto device = (*ts.begin())->device();
+    for (const Tensor *t : ts)
+      if (t) TORCH_CHECK(t->is_cuda() && t->device() == device, "dhellam operators need their tensors on one GPU");
+    TORCH_CHECK(stream.is_none() || THPStream_Check(stream.ptr()), "stream: None or a torch.cuda.Stream");
+    TORCH_CHECK(stream.is_none() || On::of(stream).device_index() == device.index(), "the stream belongs to another GPU than the tensors");
+    guard_.emplace(device.index());
+    on_.emplace(stream);
+  }
+  void *get() const { return on_->get(); }
+
+ private:
+  std::optional<c10::hip::HIPGuard> guard_;
+  std::optional<On> on_;
+};
+const Tensor *opt(const OptTensor &t) { return t.has_value() ? &*t : nullptr; }
+
 const void *ptr(const OptTensor &t) { return t.has_value() ? t->data_ptr() : nullptr; }
 void *mptr(const OptTensor &t) { return t.has_value() ? t->data_ptr() : nullptr; }
 
@@ -321,6 +342,56 @@ std::tuple<Tensor, OptTensor> rope(const Tensor &q, const OptTensor &k, const Te
     return dh_rope(q.data_ptr(), ptr(k), qo.data_ptr(), mptr(ko), inv_freq.data_ptr<float>(),
                    (const int32_t *)ptr(positions), q.size(0), (int)q.size(1), k.has_value() ? (int)k->size(1) : 0, (int)d,
                    qs, ks, head_rows_stride(qo), ko.has_value() ? head_rows_stride(*ko) : 0, seq_len, backward, type, on.get());
+  });
+  return {qo, ko};
+}
+
+// Rows of heads with any strides, contiguous inside a head; written to only if no two elements share memory.
+void check_heads(const Tensor &t, bool written) {
+  PY_ASSERT(t.dim() == 3 && (t.stride(2) == 1 || t.size(2) <= 1), "rotary: expected [tokens, heads, d] with contiguous heads");
+  if (!written || t.numel() == 0) return;
+  std::array<std::pair<int64_t, int64_t>, 2> dims{{{t.stride(0), t.size(0)}, {t.stride(1), t.size(1)}}};
+  std::sort(dims.begin(), dims.end());
+  int64_t extent = t.size(2);
+  for (const auto &[stride, size] : dims) {
+    if (size <= 1) continue;
+    PY_ASSERT(stride >= extent, "rotary: elements that share memory cannot be turned in place");
+    extent += stride * (size - 1);
+  }
+}
+
+// `steps`: rot / 2 whole numbers (dh_rotary) -> (q turned, k turned or None)
+std::tuple<Tensor, OptTensor> rotary(const Tensor &q, const OptTensor &k, const Tensor &steps, int64_t rot, bool interleaved,
+                                     double factor, const OptTensor &positions, int64_t seq_len, bool backward, bool inplace,
+                                     const OptStream &stream) {
+  OnGpu on({&q, opt(k), &steps, opt(positions)}, stream);
+  check_heads(q, inplace);
+  const int64_t tokens = q.size(0), d = q.size(2);
+  PY_ASSERT(rot >= 2 && rot % 2 == 0 && rot <= d, "rotary: the table turns more elements than a head has");
+  PY_ASSERT(steps.scalar_type() == at::kLong && steps.is_contiguous() && steps.numel() == rot / 2, "rotary: not a table of rotary_table()");
+  PY_ASSERT(seq_len >= 0, "rotary: seq_len must not be negative");
+  int position_bytes = 0;
+  if (positions.has_value()) {
+    PY_ASSERT((positions->scalar_type() == at::kInt || positions->scalar_type() == at::kLong) && positions->is_contiguous() &&
+                  positions->numel() == tokens,
+              "rotary: positions must be contiguous int32 or int64, one per token");
+    position_bytes = (int)positions->element_size();
+  }
+  if (k.has_value()) {
+    check_heads(*k, inplace);
+    PY_ASSERT(k->size(0) == tokens && k->size(2) == d && k->scalar_type() == q.scalar_type(), "rotary: q and k differ");
+    PY_ASSERT(!inplace || q.numel() == 0 || k->numel() == 0 || q.data_ptr() != k->data_ptr(), "rotary: q and k are the same tensor");
+  }
+  const int type = dt(q);
+  Tensor qo = inplace ? q : at::empty(q.sizes(), q.options());
+  OptTensor ko;
+  if (k.has_value()) ko = inplace ? *k : at::empty(k->sizes(), k->options());
+  launch([&] {
+    return dh_rotary(q.data_ptr(), ptr(k), qo.data_ptr(), mptr(ko), (const uint64_t *)steps.data_ptr(), ptr(positions), position_bytes,
+                     tokens, (int)q.size(1), k.has_value() ? (int)k->size(1) : 0, (int)d, (int)rot, q.stride(0), q.stride(1),
+                     k.has_value() ? k->stride(0) : 0, k.has_value() ? k->stride(1) : 0, qo.stride(0), qo.stride(1),
+                     ko.has_value() ? ko->stride(0) : 0, ko.has_value() ? ko->stride(1) : 0, seq_len, interleaved, backward,
+                     (float)factor, type, on.get());
   });
   return {qo, ko};
 }
@@ -767,6 +838,66 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> moe_sort(const Tensor &topk_idx, int 
   return {tpe, offs, order, dest};
 }
 
+void check_router(const Tensor &logits, const Tensor &idx, const OptTensor &mask) {
+  PY_ASSERT(logits.scalar_type() == at::kFloat && logits.is_contiguous() && logits.dim() == 2,
+            "router: logits must be a contiguous fp32 [T, E] GPU tensor");
+  PY_ASSERT(idx.scalar_type() == at::kInt && idx.is_contiguous() && idx.dim() == 2 && idx.size(0) == logits.size(0),
+            "router: topk_idx must be a contiguous int32 [T, k] GPU tensor");
+  PY_ASSERT(!mask.has_value() || (mask->scalar_type() == at::kBool && mask->is_contiguous() && mask->numel() == logits.size(0)),
+            "router: mask must be a contiguous bool tensor, one value per token");
+}
+
+// -> (losses [2], counts int32 [E], prob_sum [E], tokens int32 [1], lse [T])
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> balance_loss_fwd(const Tensor &logits, const Tensor &idx, const OptTensor &mask,
+                                                                    double balance_coef, double z_coef, const OptStream &stream) {
+  OnGpu on({&logits, &idx, opt(mask)}, stream);
+  check_router(logits, idx, mask);
+  const int64_t t = logits.size(0), e = logits.size(1);
+  Tensor losses = at::empty({2}, logits.options()), prob = at::empty({e}, logits.options()), lse = at::empty({t}, logits.options());
+  Tensor counts = at::empty({e}, idx.options()), n = at::empty({1}, idx.options());
+  const int64_t bytes = (int64_t)dh_balance_loss_workspace_bytes(t, (int)e);
+  // of this call alone: a stream's shared scratch would be that of every graph captured on it
+  Tensor ws;
+  if (bytes) ws = at::empty({bytes}, logits.options().dtype(at::kByte));
+  launch([&] {
+    return dh_balance_loss_fwd(logits.data_ptr<float>(), idx.data_ptr<int>(), (const uint8_t *)ptr(mask), t, (int)e, (int)idx.size(1),
+                               (float)balance_coef, (float)z_coef, losses.data_ptr<float>(), counts.data_ptr<int>(),
+                               prob.data_ptr<float>(), n.data_ptr<int>(), lse.data_ptr<float>(), bytes ? ws.data_ptr() : nullptr,
+                               (size_t)bytes, on.get());
+  });
+  return {losses, counts, prob, n, lse};
+}
+
+// lse, counts and n: all or none; gates and dgates: both or none
+Tensor route_bwd(const Tensor &logits, const Tensor &idx, const OptTensor &gates, const OptTensor &dgates, const OptTensor &mask,
+                 const OptTensor &lse, const OptTensor &counts, const OptTensor &n, const OptTensor &dlosses, double balance_coef,
+                 double z_coef, const OptStream &stream) {
+  OnGpu on({&logits, &idx, opt(gates), opt(dgates), opt(mask), opt(lse), opt(counts), opt(n), opt(dlosses)}, stream);
+  check_router(logits, idx, mask);
+  const int64_t t = logits.size(0), e = logits.size(1);
+  for (const OptTensor *g : {&gates, &dgates})
+    PY_ASSERT(!g->has_value() || ((*g)->scalar_type() == at::kFloat && (*g)->is_contiguous() && (*g)->sizes() == idx.sizes()),
+              "route_bwd: gates and dgates must be contiguous fp32 [T, k]");
+  PY_ASSERT(!dgates.has_value() || gates.has_value(), "route_bwd: dgates without gates");
+  PY_ASSERT(dgates.has_value() || lse.has_value(), "route_bwd: neither dgates nor a balance loss");
+  if (lse.has_value()) {
+    PY_ASSERT(lse->scalar_type() == at::kFloat && lse->is_contiguous() && lse->numel() == t, "route_bwd: lse is not of these logits");
+    PY_ASSERT(counts.has_value() && counts->scalar_type() == at::kInt && counts->is_contiguous() && counts->numel() == e && n.has_value() &&
+                  n->scalar_type() == at::kInt && n->numel() == 1,
+              "route_bwd: counts must be contiguous int32 [E] and tokens int32 [1]");
+    PY_ASSERT(!dlosses.has_value() || (dlosses->scalar_type() == at::kFloat && dlosses->is_contiguous() && dlosses->numel() == 2),
+              "route_bwd: dlosses must be contiguous fp32 [2]");
+  }
+  Tensor d = at::empty_like(logits);
+  launch([&] {
+    return dh_moe_route_bwd(logits.data_ptr<float>(), idx.data_ptr<int>(), (const float *)ptr(gates), (const float *)ptr(dgates),
+                            (const uint8_t *)ptr(mask), (const float *)ptr(lse), (const int32_t *)ptr(counts), (const int32_t *)ptr(n),
+                            (const float *)ptr(dlosses), t, (int)e, (int)idx.size(1), (float)balance_coef, (float)z_coef,
+                            d.data_ptr<float>(), on.get());
+  });
+  return d;
+}
+
 Tensor moe_gather(const Tensor &x, const Tensor &sorted_idx, const OptTensor &row_scale, const Tensor &offs, int e_lo, int e_hi,
                   int64_t max_rows, int k, const OptStream &stream) {
   PY_ASSERT(x.is_cuda() && x.is_contiguous() && x.dim() == 2, "permute: rows must be a contiguous 2-D GPU tensor");
@@ -952,6 +1083,83 @@ Tensor cross_entropy_bwd(const Tensor &logits, const Tensor &row_max, const Tens
   return g.view(logits.sizes());
 }
 
+// The operands of the distillation loss as rows, checked.
+struct Distill {
+  Tensor x, ids, teacher;
+  OptTensor target;
+  int64_t rows, cols, k;
+  int type, teacher_type;
+  Distill(const Tensor &logits, const Tensor &ids_in, const Tensor &teacher_in, const OptTensor &target_in, double alpha) {
+    PY_ASSERT(logits.dim() >= 1 && logits.stride(-1) == 1, "distill: logits of unit inner stride");
+    const auto rows_of_them = logits.sizes().slice(0, logits.dim() - 1);
+    cols = logits.size(-1);
+    PY_ASSERT(cols > 0, "distill: no columns");
+    PY_ASSERT(ids_in.dim() == logits.dim() && ids_in.sizes().slice(0, ids_in.dim() - 1) == rows_of_them && ids_in.sizes() == teacher_in.sizes() &&
+                  (ids_in.scalar_type() == at::kLong || ids_in.scalar_type() == at::kInt),
+              "distill: teacher ids (int32 or int64) and logits must be [..., K] for logits of [..., vocabulary]");
+    k = ids_in.size(-1);
+    PY_ASSERT(alpha == 1.0 || (target_in.has_value() && target_in->scalar_type() == at::kLong && target_in->sizes() == rows_of_them),
+              "distill: alpha below 1 needs one int64 target per row");
+    type = dt(logits);
+    teacher_type = dt(teacher_in);
+    rows = logits.numel() / cols;
+    x = logits.dim() == 1 ? logits.unsqueeze(0) : rows_of(logits, cols);
+    ids = ids_in.contiguous();
+    teacher = teacher_in.contiguous();
+    if (alpha < 1.0) target = target_in->contiguous();
+  }
+};
+
+// -> statistics [10, rows] (dh_distill_fwd)
+Tensor distill_fwd(const Tensor &logits, const Tensor &ids, const Tensor &teacher, const OptTensor &teacher_lse, const OptTensor &target,
+                   int64_t vocab_start, int64_t vocab_total, double temperature, double alpha) {
+  OnGpu on({&logits, &ids, &teacher, opt(teacher_lse), opt(target)}, py::none{});
+  const Distill a(logits, ids, teacher, target, alpha);
+  OptTensor lse;
+  if (teacher_lse.has_value()) {
+    PY_ASSERT(teacher_lse->scalar_type() == at::kFloat && teacher_lse->numel() == a.rows, "distill: teacher_lse must be fp32, one per row");
+    lse = teacher_lse->contiguous();
+  }
+  Tensor stats = at::empty({10, a.rows}, logits.options().dtype(at::kFloat));
+  const int64_t bytes = (int64_t)dh_distill_workspace_bytes(a.rows, a.cols);
+  Tensor ws;                                               // of this call alone
+  if (bytes) ws = at::empty({bytes}, logits.options().dtype(at::kByte));
+  launch([&] {
+    return dh_distill_fwd(a.x.data_ptr(), a.rows > 1 ? a.x.stride(0) : a.cols, a.ids.data_ptr(), (int)a.ids.element_size(),
+                          a.teacher.data_ptr(), a.teacher_type, (const float *)ptr(lse), (const int64_t *)ptr(a.target), a.rows, a.cols,
+                          (int)a.k, vocab_start, vocab_total, (float)temperature, (float)alpha, a.type, stats.data_ptr<float>(), a.rows,
+                          bytes ? ws.data_ptr() : nullptr, (size_t)bytes, on.get());
+  });
+  return stats;
+}
+
+Tensor distill_bwd(const Tensor &logits, const Tensor &ids, const Tensor &teacher, const OptTensor &target, const Tensor &stats,
+                   const Tensor &dout, int64_t vocab_start, int64_t vocab_total, double temperature, double alpha,
+                   const OptTensor &grad_out) {
+  OnGpu on({&logits, &ids, &teacher, opt(target), &stats, &dout, opt(grad_out)}, py::none{});
+  const Distill a(logits, ids, teacher, target, alpha);
+  PY_ASSERT(stats.scalar_type() == at::kFloat && stats.dim() == 2 && stats.size(0) == 10 && stats.size(1) == a.rows && stats.is_contiguous(),
+            "distill: statistics of another call");
+  const Tensor d = dout.to(at::kFloat).contiguous();
+  PY_ASSERT(d.numel() == a.rows, "distill: one gradient per row");
+  Tensor g;
+  if (grad_out.has_value()) {
+    PY_ASSERT(grad_out->scalar_type() == logits.scalar_type() && grad_out->sizes() == logits.sizes(),
+              "distill: grad_out must have the logits' shape and type");
+    g = grad_out->view({-1, a.cols});
+    PY_ASSERT(g.stride(1) == 1 || a.cols == 1, "distill: grad_out of unit inner stride");
+  } else {
+    g = at::empty({a.rows, a.cols}, logits.options());
+  }
+  launch([&] {
+    return dh_distill_bwd(a.x.data_ptr(), a.rows > 1 ? a.x.stride(0) : a.cols, a.ids.data_ptr(), (int)a.ids.element_size(),
+                          a.teacher.data_ptr(), a.teacher_type, (const int64_t *)ptr(a.target), stats.data_ptr<float>(), a.rows,
+                          d.data_ptr<float>(), a.rows, a.cols, (int)a.k, vocab_start, vocab_total, (float)temperature, (float)alpha,
+                          a.type, g.data_ptr(), a.rows > 1 ? g.stride(0) : a.cols, on.get());
+  });
+  return grad_out.has_value() ? *grad_out : g.view(logits.sizes());
+}
+
 // -> (out fp32 [2]: loss, mask sum; mask in fp32)
 std::tuple<Tensor, Tensor> masked_mean_fwd(const Tensor &losses, const Tensor &mask, double scale) {
   need_gpu({&losses, &mask});
@@ -1004,6 +1212,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("swiglu_bwd", &swiglu_bwd);
   m.def("residual_add", &residual_add);
   m.def("rope", &rope);
+  m.def("rotary", &rotary);
   m.def("dense_gemm", &dense_gemm);
   m.def("linear", &linear);
   m.def("matmul", &matmul);
@@ -1019,6 +1228,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attn_merge", &attn_merge);
   m.def("attn_merge_new", &attn_merge_new);
   m.def("moe_route", &moe_route);
+  m.def("balance_loss_fwd", &balance_loss_fwd);
+  m.def("route_bwd", &route_bwd);
   m.def("moe_sort", &moe_sort);
   m.def("moe_gather", &moe_gather);
   m.def("moe_scatter", &moe_scatter);
@@ -1034,6 +1245,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("embedding_bwd", &embedding_bwd);
   m.def("cross_entropy_fwd", &cross_entropy_fwd);
   m.def("cross_entropy_bwd", &cross_entropy_bwd);
+  m.def("distill_fwd", &distill_fwd);
+  m.def("distill_bwd", &distill_bwd);
   m.def("masked_mean_fwd", &masked_mean_fwd);
   m.def("masked_mean_bwd", &masked_mean_bwd);
   m.def("zero_all", &zero_all);

@@ -72,6 +72,58 @@ def cross_entropy_bwd(context, dout, grad_out=None):
     return sm
 
 
+def _vocabulary(cols):
+    """(first id of this rank's slice, ids of all ranks)"""
+    world = get_tensor_model_parallel_world_size()
+    start, _ = vocab_range_from_per_partition_vocab_size(cols, get_tensor_model_parallel_rank(), world)
+    return start, cols * world
+
+
+def distill_fwd(inputs, temperature=1.0, alpha=1.0):
+    """Distillation from a teacher's top logits, mixed with the labels' cross entropy.  inputs:
+
+    * ``vocab_parallel_logits`` [..., cols]: the student's, x
+    * ``teacher_ids`` int32 or int64 [..., K], ``teacher_logits`` [..., K] (any of the float types): the teacher's largest logits t and
+      the ids of the WHOLE vocabulary that they belong to, K <= 1024.  An id outside it (-1) is no entry; an entry listed twice counts twice
+    * ``teacher_lse`` fp32 [...] or None: log-sum-exp of the teacher's t / temperature over its whole vocabulary.  With it the teacher's
+      probabilities are what it gave them and what lies behind its list is left out; without it the list is normalised to one
+    * ``target`` int64 [...], needed for alpha < 1
+
+    p = exp(t / temperature - lse), q = softmax(x / temperature):
+
+        loss = alpha temperature^2 sum_k p_k (log p_k - log q_k) + (1 - alpha) cross entropy(x, target)
+
+    A row without entries has no first term.  With a tensor-parallel world above one the outputs are this rank's share: with
+    M = max_r row_max_r, ``sum_exp_t`` (at the temperature) and ``sum_exp`` joined as the cross entropy's sums are, each at its temperature, and
+
+        D = sum_r dot_r + mass_local_r (row_max_r - M) / temperature,   P as the cross entropy's
+
+    the loss is alpha temperature^2 (entropy - D + mass log sum_exp_t) + (1 - alpha) (log sum_exp - P), and ``distill_bwd`` gives a rank's
+    share of the gradient from a context whose ``stats`` rows 1, 2 and 3 hold M and the joined sums."""
+    logits, target = inputs["vocab_parallel_logits"], inputs.get("target")
+    start, total = _vocabulary(logits.shape[-1])
+    stats = _host.distill_fwd(logits, inputs["teacher_ids"], inputs["teacher_logits"], inputs.get("teacher_lse"), target, start, total,
+                              temperature, alpha)
+    loss, row_max, sum_exp_t, sum_exp, _, mass, dot, mass_local, entropy, predicted = stats.unbind(0)
+    hard = alpha < 1.0
+    return {
+        "loss": loss.view(logits.shape[:-1]),
+        "temperature": temperature, "alpha": alpha, "vocab_size": logits.shape[-1], "stats": stats,
+        "row_max": row_max, "sum_exp_t": sum_exp_t, "sum_exp": sum_exp if hard else None, "mass": mass, "dot": dot,
+        "mass_local": mass_local, "entropy": entropy, "predicted": predicted.view(logits.shape[:-1]) if hard else None,
+    }
+
+
+def distill_bwd(context, dout, grad_out=None):
+    """d loss / d logits of ``distill_fwd`` scaled by ``dout`` per row, into ``grad_out`` (default: a new tensor; pass the logits themselves
+    to overwrite them).  A row whose dout is 0 gets zeros, whatever it holds."""
+    inputs, out = context[0], context[1]
+    logits = inputs["vocab_parallel_logits"]
+    start, total = _vocabulary(out["vocab_size"])
+    return _host.distill_bwd(logits, inputs["teacher_ids"], inputs["teacher_logits"], inputs.get("target"), out["stats"], dout, start, total,
+                             out["temperature"], out["alpha"], grad_out)
+
+
 def mask_scale_loss_fwd(inputs):
     """loss = sum(losses * mask) / sum(mask) / num_microbatch * loss_scale (loss.py:131-153).  The NaN
     assertion of the reference needs a host sync and is left to the caller."""

@@ -10,6 +10,7 @@ buffers are sized by the caller-provided ``max_rows`` bound.
 from __future__ import annotations
 
 from dataclasses import dataclass
+from typing import Optional
 
 import torch
 
@@ -35,6 +36,42 @@ def route_topk(logits, k, stream=None, profiling=False):
     logit, ties to the lower expert id; gates = softmax over the k selected logits."""
     (idx, gates), ms = issue(_host.moe_route, stream, profiling, logits, k)
     return idx, gates, ms
+
+
+@dataclass
+class BalanceLoss:
+    """What ``balance_loss_fwd`` found, for ``route_bwd``.  ``counts``, ``prob_sum`` and ``tokens`` of several ranks add up; a rank's
+    gradient of the loss over all of them comes from a copy with ``counts`` and ``tokens`` replaced by the sums."""
+    counts: torch.Tensor              # int32 [E]: choices of each expert
+    prob_sum: torch.Tensor            # fp32 [E]: sum over the tokens of softmax(logits)
+    tokens: torch.Tensor              # int32 [1]: tokens that count
+    lse: torch.Tensor                 # fp32 [T]: log-sum-exp of each row of logits
+    mask: Optional[torch.Tensor]
+    balance_coef: float
+    z_coef: float
+
+
+def balance_loss_fwd(logits, topk_idx, mask=None, balance_coef=1.0, z_coef=0.0, stream=None, profiling=False):
+    """Losses that keep the experts in balance.  logits fp32 [T, E] and topk_idx int32 [T, k] as ``route_topk`` has them; mask bool [T]
+    leaves tokens out (padding; such a token's logits may be anything).  With p = softmax(logits) over all experts, N tokens that count,
+    counts and prob_sum over them:
+
+        losses[0] = balance_coef * E / (k N^2) * sum_e counts[e] prob_sum[e]        (balance_coef where all is even)
+        losses[1] = z_coef / N * sum_t logsumexp(logits_t)^2
+
+    both 0 when no token counts.  Returns (losses fp32 [2], BalanceLoss, ms)."""
+    (losses, *found), ms = issue(_host.balance_loss_fwd, stream, profiling, logits, topk_idx, mask, balance_coef, z_coef)
+    return losses, BalanceLoss(*found, mask, balance_coef, z_coef), ms
+
+
+def route_bwd(logits, topk_idx, gates=None, dgates=None, balance=None, dlosses=None, stream=None, profiling=False):
+    """Gradient of the router's logits: through the gates (dgates fp32 [T, k], as ``unpermute_bwd`` returns them, of every token, padding
+    included) and of the losses of ``balance_loss_fwd`` (``balance``), times ``dlosses`` (fp32 [2] on the GPU; None: 1).  Either may be
+    absent.  The choice of experts and their counts are constants.  Returns (dlogits fp32 [T, E], ms)."""
+    b = balance
+    return issue(_host.route_bwd, stream, profiling, logits, topk_idx, gates if dgates is not None else None, dgates,
+                 *((b.mask, b.lse, b.counts, b.tokens) if b is not None else (None,) * 4), dlosses if b is not None else None,
+                 *((b.balance_coef, b.z_coef) if b is not None else (0.0, 0.0)))
 
 
 def sort_assignments(topk_idx, num_experts, stream=None, profiling=False):

@@ -146,6 +146,26 @@ int dh_rope(const void *q, const void *k, void *q_out, void *k_out,
             int backward, int dtype, void *stream);
 
 /* ------------------------------------------------------------------------
+ * Rotary positions in their general form (no counterpart in the reference).
+ * The first rot elements of a head (even, 2 <= rot <= d) are turned in pairs:
+ * (j, j + rot / 2), or (2j, 2j + 1) with interleaved != 0; the rest is passed
+ * through.  A pair's angle is position * steps[j] * 2^-64 turns, exact for
+ * every position; cos and sin are multiplied by factor.  backward != 0: sin ->
+ * -sin.  steps: rot / 2 whole numbers, the pair's frequency / (2 pi) * 2^64.
+ * positions: int32 or int64 (position_bytes 4 or 8) per token, or NULL for
+ * t % seq_len (t when seq_len <= 0).  Token and head strides in elements, any
+ * alignment; elements of a head are contiguous.  Output may be the input
+ * itself (same strides), else it does not overlap it.
+ * ---------------------------------------------------------------------- */
+int dh_rotary(const void *q, const void *k, void *q_out, void *k_out,
+              const uint64_t *steps, const void *positions, int position_bytes,
+              int64_t tokens, int hq, int hk, int d, int rot, int64_t q_token,
+              int64_t q_head, int64_t k_token, int64_t k_head, int64_t qo_token,
+              int64_t qo_head, int64_t ko_token, int64_t ko_head,
+              int64_t seq_len, int interleaved, int backward, float factor,
+              int dtype, void *stream);
+
+/* ------------------------------------------------------------------------
  * Variable-length flash attention.  csrc/operators/ops.h:18-32 /
  * csrc/operators/flash_atten.cu:220-434 (forward) and ops.h:34-52 /
  * flash_atten.cu:479-757 (backward).
@@ -330,6 +350,34 @@ int dh_moe_route_topk(const float *logits, int32_t *topk_idx, float *gates,
                       int64_t tokens, int experts, int k, void *stream);
 /* Lanes that such a call gives a token (1: a scan of its row); 0: nothing to do. */
 int dh_moe_route_lanes(int64_t tokens, int experts, int k);
+/* Losses that keep the experts in balance, and counts.  p = softmax of a row of
+ * logits over all experts, lse its log-sum-exp, N the tokens that count (mask
+ * byte not 0; mask NULL: all).  counts[e] = choices of e, prob_sum[e] = sum p_e,
+ * n_tokens[0] = N, all over the tokens that count; lse fp32 [tokens].
+ * losses[0] = balance_coef experts / (k N^2) sum_e counts[e] prob_sum[e],
+ * losses[1] = z_coef / N sum lse^2; both 0 when N is 0.  A token that does not
+ * count may hold anything.  Choices outside [0, experts) are left out.
+ * experts <= 64, k <= 8, tokens < 2^28.  workspace may be NULL when
+ * dh_balance_loss_workspace_bytes is 0. */
+size_t dh_balance_loss_workspace_bytes(int64_t tokens, int experts);
+int dh_balance_loss_fwd(const float *logits, const int32_t *topk_idx,
+                        const uint8_t *mask, int64_t tokens, int experts, int k,
+                        float balance_coef, float z_coef, float *losses,
+                        int32_t *counts, float *prob_sum, int32_t *n_tokens,
+                        float *lse, void *workspace, size_t workspace_bytes,
+                        void *stream);
+/* dlogits fp32 [tokens, experts], every element written: the gradient of the
+ * losses (lse, counts, n_tokens of the forward; lse NULL: without them) times
+ * dlosses[0] and dlosses[1] (device, NULL: 1), plus the gradient through the
+ * gates g: g_j (dg_j - sum_i g_i dg_i) on the chosen logits (dgates NULL:
+ * without it), for every token, whatever the mask says. */
+int dh_moe_route_bwd(const float *logits, const int32_t *topk_idx,
+                     const float *gates, const float *dgates,
+                     const uint8_t *mask, const float *lse,
+                     const int32_t *counts, const int32_t *n_tokens,
+                     const float *dlosses, int64_t tokens, int experts, int k,
+                     float balance_coef, float z_coef, float *dlogits,
+                     void *stream);
 
 size_t dh_moe_sort_workspace_bytes(int64_t n_assign, int experts);
 /* Stable counting sort of the flat assignment list topk_idx [n_assign]
@@ -565,6 +613,36 @@ int dh_cross_entropy_bwd(const void *src, int64_t ld_src, int from_logits, const
                          const float *sum_exp, const int64_t *target, const float *dout,
                          int64_t rows, int64_t cols, int64_t vocab_start, float label_smoothing,
                          int dtype, void *grad, int64_t ld_grad, void *stream);
+
+/* Distillation from a teacher's top logits, mixed with the labels' cross entropy; fp32 arithmetic.
+ * A row has k teacher entries: ids (int32 / int64, id_bytes 4 / 8) of the whole vocabulary and logits t (fp32, bf16 or
+ * fp16), both [rows, k].  Ids outside [0, vocab_total) are no entries.  p = exp(t / temperature - l) with l the
+ * log-sum-exp of the row's t / temperature, or teacher_lse[row] where that is given (the teacher's over its whole
+ * vocabulary, at the temperature).  q = softmax(x / temperature) of the student.
+ *   loss = alpha temperature^2 sum p (log p - log q) + (1 - alpha) cross entropy(x, target)
+ * alpha < 1 needs targets (int64), alpha = 1 takes none.  An entry listed twice counts twice; a row without entries has no
+ * first term.  stats: 10 rows of `pitch` floats:
+ *   0 loss, 1 max x = m, 2 S = sum exp((x - m) / temperature), 3 sum exp(x - m) (alpha < 1), 4 l, 5 M = sum p,
+ *   6 D = sum over the entries of this slice p (x - m) / temperature, 7 sum of their p, 8 H = sum p log p,
+ *   9 x[target] - m (0 outside the slice)
+ * with loss = alpha temperature^2 (H - D + M log S) + (1 - alpha) (log stats[3] - stats[9]).
+ * k <= 1024, rows < 2^24, cols < 2^30, temperature in [1e-6, 1e6].  workspace may be NULL when
+ * dh_distill_workspace_bytes is 0. */
+size_t dh_distill_workspace_bytes(int64_t rows, int64_t cols);
+int dh_distill_fwd(const void *logits, int64_t ld, const void *ids, int id_bytes, const void *teacher,
+                   int teacher_dtype, const float *teacher_lse, const int64_t *target, int64_t rows,
+                   int64_t cols, int k, int64_t vocab_start, int64_t vocab_total, float temperature,
+                   float alpha, int dtype, float *stats, int64_t pitch, void *workspace,
+                   size_t workspace_bytes, void *stream);
+
+/* grad = dout[row] (alpha temperature (M q - sum p onehot(id)) + (1 - alpha) (softmax(x) - onehot(target))) from the logits
+ * and rows 1 to 5 of stats.  A row whose dout is 0, or that has neither entries nor a target, gets zeros whatever it
+ * holds.  grad may be the logits. */
+int dh_distill_bwd(const void *logits, int64_t ld, const void *ids, int id_bytes, const void *teacher,
+                   int teacher_dtype, const int64_t *target, const float *stats, int64_t pitch,
+                   const float *dout, int64_t rows, int64_t cols, int k, int64_t vocab_start,
+                   int64_t vocab_total, float temperature, float alpha, int dtype, void *grad,
+                   int64_t ld_grad, void *stream);
 
 /* out[i, :] = vocab[ids[i] - vocab_start, :], zero rows for ids outside
  * [vocab_start, vocab_start + vocab_rows): dhellam/operators/embedding.py:16-39. */

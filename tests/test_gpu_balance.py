@@ -1,0 +1,220 @@
+"""The router's losses, counts and gradients against 64-bit autograd and against differences."""
+import pytest
+import torch
+
+from dhellam_amd.operators.moe import BalanceLoss, balance_loss_fwd, route_bwd, route_topk
+
+pytestmark = pytest.mark.gpu
+
+A, B = 0.01, 0.001
+
+
+def router(t, e, k, seed=0, masked=False):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    logits = torch.randn(t, e, generator=g, device="cuda") * 2 + torch.randn(e, generator=g, device="cuda")
+    idx, gates, _ = route_topk(logits, k)
+    dgates = torch.randn(t, k, generator=g, device="cuda")
+    mask = torch.rand(t, generator=g, device="cuda") < 0.7 if masked else None
+    return logits, idx, gates, dgates, mask
+
+
+def plain(logits, idx, gates, dgates, mask, w=(1.0, 1.0), a=A, b=B):
+    """losses, counts, prob_sum, dlogits in 64 bits, and the size of the terms that the gradient is a sum of."""
+    t, e = logits.shape
+    k = idx.shape[1]
+    m = mask if mask is not None else torch.ones(t, dtype=torch.bool, device=logits.device)
+    x = torch.where(m[:, None], logits.double(), 0.0).requires_grad_(True)
+    n = max(int(m.sum()), 1)
+    counts = torch.stack([((idx == i) & m[:, None]).sum() for i in range(e)])
+    lse, p = torch.logsumexp(x, 1), torch.softmax(x, 1)
+    probs = (p * m[:, None]).sum(0)
+    losses = torch.stack((a * e / (k * n * n) * (counts * probs).sum(), b / n * (lse ** 2 * m).sum()))
+    (d,) = torch.autograd.grad((losses * torch.tensor(w, dtype=torch.float64, device=x.device)).sum(), x)
+    p, lse = p.detach() * m[:, None], lse.detach() * m
+    size = abs(w[0]) * a * e / (k * n * n) * p * (counts + (counts * p).sum(1, keepdim=True)) + abs(w[1]) * 2 * b / n * lse.abs()[:, None] * p
+    if dgates is not None:
+        g, dg = gates.double(), dgates.double()
+        d = d.scatter_add(1, idx.long(), g * (dg - (g * dg).sum(1, keepdim=True)))
+        size = size.scatter_add(1, idx.long(), g * (dg.abs() + (g * dg.abs()).sum(1, keepdim=True)))
+    return losses.detach(), counts, probs.detach(), d, size
+
+
+def close(got, want, size, tol=1e-5):
+    """An exponential's relative error is (|x - max| + 3) 2^-24, at most 20 2^-24 here; sums are of at most 100 terms one behind the other
+    (16 of a lane, 6 exchanges, 4 and 32 and 16 partial sums): 120 2^-24 = 7e-6 of the terms' size."""
+    assert ((got.double() - want).abs() <= tol * size + 1e-30).all(), ((got.double() - want).abs() / (size + 1e-30)).max()
+
+
+SIZES = [(1, 1, 1), (1, 8, 2), (3, 2, 1), (64, 5, 3), (63, 64, 8), (1000, 8, 2), (257, 24, 2), (4096, 16, 4), (5000, 60, 6), (2049, 7, 7), (20011, 64, 8),
+         (70001, 8, 2), (131072, 33, 5)]
+
+
+@pytest.mark.parametrize("t,e,k", SIZES)
+@pytest.mark.parametrize("masked", [False, True])
+def test_losses_counts_and_gradients(t, e, k, masked):
+    logits, idx, gates, dgates, mask = router(t, e, k, seed=t, masked=masked)
+    losses, bal, ms = balance_loss_fwd(logits, idx, mask, A, B)
+    want = plain(logits, idx, gates, dgates, mask)
+    assert ms == 0 and bal.counts.dtype == torch.int32 and torch.equal(bal.counts.long(), want[1])
+    assert bal.tokens.item() == (t if mask is None else int(mask.sum()))
+    close(losses, want[0], want[0].abs())
+    close(bal.prob_sum, want[2], want[2])
+    d, _ = route_bwd(logits, idx, gates, dgates, bal)
+    close(d, want[3], want[4])
+    # each part alone, and the losses' gradients scaled
+    none = plain(logits, idx, gates, None, mask, (0.5, -3.0))
+    close(route_bwd(logits, idx, gates, None, bal, torch.tensor([0.5, -3.0], device="cuda"))[0], none[3], none[4])
+    alone = plain(logits, idx, gates, dgates, mask, (0.0, 0.0))
+    close(route_bwd(logits, idx, gates, dgates)[0], alone[3], alone[4])
+
+
+def test_gradient_against_differences():
+    """The losses as a function of the logits with the choices held fixed; a step of h errs by its third derivative, below h^2."""
+    logits, idx, gates, dgates, _ = router(6, 8, 2)
+    _, bal, _ = balance_loss_fwd(logits, idx, None, 1.0, 0.1)
+    d = route_bwd(logits, idx, gates, None, bal)[0]
+    f = lambda x: plain(x, idx, gates, None, None, a=1.0, b=0.1)[0].sum().item()
+    h = 1e-4
+    for t in range(6):
+        for e in range(8):
+            up, down = logits.double().clone(), logits.double().clone()
+            up[t, e] += h
+            down[t, e] -= h
+            assert abs((f(up) - f(down)) / (2 * h) - d[t, e].item()) <= 1e-6
+
+
+def test_an_even_router_has_the_coefficient_as_its_loss():
+    logits = torch.zeros(64, 8, device="cuda")
+    idx = (torch.arange(64, device="cuda", dtype=torch.int32)[:, None] * 2 + torch.arange(2, device="cuda", dtype=torch.int32)) % 8
+    losses, bal, _ = balance_loss_fwd(logits, idx, None, 0.5, 1.0)
+    torch.testing.assert_close(losses, torch.tensor([0.5, torch.tensor(8.0).log() ** 2], device="cuda"), rtol=1e-6, atol=0)
+    assert (bal.counts == 16).all()
+    assert route_bwd(logits, idx, balance=BalanceLoss(bal.counts, bal.prob_sum, bal.tokens, bal.lse, None, 0.5, 0.0))[0].abs().max() <= 1e-8
+
+
+@pytest.mark.parametrize("t,e,k", [(40, 8, 2), (9000, 64, 4), (5, 5, 2)])
+def test_masked_tokens_may_hold_anything(t, e, k):
+    logits, idx, gates, dgates, mask = router(t, e, k, masked=True)
+    mask[0], mask[-1] = False, True
+    want = balance_loss_fwd(logits, idx, mask, A, B)
+    dwant = route_bwd(logits, idx, gates, None, want[1])[0]
+    bad = logits.clone()
+    bad[~mask] = torch.tensor([torch.nan, torch.inf, -torch.inf, torch.finfo(torch.float32).min], device="cuda").repeat(t)[:e * t].view(-1)[:e]
+    worse = idx.clone()
+    worse[~mask] = -7
+    got = balance_loss_fwd(bad, worse, mask, A, B)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1].counts, want[1].counts) and torch.equal(got[1].prob_sum, want[1].prob_sum)
+    d = route_bwd(bad, worse, gates, None, got[1])[0]
+    assert torch.equal(d, dwant) and (d[~mask] == 0).all()
+
+
+def test_nothing_counts():
+    logits, idx, gates, dgates, _ = router(100, 8, 2)
+    off = torch.zeros(100, dtype=torch.bool, device="cuda")
+    losses, bal, _ = balance_loss_fwd(logits * torch.nan, idx, off, A, B)
+    assert (losses == 0).all() and (bal.counts == 0).all() and (bal.prob_sum == 0).all() and bal.tokens.item() == 0
+    assert (route_bwd(logits, idx, gates, None, bal)[0] == 0).all()
+    losses, bal, _ = balance_loss_fwd(logits[:0], idx[:0], None, A, B)
+    assert (losses == 0).all() and (bal.counts == 0).all() and bal.tokens.item() == 0
+    assert route_bwd(logits[:0], idx[:0], gates[:0], dgates[:0], bal)[0].shape == (0, 8)
+
+
+def test_experts_that_are_switched_off():
+    """Logits of -inf, and of the type's lowest value, are probabilities of zero; choices outside [0, E) are not counted."""
+    logits, idx, gates, dgates, _ = router(500, 8, 2)
+    for low in (-torch.inf, torch.finfo(torch.float32).min):
+        x = logits.clone()
+        x[:, 5] = low
+        i, g, _ = route_topk(x, 2)
+        losses, bal, _ = balance_loss_fwd(x, i, None, A, B)
+        assert bal.counts[5] == 0 and bal.prob_sum[5] == 0 and torch.isfinite(losses).all()
+        d = route_bwd(x, i, g, dgates, bal)[0]
+        assert (d[:, 5] == 0).all()
+        keep = [0, 1, 2, 3, 4, 6, 7]
+        small = i - (i > 5).int()
+        want = plain(x[:, keep], small, g, dgates, None, a=A * 8 / 7)
+        close(d[:, keep], want[3], want[4])
+    out = idx.clone()
+    out[::2, 0], out[1::2, 1] = -1, 8
+    _, bal, _ = balance_loss_fwd(logits, out, None, A, B)
+    assert bal.counts.sum() == 500
+
+
+def test_an_expert_chosen_twice_counts_twice():
+    logits, idx, gates, dgates, _ = router(50, 8, 2)
+    idx[:, 1] = idx[:, 0]
+    losses, bal, _ = balance_loss_fwd(logits, idx, None, A, B)
+    want = plain(logits, idx, gates, dgates, None)
+    assert torch.equal(bal.counts.long(), torch.bincount(idx.flatten().long(), minlength=8))
+    d = route_bwd(logits, idx, gates, dgates)[0]
+    g, dg = gates.double(), dgates.double()
+    ref = torch.zeros(50, 8, dtype=torch.float64, device="cuda").scatter_add(1, idx.long(), g * (dg - (g * dg).sum(1, keepdim=True)))
+    close(d, ref, torch.zeros_like(ref).scatter_add(1, idx.long(), g * (dg.abs() + (g * dg.abs()).sum(1, keepdim=True))))
+
+
+def test_ranks_join_their_counts():
+    logits, idx, gates, dgates, mask = router(4000, 16, 2, masked=True)
+    whole = balance_loss_fwd(logits, idx, mask, A, B)
+    parts = [balance_loss_fwd(logits[s].contiguous(), idx[s].contiguous(), mask[s].contiguous(), A, B) for s in (slice(0, 1500), slice(1500, 4000))]
+    counts, tokens = sum(p[1].counts for p in parts), sum(p[1].tokens for p in parts)
+    assert torch.equal(counts, whole[1].counts) and torch.equal(tokens, whole[1].tokens)
+    probs = sum(p[1].prob_sum for p in parts)
+    n = tokens.double()
+    torch.testing.assert_close((A * 16 / (2 * n * n) * (counts.double() * probs.double()).sum()).float()[0], whole[0][0], rtol=1e-5, atol=0)
+    want = route_bwd(logits, idx, None, None, whole[1])[0]
+    for p, s in zip(parts, (slice(0, 1500), slice(1500, 4000))):
+        bal = BalanceLoss(counts, probs, tokens, p[1].lse, p[1].mask, A, B)
+        assert torch.equal(route_bwd(logits[s].contiguous(), idx[s].contiguous(), None, None, bal)[0], want[s])
+
+
+def test_the_same_every_time_on_streams_and_in_graphs():
+    """Two graphs captured on one stream, replayed at the same time on two: neither shares scratch with the other."""
+    data = [router(60000 + i, 64, 8, seed=i) for i in range(2)]
+    want = []
+    for logits, idx, gates, dgates, mask in data:
+        losses, bal, _ = balance_loss_fwd(logits, idx, mask, A, B)
+        want.append((losses, bal.counts, bal.prob_sum, route_bwd(logits, idx, gates, dgates, bal)[0]))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    logits, idx, gates, dgates, mask = data[0]
+    losses, bal, ms = balance_loss_fwd(logits, idx, mask, A, B, stream=side, profiling=True)
+    d, _ = route_bwd(logits, idx, gates, dgates, bal, stream=side)
+    torch.cuda.synchronize()
+    assert ms > 0 and torch.equal(losses, want[0][0]) and torch.equal(d, want[0][3])
+    graphs, outs = [], []
+    for logits, idx, gates, dgates, mask in data:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            losses, bal, _ = balance_loss_fwd(logits, idx, mask, A, B)
+            outs.append((losses, bal.counts, bal.prob_sum, route_bwd(logits, idx, gates, dgates, bal)[0]))
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        for o in outs:
+            for x in o:
+                x.zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for got, ref in zip(outs, want):
+            assert all(torch.equal(x, y) for x, y in zip(got, ref))
+
+
+def test_refusals():
+    logits, idx, gates, dgates, _ = router(10, 8, 2)
+    _, bal, _ = balance_loss_fwd(logits, idx)
+    ok = torch.ones(10, dtype=torch.bool, device="cuda")
+    for bad in [lambda: balance_loss_fwd(logits.half(), idx), lambda: balance_loss_fwd(logits[:, :4], idx), lambda: balance_loss_fwd(logits, idx.long()),
+                lambda: balance_loss_fwd(logits, idx[:9]), lambda: balance_loss_fwd(logits, idx, ok.float()), lambda: balance_loss_fwd(logits, idx, ok[:9]),
+                lambda: route_bwd(logits, idx), lambda: route_bwd(logits, idx, None, dgates), lambda: route_bwd(logits, idx, gates.half(), dgates),
+                lambda: route_bwd(logits, idx, gates[:9], dgates), lambda: route_bwd(logits[:9], idx[:9], None, None, bal),
+                lambda: route_bwd(logits, idx, None, None, bal, torch.ones(3, device="cuda"))]:
+        with pytest.raises(AssertionError):
+            bad()
+    for bad in [lambda: balance_loss_fwd(logits, idx.cpu()), lambda: balance_loss_fwd(torch.zeros(4, 65, device="cuda"), idx[:4]),
+                lambda: balance_loss_fwd(logits, torch.zeros(10, 9, dtype=torch.int32, device="cuda")),
+                lambda: route_bwd(logits, idx, gates, dgates.cpu()), lambda: balance_loss_fwd(logits, idx, stream=3)]:
+        with pytest.raises(RuntimeError):
+            bad()

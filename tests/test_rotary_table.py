@@ -1,0 +1,71 @@
+"""Frequencies and tables of the general rotary positions (no GPU)."""
+import math
+from decimal import Decimal, getcontext
+
+import pytest
+import torch
+
+from dhellam_amd.operators.rope import rotary_frequencies, rotary_table
+
+PI = Decimal("3.14159265358979323846264338327950288419716939937510582097494459")
+
+
+def test_a_table_holds_the_turns_of_a_position():
+    """A step is theta^(-2j / dim) / (2 pi) turns: 2^-53 of it from the 64-bit power and two more roundings."""
+    getcontext().prec = 50
+    theta, dim = 500000.0, 128
+    t = rotary_table(theta, dim, "cpu")
+    assert t.steps.dtype == torch.int64 and t.steps.shape == (dim // 2,) and not t.interleaved and t.factor == 1.0
+    for j, u in enumerate(t.steps.tolist()):
+        want = (Decimal(theta).ln() * (Decimal(-2 * j) / Decimal(dim))).exp() / (2 * PI)
+        assert abs(Decimal(u) / 2 ** 64 - want) <= want * Decimal(2.0 ** -50) + Decimal(2.0 ** -64)
+
+
+def test_steps_past_half_a_turn_are_negative_numbers():
+    t = rotary_table(10000.0, 4, "cpu", scaling={"kind": "linear", "factor": 0.25})      # 4 radians a position
+    assert t.steps[0].item() < 0
+    assert abs(t.steps[0].item() % 2 ** 64 / 2 ** 64 - 4 / (2 * math.pi)) < 1e-15
+
+
+@pytest.mark.parametrize("dim", [2, 20, 64, 128])
+def test_scaled_frequencies(dim):
+    theta, s = 10000.0, 8.0
+    plain, one = rotary_frequencies(theta, dim)
+    assert one == 1.0 and plain[0] == 1.0 and len(plain) == dim // 2
+    assert rotary_frequencies(theta, dim, {"kind": "linear", "factor": s})[0] == [x / s for x in plain]
+    ntk, _ = rotary_frequencies(theta, dim, {"kind": "ntk", "factor": s})
+    assert ntk[0] == 1.0
+    if dim > 2:
+        assert math.isclose(ntk[-1], plain[-1] / s, rel_tol=1e-12)                        # the slowest pair is interpolated, the fastest stays
+    length = 4096
+    bands, one = rotary_frequencies(theta, dim, {"kind": "bands", "factor": s, "original_length": length})
+    parts, m = rotary_frequencies(theta, dim, {"kind": "parts", "factor": s, "original_length": length})
+    assert one == 1.0 and math.isclose(m, 0.1 * math.log(s) + 1)
+    for got in (bands, parts):
+        assert all(x / s * (1 - 1e-12) <= y <= x * (1 + 1e-12) for x, y in zip(plain, got))
+        ratio = [y / x for x, y in zip(plain, got)]
+        assert ratio == sorted(ratio, reverse=True) or all(a >= b - 1e-12 for a, b in zip(ratio, ratio[1:]))
+    for x, y in zip(plain, bands):
+        turns = length * x / (2 * math.pi)
+        if turns > 4:
+            assert y == x
+        if turns < 1:
+            assert y == x / s
+    for x, y in zip(plain, parts):                      # a pair's index is rounded outwards: two more pairs on either side of the line
+        step = theta ** (2.0 / dim)
+        if length * x / (2 * math.pi) > 32 * step ** 2:
+            assert math.isclose(y, x, rel_tol=1e-12)
+        if length * x / (2 * math.pi) < step ** -2:
+            assert math.isclose(y, x / s, rel_tol=1e-12)
+    assert rotary_frequencies(theta, dim, {"kind": "parts", "factor": s, "original_length": length, "attention_factor": 1.5})[1] == 1.5
+
+
+@pytest.mark.parametrize("args", [
+    (10000.0, 3), (10000.0, 0), (10000.0, 2.0), (0.0, 4), (math.nan, 4), (10000.0, 4, {}), (10000.0, 4, {"kind": "other", "factor": 2.0}),
+    (10000.0, 4, {"kind": "linear"}), (10000.0, 4, {"kind": "linear", "factor": -1.0}), (10000.0, 4, {"kind": "linear", "factor": 2.0, "low": 1}),
+    (10000.0, 4, {"kind": "bands", "factor": 2.0}), (10000.0, 4, {"kind": "bands", "factor": 2.0, "original_length": 64, "low": 4.0, "high": 4.0}),
+    (10000.0, 4, {"kind": "parts", "factor": 2.0, "original_length": 64, "beta_fast": 1.0, "beta_slow": 2.0}),
+    (1.0, 4, {"kind": "parts", "factor": 2.0, "original_length": 64})])
+def test_refused_frequencies(args):
+    with pytest.raises(ValueError):
+        rotary_frequencies(*args)
