@@ -10,31 +10,43 @@
 // once with a running maximum and one or two sums of exponentials beside it, and K single logits; the backward reads it once more
 // and writes the gradient.  The K listed columns (and the target's) are corrected behind the row's stores, so nothing
 // per element depends on the column.
+//
+// 4096 x 128256 in bf16, K = 128, alpha 0.5, tau 1: forward 167 us (6.3 TB/s), backward 361 us (5.8 TB/s); a copy on this card 5.9 TB/s.
 #include "common.h"
 
 namespace dh {
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int BT = 256, MAX_K = 1024, SLOTS = MAX_K / BT;      // threads of a row's workgroup; entries of a list; of a thread
+constexpr int BT = 256, MAX_K = 1024;      // threads of a workgroup; entries of a list
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // 16 bytes aligned as single elements are: rows of any pitch and any start.
 typedef uint32_t raw16 __attribute__((ext_vector_type(4), aligned(2)));
-template <typename T> __device__ __forceinline__ Vec<T> load16(const T *p) {
-  return __builtin_bit_cast(Vec<T>, *reinterpret_cast<const raw16 *>(p));
+template <bool NT, typename T> __device__ __forceinline__ Vec<T> load16(const T *p) {
+  const raw16 *q = reinterpret_cast<const raw16 *>(p);
+  return __builtin_bit_cast(Vec<T>, NT ? __builtin_nontemporal_load(q) : *q);
 }
-template <typename T> __device__ __forceinline__ void store16(T *p, const Vec<T> &x) {
-  *reinterpret_cast<raw16 *>(p) = __builtin_bit_cast(raw16, x);
+template <bool NT, typename T> __device__ __forceinline__ void store16(T *p, const Vec<T> &x) {
+  const raw16 v = __builtin_bit_cast(raw16, x);
+  if (NT) __builtin_nontemporal_store(v, reinterpret_cast<raw16 *>(p));
+  else *reinterpret_cast<raw16 *>(p) = v;
 }
 
-__device__ __forceinline__ float block_max(float v, float *red) {
-  v = wave_max(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+// How the exponential at temperature one comes from that at tau, e: it is the same (tau 1, or no targets), e^2 (tau 2), e^4 (tau 4), or
+// needs one of its own.  An exponential is four of the fifteen issue slots that an element takes with two of them, which is
+// more than its two bytes take to arrive: forward of 4096 x 16032 in bf16 at tau 2, alpha 0.5, 30.8 us with two, 26.8 squared.
+enum Hard { SAME, SQUARE, FOURTH, OWN };
+Hard hard_of(float temperature, float alpha) {
+  if (alpha == 1.f || temperature == 1.f) return SAME;
+  return temperature == 2.f ? SQUARE : temperature == 4.f ? FOURTH : OWN;
+}
+template <Hard H> __device__ __forceinline__ float exp_one(float e, float y) {      // y = x - reference
+  if (H == SAME) return e;
+  if (H == SQUARE) return e * e;
+  if (H == FOURTH) return (e * e) * (e * e);
+  return exp2_fast(y * LOG2E);
 }
 
 struct Teacher {
@@ -67,302 +79,370 @@ struct Teacher {
 // The per-row statistics, `pitch` floats apart.
 enum { LOSS, ROW_MAX, SUM_TAU, SUM_ONE, NORM, MASS, DOT, MASS_LOCAL, ENTROPY, PREDICTED, N_STATS };
 
-// Running maximum and sums of exponentials against it: s at the temperature, s1 at one (TWO).
-template <bool TWO> struct Running {
-  float m = -INFINITY, s = 0.f, s1 = 0.f;
+// Sums of exponentials, s at the temperature and s1 at one (TWO), against a reference m that is moved only when a value
+// passes it by 2^16: the sums are then as exact as against the maximum (a float's precision does not depend on its scale), and a
+// wavefront hardly ever branches once it has seen its first values.  The lowest float to begin with: -inf adds nothing to it, and
+// a row of lowest floats is a row of equal ones.
+template <Hard H> struct Running {
+  float m = -3.402823466e38f, top = -INFINITY, s = 0.f, s1 = 0.f;
   __device__ __forceinline__ void move(float to, float k) {
     s *= exp2_fast((m - to) * k);
-    if (TWO) s1 *= exp2_fast((m - to) * LOG2E);
+    if (H != SAME) s1 *= exp2_fast((m - to) * LOG2E);
     m = to;
   }
-  template <int N> __device__ __forceinline__ void add(const float *x, float k) {
-    float top = x[0];
+  template <int N> __device__ __forceinline__ void add(const float *x, float k, float slack) {
+    float t = x[0];
 #pragma unroll
-    for (int i = 1; i < N; ++i) top = fmaxf(top, x[i]);
-    if (top > m) move(top, k);                      // m = -inf: 0 * exp2(-inf) = 0
-    if (m == -INFINITY && top == -INFINITY) return;      // nothing but -inf so far
+    for (int i = 1; i < N; ++i) t = fmaxf(t, x[i]);
+    top = fmaxf(top, t);
+    if (t > m + slack) move(t, k);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       // (x - m) first: the difference of two close numbers is exact
-      s += exp2_fast((x[i] - m) * k);
-      if (TWO) s1 += exp2_fast((x[i] - m) * LOG2E);
+      const float y = x[i] - m;
+      const float e = exp2_fast(y * k);
+      s += e;
+      if (H != SAME) s1 += exp_one<H>(e, y);
     }
-  }
-  // brought to a maximum that others share
-  __device__ __forceinline__ void align(float to, float k) {
-    if (m > -INFINITY) move(to, k);
   }
 };
 
-template <bool TWO, typename T>
-__device__ __forceinline__ void scan_row(const T *row, int64_t from, int64_t to, float k, Running<TWO> &run) {
-  constexpr int N = Vec<T>::N, U = 4;                // vectors in flight
-  const int64_t nvec = (to - from) / N;
+template <bool NT, Hard H, typename T>
+__device__ __forceinline__ void scan_row(const T *row, int64_t from, int64_t to, float k, Running<H> &run) {
+  constexpr int N = Vec<T>::N, U = 2;                // vectors in flight: 4096 x 16032 in bf16, not in any cache, 30.3 us, with 4 32.8, with 8 39.2
+  const float slack = 16.f / fmaxf(k, LOG2E);        // 2^16 at either temperature
+  const int nvec = (int)((to - from) / N);
   const T *base = row + from;
-  int64_t v = threadIdx.x;
-  for (; v + (U - 1) * BT < nvec; v += U * BT) {
+  for (int v = threadIdx.x; v < nvec; v += U * BT) {
     Vec<T> x[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) x[u] = load16(base + (v + u * BT) * N);
+    for (int u = 0; u < U; ++u)
+      if (v + u * BT < nvec) x[u] = load16<NT>(base + (int64_t)(v + u * BT) * N);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float f[N];
+    for (int u = 0; u < U; ++u)
+      if (v + u * BT < nvec) {
+        float f[N];
 #pragma unroll
-      for (int e = 0; e < N; ++e) f[e] = to_f(x[u].v[e]);
-      run.template add<N>(f, k);
-    }
+        for (int e = 0; e < N; ++e) f[e] = to_f(x[u].v[e]);
+        run.template add<N>(f, k, slack);
+      }
   }
-  for (; v < nvec; v += BT) {
-    const Vec<T> x = load16(base + v * N);
-    float f[N];
-#pragma unroll
-    for (int e = 0; e < N; ++e) f[e] = to_f(x.v[e]);
-    run.template add<N>(f, k);
-  }
-  for (int64_t c = nvec * N + threadIdx.x; c < to - from; c += BT) {
+  for (int64_t c = (int64_t)nvec * N + threadIdx.x; c < to - from; c += BT) {
     const float f = to_f(base[c]);
-    run.template add<1>(&f, k);
+    run.template add<1>(&f, k, slack);
   }
 }
 
-// The row's statistics from its maximum and sums, by a whole workgroup.
-template <typename T>
-__device__ __forceinline__ void finish_row(const Teacher &t, const T *row, int64_t r, float m, float s, float s1, float *stats,
-                                           int64_t pitch, float *red) {
-  float a[SLOTS], x[SLOTS];                          // t / tau, the student's logit (local entries)
-  bool local[SLOTS];
-  float top = -INFINITY;
+// A row's teacher entries, by one wavefront, 256 at a time: what is read is asked for before the row is scanned.
+struct Entries {
+  static constexpr int U = 4;
+  float a[U], x[U];                                  // t / tau (-inf: none), the student's logit
+  uint32_t local;                                    // bit i: entry i lies in this slice
+  template <typename T> __device__ __forceinline__ void load(const Teacher &t, const T *row, int64_t r, int first) {
+    int64_t id[U];
 #pragma unroll
-  for (int i = 0; i < SLOTS; ++i) {
-    const int j = i * BT + (int)threadIdx.x;
-    a[i] = -INFINITY;
-    x[i] = 0.f;
-    local[i] = false;
-    if (j < t.k) {
-      const int64_t id = t.id(r, j);
-      if (t.there(id)) {
+    for (int i = 0; i < U; ++i) {
+      const int j = first + i * 64 + (int)(threadIdx.x & 63);
+      id[i] = -1;
+      a[i] = -INFINITY;
+      if (j < t.k) {
+        id[i] = t.id(r, j);
         a[i] = t.logit(r, j);
-        const int64_t c = t.column(id);
-        local[i] = c >= 0;
-        if (local[i]) x[i] = to_f(row[c]);
       }
     }
-    top = fmaxf(top, a[i]);
-  }
-  float norm;
-  if (t.lse) {
-    norm = t.lse[r];
-  } else {
-    top = block_max(top, red);
-    float sum = 0.f;
+    local = 0;
 #pragma unroll
-    for (int i = 0; i < SLOTS; ++i)
-      if (a[i] != -INFINITY) sum += expf(a[i] - top);
-    sum = block_sum<BT>(sum, red);
-    norm = sum != 0.f ? top + logf(sum) : 0.f;       // no entries: no mass either
+    for (int i = 0; i < U; ++i) {
+      x[i] = 0.f;
+      if (!t.there(id[i])) {
+        a[i] = -INFINITY;
+        continue;
+      }
+      const int64_t c = t.column(id[i]);
+      if (c >= 0) {
+        x[i] = to_f(row[c]);
+        local |= 1u << i;
+      }
+    }
   }
-  float mass = 0.f, mine = 0.f, dot = 0.f, ent = 0.f;
+};
+
+// The sums over a row's entries in one pass: weights exp(a - ref) against a running reference, logits against `m`.
+struct Sums {
+  float norm, mass, dot, mine, ent;
+  template <typename T>
+  __device__ __forceinline__ void run(const Teacher &t, const T *row, int64_t r, float m, Entries &e) {
+    float ref = -INFINITY, w0 = 0.f, wa = 0.f, wx = 0.f, wl = 0.f;
+    for (int first = 0;;) {
+      float top = fmaxf(fmaxf(e.a[0], e.a[1]), fmaxf(e.a[2], e.a[3]));
+      top = fmaxf(wave_max(top), ref);
+      if (ref > -INFINITY) {
+        const float f = expf(ref - top);
+        wa = (wa + (ref - top) * w0) * f;
+        w0 *= f, wx *= f, wl *= f;
+      }
+      ref = top;
 #pragma unroll
-  for (int i = 0; i < SLOTS; ++i)
-    if (a[i] != -INFINITY) {
-      const float p = expf(a[i] - norm);
-      if (p != 0.f) {
-        mass += p;
-        ent += p * (a[i] - norm);
-        if (local[i]) {
-          mine += p;
-          dot += p * ((x[i] - m) * t.inv_tau);
+      for (int i = 0; i < Entries::U; ++i)
+        if (e.a[i] != -INFINITY) {
+          const float y = e.a[i] - ref, w = expf(y);
+          if (w != 0.f) {
+            w0 += w;
+            wa += w * y;
+            if (e.local >> i & 1) {
+              wl += w;
+              wx += w * ((e.x[i] - m) * t.inv_tau);
+            }
+          }
         }
-      }
+      first += Entries::U * 64;
+      if (first >= t.k) break;
+      e.load(t, row, r, first);
     }
-  mass = block_sum<BT>(mass, red);
-  mine = block_sum<BT>(mine, red);
-  dot = block_sum<BT>(dot, red);
-  ent = block_sum<BT>(ent, red);
-  if (threadIdx.x == 0) {
-    float loss = 0.f, pred = 0.f;
-    if (mass != 0.f && t.alpha > 0.f) loss = t.alpha * t.tau * t.tau * (ent - dot + mass * logf(s));
-    if (t.target) {
-      const int64_t c = t.column(t.target[r]);
-      if (c >= 0) pred = to_f(row[c]) - m;
-      loss += (1.f - t.alpha) * (logf(s1) - pred);
-    }
-    float *o = stats + r;
-    o[LOSS * pitch] = loss;
-    o[ROW_MAX * pitch] = m;
-    o[SUM_TAU * pitch] = s;
-    o[SUM_ONE * pitch] = s1;
-    o[NORM * pitch] = norm;
-    o[MASS * pitch] = mass;
-    o[DOT * pitch] = dot;
-    o[MASS_LOCAL * pitch] = mine;
-    o[ENTROPY * pitch] = ent;
-    o[PREDICTED * pitch] = pred;
+    w0 = wave_sum(w0), wa = wave_sum(wa), wx = wave_sum(wx), wl = wave_sum(wl);
+    norm = mass = dot = mine = ent = 0.f;
+    if (w0 == 0.f) return;                           // no entries
+    norm = t.lse ? t.lse[r] : ref + logf(w0);
+    const float scale = t.lse ? expf(ref - norm) : 1.f / w0;
+    mass = t.lse ? w0 * scale : 1.f;
+    dot = wx * scale;
+    mine = t.lse || wl != w0 ? wl * scale : 1.f;
+    ent = wa * scale + (ref - norm) * mass;
   }
+};
+
+__device__ __forceinline__ void write_stats(const Teacher &t, float *stats, int64_t pitch, float m, float s, float s1, const Sums &e,
+                                            float pred) {
+  float loss = 0.f;
+  if (e.mass != 0.f && t.alpha > 0.f) loss = t.alpha * t.tau * t.tau * (e.ent - e.dot + e.mass * logf(s));
+  if (t.target) loss += (1.f - t.alpha) * (logf(s1) - pred);
+  stats[LOSS * pitch] = loss;
+  stats[ROW_MAX * pitch] = m;
+  stats[SUM_TAU * pitch] = s;
+  stats[SUM_ONE * pitch] = s1;
+  stats[NORM * pitch] = e.norm;
+  stats[MASS * pitch] = e.mass;
+  stats[DOT * pitch] = e.dot;
+  stats[MASS_LOCAL * pitch] = e.mine;
+  stats[ENTROPY * pitch] = e.ent;
+  stats[PREDICTED * pitch] = pred;
 }
 
-// One workgroup a row, or a segment of one (partial sums in `parts`: [rows][segments][3]).
-template <typename T, bool TWO>
+// What a row's segments leave for the join: three floats each, and the first one's sums over the entries (dot and the target's
+// logit against the first segment's maximum).
+enum { PART_SUMS = 6 };
+
+// One workgroup a row, or a segment of one.
+template <typename T, Hard H, bool NT>
 __global__ void __launch_bounds__(BT)
-distill_fwd_kernel(const T *__restrict__ logits, int64_t ld, int64_t segment, Teacher t, float *__restrict__ stats, int64_t pitch,
-                   float *__restrict__ parts) {
-  __shared__ float red[4];
-  const int64_t r = blockIdx.x;
+distill_fwd_kernel(const T *__restrict__ logits, int64_t ld, int64_t segment, int segments, Teacher t, float *__restrict__ stats,
+                   int64_t pitch, float *__restrict__ parts) {
+  __shared__ float red[BT / 64][3];
+  const int64_t r = blockIdx.x / (unsigned)segments;
+  const int y = blockIdx.x % (unsigned)segments, w = threadIdx.x >> 6;
   const T *row = logits + r * ld;
   const float k = t.inv_tau * LOG2E;
-  const int64_t from = (int64_t)blockIdx.y * segment, to = from + segment < t.cols ? from + segment : t.cols;
-  Running<TWO> run;
-  scan_row<TWO>(row, from, to, k, run);
-  const float m = block_max(run.m, red);
-  run.align(m, k);
-  const float s = block_sum<BT>(run.s, red), s1 = TWO ? block_sum<BT>(run.s1, red) : s;
+  const int64_t from = (int64_t)y * segment, to = from + segment < t.cols ? from + segment : t.cols;
+  Entries e;
+  float xt = 0.f;
+  bool has_target = false;
+  if (y == 0 && w == 0) {
+    e.load(t, row, r, 0);
+    if (t.target) {
+      const int64_t c = t.column(t.target[r]);
+      has_target = c >= 0;
+      if (has_target) xt = to_f(row[c]);
+    }
+  }
+  Running<H> run;
+  scan_row<NT>(row, from, to, k, run);
+  float m = wave_max(run.top);
+  if (m > -INFINITY) run.move(m, k);
+  float s = wave_sum(run.s), s1 = H != SAME ? wave_sum(run.s1) : s;
+  if ((threadIdx.x & 63) == 0) {
+    red[w][0] = m;
+    red[w][1] = s;
+    red[w][2] = s1;
+  }
+  __syncthreads();
+  if (w != 0) return;
+  m = fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0]));
+  s = s1 = 0.f;
+#pragma unroll
+  for (int i = 0; i < BT / 64; ++i) {
+    const float d = red[i][0] - m;
+    if (d > -INFINITY || red[i][1] != 0.f) s += red[i][1] * exp2_fast(d * k);      // (a wavefront of -inf only adds nothing)
+    if (H != SAME && (d > -INFINITY || red[i][2] != 0.f)) s1 += red[i][2] * exp2_fast(d * LOG2E);
+  }
+  if (H == SAME) s1 = s;
+  float *o = parts ? parts + (r * segments + y) * 3 : nullptr;
+  if (parts && threadIdx.x == 0) {
+    o[0] = m;
+    o[1] = s;
+    o[2] = s1;
+  }
+  if (y != 0) return;
+  Sums sums;
+  sums.run(t, row, r, m, e);
+  const float pred = has_target ? xt - m : 0.f;
+  if (threadIdx.x != 0) return;
   if (parts) {
-    if (threadIdx.x == 0) {
-      float *o = parts + (r * gridDim.y + blockIdx.y) * 3;
-      o[0] = m;
-      o[1] = s;
-      o[2] = s1;
-    }
-    return;
+    o = parts + gridDim.x * 3 + r * PART_SUMS;
+    o[0] = sums.norm;
+    o[1] = sums.mass;
+    o[2] = sums.dot;
+    o[3] = sums.mine;
+    o[4] = sums.ent;
+    o[5] = has_target ? xt : -INFINITY;
+  } else {
+    write_stats(t, stats + r, pitch, m, s, s1, sums, pred);
   }
-  finish_row(t, row, r, m, s, s1, stats, pitch, red);
 }
 
-// The segments of a row, joined, and the row's statistics.
-template <typename T>
-__global__ void __launch_bounds__(BT)
-distill_join_kernel(const T *__restrict__ logits, int64_t ld, int segments, Teacher t, float *__restrict__ stats, int64_t pitch,
-                    const float *__restrict__ parts) {
-  __shared__ float red[4];
+// The segments of a row, joined by one wavefront.
+__global__ void __launch_bounds__(64)
+distill_join_kernel(int segments, Teacher t, float *__restrict__ stats, int64_t pitch, const float *__restrict__ parts) {
   const int64_t r = blockIdx.x;
-  const float k = t.inv_tau * LOG2E, *p = parts + r * segments * 3;
-  Running<true> run;
-  for (int i = threadIdx.x; i < segments; i += BT) {
-    const float m = p[3 * i], to = fmaxf(m, run.m);
-    float s = p[3 * i + 1], s1 = p[3 * i + 2];
-    if (m > -INFINITY) {
-      s *= exp2_fast((m - to) * k);
-      s1 *= exp2_fast((m - to) * LOG2E);
+  const float k = t.inv_tau * LOG2E, *p = parts + r * segments * 3, *e = parts + (int64_t)gridDim.x * segments * 3 + r * PART_SUMS;
+  float top = -INFINITY;
+  for (int i = threadIdx.x; i < segments; i += 64) top = fmaxf(top, p[3 * i]);
+  const float m = wave_max(top);
+  float s = 0.f, s1 = 0.f;
+  for (int i = threadIdx.x; i < segments; i += 64) {
+    const float d = p[3 * i] - m;
+    if (d > -INFINITY || p[3 * i + 1] != 0.f) {
+      s += p[3 * i + 1] * exp2_fast(d * k);
+      s1 += p[3 * i + 2] * exp2_fast(d * LOG2E);
     }
-    run.align(to, k);
-    run.m = to;
-    run.s += s;
-    run.s1 += s1;
   }
-  const float m = block_max(run.m, red);
-  run.align(m, k);
-  const float s = block_sum<BT>(run.s, red), s1 = block_sum<BT>(run.s1, red);
-  finish_row(t, logits + r * ld, r, m, s, s1, stats, pitch, red);
+  s = wave_sum(s), s1 = wave_sum(s1);
+  if (threadIdx.x != 0) return;
+  Sums sums;
+  sums.norm = e[0], sums.mass = e[1], sums.mine = e[3], sums.ent = e[4];
+  sums.dot = sums.mine != 0.f ? e[2] + sums.mine * ((p[0] - m) * t.inv_tau) : 0.f;
+  write_stats(t, stats + r, pitch, m, s, s1, sums, t.target && t.column(t.target[r]) >= 0 ? e[5] - m : 0.f);
 }
 
-// One workgroup a segment of a row.  grad may be the logits (each element is read, then written, by the same thread; the listed
-// ones are read before any store of the row).
-template <typename T, bool TWO>
+// One workgroup a segment of a row.  Its wavefronts look up the listed columns that lie in the segment, 64 each, then all stream the
+// segment, and behind its stores the listed columns are corrected.  grad may be the logits: the listed ones are read before any store.
+// A segment is short, four vectors a thread, so that the workgroups of a moment read and write neighbouring memory, at the price of looking
+// at a row's list once a segment.  4096 x 128256 in bf16, 129 columns a row, us by KB a segment: 8 473, 12 395, 16 361 (5.8 TB/s, what a
+// copy reaches), 24 391, 32 404, 64 420, 256 447; 4096 x 16032: 8 56, 16 48, 32 49.
+constexpr int64_t BWD_BYTES = 16384;
+template <typename T, Hard H, bool NT>
 __global__ void __launch_bounds__(BT)
-distill_bwd_kernel(const T *logits, int64_t ld, int64_t segment, Teacher t, const float *__restrict__ stats, int64_t pitch,
-                   const float *__restrict__ dout, T *grad, int64_t ld_grad) {
-  constexpr int N = Vec<T>::N, U = 4, HOLD = SLOTS + 1;      // + 1: the target
-  __shared__ int32_t cols_of[MAX_K + 4];                     // columns of the segment, -1 elsewhere
-  __shared__ float weight[MAX_K + 4];
-  const int64_t r = blockIdx.x;
+distill_bwd_kernel(const T *logits, int64_t ld, int64_t segment, int segments, Teacher t, const float *__restrict__ stats,
+                   int64_t pitch, const float *__restrict__ dout, T *grad, int64_t ld_grad) {
+  constexpr int N = Vec<T>::N, U = 4;                        // vectors in flight
+  __shared__ __align__(16) int32_t cols_of[MAX_K + 4];       // columns in the segment, -1 elsewhere
+  __shared__ __align__(16) float weight[MAX_K + 4];          // what is taken off them
+  const int64_t r = blockIdx.x / (unsigned)segments;
   const int tid = threadIdx.x;
-  const int64_t from = (int64_t)blockIdx.y * segment, to = from + segment < t.cols ? from + segment : t.cols;
+  const int64_t from = (int64_t)(blockIdx.x % (unsigned)segments) * segment, to = from + segment < t.cols ? from + segment : t.cols;
   const T *row = logits + r * ld + from;
   T *out = grad + r * ld_grad + from;
   const float *st = stats + r;
   const float m = st[ROW_MAX * pitch], mass = st[MASS * pitch], norm = st[NORM * pitch], d = dout[r];
   const float k = t.inv_tau * LOG2E;
   const float scale = mass != 0.f ? t.alpha * t.tau * d : 0.f;
-  const float ks = scale != 0.f ? scale * mass / st[SUM_TAU * pitch] : 0.f;
   const float hard = t.target ? (1.f - t.alpha) * d : 0.f;
-  const float k1 = hard != 0.f ? hard / st[SUM_ONE * pitch] : 0.f;
-  const int64_t len = to - from, nvec = len / N;
+  const int len = (int)(to - from), nvec = len / N;
   if (d == 0.f || (scale == 0.f && hard == 0.f)) {           // a row that is left out: zeros, whatever it holds
     Vec<T> zero;
 #pragma unroll
     for (int e = 0; e < N; ++e) zero.v[e] = from_f<T>(0.f);
-    for (int64_t v = tid; v < nvec; v += BT) store16(out + v * N, zero);
-    for (int64_t c = nvec * N + tid; c < len; c += BT) out[c] = from_f<T>(0.f);
+    for (int v = tid; v < nvec; v += BT) store16<NT>(out + (int64_t)v * N, zero);
+    for (int c = nvec * N + tid; c < len; c += BT) out[c] = from_f<T>(0.f);
     return;
   }
+  const float ks = scale != 0.f ? scale * mass / st[SUM_TAU * pitch] : 0.f;
+  const float k1 = hard != 0.f ? hard / st[SUM_ONE * pitch] : 0.f;
   auto value = [&](float x) {
-    if (TWO) return fmaf(exp2_fast((x - m) * k), ks, exp2_fast((x - m) * LOG2E) * k1);
-    return exp2_fast((x - m) * k) * (ks + k1);
+    const float e = exp2_fast((x - m) * k);
+    if (H == SAME) return e * (ks + k1);
+    return fmaf(e, ks, exp_one<H>(e, x - m) * k1);
   };
-  // the entries that lie in this segment: weight and value without them, from the logits before they are overwritten
-  const int entries = t.k + (t.target ? 1 : 0);
-  float base[HOLD];
+  const int entries = t.k + (t.target ? 1 : 0);              // the target behind the teacher's
+  constexpr int SLOTS = MAX_K / BT + 1;
+  float base[SLOTS];                                         // of the thread's entries: the value without what is taken off
 #pragma unroll
-  for (int i = 0; i < HOLD; ++i) {
+  for (int i = 0; i < SLOTS; ++i) {
     const int j = i * BT + tid;
     base[i] = 0.f;
-    if (j < entries) {
+    if (i * BT < entries && j < ((entries + 3) & ~3)) {
       int64_t c = -1;
-      float w = 0.f;
-      if (j == t.k) {
-        c = t.column(t.target[r]);
-        w = hard;
-      } else {
+      float w = hard;
+      if (j < t.k) {
         const int64_t id = t.id(r, j);
-        if (t.there(id)) {
-          c = t.column(id);
-          const float a = t.logit(r, j);
-          w = a != -INFINITY ? scale * expf(a - norm) : 0.f;
-        }
+        const float a = t.logit(r, j);
+        if (t.there(id)) c = id - t.vocab_start - from;
+        w = a != -INFINITY ? scale * expf(a - norm) : 0.f;
+      } else if (j < entries) {
+        c = t.target[r] - t.vocab_start - from;
       }
-      if (c < from || c >= to) c = -1;
-      else base[i] = value(to_f(row[c - from]));
-      cols_of[j] = c < 0 ? -1 : (int32_t)(c - from);
+      if (c < 0 || c >= len) c = -1;
+      else base[i] = value(to_f(row[c]));
+      cols_of[j] = (int32_t)c;
       weight[j] = w;
     }
   }
-  if (tid < 4 && entries + tid < MAX_K + 4) cols_of[entries + tid] = -1;
-  __syncthreads();
-  int64_t v = tid;
-  auto emit = [&](int64_t at, const Vec<T> &x) {
-    Vec<T> o;
-#pragma unroll
-    for (int e = 0; e < N; ++e) o.v[e] = from_f<T>(value(to_f(x.v[e])));
-    store16(out + at * N, o);
-  };
-  for (; v + (U - 1) * BT < nvec; v += U * BT) {
+  if (logits == grad) __syncthreads();
+  for (int v = tid; v < nvec; v += U * BT) {
     Vec<T> x[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) x[u] = load16(row + (v + u * BT) * N);
+    for (int u = 0; u < U; ++u)
+      if (v + u * BT < nvec) x[u] = load16<false>(row + (int64_t)(v + u * BT) * N);
 #pragma unroll
-    for (int u = 0; u < U; ++u) emit(v + u * BT, x[u]);
+    for (int u = 0; u < U; ++u)
+      if (v + u * BT < nvec) {
+        Vec<T> o;
+#pragma unroll
+        for (int e = 0; e < N; ++e) o.v[e] = from_f<T>(value(to_f(x[u].v[e])));
+        store16<NT>(out + (int64_t)(v + u * BT) * N, o);
+      }
   }
-  for (; v < nvec; v += BT) emit(v, load16(row + v * N));
-  for (int64_t c = nvec * N + tid; c < len; c += BT) out[c] = from_f<T>(value(to_f(row[c])));
-  __syncthreads();                                           // the segment's stores are complete
+  for (int c = nvec * N + tid; c < len; c += BT) out[c] = from_f<T>(value(to_f(row[c])));
+  __syncthreads();                                           // the segment's stores are complete, the lists too
   // the first entry of a column takes off the weights of all that name it, in the list's order
 #pragma unroll
-  for (int i = 0; i < HOLD; ++i) {
+  for (int i = 0; i < SLOTS; ++i) {
+    if (i * BT >= entries) break;
     const int j = i * BT + tid;
     const int c = j < entries ? cols_of[j] : -1;
-    if (c >= 0) {
-      bool first = true;
-      float w = 0.f;
-      for (int o = 0; o < entries; ++o)
-        if (cols_of[o] == c) {
-          first &= o >= j;
-          w += weight[o];
-        }
-      if (first) out[c] = from_f<T>(base[i] - w);
+    if (c < 0) continue;
+    bool first = true;
+    float off = 0.f;
+    for (int o = 0; o < entries; o += 4) {
+      const int4 cc = *reinterpret_cast<const int4 *>(cols_of + o);
+      const float4 ww = *reinterpret_cast<const float4 *>(weight + o);
+      off += cc.x == c ? ww.x : 0.f;
+      off += cc.y == c ? ww.y : 0.f;
+      off += cc.z == c ? ww.z : 0.f;
+      off += cc.w == c ? ww.w : 0.f;
+      first &= !((cc.x == c && o < j) || (cc.y == c && o + 1 < j) || (cc.z == c && o + 2 < j) || (cc.w == c && o + 3 < j));
     }
+    if (first) out[c] = from_f<T>(base[i] - off);
   }
 }
+
+#define DISTILL_KERNEL(name, out)                                                                          \
+  switch (hard_of(temperature, alpha)) {                                                                   \
+    case SAME: out = nt ? name<T, SAME, true> : name<T, SAME, false>; break;                               \
+    case SQUARE: out = nt ? name<T, SQUARE, true> : name<T, SQUARE, false>; break;                         \
+    case FOURTH: out = nt ? name<T, FOURTH, true> : name<T, FOURTH, false>; break;                         \
+    default: out = nt ? name<T, OWN, true> : name<T, OWN, false>;                                          \
+  }
 
 // Segments of a row: one where the rows alone fill the chip; then pieces of at least 4096 columns until they do.
 int64_t segments_of(int64_t rows, int64_t cols, int64_t least, int64_t want) {
   int64_t n = cdiv(want, rows);
   const int64_t most = cdiv(cols, least);
   if (n > most) n = most;
-  return n < 1 ? 1 : n > 65535 ? 65535 : n;
+  return n < 1 ? 1 : n;
 }
-int64_t fwd_segments(int64_t rows, int64_t cols) { return rows >= 1024 ? 1 : segments_of(rows, cols, 4096, 2048); }
-// a segment's length, whole 16-byte pieces of any type
-int64_t segment_of(int64_t cols, int64_t segments) { return cdiv(cdiv(cols, segments), 8) * 8; }
+// a segment's length, whole cache lines of any type (4096 x 128256 backward, when it was 398 us: -10)
+int64_t segment_of(int64_t cols, int64_t segments) { return cdiv(cdiv(cols, segments), 64) * 64; }
+int64_t fwd_segment(int64_t rows, int64_t cols) { return segment_of(cols, rows >= 1024 ? 1 : segments_of(rows, cols, 4096, 2048)); }
 
 }  // namespace
 }  // namespace dh
@@ -390,8 +470,8 @@ static int distill_check(const void *logits, int64_t ld, const void *ids, int id
 
 extern "C" size_t dh_distill_workspace_bytes(int64_t rows, int64_t cols) {
   if (rows <= 0 || cols <= 0) return 0;
-  const int64_t n = fwd_segments(rows, cols);
-  return n > 1 ? (size_t)(rows * n * 3 * (int64_t)sizeof(float)) : 0;
+  const int64_t n = cdiv(cols, fwd_segment(rows, cols));
+  return n > 1 ? (size_t)(rows * (n * 3 + PART_SUMS) * (int64_t)sizeof(float)) : 0;
 }
 
 extern "C" int dh_distill_fwd(const void *logits, int64_t ld, const void *ids, int id_bytes, const void *teacher, int teacher_dtype,
@@ -406,18 +486,19 @@ extern "C" int dh_distill_fwd(const void *logits, int64_t ld, const void *ids, i
   DH_CHECK(need == 0 || (workspace && workspace_bytes >= need), "workspace of %zu bytes, %zu are needed", workspace_bytes, need);
   const Teacher t{ids, teacher, teacher_lse, alpha < 1.f ? target : nullptr, vocab_start, vocab_total, cols, k, id_bytes == 8,
                   teacher_dtype, 1.f / temperature, temperature, alpha};
-  const int64_t segment = segment_of(cols, fwd_segments(rows, cols)), n = cdiv(cols, segment);
-  const bool two = alpha < 1.f && temperature != 1.f;
+  const int64_t segment = fwd_segment(rows, cols), n = cdiv(cols, segment);
   float *parts = need ? (float *)workspace : nullptr;
   const hipStream_t st = (hipStream_t)stream;
   DH_DISPATCH_DTYPE(dtype, {
-    const auto kernel = two ? distill_fwd_kernel<T, true> : distill_fwd_kernel<T, false>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)rows, (unsigned)n), dim3(BT), 0, st, (const T *)logits, ld, segment, t, stats, pitch,
-                       parts);
-    if (parts)
-      hipLaunchKernelGGL((distill_join_kernel<T>), dim3((unsigned)rows), dim3(BT), 0, st, (const T *)logits, ld, (int)n, t, stats,
-                         pitch, (const float *)parts);
+    // rows that do not fit in the last-level cache do not go through it: 4096 x 128256 in bf16 191 -> 165 us; 1000 x 50257 in fp32 with the
+    // hint 34.5 -> 36.8, and the backward then finds nothing of it (97 -> 113 both)
+    const bool nt = stream_hint(rows * cols * (int64_t)sizeof(T));
+    decltype(&distill_fwd_kernel<T, SAME, false>) kernel;
+    DISTILL_KERNEL(distill_fwd_kernel, kernel)
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * n)), dim3(BT), 0, st, (const T *)logits, ld, segment, (int)n, t, stats, pitch, parts);
   });
+  if (parts)
+    hipLaunchKernelGGL(distill_join_kernel, dim3((unsigned)rows), dim3(64), 0, st, (int)n, t, stats, pitch, (const float *)parts);
   DH_LAUNCH_CHECK();
   return DH_OK;
 }
@@ -439,14 +520,16 @@ extern "C" int dh_distill_bwd(const void *logits, int64_t ld, const void *ids, i
   }
   const Teacher t{ids, teacher, nullptr, alpha < 1.f ? target : nullptr, vocab_start, vocab_total, cols, k, id_bytes == 8,
                   teacher_dtype, 1.f / temperature, temperature, alpha};
-  const int64_t want = segments_of(rows, cols, 2048, 2048), whole = cdiv(cols, 16384);
+  const int64_t want = segments_of(rows, cols, 2048, 2048), whole = cdiv(cols * (int64_t)dtype_size(dtype), BWD_BYTES);
   const int64_t segment = segment_of(cols, want > whole ? want : whole), n = cdiv(cols, segment);
-  DH_CHECK(n <= 65535, "too many columns");
-  const bool two = alpha < 1.f && temperature != 1.f;
+  DH_CHECK(rows * n < 1ll << 24, "rows=%lld of cols=%lld: too many for one call", (long long)rows, (long long)cols);
   const hipStream_t st = (hipStream_t)stream;
   DH_DISPATCH_DTYPE(dtype, {
-    const auto kernel = two ? distill_bwd_kernel<T, true> : distill_bwd_kernel<T, false>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)rows, (unsigned)n), dim3(BT), 0, st, (const T *)logits, ld, segment, t, stats, pitch, dout,
+    // the same for the gradient's stores, reads and writes together: 1000 x 50257 in fp32 76 -> 62 us; at 4096 x 16032 in bf16 they fit
+    const bool nt = stream_hint(2 * rows * cols * (int64_t)sizeof(T));
+    decltype(&distill_bwd_kernel<T, SAME, false>) kernel;
+    DISTILL_KERNEL(distill_bwd_kernel, kernel)
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * n)), dim3(BT), 0, st, (const T *)logits, ld, segment, (int)n, t, stats, pitch, dout,
                        (T *)grad, ld_grad);
   });
   DH_LAUNCH_CHECK();

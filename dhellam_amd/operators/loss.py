@@ -93,25 +93,29 @@ def distill_fwd(inputs, temperature=1.0, alpha=1.0):
 
         loss = alpha temperature^2 sum_k p_k (log p_k - log q_k) + (1 - alpha) cross entropy(x, target)
 
-    A row without entries has no first term.  With a tensor-parallel world above one the outputs are this rank's share: with
-    M = max_r row_max_r, ``sum_exp_t`` (at the temperature) and ``sum_exp`` joined as the cross entropy's sums are, each at its temperature, and
-
-        D = sum_r dot_r + mass_local_r (row_max_r - M) / temperature,   P as the cross entropy's
-
-    the loss is alpha temperature^2 (entropy - D + mass log sum_exp_t) + (1 - alpha) (log sum_exp - P), and ``distill_bwd`` gives a rank's
-    share of the gradient from a context whose ``stats`` rows 1, 2 and 3 hold M and the joined sums."""
+    A row without entries has no first term.  Returns {"loss" [...], "stats" (what the backward needs and ``distill_statistics`` names),
+    "temperature", "alpha", "vocab_size"}."""
     logits, target = inputs["vocab_parallel_logits"], inputs.get("target")
     start, total = _vocabulary(logits.shape[-1])
     stats = _host.distill_fwd(logits, inputs["teacher_ids"], inputs["teacher_logits"], inputs.get("teacher_lse"), target, start, total,
                               temperature, alpha)
-    loss, row_max, sum_exp_t, sum_exp, _, mass, dot, mass_local, entropy, predicted = stats.unbind(0)
-    hard = alpha < 1.0
-    return {
-        "loss": loss.view(logits.shape[:-1]),
-        "temperature": temperature, "alpha": alpha, "vocab_size": logits.shape[-1], "stats": stats,
-        "row_max": row_max, "sum_exp_t": sum_exp_t, "sum_exp": sum_exp if hard else None, "mass": mass, "dot": dot,
-        "mass_local": mass_local, "entropy": entropy, "predicted": predicted.view(logits.shape[:-1]) if hard else None,
-    }
+    return {"loss": stats[0].view(logits.shape[:-1]), "stats": stats, "temperature": temperature, "alpha": alpha,
+            "vocab_size": logits.shape[-1]}
+
+
+def distill_statistics(out):
+    """The rows of ``out["stats"]`` by name, views of [rows].  With a tensor-parallel world above one the outputs of ``distill_fwd`` are
+    this rank's share and the caller joins them: with M = max_r row_max_r,
+
+        S  = sum_r sum_exp_t_r exp((row_max_r - M) / temperature),   S1 = sum_r sum_exp_r exp(row_max_r - M)      (alpha < 1)
+        D  = sum_r dot_r + mass_local_r (row_max_r - M) / temperature
+        P  = sum over the rank that holds the target of (predicted_r + row_max_r - M)
+        loss = alpha temperature^2 (entropy - D + mass log S) + (1 - alpha) (log S1 - P)
+
+    and each rank's share of the gradient comes from ``distill_bwd`` after M, S and S1 are written over ``row_max``, ``sum_exp_t`` and
+    ``sum_exp``."""
+    names = ("loss", "row_max", "sum_exp_t", "sum_exp", "teacher_norm", "mass", "dot", "mass_local", "entropy", "predicted")
+    return dict(zip(names, out["stats"].unbind(0)))
 
 
 def distill_bwd(context, dout, grad_out=None):

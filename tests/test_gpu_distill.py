@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from dhellam_amd.common import parallel_state
-from dhellam_amd.operators.loss import cross_entropy_bwd, cross_entropy_fwd, distill_bwd, distill_fwd
+from dhellam_amd.operators.loss import cross_entropy_bwd, cross_entropy_fwd, distill_bwd, distill_fwd, distill_statistics
 
 pytestmark = pytest.mark.gpu
 
@@ -67,13 +67,6 @@ def plain(inputs, tau, alpha):
 def tolerance(cols, tau):
     """Sums of cols / 256 terms one behind the other and 20 joins, an exponential of an argument of up to 40 / tau: half steps of 2^-23."""
     return (cols / 256 + 20 + 2 * 40 / min(tau, 1.0) + 10) * 2.0 ** -24
-
-
-def check(inputs, dout, tau, alpha, **kw):
-    out = distill_fwd(inputs, tau, alpha)
-    d = distill_bwd([inputs, out], dout, **kw)
-    x = inputs["vocab_parallel_logits"] if not kw else None
-    return out, d
 
 
 def compare(out, d, want, dout, dtype, cols, tau):
@@ -204,7 +197,7 @@ def test_slices_of_the_vocabulary_join(rows, tau, alpha):
             parallel_state.set_tensor_model_parallel(rank, 2)
             part = dict(inputs, vocab_parallel_logits=inputs["vocab_parallel_logits"][:, rank * cols:(rank + 1) * cols])
             parts.append(part)
-            outs.append(distill_fwd(part, tau, alpha))
+            outs.append(distill_statistics(distill_fwd(part, tau, alpha)))
         m = torch.maximum(outs[0]["row_max"], outs[1]["row_max"])
         s = sum(o["sum_exp_t"] * torch.exp((o["row_max"] - m) / tau) for o in outs)
         dot = sum(o["dot"] + o["mass_local"] * (o["row_max"] - m) / tau for o in outs)
@@ -219,8 +212,9 @@ def test_slices_of_the_vocabulary_join(rows, tau, alpha):
         torch.testing.assert_close(loss, whole["loss"], rtol=2e-5, atol=2e-5)
         for rank in range(2):
             parallel_state.set_tensor_model_parallel(rank, 2)
-            o = dict(outs[rank], stats=outs[rank]["stats"].clone())
-            o["stats"][1], o["stats"][2], o["stats"][3] = m, s, s1
+            o = distill_fwd(parts[rank], tau, alpha)
+            for name, joined in (("row_max", m), ("sum_exp_t", s), ("sum_exp", s1)):
+                distill_statistics(o)[name].copy_(joined)
             got = distill_bwd([parts[rank], o], dout)
             torch.testing.assert_close(got, want[:, rank * cols:(rank + 1) * cols], rtol=1e-4, atol=1e-7)
     finally:
