@@ -525,8 +525,10 @@ extern "C" int dh_distill_bwd(const void *logits, int64_t ld, const void *ids, i
   DH_CHECK(rows * n < 1ll << 24, "rows=%lld of cols=%lld: too many for one call", (long long)rows, (long long)cols);
   const hipStream_t st = (hipStream_t)stream;
   DH_DISPATCH_DTYPE(dtype, {
-    // the same for the gradient's stores, reads and writes together: 1000 x 50257 in fp32 76 -> 62 us; at 4096 x 16032 in bf16 they fit
-    const bool nt = stream_hint(2 * rows * cols * (int64_t)sizeof(T));
+    // the gradient's stores go past the caches where that and the logits are more than a part of the last one.  us, forward, backward and a
+    // reader of the gradient behind them, in the caches / past them, 16032 columns in bf16: 1024 rows 36.4 / 38.7, 2048 64.0 / 63.2, 4096
+    // 110.9 / 108.8 (92.2 / 88.3 without the reader), 8192 220 / 208; 1000 x 50257 in fp32 160 / 148
+    const bool nt = 2 * rows * cols * (int64_t)sizeof(T) > 96ll << 20;
     decltype(&distill_bwd_kernel<T, SAME, false>) kernel;
     DISTILL_KERNEL(distill_bwd_kernel, kernel)
     hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * n)), dim3(BT), 0, st, (const T *)logits, ld, segment, (int)n, t, stats, pitch, dout,

@@ -42,7 +42,8 @@ def rand(*shape, dtype, seed=0):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("tokens,hq,hk,d,rot", [
     (1, 1, 1, 2, 2), (1, 32, 8, 128, 128), (7, 8, 1, 128, 64), (33, 3, 2, 80, 20), (5, 4, 4, 100, 50), (3, 2, 1, 13, 6), (64, 12, 4, 96, 96),
-    (300, 5, 5, 72, 18), (1000, 8, 1, 256, 256), (2, 130, 3, 64, 32), (9, 0, 2, 64, 64), (17, 1, 0, 65, 64)])
+    (300, 5, 5, 72, 18), (1000, 8, 1, 256, 256), (2, 130, 3, 64, 32), (9, 0, 2, 64, 64), (17, 1, 0, 65, 64),
+    (130, 3, 2, 128, 64), (64, 5, 1, 192, 128), (201, 7, 3, 64, 32), (4100, 9, 0, 64, 64), (63, 1, 1, 40, 6)])
 @pytest.mark.parametrize("interleaved", [False, True])
 def test_forward_and_backward(tokens, hq, hk, d, rot, interleaved, dtype):
     q, k = rand(tokens, hq, d, dtype=dtype), rand(tokens, hk, d, dtype=dtype, seed=1)
@@ -166,6 +167,33 @@ def test_another_stream_and_replays_of_a_graph():
         torch.cuda.synchronize()
         want = rotary_fwd(q, k, t)[:2]
         assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+def test_more_lanes_than_one_launch():
+    """2^30 + 70 tokens of two heads of two elements: two launches, positions past 2^30, addresses past 2^32."""
+    n = (1 << 30) + 70
+    t = rotary_table(10000.0, 2, "cuda")
+    q = torch.empty(n, 2, 2, dtype=torch.bfloat16, device="cuda")
+    q.view(-1).view(torch.int64).fill_(0x3F8040003F804040)                # four ordinary values
+    ends = [slice(0, 100), slice((1 << 30) - 30, (1 << 30) + 70)]
+    rows = [q[s].clone() for s in ends]
+    rotary_fwd(q, None, t, inplace=True)
+    for s, x in zip(ends, rows):
+        check(q[s], x, 10000.0, 2, False, None, torch.arange(s.start, s.stop, device="cuda"))
+
+
+def test_one_of_the_two_in_place():
+    """The C entry takes q in place and k not: every element of both is turned once, also where a part is no whole number of pieces."""
+    from dhellam_amd import _lib
+    t, at = rotary_table(10000.0, 20, "cuda"), torch.arange(70, device="cuda", dtype=torch.int32)
+    q, k = rand(70, 3, 41, dtype=torch.float16), rand(70, 2, 41, dtype=torch.float16, seed=1)
+    want = rotary_fwd(q, k, t, at)[:2]
+    a, b = q.clone(), torch.full_like(k, 7.0)
+    call = lambda head: _lib.load().dh_rotary(a.data_ptr(), k.data_ptr(), a.data_ptr(), b.data_ptr(), t.steps.data_ptr(), at.data_ptr(), 4, 70, 3, 2, 41, 20,
+                                              123, 41, 82, 41, 123, head, 82, 41, 0, 0, 0, 1.0, 2, torch.cuda.current_stream().cuda_stream)
+    _lib.check(call(41))
+    assert torch.equal(a, want[0]) and torch.equal(b, want[1])
+    assert call(42) == -1 and "strides" in _lib.load().dh_last_error().decode()
 
 
 def test_refusals():
