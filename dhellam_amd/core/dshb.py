@@ -27,7 +27,8 @@ from .._Clib import keep_transposed
 from ..operators.embedding import word_embedding_bwd, word_embedding_fwd
 from ..operators.layernorm import pylayernorm_bwd, pylayernorm_fwd
 from ..operators.layernorm_column import dgrad_bwd, gemm_fwd, wgrad_bwd
-from ..operators.loss import cross_entropy_bwd, cross_entropy_fwd, mask_scale_loss_bwd, mask_scale_loss_fwd
+from ..operators.loss import (cross_entropy_bwd, cross_entropy_fwd, distill_bwd, distill_fwd, mask_scale_loss_bwd,
+                              mask_scale_loss_fwd)
 
 
 def pre_process(token_ids: torch.Tensor, word_embedding_weight: torch.Tensor, batch_first: bool = False):
@@ -46,17 +47,27 @@ def pre_process_bwd(context, d_hidden: torch.Tensor, batch_first: bool = False) 
 
 def post_process(hidden_states: torch.Tensor, ln_weight: torch.Tensor, ln_bias: Optional[torch.Tensor],
                  labels: torch.Tensor, loss_mask: torch.Tensor, word_embedding_weight: torch.Tensor, num_mb: int,
-                 loss_scale: float = 1.0, eps: float = 1e-5, label_smoothing: float = 0.0, batch_first: bool = False):
+                 loss_scale: float = 1.0, eps: float = 1e-5, label_smoothing: float = 0.0, batch_first: bool = False,
+                 teacher: Optional[Dict] = None):
     """hidden_states [s, b, h] (or [b, s, h] with ``batch_first``), labels / loss_mask [b, s],
     word_embedding_weight [vocab/tp, h].  Returns (loss, context); loss is a 0-d fp32 tensor
-    (dshb.py:98-112)."""
+    (dshb.py:98-112).  ``teacher``: {"ids", "logits" [b, s, K], "lse" [b, s] (may be absent), "temperature", "alpha" (1 if
+    absent)} for the distillation loss (``operators.loss.distill_fwd``) in the place of the cross entropy; it takes no label smoothing."""
     h = hidden_states.shape[-1]
     ln_out, mu, rsigma, _ = pylayernorm_fwd(hidden_states, ln_weight, ln_bias, eps, 0, False, None)
     logits, _ = gemm_fwd(None, ln_out.view(-1, h), word_embedding_weight, None, "TN", False, 0, True, None)
     # the reference's hidden states are sequence-first and its labels batch-first (dshb.py:105)
     target = labels.contiguous() if batch_first else labels.transpose(0, 1).contiguous()
     ce_in = {"vocab_parallel_logits": logits.view(*hidden_states.shape[:2], -1), "target": target}
-    ce_out = cross_entropy_fwd(ce_in, label_smoothing, keep_softmax=False)
+    if teacher is not None:
+        if label_smoothing != 0.0:
+            raise ValueError("post_process: no label smoothing beside a teacher")
+        for name in ("ids", "logits", "lse"):
+            t = teacher.get(name)
+            ce_in["teacher_" + name] = t if t is None or batch_first else t.transpose(0, 1).contiguous()
+        ce_out = distill_fwd(ce_in, teacher.get("temperature", 1.0), teacher.get("alpha", 1.0))
+    else:
+        ce_out = cross_entropy_fwd(ce_in, label_smoothing, keep_softmax=False)
     token_loss = ce_out["loss"] if batch_first else ce_out["loss"].transpose(0, 1).contiguous()      # [b, s]
     mm_in = {"loss_mask": loss_mask, "output_tensor": token_loss, "num_microbatch": num_mb, "loss_scale": loss_scale}
     mm_out = mask_scale_loss_fwd(mm_in)
@@ -74,7 +85,8 @@ def post_process_bwd(ctx: Dict) -> torch.Tensor:
     ce_in, ce_out = ctx["ce"]
     logits = ce_in["vocab_parallel_logits"]
     d_rows = d_token if ctx["batch_first"] else d_token.transpose(0, 1).contiguous()
-    d_logits = cross_entropy_bwd(ctx["ce"], d_rows, grad_out=logits)
+    loss_bwd = distill_bwd if "teacher_ids" in ce_in else cross_entropy_bwd
+    d_logits = loss_bwd(ctx["ce"], d_rows, grad_out=logits)
     d2 = d_logits.view(-1, d_logits.shape[-1])
     w = ctx["weight"]
     d_ln_out, _ = dgrad_bwd(None, d2, w, None, "NN", False, 0, True, None)

@@ -53,7 +53,7 @@ from ..operators.bda import bda_bwd, bda_fwd
 from ..operators.layernorm import pylayernorm_bwd, pylayernorm_fwd
 from ..operators.layernorm_column import dgrad_bwd, gemm_fwd, wgrad_bwd
 from ..operators.ring_attn import RingGroup, fa_cp_block_bwd, fa_cp_block_fwd
-from ..operators.rope import rope_bwd, rope_fwd, rope_inv_freq
+from ..operators.rope import cached_rotary_table, rope_bwd, rope_fwd, rope_inv_freq, rotary_bwd, rotary_fwd
 from ..operators.swiglu import swiglu, swiglu_back
 
 
@@ -130,6 +130,10 @@ class LayerConfig:
     fuse_adjacent: bool = True        # ops a plan lists next to each other run as one kernel where one exists (bda_attn + ln_mlp)
     gather_in_place: bool = True      # the op in front of a sequence-parallel all-gather writes straight into its rows of the gathered buffer
     resident_weight_transposes: bool = True   # projection weights are kept as W and W^T: the data-gradient GEMMs then run in the forward's layout
+    # rotary positions other than the halves of whole heads by theta^(-2j / d) (``operators.rope.rotary_table``)
+    rotary_dim: Optional[int] = None  # elements at the front of a head that are turned; None: all
+    rotary_interleaved: bool = False  # pairs (2j, 2j + 1)
+    rope_scaling: Optional[dict] = None
 
     @property
     def head_dim(self) -> int:
@@ -162,6 +166,22 @@ class LayerConfig:
     @property
     def softmax_scale(self) -> float:
         return 1.0 / math.sqrt(self.head_dim)
+
+    @property
+    def general_rotary(self) -> bool:
+        """Rotary positions in a form that only the ``rotary_*`` operators have."""
+        return self.rope_theta is not None and (self.rotary_interleaved or self.rope_scaling is not None
+                                                or self.rotary_dim not in (None, self.head_dim))
+
+
+def _turn(config: LayerConfig, q, k, positions, stream, backward=False):
+    """Rotary positions on q and k (backward: on their gradients), in place."""
+    if config.general_rotary:
+        table = cached_rotary_table(config.rope_theta, config.rotary_dim or config.head_dim, q.device, config.rotary_interleaved,
+                                    config.rope_scaling)
+        (rotary_bwd if backward else rotary_fwd)(q, k, table, positions, config.seq_length, stream, False, inplace=True)
+    else:
+        (rope_bwd if backward else rope_fwd)(q, k, positions, config.rope_theta, config.seq_length, stream, False, inplace=True)
 
 
 def _use(t, stream):
@@ -252,14 +272,14 @@ class DCFunc:
         if config.rope_theta is None or config.groups_per_rank != 1:
             return qkv
         q, k, _ = _split_qkv(config, qkv)
-        rope_fwd(q, k, None, config.rope_theta, config.seq_length, stream, False, inplace=True)
+        _turn(config, q, k, None, stream)
         return qkv
 
     @staticmethod
     def attn(config, data, stream, apply_rope=False):
         qkv, cu_seqlens_q, cu_seqlens_kv = data
         s = config.seq_length
-        if _kernel_head_dim(qkv, config.head_dim) == config.head_dim:
+        if _kernel_head_dim(qkv, config.head_dim) == config.head_dim and not (apply_rope and config.general_rotary):
             inv = rope_inv_freq(config.rope_theta, config.head_dim, qkv.device) if apply_rope and config.rope_theta is not None else None
             out, q, k, v, lse = _host.attn_fwd_packed(qkv, cu_seqlens_q, cu_seqlens_kv, config.heads_per_rank,
                                                       config.groups_per_rank, config.head_dim, s, config.softmax_scale, inv,
@@ -268,7 +288,7 @@ class DCFunc:
         with torch.cuda.stream(stream):
             q, k, v = _split_qkv(config, qkv)
             if apply_rope and config.rope_theta is not None:
-                rope_fwd(q, k, None, config.rope_theta, s, stream, False, inplace=True)
+                _turn(config, q, k, None, stream)
             out, q_p, k_p, v_p, out_p, lse, _, rng_state = pymha_varlen_fwd(
                 q, k, v, cu_seqlens_q, cu_seqlens_kv, s, s, 0.0, config.softmax_scale, True, False, 0, False)
             output = out.view(config.tokens, -1)
@@ -289,7 +309,7 @@ class DCFunc:
                     raise RuntimeError(f"ring attention needs the micro-batch's {cp - 1} visiting KV chunks")
                 q, k, v = _split_qkv(config, input)
                 if config.rope_theta is not None:
-                    rope_fwd(q, k, positions, config.rope_theta, s, stream, False, inplace=True)
+                    _turn(config, q, k, positions, stream)
                 own = torch.stack((k.reshape(b, 2, s // 2, hk, d), v.reshape(b, 2, s // 2, hk, d)))
                 input = [q.view(b, 2, s // 2, hq, d), [own, *visiting], None, None, None, None, None, 0]
             i = input[7]
@@ -324,7 +344,7 @@ class DCFunc:
             dq = dq.reshape(T, hq, d)
             dk, dv = dkv[0][0].reshape(T, hk, d), dkv[0][1].reshape(T, hk, d)
             if config.rope_theta is not None:
-                rope_bwd(dq, dk, positions, config.rope_theta, s, stream, False, inplace=True)
+                _turn(config, dq, dk, positions, stream, backward=True)
             dqkv = torch.empty((T, config.qkv_per_rank), dtype=dq.dtype, device=dq.device)
             rr = hq // hk
             torch.cat((dq.view(T, hk, rr * d), dk, dv), dim=2, out=dqkv.view(T, hk, (rr + 2) * d))
@@ -407,7 +427,7 @@ class DCFunc:
         grad_output, q, k, v, out, lse, cu_seqlens_q, cu_seqlens_kv, rng_state = data
         hq, hk, d = config.heads_per_rank, config.groups_per_rank, config.head_dim
         T = grad_output.shape[0]
-        if q.shape[-1] == d:
+        if q.shape[-1] == d and not (apply_rope and config.general_rotary):
             inv = rope_inv_freq(config.rope_theta, d, q.device) if apply_rope and config.rope_theta is not None else None
             return _host.attn_bwd_packed(grad_output, q, k, v, out, lse, cu_seqlens_q, cu_seqlens_kv, config.seq_length,
                                          config.softmax_scale, inv, stream)
@@ -421,7 +441,7 @@ class DCFunc:
             _attn_bwd_raw(dout, q, k, v, out, lse, dq, dk, dv, None, cu_seqlens_q, cu_seqlens_kv, config.seq_length,
                           config.seq_length, config.softmax_scale, True, stream)
             if apply_rope and config.rope_theta is not None:
-                rope_bwd(dq, dk, None, config.rope_theta, config.seq_length, stream, False, inplace=True)
+                _turn(config, dq, dk, None, stream, backward=True)
             if hk != 1:
                 r = hq // hk
                 torch.cat((dq.view(T, hk, r * d), dk, dv), dim=2, out=dqkv.view(T, hk, (r + 2) * d))
@@ -433,7 +453,7 @@ class DCFunc:
         if config.rope_theta is None or config.groups_per_rank != 1:   # several groups: done inside attn_bwd
             return dqkv
         dq, dk, _ = _split_qkv(config, dqkv)
-        rope_bwd(dq, dk, None, config.rope_theta, config.seq_length, stream, False, inplace=True)
+        _turn(config, dq, dk, None, stream, backward=True)
         return dqkv
 
     @staticmethod

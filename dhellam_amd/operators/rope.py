@@ -143,6 +143,18 @@ def rotary_table(theta: float, dim: int, device, interleaved: bool = False, scal
     return RotaryTable(torch.tensor(steps, dtype=torch.int64).to(device), dim, bool(interleaved), factor)
 
 
+_table_cache: dict = {}
+
+
+def cached_rotary_table(theta, dim, device, interleaved=False, scaling=None) -> RotaryTable:
+    """``rotary_table``, made once for equal arguments (what a layer's configuration holds)."""
+    key = (theta, dim, device, interleaved, tuple(sorted(scaling.items())) if scaling is not None else None)
+    t = _table_cache.get(key)
+    if t is None:
+        t = _table_cache[key] = rotary_table(theta, dim, device, interleaved, scaling)
+    return t
+
+
 def _rotary(q, k, table, positions, seq_len, backward, stream, profiling, inplace):
     (qo, ko), ms = issue(_host.rotary, stream, profiling, q, k, table.steps, table.dim, table.interleaved, table.factor, positions,
                          int(seq_len or 0), backward, inplace)
