@@ -20,7 +20,8 @@ __all__ = ["add_tensors", "pygemm", "dense_gemm", "dense_ok", "keep_transposed",
            "pyrmsnorm_fwd", "pyrmsnorm_bwd", "pyrope_fwd", "pyrope_bwd", "pyswiglu_fwd", "pyswiglu_bwd",
            "pymoe_route_topk", "pymoe_sort", "pymoe_permute", "pymoe_unpermute", "pygrouped_gemm_nt",
            "pygrouped_gemm_nn", "pygrouped_gemm_tn", "pycross_entropy_fwd", "pycross_entropy_bwd",
-           "pyembedding_fwd", "pyembedding_bwd"]
+           "pyembedding_fwd", "pyembedding_bwd", "pyrotary_fwd", "pyrotary_bwd", "pymoe_balance_loss", "pymoe_route_bwd",
+           "pydistill_fwd", "pydistill_bwd"]
 
 
 def _timed(profiling: bool, stream, fn):
@@ -556,6 +557,19 @@ def pyrope_bwd(dq, dk, positions, theta, profiling=False):
     return _ret((a, b), ms, profiling)
 
 
+def pyrotary_fwd(q, k, table, positions, profiling=False):
+    """-> [q_rot, k_rot]; table of ``operators.rope.rotary_table``, positions None = 0..T-1"""
+    from .operators.rope import rotary_fwd
+    qr, kr, ms = rotary_fwd(q, k, table, positions, None, None, profiling)
+    return _ret((qr, kr), ms, profiling)
+
+
+def pyrotary_bwd(dq, dk, table, positions, profiling=False):
+    from .operators.rope import rotary_bwd
+    a, b, ms = rotary_bwd(dq, dk, table, positions, None, None, profiling)
+    return _ret((a, b), ms, profiling)
+
+
 def pyswiglu_fwd(y, profiling=False):
     from .operators.swiglu import swiglu
     out, ms = swiglu(y, None, profiling)
@@ -573,6 +587,20 @@ def pymoe_route_topk(logits, k, profiling=False):
     from .operators.moe import route_topk
     idx, gates, ms = route_topk(logits, k, None, profiling)
     return _ret((idx, gates), ms, profiling)
+
+
+def pymoe_balance_loss(logits, topk_idx, mask, balance_coef, z_coef, profiling=False):
+    """-> [losses fp32 [2], ``operators.moe.BalanceLoss``]"""
+    from .operators.moe import balance_loss_fwd
+    losses, balance, ms = balance_loss_fwd(logits, topk_idx, mask, balance_coef, z_coef, None, profiling)
+    return _ret((losses, balance), ms, profiling)
+
+
+def pymoe_route_bwd(logits, topk_idx, gates, dgates, balance, dlosses, profiling=False):
+    """-> [dlogits fp32 [T, E]]"""
+    from .operators.moe import route_bwd
+    d, ms = route_bwd(logits, topk_idx, gates, dgates, balance, dlosses, None, profiling)
+    return _ret((d,), ms, profiling)
 
 
 def pymoe_sort(topk_idx, num_experts, profiling=False):
@@ -620,6 +648,19 @@ def pycross_entropy_bwd(vocab_parallel_logits, target, fwd_out, dout, grad_out=N
     from .operators.loss import cross_entropy_bwd
     return cross_entropy_bwd([{"vocab_parallel_logits": vocab_parallel_logits, "target": target}, fwd_out], dout,
                              grad_out)
+
+
+def pydistill_fwd(vocab_parallel_logits, teacher_ids, teacher_logits, teacher_lse, target, temperature=1.0, alpha=1.0):
+    """-> the output dict of ``operators.loss.distill_fwd``; teacher_lse and target may be None"""
+    from .operators.loss import distill_fwd
+    return distill_fwd({"vocab_parallel_logits": vocab_parallel_logits, "teacher_ids": teacher_ids, "teacher_logits": teacher_logits,
+                        "teacher_lse": teacher_lse, "target": target}, temperature, alpha)
+
+
+def pydistill_bwd(vocab_parallel_logits, teacher_ids, teacher_logits, target, fwd_out, dout, grad_out=None):
+    from .operators.loss import distill_bwd
+    return distill_bwd([{"vocab_parallel_logits": vocab_parallel_logits, "teacher_ids": teacher_ids, "teacher_logits": teacher_logits,
+                         "target": target}, fwd_out], dout, grad_out)
 
 
 def pyembedding_fwd(vocab, token_ids):

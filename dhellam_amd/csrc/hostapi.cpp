@@ -14,6 +14,7 @@
 #include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <c10/util/strides.h>
 #include <torch/csrc/Stream.h>
 
 #include <array>
@@ -1110,8 +1111,8 @@ struct Distill {
   }
 };
 
-// -> statistics [10, rows] (dh_distill_fwd)
-Tensor distill_fwd(const Tensor &logits, const Tensor &ids, const Tensor &teacher, const OptTensor &teacher_lse, const OptTensor &target,
+// -> (loss [...], its row of the statistics [10, rows] of dh_distill_fwd, which come second)
+std::tuple<Tensor, Tensor> distill_fwd(const Tensor &logits, const Tensor &ids, const Tensor &teacher, const OptTensor &teacher_lse, const OptTensor &target,
                    int64_t vocab_start, int64_t vocab_total, double temperature, double alpha) {
   OnGpu on({&logits, &ids, &teacher, opt(teacher_lse), opt(target)}, py::none{});
   const Distill a(logits, ids, teacher, target, alpha);
@@ -1130,7 +1131,8 @@ Tensor distill_fwd(const Tensor &logits, const Tensor &ids, const Tensor &teache
                           (int)a.k, vocab_start, vocab_total, (float)temperature, (float)alpha, a.type, stats.data_ptr<float>(), a.rows,
                           bytes ? ws.data_ptr() : nullptr, (size_t)bytes, on.get());
   });
-  return stats;
+  const auto shape = logits.sizes().slice(0, logits.dim() - 1);
+  return {stats.as_strided(shape, c10::contiguous_strides(shape)), stats};
 }
 
 Tensor distill_bwd(const Tensor &logits, const Tensor &ids, const Tensor &teacher, const OptTensor &target, const Tensor &stats,

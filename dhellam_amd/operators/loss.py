@@ -97,9 +97,9 @@ def distill_fwd(inputs, temperature=1.0, alpha=1.0):
     "temperature", "alpha", "vocab_size"}."""
     logits, target = inputs["vocab_parallel_logits"], inputs.get("target")
     start, total = _vocabulary(logits.shape[-1])
-    stats = _host.distill_fwd(logits, inputs["teacher_ids"], inputs["teacher_logits"], inputs.get("teacher_lse"), target, start, total,
-                              temperature, alpha)
-    return {"loss": stats[0].view(logits.shape[:-1]), "stats": stats, "temperature": temperature, "alpha": alpha,
+    loss, stats = _host.distill_fwd(logits, inputs["teacher_ids"], inputs["teacher_logits"], inputs.get("teacher_lse"), target, start, total,
+                                    temperature, alpha)
+    return {"loss": loss, "stats": stats, "temperature": temperature, "alpha": alpha,
             "vocab_size": logits.shape[-1]}
 
 

@@ -108,6 +108,17 @@ def test_masked_tokens_may_hold_anything(t, e, k):
     assert torch.equal(d, dwant) and (d[~mask] == 0).all()
 
 
+@pytest.mark.parametrize("t", [30, 5000])
+def test_logits_that_do_not_start_a_vector(t):
+    """Contiguous logits four bytes off the 16-byte grid: the same results."""
+    logits, idx, gates, dgates, mask = router(t, 8, 2, masked=True)
+    room = torch.zeros(8 * t + 1, device="cuda")
+    off = room[1:].view(t, 8).copy_(logits)
+    want, got = balance_loss_fwd(logits, idx, mask, A, B), balance_loss_fwd(off, idx, mask, A, B)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1].prob_sum, want[1].prob_sum)
+    assert torch.equal(route_bwd(off, idx, gates, dgates, got[1])[0], route_bwd(logits, idx, gates, dgates, want[1])[0])
+
+
 def test_nothing_counts():
     logits, idx, gates, dgates, _ = router(100, 8, 2)
     off = torch.zeros(100, dtype=torch.bool, device="cuda")

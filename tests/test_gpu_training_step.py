@@ -200,3 +200,25 @@ def test_a_step_of_a_mixture_model():
     got = dict(x=dx, wqkv=wqkv.main_grad, wo=wo.main_grad, wr=dwr, w1=dw1, w2=dw2, table=table.main_grad, ln=ln.main_grad)
     far = {name: rel_err(got[name], leaf[name].grad) for name in got}
     assert max(far.values()) <= 2 * 4 * 2.0 ** -9, far
+
+
+def test_binding_level_names():
+    """They forward to the operators of the same kind."""
+    from dhellam_amd import _Clib as C
+    from dhellam_amd.operators import loss, moe, rope
+    g = torch.Generator(device="cuda").manual_seed(1)
+    rand = lambda *n: torch.randn(*n, generator=g, device="cuda")
+    t, q, k, at = rope.rotary_table(10000.0, 32, "cuda", True), rand(9, 4, 64), rand(9, 1, 64), torch.arange(9, device="cuda")
+    for name, f in (("pyrotary_fwd", rope.rotary_fwd), ("pyrotary_bwd", rope.rotary_bwd)):
+        got = getattr(C, name)(q, k, t, at, True)
+        assert all(torch.equal(a, b) for a, b in zip(got, f(q, k, t, at)[:2])) and got[2] > 0
+    lg = rand(9, 8)
+    idx, gates, _ = moe.route_topk(lg, 2)
+    losses, bal = C.pymoe_balance_loss(lg, idx, None, 0.1, 0.01)
+    assert torch.equal(losses, moe.balance_loss_fwd(lg, idx, None, 0.1, 0.01)[0])
+    assert torch.equal(C.pymoe_route_bwd(lg, idx, gates, gates, bal, None)[0], moe.route_bwd(lg, idx, gates, gates, bal)[0])
+    x, ids, tl, target = rand(9, 50), torch.randint(0, 50, (9, 3), generator=g, device="cuda"), rand(9, 3), torch.arange(9, device="cuda")
+    inputs = {"vocab_parallel_logits": x, "teacher_ids": ids, "teacher_logits": tl, "target": target}
+    out, want = C.pydistill_fwd(x, ids, tl, None, target, 2.0, 0.5), loss.distill_fwd(inputs, 2.0, 0.5)
+    assert torch.equal(out["loss"], want["loss"])
+    assert torch.equal(C.pydistill_bwd(x, ids, tl, target, out, losses.new_ones(9)), loss.distill_bwd([inputs, want], losses.new_ones(9)))
