@@ -839,6 +839,15 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> moe_sort(const Tensor &topk_idx, int 
   return {tpe, offs, order, dest};
 }
 
+// A contiguous tensor of 4-byte elements of `like`'s type in the memory of `all`, from its element `used` on, which moves behind it.
+Tensor part_of(const Tensor &all, int64_t &used, at::IntArrayRef sizes, const Tensor &like) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), like.dtype());
+  t.unsafeGetTensorImpl()->set_storage_offset(used);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+  used += (t.numel() + 3) / 4 * 4;
+  return t;
+}
+
 void check_router(const Tensor &logits, const Tensor &idx, const OptTensor &mask) {
   PY_ASSERT(logits.scalar_type() == at::kFloat && logits.is_contiguous() && logits.dim() == 2,
             "router: logits must be a contiguous fp32 [T, E] GPU tensor");
@@ -854,8 +863,11 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> balance_loss_fwd(const Tensor
   OnGpu on({&logits, &idx, opt(mask)}, stream);
   check_router(logits, idx, mask);
   const int64_t t = logits.size(0), e = logits.size(1);
-  Tensor losses = at::empty({2}, logits.options()), prob = at::empty({e}, logits.options()), lse = at::empty({t}, logits.options());
-  Tensor counts = at::empty({e}, idx.options()), n = at::empty({1}, idx.options());
+  // one allocation for the five results, 16 bytes apart at least
+  Tensor all = at::empty({(t + 3) / 4 * 4 + 2 * ((e + 3) / 4 * 4) + 8}, logits.options());
+  int64_t used = 0;
+  Tensor lse = part_of(all, used, {t}, logits), prob = part_of(all, used, {e}, logits), losses = part_of(all, used, {2}, logits);
+  Tensor counts = part_of(all, used, {e}, idx), n = part_of(all, used, {1}, idx);
   const int64_t bytes = (int64_t)dh_balance_loss_workspace_bytes(t, (int)e);
   // of this call alone: a stream's shared scratch would be that of every graph captured on it
   Tensor ws;
