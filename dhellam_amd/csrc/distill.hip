@@ -11,7 +11,7 @@
 // and writes the gradient.  The K listed columns (and the target's) are corrected behind the row's stores, so nothing
 // per element depends on the column.
 //
-// 4096 x 128256 in bf16, K = 128, alpha 0.5, tau 1: forward 167 us (6.3 TB/s), backward 361 us (5.8 TB/s); a copy on this card 5.9 TB/s.
+// 4096 x 128256 in bf16, K = 128, alpha 0.5, tau 1: forward 167 us (6.3 TB/s), backward 352 us (6.0 TB/s); a copy on this card 5.9 TB/s.
 #include "common.h"
 
 namespace dh {
@@ -325,17 +325,19 @@ distill_join_kernel(int segments, Teacher t, float *__restrict__ stats, int64_t 
 
 // One workgroup a segment of a row.  Its wavefronts look up the listed columns that lie in the segment, 64 each, then all stream the
 // segment, and behind its stores the listed columns are corrected.  grad may be the logits: the listed ones are read before any store.
-// A segment is short, four vectors a thread, so that the workgroups of a moment read and write neighbouring memory, at the price of looking
-// at a row's list once a segment.  4096 x 128256 in bf16, 129 columns a row, us by KB a segment: 8 473, 12 395, 16 361 (5.8 TB/s, what a
-// copy reaches), 24 391, 32 404, 64 420, 256 447; 4096 x 16032: 8 56, 16 48, 32 49.
+// A segment is short, four vectors a thread, so that the workgroups of a moment read and write neighbouring memory, at the price of
+// looking at a row's list once a segment.  4096 x 128256 in bf16, 129 columns a row, us by KB a segment: 8 473, 12 395, 16 361 (5.8 TB/s, what
+// a copy reaches), 24 391, 32 404, 64 420, 256 447; 4096 x 16032: 8 56, 16 48, 32 49.  (All before the bits below, which took 9 off the first.)
 constexpr int64_t BWD_BYTES = 16384;
 template <typename T, Hard H, bool NT>
 __global__ void __launch_bounds__(BT)
 distill_bwd_kernel(const T *logits, int64_t ld, int64_t segment, int segments, Teacher t, const float *__restrict__ stats,
                    int64_t pitch, const float *__restrict__ dout, T *grad, int64_t ld_grad) {
   constexpr int N = Vec<T>::N, U = 4;                        // vectors in flight
-  __shared__ __align__(16) int32_t cols_of[MAX_K + 4];       // columns in the segment, -1 elsewhere
-  __shared__ __align__(16) float weight[MAX_K + 4];          // what is taken off them
+  __shared__ __align__(16) int32_t cols_of[MAX_K];           // columns in the segment, -1 elsewhere
+  __shared__ __align__(16) float weight[MAX_K];              // what is taken off them
+  __shared__ uint32_t named[BWD_BYTES / 2 / 32];             // a bit a column: listed
+  __shared__ int twice;                                      // a column is listed twice
   const int64_t r = blockIdx.x / (unsigned)segments;
   const int tid = threadIdx.x;
   const int64_t from = (int64_t)(blockIdx.x % (unsigned)segments) * segment, to = from + segment < t.cols ? from + segment : t.cols;
@@ -362,28 +364,43 @@ distill_bwd_kernel(const T *logits, int64_t ld, int64_t segment, int segments, T
     if (H == SAME) return e * (ks + k1);
     return fmaf(e, ks, exp_one<H>(e, x - m) * k1);
   };
-  const int entries = t.k + (t.target ? 1 : 0);              // the target behind the teacher's
-  constexpr int SLOTS = MAX_K / BT + 1;
+  static_assert(BWD_BYTES / 2 / 32 == BT, "a word of the bits a thread");
+  named[tid] = 0;
+  if (tid == 0) twice = 0;
+  __syncthreads();
+  constexpr int SLOTS = MAX_K / BT;
   float base[SLOTS];                                         // of the thread's entries: the value without what is taken off
 #pragma unroll
   for (int i = 0; i < SLOTS; ++i) {
     const int j = i * BT + tid;
     base[i] = 0.f;
-    if (i * BT < entries && j < ((entries + 3) & ~3)) {
+    if (i * BT < t.k && j < ((t.k + 3) & ~3)) {
       int64_t c = -1;
-      float w = hard;
+      float w = 0.f;
       if (j < t.k) {
         const int64_t id = t.id(r, j);
         const float a = t.logit(r, j);
         if (t.there(id)) c = id - t.vocab_start - from;
         w = a != -INFINITY ? scale * expf(a - norm) : 0.f;
-      } else if (j < entries) {
-        c = t.target[r] - t.vocab_start - from;
       }
-      if (c < 0 || c >= len) c = -1;
-      else base[i] = value(to_f(row[c]));
+      if (c < 0 || c >= len) {
+        c = -1;
+      } else {
+        base[i] = value(to_f(row[c]));
+        const uint32_t bit = 1u << (c & 31);
+        if (atomicOr(&named[c >> 5], bit) & bit) twice = 1;
+      }
       cols_of[j] = (int32_t)c;
       weight[j] = w;
+    }
+  }
+  int target = -1;                                           // the label's column
+  float at_target = 0.f;
+  if (t.target) {
+    const int64_t c = t.target[r] - t.vocab_start - from;
+    if (c >= 0 && c < len) {
+      target = (int)c;
+      at_target = value(to_f(row[c]));
     }
   }
   if (logits == grad) __syncthreads();
@@ -403,16 +420,20 @@ distill_bwd_kernel(const T *logits, int64_t ld, int64_t segment, int segments, T
   }
   for (int c = nvec * N + tid; c < len; c += BT) out[c] = from_f<T>(value(to_f(row[c])));
   __syncthreads();                                           // the segment's stores are complete, the lists too
-  // the first entry of a column takes off the weights of all that name it, in the list's order
+  // the label's weight goes with the entry of its column, or alone
+  if (tid == 0 && target >= 0 && !(named[target >> 5] >> (target & 31) & 1)) out[target] = from_f<T>(at_target - hard);
+  // no column twice, as a rule; else the first entry of a column takes off the weights of all that name it, in the list's order.  (Without the
+  // bits, every entry looking for others of its column, 2000 x 4001 with 256 entries a row took 70 us, so 12.)
+  const bool once = twice == 0;
 #pragma unroll
   for (int i = 0; i < SLOTS; ++i) {
-    if (i * BT >= entries) break;
+    if (i * BT >= t.k) break;
     const int j = i * BT + tid;
-    const int c = j < entries ? cols_of[j] : -1;
+    const int c = j < t.k ? cols_of[j] : -1;
     if (c < 0) continue;
     bool first = true;
-    float off = 0.f;
-    for (int o = 0; o < entries; o += 4) {
+    float off = once ? weight[j] : 0.f;
+    for (int o = 0; !once && o < t.k; o += 4) {
       const int4 cc = *reinterpret_cast<const int4 *>(cols_of + o);
       const float4 ww = *reinterpret_cast<const float4 *>(weight + o);
       off += cc.x == c ? ww.x : 0.f;
@@ -421,7 +442,7 @@ distill_bwd_kernel(const T *logits, int64_t ld, int64_t segment, int segments, T
       off += cc.w == c ? ww.w : 0.f;
       first &= !((cc.x == c && o < j) || (cc.y == c && o + 1 < j) || (cc.z == c && o + 2 < j) || (cc.w == c && o + 3 < j));
     }
-    if (first) out[c] = from_f<T>(base[i] - off);
+    if (first) out[c] = from_f<T>(base[i] - (c == target ? off + hard : off));
   }
 }
 

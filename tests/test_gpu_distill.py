@@ -91,7 +91,7 @@ def test_loss_and_gradient(rows, cols, k, tau, alpha, dtype):
 
 
 @pytest.mark.parametrize("padded,twice,whole", [(True, False, False), (False, True, False), (False, False, True), (True, True, True)])
-@pytest.mark.parametrize("rows,cols,k", [(40, 1000, 8), (6, 30001, 130), (1100, 777, 33)])
+@pytest.mark.parametrize("rows,cols,k", [(40, 1000, 8), (6, 30001, 130), (1100, 777, 33), (2, 9000, 1024)])
 @pytest.mark.parametrize("alpha", [1.0, 0.4])
 @pytest.mark.parametrize("ids,teacher", [(torch.int64, torch.float32), (torch.int32, torch.bfloat16), (torch.int32, torch.float16)])
 def test_padded_repeated_and_unnormalised_lists(rows, cols, k, padded, twice, whole, alpha, ids, teacher):
