@@ -18,7 +18,7 @@ namespace dh {
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int BT = 256, MAX_K = 1024;      // threads of a workgroup; entries of a list
+constexpr int MAX_K = 1024;                // entries of a list
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -107,7 +107,7 @@ template <Hard H> struct Running {
   }
 };
 
-template <bool NT, Hard H, typename T>
+template <bool NT, int BT, Hard H, typename T>
 __device__ __forceinline__ void scan_row(const T *row, int64_t from, int64_t to, float k, Running<H> &run) {
   constexpr int N = Vec<T>::N, U = 2;                // vectors in flight: 4096 x 16032 in bf16, not in any cache, 30.3 us, with 4 32.8, with 8 39.2
   const float slack = 16.f / fmaxf(k, LOG2E);        // 2^16 at either temperature
@@ -233,7 +233,7 @@ __device__ __forceinline__ void write_stats(const Teacher &t, float *stats, int6
 enum { PART_SUMS = 6 };
 
 // One workgroup a row, or a segment of one.
-template <typename T, Hard H, bool NT>
+template <typename T, Hard H, bool NT, int BT>
 __global__ void __launch_bounds__(BT)
 distill_fwd_kernel(const T *__restrict__ logits, int64_t ld, int64_t segment, int segments, Teacher t, float *__restrict__ stats,
                    int64_t pitch, float *__restrict__ parts) {
@@ -255,7 +255,7 @@ distill_fwd_kernel(const T *__restrict__ logits, int64_t ld, int64_t segment, in
     }
   }
   Running<H> run;
-  scan_row<NT>(row, from, to, k, run);
+  scan_row<NT, BT>(row, from, to, k, run);
   float m = wave_max(run.top);
   if (m > -INFINITY) run.move(m, k);
   float s = wave_sum(run.s), s1 = H != SAME ? wave_sum(run.s1) : s;
@@ -266,7 +266,9 @@ distill_fwd_kernel(const T *__restrict__ logits, int64_t ld, int64_t segment, in
   }
   __syncthreads();
   if (w != 0) return;
-  m = fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0]));
+  m = red[0][0];
+#pragma unroll
+  for (int i = 1; i < BT / 64; ++i) m = fmaxf(m, red[i][0]);
   s = s1 = 0.f;
 #pragma unroll
   for (int i = 0; i < BT / 64; ++i) {
@@ -329,7 +331,7 @@ distill_join_kernel(int segments, Teacher t, float *__restrict__ stats, int64_t 
 // looking at a row's list once a segment.  4096 x 128256 in bf16, 129 columns a row, us by KB a segment: 8 473, 12 395, 16 361 (5.8 TB/s, what
 // a copy reaches), 24 391, 32 404, 64 420, 256 447; 4096 x 16032: 8 56, 16 48, 32 49.  (All before the bits below, which took 9 off the first.)
 constexpr int64_t BWD_BYTES = 16384;
-template <typename T, Hard H, bool NT>
+template <typename T, Hard H, bool NT, int BT>
 __global__ void __launch_bounds__(BT)
 distill_bwd_kernel(const T *logits, int64_t ld, int64_t segment, int segments, Teacher t, const float *__restrict__ stats,
                    int64_t pitch, const float *__restrict__ dout, T *grad, int64_t ld_grad) {
@@ -364,11 +366,11 @@ distill_bwd_kernel(const T *logits, int64_t ld, int64_t segment, int segments, T
     if (H == SAME) return e * (ks + k1);
     return fmaf(e, ks, exp_one<H>(e, x - m) * k1);
   };
-  static_assert(BWD_BYTES / 2 / 32 == BT, "a word of the bits a thread");
-  named[tid] = 0;
+#pragma unroll
+  for (int i = 0; i < BWD_BYTES / 2 / 32; i += BT) named[i + tid] = 0;
   if (tid == 0) twice = 0;
   __syncthreads();
-  constexpr int SLOTS = MAX_K / BT;
+  constexpr int SLOTS = 4;                                   // entries of a thread: lists of up to 4 BT
   float base[SLOTS];                                         // of the thread's entries: the value without what is taken off
 #pragma unroll
   for (int i = 0; i < SLOTS; ++i) {
@@ -446,15 +448,15 @@ distill_bwd_kernel(const T *logits, int64_t ld, int64_t segment, int segments, T
   }
 }
 
-#define DISTILL_KERNEL(name, out)                                                                          \
-  switch (hard_of(temperature, alpha)) {                                                                   \
-    case SAME: out = nt ? name<T, SAME, true> : name<T, SAME, false>; break;                               \
-    case SQUARE: out = nt ? name<T, SQUARE, true> : name<T, SQUARE, false>; break;                         \
-    case FOURTH: out = nt ? name<T, FOURTH, true> : name<T, FOURTH, false>; break;                         \
-    default: out = nt ? name<T, OWN, true> : name<T, OWN, false>;                                          \
+#define DISTILL_KERNEL(name, out)                                                                                        \
+  switch (hard_of(temperature, alpha)) {                                                                                 \
+    case SAME: out = nt ? name<T, SAME, true, 256> : narrow ? name<T, SAME, false, 64> : name<T, SAME, false, 256>; break;          \
+    case SQUARE: out = nt ? name<T, SQUARE, true, 256> : narrow ? name<T, SQUARE, false, 64> : name<T, SQUARE, false, 256>; break;  \
+    case FOURTH: out = nt ? name<T, FOURTH, true, 256> : narrow ? name<T, FOURTH, false, 64> : name<T, FOURTH, false, 256>; break;  \
+    default: out = nt ? name<T, OWN, true, 256> : narrow ? name<T, OWN, false, 64> : name<T, OWN, false, 256>;                      \
   }
 
-// Segments of a row: one where the rows alone fill the chip; then pieces of at least 4096 columns until they do.
+// Segments of a row: at least `least` columns, no more of them than make `want` workgroups of all rows.
 int64_t segments_of(int64_t rows, int64_t cols, int64_t least, int64_t want) {
   int64_t n = cdiv(want, rows);
   const int64_t most = cdiv(cols, least);
@@ -463,7 +465,11 @@ int64_t segments_of(int64_t rows, int64_t cols, int64_t least, int64_t want) {
 }
 // a segment's length, whole cache lines of any type (4096 x 128256 backward, when it was 398 us: -10)
 int64_t segment_of(int64_t cols, int64_t segments) { return cdiv(cdiv(cols, segments), 64) * 64; }
-int64_t fwd_segment(int64_t rows, int64_t cols) { return segment_of(cols, rows >= 1024 ? 1 : segments_of(rows, cols, 4096, 2048)); }
+// The forward's: one where the rows alone fill the chip, and up to 32768 columns, which a workgroup reads in less than a second launch takes.
+// us, whole rows / segments of 4096, bf16, 16 rows: 16032 columns 5.7 / 8.0, 32000 7.2 / 8.1, 50257 9.7 / 7.9, 128256 10.1 / 7.8
+int64_t fwd_segment(int64_t rows, int64_t cols) {
+  return segment_of(cols, rows >= 1024 || cols <= 32768 ? 1 : segments_of(rows, cols, 4096, 2048));
+}
 
 }  // namespace
 }  // namespace dh
@@ -514,9 +520,12 @@ extern "C" int dh_distill_fwd(const void *logits, int64_t ld, const void *ids, i
     // rows that do not fit in the last-level cache do not go through it: 4096 x 128256 in bf16 191 -> 165 us; 1000 x 50257 in fp32 with the
     // hint 34.5 -> 36.8, and the backward then finds nothing of it (97 -> 113 both)
     const bool nt = stream_hint(rows * cols * (int64_t)sizeof(T));
-    decltype(&distill_fwd_kernel<T, SAME, false>) kernel;
+    // short rows: a wavefront a row, where four of them mostly wait for each other.  us, 256 threads / 64, bf16: 2000 x 1000 5.8 / 5.2, 8000 x 1000
+    // 14.4 / 8.7, 8000 x 2000 17.2 / 11.2, 8000 x 4001 21.5 / 16.9, but 2000 x 4001 7.3 / 7.9, 512 x 8008 5.3 / 7.3
+    const bool narrow = !nt && (cols <= 2048 || (cols <= 4096 && rows >= 4096));
+    decltype(&distill_fwd_kernel<T, SAME, false, 256>) kernel;
     DISTILL_KERNEL(distill_fwd_kernel, kernel)
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * n)), dim3(BT), 0, st, (const T *)logits, ld, segment, (int)n, t, stats, pitch, parts);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * n)), dim3(narrow ? 64 : 256), 0, st, (const T *)logits, ld, segment, (int)n, t, stats, pitch, parts);
   });
   if (parts)
     hipLaunchKernelGGL(distill_join_kernel, dim3((unsigned)rows), dim3(64), 0, st, (int)n, t, stats, pitch, (const float *)parts);
@@ -550,9 +559,12 @@ extern "C" int dh_distill_bwd(const void *logits, int64_t ld, const void *ids, i
     // reader of the gradient behind them, in the caches / past them, 16032 columns in bf16: 1024 rows 36.4 / 38.7, 2048 64.0 / 63.2, 4096
     // 110.9 / 108.8 (92.2 / 88.3 without the reader), 8192 220 / 208; 1000 x 50257 in fp32 160 / 148
     const bool nt = 2 * rows * cols * (int64_t)sizeof(T) > 96ll << 20;
-    decltype(&distill_bwd_kernel<T, SAME, false>) kernel;
+    // short rows as in the forward: 2000 x 1000 6.1 / 4.8 us, 8000 x 1000 17.0 / 11.5, 8000 x 2000 19.6 / 16.0, 8000 x 4001 29.0 / 29.1; a wavefront
+    // holds lists of up to 256
+    const bool narrow = !nt && cols <= 2048 && k <= 256;
+    decltype(&distill_bwd_kernel<T, SAME, false, 256>) kernel;
     DISTILL_KERNEL(distill_bwd_kernel, kernel)
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * n)), dim3(BT), 0, st, (const T *)logits, ld, segment, (int)n, t, stats, pitch, dout,
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * n)), dim3(narrow ? 64 : 256), 0, st, (const T *)logits, ld, segment, (int)n, t, stats, pitch, dout,
                        (T *)grad, ld_grad);
   });
   DH_LAUNCH_CHECK();
