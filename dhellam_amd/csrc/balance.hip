@@ -10,7 +10,7 @@
 // stay in registers, then LDS, then one partial sum a workgroup (one of 1024 threads a compute unit) that a second launch adds in order: no
 // atomics on floats, the same result every time.
 //
-// 131072 tokens x 64 experts, k 8: losses 13.9 us (38 MB; 3 of them the second launch), gradient 17.3 us (80 MB, 4.6 TB/s).  Small calls are
+// 131072 tokens x 64 experts, k 8: losses 13.9 us (38 MB; 3 of them the second launch), gradient 15.7 us (80 MB, 5.1 TB/s).  Small calls are
 // launches: 64 tokens x 8 experts 3.9 and 2.9 us.
 #include "common.h"
 
@@ -227,6 +227,12 @@ balance_join_kernel(const BalancePartial *__restrict__ partials, int blocks, int
   }
 }
 
+// What a wavefront writes to LDS before this, its lanes read behind it (they access it in order; the compiler is to keep that).
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 template <int L>
 __global__ void __launch_bounds__(256)
 route_bwd_kernel(const float *__restrict__ logits, const int32_t *__restrict__ idx, const float *__restrict__ gates,
@@ -234,7 +240,13 @@ route_bwd_kernel(const float *__restrict__ logits, const int32_t *__restrict__ i
                  const int32_t *__restrict__ counts, const int32_t *__restrict__ n_tokens, const float *__restrict__ dlosses,
                  int64_t tokens, int E, int K, float a, float b, float *__restrict__ dlogits, bool vec) {
   constexpr int TPB = 256 / L, S = (BAL_MAX_K + L - 1) / L;       // choices a lane holds
+  __shared__ __align__(16) float tile[L >= 8 ? TPB : 1][4 * L];    // a token's gradient through its gates; all zero between tokens
+  __shared__ int32_t marks[L >= 8 ? TPB : 1][4 * L];
   const int tid = threadIdx.x, l = tid % L, e0 = 4 * l, first = (tid & 63) - l;
+  if constexpr (L >= 8) {
+    *reinterpret_cast<float4 *>(&tile[tid / L][e0]) = make_float4(0.f, 0.f, 0.f, 0.f);
+    wave_order();                                   // (a token's lanes are of one wavefront)
+  }
   float ca = 0.f, cb = 0.f, c[4] = {0.f, 0.f, 0.f, 0.f};
   if (lse) {
     const int n = n_tokens[0];
@@ -283,9 +295,30 @@ route_bwd_kernel(const float *__restrict__ logits, const int32_t *__restrict__ i
       sum = lanes_sum<L>(sum);
 #pragma unroll
       for (int s = 0; s < S; ++s) v[s] = g[s] * (v[s] - sum);
+      bool spread = false;
+      if constexpr (L >= 8) {
+        // a choice a lane: through a row of LDS, where no expert is chosen twice (each lane finds its own mark there); 131072 tokens x 64
+        // experts, k 8, by exchanges and four comparisons a choice 17.6 us, so 15.7
+        const bool chose = (unsigned)e[0] < (unsigned)E;
+        float *to = tile[tid / L];
+        int32_t *mark = marks[tid / L];
+        if (chose) {
+          to[e[0]] = v[0];
+          mark[e[0]] = l;
+        }
+        wave_order();
+        spread = !__any(chose && mark[e[0]] != l);
+        if (spread) {
+          const float4 got = *reinterpret_cast<const float4 *>(to + e0);
+          d[0] += got.x, d[1] += got.y, d[2] += got.z, d[3] += got.w;
+        }
+        wave_order();
+        if (chose) to[e[0]] = 0.f;
+        wave_order();
+      }
 #pragma unroll
       for (int j = 0; j < BAL_MAX_K; ++j)
-        if (j < K) {                                // choice j, to the lane that holds its expert
+        if (!spread && j < K) {                     // choice j, to the lane that holds its expert
           const int to = __shfl(e[j / L], first + j % L, 64) - e0;
           const float val = __shfl(v[j / L], first + j % L, 64);
 #pragma unroll

@@ -151,16 +151,25 @@ def test_experts_that_are_switched_off():
     assert bal.counts.sum() == 500
 
 
-def test_an_expert_chosen_twice_counts_twice():
-    logits, idx, gates, dgates, _ = router(50, 8, 2)
-    idx[:, 1] = idx[:, 0]
+@pytest.mark.parametrize("e,k", [(8, 2), (24, 2), (32, 5), (64, 8)])
+def test_an_expert_chosen_twice_counts_twice(e, k):
+    """In some tokens, beside others that choose each expert once; once three times."""
+    logits, idx, gates, dgates, _ = router(150, e, k)
+    idx[::3, 1] = idx[::3, 0]
+    idx[5, :3] = idx[5, 0].clone()
     losses, bal, _ = balance_loss_fwd(logits, idx, None, A, B)
-    want = plain(logits, idx, gates, dgates, None)
-    assert torch.equal(bal.counts.long(), torch.bincount(idx.flatten().long(), minlength=8))
+    assert torch.equal(bal.counts.long(), torch.bincount(idx.flatten().long(), minlength=e))
     d = route_bwd(logits, idx, gates, dgates)[0]
     g, dg = gates.double(), dgates.double()
-    ref = torch.zeros(50, 8, dtype=torch.float64, device="cuda").scatter_add(1, idx.long(), g * (dg - (g * dg).sum(1, keepdim=True)))
+    ref = torch.zeros(150, e, dtype=torch.float64, device="cuda").scatter_add(1, idx.long(), g * (dg - (g * dg).sum(1, keepdim=True)))
     close(d, ref, torch.zeros_like(ref).scatter_add(1, idx.long(), g * (dg.abs() + (g * dg.abs()).sum(1, keepdim=True))))
+    out = idx.clone()
+    out[1::4, 0] = -1
+    out[2::4, 1] = e
+    d = route_bwd(logits, out, gates, dgates)[0]                          # a choice that is none has no logit
+    at = out.long().clamp(0, e - 1)
+    val = (g * (dg - (g * dg).sum(1, keepdim=True))) * ((out >= 0) & (out < e))
+    close(d, torch.zeros_like(ref).scatter_add(1, at, val), torch.zeros_like(ref).scatter_add(1, at, g * (dg.abs() + (g * dg.abs()).sum(1, keepdim=True))))
 
 
 def test_ranks_join_their_counts():
