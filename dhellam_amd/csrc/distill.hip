@@ -79,7 +79,7 @@ struct Teacher {
 // The per-row statistics, `pitch` floats apart.
 enum { LOSS, ROW_MAX, SUM_TAU, SUM_ONE, NORM, MASS, DOT, MASS_LOCAL, ENTROPY, PREDICTED, N_STATS };
 
-// Sums of exponentials, s at the temperature and s1 at one (TWO), against a reference m that is moved only when a value
+// Sums of exponentials, s at the temperature and s1 at one, against a reference m that is moved only when a value
 // passes it by 2^16: the sums are then as exact as against the maximum (a float's precision does not depend on its scale), and a
 // wavefront hardly ever branches once it has seen its first values.  The lowest float to begin with: -inf adds nothing to it, and
 // a row of lowest floats is a row of equal ones.
@@ -228,9 +228,9 @@ __device__ __forceinline__ void write_stats(const Teacher &t, float *stats, int6
   stats[PREDICTED * pitch] = pred;
 }
 
-// What a row's segments leave for the join: three floats each, and the first one's sums over the entries (dot and the target's
-// logit against the first segment's maximum).
-enum { PART_SUMS = 6 };
+// What a row's segments leave for the join: three floats each, and the first one's sums over the entries, with dot against a reference of
+// the entries' own, for the first segment's maximum may be any low value.
+enum { PART_NORM, PART_MASS, PART_DOT, PART_MINE, PART_ENT, PART_REF, PART_TARGET, PART_SUMS };
 
 // One workgroup a row, or a segment of one.
 template <typename T, Hard H, bool NT, int BT>
@@ -285,19 +285,27 @@ distill_fwd_kernel(const T *__restrict__ logits, int64_t ld, int64_t segment, in
   }
   if (y != 0) return;
   Sums sums;
-  sums.run(t, row, r, m, e);
-  const float pred = has_target ? xt - m : 0.f;
-  if (threadIdx.x != 0) return;
-  if (parts) {
-    o = parts + gridDim.x * 3 + r * PART_SUMS;
-    o[0] = sums.norm;
-    o[1] = sums.mass;
-    o[2] = sums.dot;
-    o[3] = sums.mine;
-    o[4] = sums.ent;
-    o[5] = has_target ? xt : -INFINITY;
-  } else {
-    write_stats(t, stats + r, pitch, m, s, s1, sums, pred);
+  if (!parts) {
+    sums.run(t, row, r, m, e);
+    if (threadIdx.x == 0) write_stats(t, stats + r, pitch, m, s, s1, sums, has_target ? xt - m : 0.f);
+    return;
+  }
+  float ref = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < Entries::U; ++i)
+    if (e.local >> i & 1) ref = fmaxf(ref, e.x[i]);
+  ref = wave_max(ref);
+  if (ref == -INFINITY) ref = 0.f;
+  sums.run(t, row, r, ref, e);
+  if (threadIdx.x == 0) {
+    o = parts + (int64_t)gridDim.x * 3 + r * PART_SUMS;
+    o[PART_NORM] = sums.norm;
+    o[PART_MASS] = sums.mass;
+    o[PART_DOT] = sums.dot;
+    o[PART_MINE] = sums.mine;
+    o[PART_ENT] = sums.ent;
+    o[PART_REF] = ref;
+    o[PART_TARGET] = xt;
   }
 }
 
@@ -320,9 +328,9 @@ distill_join_kernel(int segments, Teacher t, float *__restrict__ stats, int64_t 
   s = wave_sum(s), s1 = wave_sum(s1);
   if (threadIdx.x != 0) return;
   Sums sums;
-  sums.norm = e[0], sums.mass = e[1], sums.mine = e[3], sums.ent = e[4];
-  sums.dot = sums.mine != 0.f ? e[2] + sums.mine * ((p[0] - m) * t.inv_tau) : 0.f;
-  write_stats(t, stats + r, pitch, m, s, s1, sums, t.target && t.column(t.target[r]) >= 0 ? e[5] - m : 0.f);
+  sums.norm = e[PART_NORM], sums.mass = e[PART_MASS], sums.mine = e[PART_MINE], sums.ent = e[PART_ENT];
+  sums.dot = sums.mine != 0.f ? e[PART_DOT] + sums.mine * ((e[PART_REF] - m) * t.inv_tau) : 0.f;
+  write_stats(t, stats + r, pitch, m, s, s1, sums, t.target && t.column(t.target[r]) >= 0 ? e[PART_TARGET] - m : 0.f);
 }
 
 // One workgroup a segment of a row.  Its wavefronts look up the listed columns that lie in the segment, 64 each, then all stream the

@@ -184,6 +184,19 @@ def test_rows_and_columns_that_are_switched_off(rows, cols, alpha):
     assert again["loss"][0] == torch.inf and torch.isfinite(distill_bwd([inputs, again], dout)[0]).all()
 
 
+@pytest.mark.parametrize("low", [-torch.inf, LOW, -1e30])
+@pytest.mark.parametrize("rows,cols", [(4, 40000), (3, 3000), (1100, 900)])
+def test_a_switched_off_beginning_of_the_vocabulary(rows, cols, low):
+    """Whole segments, and whole wavefronts' shares, without a value to compare with."""
+    inputs, dout = case(rows, cols, 300 if cols > 3000 else 40, torch.float32, 0.5, tau=0.7)
+    part = cols * 3 // 5
+    inputs["vocab_parallel_logits"][:, :part] = low
+    inputs["teacher_ids"].clamp_(min=part)
+    inputs["target"].clamp_(min=part)
+    out = distill_fwd(inputs, 0.7, 0.5)
+    compare(out, distill_bwd([inputs, out], dout), plain(inputs, 0.7, 0.5), dout, torch.float32, cols, 0.7)
+
+
 @pytest.mark.parametrize("rows,cols", [(6, 1200), (1200, 1200), (3, 34000)])
 @pytest.mark.parametrize("tau,alpha", [(1.0, 1.0), (2.0, 0.4)])
 def test_slices_of_the_vocabulary_join(rows, cols, tau, alpha):
