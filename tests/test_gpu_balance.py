@@ -187,6 +187,25 @@ def test_ranks_join_their_counts():
         assert torch.equal(route_bwd(logits[s].contiguous(), idx[s].contiguous(), None, None, bal)[0], want[s])
 
 
+def test_tokens_past_32_bits_of_offset():
+    """40 million tokens of 64 experts (10 GB): 5000 tokens over and over.  A lane adds 2500 terms one behind the other, half a step each
+    at most: 2^-24 2500 = 1.5e-4 of a sum beside what ``close`` allows."""
+    logits, idx, gates, dgates, mask = router(5000, 64, 8, masked=True)
+    n = 8000
+    many = lambda t: t.repeat(n, *[1] * (t.dim() - 1))
+    x, i = many(logits), many(idx)
+    losses, bal, _ = balance_loss_fwd(x, i, many(mask), A, B)
+    want = plain(logits, idx, None, None, mask)
+    assert torch.equal(bal.counts.long(), n * want[1]) and bal.tokens.item() == n * int(mask.sum())
+    close(losses, want[0], want[0].abs(), 1.6e-4)
+    close(bal.prob_sum, n * want[2], n * want[2], 1.6e-4)
+    d = route_bwd(x, i, many(gates), many(dgates), bal)[0]
+    ref = plain(logits, idx, gates, dgates, mask)
+    losses_only, with_gates = plain(logits, idx, None, None, mask), ref[3] - want[3]
+    for at in (slice(0, 5000), slice(-5000, None)):                       # (a mean over n times as many: the losses' share is n times smaller)
+        close(d[at], losses_only[3] / n + with_gates, ref[4])
+
+
 def test_the_same_every_time_on_streams_and_in_graphs():
     """Two graphs captured on one stream, replayed at the same time on two: neither shares scratch with the other."""
     data = [router(60000 + i, 64, 8, seed=i) for i in range(2)]

@@ -234,6 +234,19 @@ def test_slices_of_the_vocabulary_join(rows, cols, tau, alpha):
         parallel_state.set_tensor_model_parallel(0, 1)
 
 
+def test_logits_past_32_bits_of_offset():
+    """20000 rows of 128256 in bf16 (5.1 GB): the last rows are what they are alone, in place too."""
+    n, cols = 20000, 128256
+    tail, dout = case(5, cols, 20, torch.bfloat16, 0.5, tau=2.0)
+    inputs = {name: (v.repeat(n // 5, *[1] * (v.dim() - 1)) if v is not None else None) for name, v in tail.items()}
+    out = distill_fwd(inputs, 2.0, 0.5)
+    want = plain(tail, 2.0, 0.5)
+    d = distill_bwd([inputs, out], dout.repeat(n // 5), grad_out=inputs["vocab_parallel_logits"])
+    for at in (slice(0, 5), slice(n - 5, n)):
+        compare({"loss": out["loss"][at]}, d[at], want, dout, torch.bfloat16, cols, 2.0)
+    assert torch.equal(out["loss"], out["loss"][:5].repeat(n // 5)) and torch.equal(d[-5:], d[:5])
+
+
 def test_the_same_every_time_in_graphs():
     """Two graphs captured behind one another replay at the same time on two streams; repeated columns are summed in the list's order."""
     data = [case(5 + i, 40000, 300, torch.bfloat16, 0.5, twice=True, seed=i) for i in range(2)]
