@@ -11,7 +11,7 @@
 // and writes the gradient.  The K listed columns (and the target's) are corrected behind the row's stores, so nothing
 // per element depends on the column.
 //
-// 4096 x 128256 in bf16, K = 128, alpha 0.5, tau 1: forward 167 us (6.3 TB/s), backward 352 us (6.0 TB/s); a copy on this card 5.9 TB/s.
+// 4096 x 128256 in bf16, K = 128, alpha 0.5, tau 1: forward 163 us (6.4 TB/s), backward 352 us (6.0 TB/s); a copy on this card 5.9 TB/s.
 #include "common.h"
 
 namespace dh {
@@ -456,13 +456,17 @@ distill_bwd_kernel(const T *logits, int64_t ld, int64_t segment, int segments, T
   }
 }
 
-#define DISTILL_KERNEL(name, out)                                                                                        \
-  switch (hard_of(temperature, alpha)) {                                                                                 \
-    case SAME: out = nt ? name<T, SAME, true, 256> : narrow ? name<T, SAME, false, 64> : name<T, SAME, false, 256>; break;          \
-    case SQUARE: out = nt ? name<T, SQUARE, true, 256> : narrow ? name<T, SQUARE, false, 64> : name<T, SQUARE, false, 256>; break;  \
-    case FOURTH: out = nt ? name<T, FOURTH, true, 256> : narrow ? name<T, FOURTH, false, 64> : name<T, FOURTH, false, 256>; break;  \
-    default: out = nt ? name<T, OWN, true, 256> : narrow ? name<T, OWN, false, 64> : name<T, OWN, false, 256>;                      \
-  }
+template <typename T, Hard H> auto fwd_kernel(int threads, bool nt) {
+  return threads == 64     ? distill_fwd_kernel<T, H, false, 64>
+         : threads == 1024 ? (nt ? distill_fwd_kernel<T, H, true, 1024> : distill_fwd_kernel<T, H, false, 1024>)
+                           : (nt ? distill_fwd_kernel<T, H, true, 256> : distill_fwd_kernel<T, H, false, 256>);
+}
+template <typename T, Hard H> auto bwd_kernel(int threads, bool nt) {
+  return threads == 64 ? distill_bwd_kernel<T, H, false, 64> : nt ? distill_bwd_kernel<T, H, true, 256> : distill_bwd_kernel<T, H, false, 256>;
+}
+#define DISTILL_PICK(pick, hard, threads, nt)                                                       \
+  (hard == SAME ? pick<T, SAME>(threads, nt) : hard == SQUARE ? pick<T, SQUARE>(threads, nt)        \
+   : hard == FOURTH ? pick<T, FOURTH>(threads, nt) : pick<T, OWN>(threads, nt))
 
 // Segments of a row: at least `least` columns, no more of them than make `want` workgroups of all rows.
 int64_t segments_of(int64_t rows, int64_t cols, int64_t least, int64_t want) {
@@ -473,10 +477,16 @@ int64_t segments_of(int64_t rows, int64_t cols, int64_t least, int64_t want) {
 }
 // a segment's length, whole cache lines of any type (4096 x 128256 backward, when it was 398 us: -10)
 int64_t segment_of(int64_t cols, int64_t segments) { return cdiv(cdiv(cols, segments), 64) * 64; }
-// The forward's: one where the rows alone fill the chip, and up to 32768 columns, which a workgroup reads in less than a second launch takes.
-// us, whole rows / segments of 4096, bf16, 16 rows: 16032 columns 5.7 / 8.0, 32000 7.2 / 8.1, 50257 9.7 / 7.9, 128256 10.1 / 7.8
-int64_t fwd_segment(int64_t rows, int64_t cols) {
-  return segment_of(cols, rows >= 1024 || cols <= 32768 ? 1 : segments_of(rows, cols, 4096, 2048));
+// The forward's: one, but for few rows of very many columns, where joining them costs a launch.  us, one workgroup of 1024 threads a row / segments
+// of 4096, bf16: 16 rows of 50257 7.2 / 7.7, of 128256 11.7 / 7.9, 64 of 128256 12.4 / 11.0, 128 12.7 / 13.5, 256 14.0 / 18.7
+int64_t fwd_segment(int64_t rows, int64_t cols) { return segment_of(cols, rows < 100 && cols > 65536 ? segments_of(rows, cols, 4096, 2048) : 1); }
+// Threads of a row's workgroup in the forward.  A wavefront where rows are short, for four of them mostly wait for each other: us, 256 threads / 64,
+// bf16: 2000 x 1000 5.8 / 5.2, 8000 x 1000 14.4 / 8.7, 8000 x 2000 17.2 / 11.2, 8000 x 4001 21.5 / 16.9, but 2000 x 4001 7.3 / 7.9, 512 x 8008 5.3 / 7.3.
+// 1024 where there are no more rows than stand on the chip at once, or long ones: us, 256 / 1024: bf16, 64 x 10000 5.2 / 5.0, 128 x 32000 9.0 / 6.4, 512 x 50257
+// 17.7 / 13.1, 700 x 128256 44.5 / 36.6, 4096 x 128256 167 / 161, but 700 x 16032 8.6 / 9.9, 3000 x 50257 67 / 73; fp32, 3000 x 50257 99 / 94.
+int fwd_threads(int64_t rows, int64_t cols, int64_t bytes) {
+  if (cols <= 2048 || (cols <= 4096 && rows >= 4096)) return 64;
+  return (rows <= 512 && cols > 8192) || bytes >= 192 << 10 ? 1024 : 256;
 }
 
 }  // namespace
@@ -527,13 +537,9 @@ extern "C" int dh_distill_fwd(const void *logits, int64_t ld, const void *ids, i
   DH_DISPATCH_DTYPE(dtype, {
     // rows that do not fit in the last-level cache do not go through it: 4096 x 128256 in bf16 191 -> 165 us; 1000 x 50257 in fp32 with the
     // hint 34.5 -> 36.8, and the backward then finds nothing of it (97 -> 113 both)
-    const bool nt = stream_hint(rows * cols * (int64_t)sizeof(T));
-    // short rows: a wavefront a row, where four of them mostly wait for each other.  us, 256 threads / 64, bf16: 2000 x 1000 5.8 / 5.2, 8000 x 1000
-    // 14.4 / 8.7, 8000 x 2000 17.2 / 11.2, 8000 x 4001 21.5 / 16.9, but 2000 x 4001 7.3 / 7.9, 512 x 8008 5.3 / 7.3
-    const bool narrow = !nt && (cols <= 2048 || (cols <= 4096 && rows >= 4096));
-    decltype(&distill_fwd_kernel<T, SAME, false, 256>) kernel;
-    DISTILL_KERNEL(distill_fwd_kernel, kernel)
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * n)), dim3(narrow ? 64 : 256), 0, st, (const T *)logits, ld, segment, (int)n, t, stats, pitch, parts);
+    const int threads = n > 1 ? 256 : fwd_threads(rows, cols, cols * (int64_t)sizeof(T));
+    const auto kernel = DISTILL_PICK(fwd_kernel, hard_of(temperature, alpha), threads, threads > 64 && stream_hint(rows * cols * (int64_t)sizeof(T)));
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * n)), dim3(threads), 0, st, (const T *)logits, ld, segment, (int)n, t, stats, pitch, parts);
   });
   if (parts)
     hipLaunchKernelGGL(distill_join_kernel, dim3((unsigned)rows), dim3(64), 0, st, (int)n, t, stats, pitch, (const float *)parts);
@@ -567,12 +573,11 @@ extern "C" int dh_distill_bwd(const void *logits, int64_t ld, const void *ids, i
     // reader of the gradient behind them, in the caches / past them, 16032 columns in bf16: 1024 rows 36.4 / 38.7, 2048 64.0 / 63.2, 4096
     // 110.9 / 108.8 (92.2 / 88.3 without the reader), 8192 220 / 208; 1000 x 50257 in fp32 160 / 148
     const bool nt = 2 * rows * cols * (int64_t)sizeof(T) > 96ll << 20;
-    // short rows as in the forward: 2000 x 1000 6.1 / 4.8 us, 8000 x 1000 17.0 / 11.5, 8000 x 2000 19.6 / 16.0, 8000 x 4001 29.0 / 29.1; a wavefront
-    // holds lists of up to 256
-    const bool narrow = !nt && cols <= 2048 && k <= 256;
-    decltype(&distill_bwd_kernel<T, SAME, false, 256>) kernel;
-    DISTILL_KERNEL(distill_bwd_kernel, kernel)
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * n)), dim3(narrow ? 64 : 256), 0, st, (const T *)logits, ld, segment, (int)n, t, stats, pitch, dout,
+    // a wavefront for short rows as in the forward: 2000 x 1000 6.1 / 4.8 us, 8000 x 1000 17.0 / 11.5, 8000 x 2000 19.6 / 16.0, 8000 x 4001 29.0 /
+    // 29.1; it holds lists of up to 256
+    const int threads = cols <= 2048 && k <= 256 ? 64 : 256;
+    const auto kernel = DISTILL_PICK(bwd_kernel, hard_of(temperature, alpha), threads, nt && threads == 256);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * n)), dim3(threads), 0, st, (const T *)logits, ld, segment, (int)n, t, stats, pitch, dout,
                        (T *)grad, ld_grad);
   });
   DH_LAUNCH_CHECK();

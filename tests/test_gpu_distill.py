@@ -82,7 +82,7 @@ def compare(out, d, want, dout, dtype, cols, tau):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("rows,cols,k", [(1, 1, 1), (1, 2, 2), (3, 7, 3), (5, 1000, 64), (2, 4097, 1), (33, 4001, 100), (2, 50257, 300), (1, 128256, 1024),
-                                         (1030, 1000, 20), (1024, 515, 257), (300, 2048, 256), (70, 2049, 255), (4100, 3000, 5)])
+                                         (1030, 1000, 20), (1024, 515, 257), (300, 2048, 256), (70, 2049, 255), (4100, 3000, 5), (101, 65600, 300), (520, 9001, 3)])
 @pytest.mark.parametrize("tau,alpha", [(1.0, 1.0), (2.0, 1.0), (1.0, 0.5), (0.7, 0.3), (4.0, 0.0)])
 def test_loss_and_gradient(rows, cols, k, tau, alpha, dtype):
     inputs, dout = case(rows, cols, k, dtype, alpha, tau=tau, seed=cols + k)
