@@ -36,7 +36,7 @@ template <bool NT, typename T> __device__ __forceinline__ void store16(T *p, con
 
 // How the exponential at temperature one comes from that at tau, e: it is the same (tau 1, or no targets), e^2 (tau 2), e^4 (tau 4), or
 // needs one of its own.  An exponential is four of the fifteen issue slots that an element takes with two of them, which is
-// more than its two bytes take to arrive: forward of 4096 x 16032 in bf16 at tau 2, alpha 0.5, 30.8 us with two, 26.8 squared.
+// more than its two bytes take to arrive: forward of 4096 x 16032 in bf16 at tau 2, alpha 0.5, 32.4 us with two, 29.8 squared.
 enum Hard { SAME, SQUARE, FOURTH, OWN };
 Hard hard_of(float temperature, float alpha) {
   if (alpha == 1.f || temperature == 1.f) return SAME;
@@ -336,8 +336,9 @@ distill_join_kernel(int segments, Teacher t, float *__restrict__ stats, int64_t 
 // One workgroup a segment of a row.  Its wavefronts look up the listed columns that lie in the segment, 64 each, then all stream the
 // segment, and behind its stores the listed columns are corrected.  grad may be the logits: the listed ones are read before any store.
 // A segment is short, four vectors a thread, so that the workgroups of a moment read and write neighbouring memory, at the price of
-// looking at a row's list once a segment.  4096 x 128256 in bf16, 129 columns a row, us by KB a segment: 8 473, 12 395, 16 361 (5.8 TB/s, what
-// a copy reaches), 24 391, 32 404, 64 420, 256 447; 4096 x 16032: 8 56, 16 48, 32 49.  (All before the bits below, which took 9 off the first.)
+// looking at a row's list once a segment.  4096 x 128256 in bf16, 129 columns a row, us by KB a segment: 8 406, 12 354, 16 353 (6.0 TB/s, what
+// a copy reaches), and with the corrections 9 us slower 16 361, 24 391, 32 404, 64 420, 256 447; 4096 x 16032: 8 52, 16 54, 32 59, but 8 87 with
+// the forward in front, 16 84.
 constexpr int64_t BWD_BYTES = 16384;
 template <typename T, Hard H, bool NT, int BT>
 __global__ void __launch_bounds__(BT)
@@ -535,8 +536,8 @@ extern "C" int dh_distill_fwd(const void *logits, int64_t ld, const void *ids, i
   float *parts = need ? (float *)workspace : nullptr;
   const hipStream_t st = (hipStream_t)stream;
   DH_DISPATCH_DTYPE(dtype, {
-    // rows that do not fit in the last-level cache do not go through it: 4096 x 128256 in bf16 191 -> 165 us; 1000 x 50257 in fp32 with the
-    // hint 34.5 -> 36.8, and the backward then finds nothing of it (97 -> 113 both)
+    // rows that do not fit in the last-level cache do not go through it: 4096 x 128256 in bf16 183 -> 163 us; 1000 x 50257 in fp32 with the
+    // hint 38.0 -> 35.4, but the backward then finds nothing of it (102 -> 113 both)
     const int threads = n > 1 ? 256 : fwd_threads(rows, cols, cols * (int64_t)sizeof(T));
     const auto kernel = DISTILL_PICK(fwd_kernel, hard_of(temperature, alpha), threads, threads > 64 && stream_hint(rows * cols * (int64_t)sizeof(T)));
     hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * n)), dim3(threads), 0, st, (const T *)logits, ld, segment, (int)n, t, stats, pitch, parts);
@@ -571,7 +572,7 @@ extern "C" int dh_distill_bwd(const void *logits, int64_t ld, const void *ids, i
   DH_DISPATCH_DTYPE(dtype, {
     // the gradient's stores go past the caches where that and the logits are more than a part of the last one.  us, forward, backward and a
     // reader of the gradient behind them, in the caches / past them, 16032 columns in bf16: 1024 rows 36.4 / 38.7, 2048 64.0 / 63.2, 4096
-    // 110.9 / 108.8 (92.2 / 88.3 without the reader), 8192 220 / 208; 1000 x 50257 in fp32 160 / 148
+    // 107.6 / 106.7 (90.2 / 83.8 without the reader), 8192 220 / 208; 1000 x 50257 in fp32 154 / 140
     const bool nt = 2 * rows * cols * (int64_t)sizeof(T) > 96ll << 20;
     // a wavefront for short rows as in the forward: 2000 x 1000 6.1 / 4.8 us, 8000 x 1000 17.0 / 11.5, 8000 x 2000 19.6 / 16.0, 8000 x 4001 29.0 /
     // 29.1; it holds lists of up to 256
