@@ -109,7 +109,7 @@ template <Hard H> struct Running {
 
 template <bool NT, int BT, Hard H, typename T>
 __device__ __forceinline__ void scan_row(const T *row, int64_t from, int64_t to, float k, Running<H> &run) {
-  constexpr int N = Vec<T>::N, U = 2;                // vectors in flight: 4096 x 16032 in bf16, not in any cache, 30.3 us, with 4 32.8, with 8 39.2
+  constexpr int N = Vec<T>::N, U = 2;                // vectors in flight: 4096 x 16032 in bf16, not in any cache, 29.8 us, with 4 32.3, with 8 38.6
   const float slack = 16.f / fmaxf(k, LOG2E);        // 2^16 at either temperature
   const int nvec = (int)((to - from) / N);
   const T *base = row + from;
@@ -336,9 +336,9 @@ distill_join_kernel(int segments, Teacher t, float *__restrict__ stats, int64_t 
 // One workgroup a segment of a row.  Its wavefronts look up the listed columns that lie in the segment, 64 each, then all stream the
 // segment, and behind its stores the listed columns are corrected.  grad may be the logits: the listed ones are read before any store.
 // A segment is short, four vectors a thread, so that the workgroups of a moment read and write neighbouring memory, at the price of
-// looking at a row's list once a segment.  4096 x 128256 in bf16, 129 columns a row, us by KB a segment: 8 406, 12 354, 16 353 (6.0 TB/s, what
-// a copy reaches), and with the corrections 9 us slower 16 361, 24 391, 32 404, 64 420, 256 447; 4096 x 16032: 8 52, 16 54, 32 59, but 8 87 with
-// the forward in front, 16 84.
+// looking at a row's list once a segment.  us by KB a segment, inputs in no cache: 4096 x 128256 in bf16, 129 columns a row, 8 406, 12 354,
+// 16 353 (6.0 TB/s, what a copy reaches), 24 382, 32 404, 128 431; 4096 x 16032, 65 columns, 8 52, 16 55, 32 59, but with the forward in
+// front 8 87, 16 84, 32 87; 1000 x 50257 in fp32 8 70, 16 77, 32 83 (99.5, 101.7, 104.3).
 constexpr int64_t BWD_BYTES = 16384;
 template <typename T, Hard H, bool NT, int BT>
 __global__ void __launch_bounds__(BT)
