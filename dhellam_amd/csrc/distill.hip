@@ -11,7 +11,7 @@
 // and writes the gradient.  The K listed columns (and the target's) are corrected behind the row's stores, so nothing
 // per element depends on the column.
 //
-// 4096 x 128256 in bf16, K = 128, alpha 0.5, tau 1: forward 163 us (6.4 TB/s), backward 352 us (6.0 TB/s); a copy on this card 5.9 TB/s.
+// 4096 x 128256 in bf16, K = 128, alpha 0.5, tau 1: forward 163 us (6.4 TB/s), backward 356 us (5.9 TB/s); a copy on this card 5.9 TB/s.
 #include "common.h"
 
 namespace dh {
@@ -336,7 +336,7 @@ distill_join_kernel(int segments, Teacher t, float *__restrict__ stats, int64_t 
 // One workgroup a segment of a row.  Its wavefronts look up the listed columns that lie in the segment, 64 each, then all stream the
 // segment, and behind its stores the listed columns are corrected.  grad may be the logits: the listed ones are read before any store.
 // A segment is short, four vectors a thread, so that the workgroups of a moment read and write neighbouring memory, at the price of
-// looking at a row's list once a segment.  us by KB a segment, inputs in no cache: 4096 x 128256 in bf16, 129 columns a row, 8 406, 12 354,
+// looking at a row's list once a segment.  us by KB a segment, inputs in no cache, before the wait below: 4096 x 128256 in bf16, 129 columns a row, 8 406, 12 354,
 // 16 353 (6.0 TB/s, what a copy reaches), 24 382, 32 404, 128 431; 4096 x 16032, 65 columns, 8 52, 16 55, 32 59, but with the forward in
 // front 8 87, 16 84, 32 87; 1000 x 50257 in fp32 8 70, 16 77, 32 83 (99.5, 101.7, 104.3).
 constexpr int64_t BWD_BYTES = 16384;
@@ -430,7 +430,10 @@ distill_bwd_kernel(const T *logits, int64_t ld, int64_t segment, int segments, T
       }
   }
   for (int c = nvec * N + tid; c < len; c += BT) out[c] = from_f<T>(value(to_f(row[c])));
-  __syncthreads();                                           // the segment's stores are complete, the lists too
+  // the segment's stores are complete, the lists too.  (The barrier by itself waits for LDS only; two stores to one address must not depend on the
+  // order that the memory keeps.  Backward, us, without the wait / with it: 4096 x 128256 in bf16 352 / 356, 4096 x 16032 53.8 / 54.6.)
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
   // the label's weight goes with the entry of its column, or alone
   if (tid == 0 && target >= 0 && !(named[target >> 5] >> (target & 31) & 1)) out[target] = from_f<T>(at_target - hard);
   // no column twice, as a rule; else the first entry of a column takes off the weights of all that name it, in the list's order.  (Without the
