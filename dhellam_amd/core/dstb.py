@@ -177,8 +177,8 @@ class LayerConfig:
 def _turn(config: LayerConfig, q, k, positions, stream, backward=False):
     """Rotary positions on q and k (backward: on their gradients), in place."""
     if config.general_rotary:
-        table = cached_rotary_table(config.rope_theta, config.rotary_dim or config.head_dim, q.device, config.rotary_interleaved,
-                                    config.rope_scaling)
+        dim = config.head_dim if config.rotary_dim is None else config.rotary_dim      # (0 is refused there, not taken for all)
+        table = cached_rotary_table(config.rope_theta, dim, q.device, config.rotary_interleaved, config.rope_scaling)
         (rotary_bwd if backward else rotary_fwd)(q, k, table, positions, config.seq_length, stream, False, inplace=True)
     else:
         (rope_bwd if backward else rope_fwd)(q, k, positions, config.rope_theta, config.seq_length, stream, False, inplace=True)

@@ -69,3 +69,13 @@ def test_scaled_frequencies(dim):
 def test_refused_frequencies(args):
     with pytest.raises(ValueError):
         rotary_frequencies(*args)
+
+
+@pytest.mark.parametrize("dim", [0, -2, 7])
+def test_a_layer_whose_turned_part_is_no_part_of_a_head_is_refused(dim):
+    """0 is not "all": a share of the head that was rounded to nothing is an error of the configuration."""
+    from dhellam_amd.core.dstb import LayerConfig, _turn
+    cfg = LayerConfig(hidden_size=256, num_attention_heads=4, num_query_groups=4, ffn_hidden_size=192, seq_length=64, rotary_dim=dim)
+    assert cfg.general_rotary
+    with pytest.raises(ValueError, match="even number"):
+        _turn(cfg, torch.zeros(64, 4, 64), torch.zeros(64, 4, 64), None, None)
