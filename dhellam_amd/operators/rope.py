@@ -102,7 +102,9 @@ def rotary_frequencies(theta: float, dim: int, scaling: Optional[dict] = None):
             raise ValueError("rotary: scaling 'parts' needs 0 < beta_slow <= beta_fast and theta above 1")
         # the index of the pair that turns beta times over the original length
         edge = lambda beta: dim * math.log(length / (beta * 2.0 * math.pi)) / (2.0 * math.log(theta))
-        lo, hi = max(math.floor(edge(fast)), 0), min(math.ceil(edge(slow)), dim - 1)
+        lo, hi = math.floor(edge(fast)), math.ceil(edge(slow))
+        if hi >= 0 and lo <= dim - 1:         # (a line that ends before the first pair, or begins behind the last, stays where it is)
+            lo, hi = max(lo, 0), min(hi, dim - 1)
         span = float(hi - lo) if hi != lo else 0.001
         ramp = [min(max((j - lo) / span, 0.0), 1.0) for j in range(dim // 2)]
         factor = scaling.get("attention_factor")

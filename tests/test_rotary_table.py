@@ -79,3 +79,25 @@ def test_a_layer_whose_turned_part_is_no_part_of_a_head_is_refused(dim):
     assert cfg.general_rotary
     with pytest.raises(ValueError, match="even number"):
         _turn(cfg, torch.zeros(64, 4, 64), torch.zeros(64, 4, 64), None, None)
+
+
+@pytest.mark.parametrize("theta,dim,length", [(10.0, 64, 100000), (10.0, 2, 1 << 20), (10000.0, 64, 4), (10000.0, 128, 0.5), (10.0, 64, 1), (2.0, 8, 300)])
+def test_parts_whose_line_lies_outside_the_pairs(theta, dim, length):
+    """All pairs turn more than 32 times over the original length and stay, or all less than once and are divided (the line's end is
+    rounded up to a pair: one that turns theta^(-2 / dim) of once may stay); nothing in between turns round."""
+    s = 8.0
+    plain, _ = rotary_frequencies(theta, dim)
+    got, _ = rotary_frequencies(theta, dim, {"kind": "parts", "factor": s, "original_length": length})
+    step = theta ** (2.0 / dim)
+    seen = set()
+    for x, y in zip(plain, got):
+        turns = length * x / (2 * math.pi)
+        if turns > 32:
+            assert math.isclose(y, x, rel_tol=1e-12)
+            seen.add("stays")
+        elif turns < 1 / step:
+            assert math.isclose(y, x / s, rel_tol=1e-12)
+            seen.add("divided")
+        else:
+            assert x / s * (1 - 1e-12) <= y <= x * (1 + 1e-12)
+    assert seen
