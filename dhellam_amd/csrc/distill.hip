@@ -19,6 +19,7 @@ namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int MAX_K = 1024;                // entries of a list
+constexpr float LOWEST = -3.402823466e38f;
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -167,11 +168,12 @@ struct Entries {
   }
 };
 
-// The sums over a row's entries in one pass: weights exp(a - ref) against a running reference, logits against `m`.
+// The sums over a row's entries in one pass: weights exp(a - ref) against a running reference, logits against `m`, the row's maximum, or
+// (FIND) against the largest logit of an entry that has a weight, which m then is.
 struct Sums {
   float norm, mass, dot, mine, ent;
-  template <typename T>
-  __device__ __forceinline__ void run(const Teacher &t, const T *row, int64_t r, float m, Entries &e) {
+  template <bool FIND, typename T>
+  __device__ __forceinline__ void run(const Teacher &t, const T *row, int64_t r, float &m, Entries &e) {
     float ref = -INFINITY, w0 = 0.f, wa = 0.f, wx = 0.f, wl = 0.f;
     for (int first = 0;;) {
       float top = fmaxf(fmaxf(e.a[0], e.a[1]), fmaxf(e.a[2], e.a[3]));
@@ -182,6 +184,15 @@ struct Sums {
         w0 *= f, wx *= f, wl *= f;
       }
       ref = top;
+      if (FIND) {
+        float to = m;
+#pragma unroll
+        for (int i = 0; i < Entries::U; ++i)
+          if (e.a[i] != -INFINITY && (e.local >> i & 1)) to = fmaxf(to, e.x[i]);
+        to = wave_max(to);
+        if (wl != 0.f) wx += wl * ((m - to) * t.inv_tau);
+        m = to;
+      }
 #pragma unroll
       for (int i = 0; i < Entries::U; ++i)
         if (e.a[i] != -INFINITY) {
@@ -286,17 +297,12 @@ distill_fwd_kernel(const T *__restrict__ logits, int64_t ld, int64_t segment, in
   if (y != 0) return;
   Sums sums;
   if (!parts) {
-    sums.run(t, row, r, m, e);
+    sums.run<false>(t, row, r, m, e);
     if (threadIdx.x == 0) write_stats(t, stats + r, pitch, m, s, s1, sums, has_target ? xt - m : 0.f);
     return;
   }
-  float ref = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < Entries::U; ++i)
-    if (e.local >> i & 1) ref = fmaxf(ref, e.x[i]);
-  ref = wave_max(ref);
-  if (ref == -INFINITY) ref = 0.f;
-  sums.run(t, row, r, ref, e);
+  float ref = LOWEST;
+  sums.run<true>(t, row, r, ref, e);
   if (threadIdx.x == 0) {
     o = parts + (int64_t)gridDim.x * 3 + r * PART_SUMS;
     o[PART_NORM] = sums.norm;

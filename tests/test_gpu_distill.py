@@ -298,3 +298,21 @@ def test_refusals():
     none = {n: (v[:0] if v is not None else None) for n, v in inputs.items()}
     o = distill_fwd(none, 1.0, 0.5)
     assert o["loss"].shape == (0,) and distill_bwd([none, o], dout[:0]).shape == (0, 100)
+
+
+@pytest.mark.parametrize("low", [-torch.inf, LOW, -1e30])
+@pytest.mark.parametrize("rows,cols", [(3, 70000), (3, 30000)])
+@pytest.mark.parametrize("tau", [1.0, 0.7])
+def test_entries_without_a_weight_on_columns_that_are_switched_off(rows, cols, tau, low):
+    """600 entries: the first 300 have no weight (the teacher's -inf) and columns without a probability, or are padding; what a row's
+    segments are joined with must not be measured against those."""
+    inputs, dout = case(rows, cols, 600, torch.float32, tau=tau)
+    x, ids, t = inputs["vocab_parallel_logits"], inputs["teacher_ids"], inputs["teacher_logits"]
+    x[:, :cols // 2] = low
+    ids[:, :300] = torch.arange(300, device="cuda")
+    ids[:, 300:] = cols - 1 - torch.arange(300, device="cuda")
+    t[:, :300] = -torch.inf
+    ids[1, :290] = -1
+    x[2] = torch.where(x[2] == low, low, x[2] + 500.0)                  # a row far from zero
+    out = distill_fwd(inputs, tau, 1.0)
+    compare(out, distill_bwd([inputs, out], dout), plain(inputs, tau, 1.0), dout, torch.float32, cols, tau)
