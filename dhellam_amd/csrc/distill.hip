@@ -82,10 +82,11 @@ enum { LOSS, ROW_MAX, SUM_TAU, SUM_ONE, NORM, MASS, DOT, MASS_LOCAL, ENTROPY, PR
 
 // Sums of exponentials, s at the temperature and s1 at one, against a reference m that is moved only when a value
 // passes it by 2^16: the sums are then as exact as against the maximum (a float's precision does not depend on its scale), and a
-// wavefront hardly ever branches once it has seen its first values.  The lowest float to begin with: -inf adds nothing to it, and
-// a row of lowest floats is a row of equal ones.
+// wavefront hardly ever branches once it has seen its first values.  The lowest float to begin with, for the reference and for the
+// maximum: -inf adds nothing to it, a row of lowest floats is a row of equal ones, and x - m is a number for every x, also where a
+// rank's slice holds nothing but -inf.
 template <Hard H> struct Running {
-  float m = -3.402823466e38f, top = -INFINITY, s = 0.f, s1 = 0.f;
+  float m = LOWEST, top = LOWEST, s = 0.f, s1 = 0.f;
   __device__ __forceinline__ void move(float to, float k) {
     s *= exp2_fast((m - to) * k);
     if (H != SAME) s1 *= exp2_fast((m - to) * LOG2E);
@@ -268,7 +269,7 @@ distill_fwd_kernel(const T *__restrict__ logits, int64_t ld, int64_t segment, in
   Running<H> run;
   scan_row<NT, BT>(row, from, to, k, run);
   float m = wave_max(run.top);
-  if (m > -INFINITY) run.move(m, k);
+  run.move(m, k);
   float s = wave_sum(run.s), s1 = H != SAME ? wave_sum(run.s1) : s;
   if ((threadIdx.x & 63) == 0) {
     red[w][0] = m;
@@ -284,8 +285,8 @@ distill_fwd_kernel(const T *__restrict__ logits, int64_t ld, int64_t segment, in
 #pragma unroll
   for (int i = 0; i < BT / 64; ++i) {
     const float d = red[i][0] - m;
-    if (d > -INFINITY || red[i][1] != 0.f) s += red[i][1] * exp2_fast(d * k);      // (a wavefront of -inf only adds nothing)
-    if (H != SAME && (d > -INFINITY || red[i][2] != 0.f)) s1 += red[i][2] * exp2_fast(d * LOG2E);
+    s += red[i][1] * exp2_fast(d * k);               // (a wavefront of -inf only adds nothing)
+    if (H != SAME) s1 += red[i][2] * exp2_fast(d * LOG2E);
   }
   if (H == SAME) s1 = s;
   float *o = parts ? parts + (r * segments + y) * 3 : nullptr;
@@ -320,16 +321,14 @@ __global__ void __launch_bounds__(64)
 distill_join_kernel(int segments, Teacher t, float *__restrict__ stats, int64_t pitch, const float *__restrict__ parts) {
   const int64_t r = blockIdx.x;
   const float k = t.inv_tau * LOG2E, *p = parts + r * segments * 3, *e = parts + (int64_t)gridDim.x * segments * 3 + r * PART_SUMS;
-  float top = -INFINITY;
+  float top = LOWEST;
   for (int i = threadIdx.x; i < segments; i += 64) top = fmaxf(top, p[3 * i]);
   const float m = wave_max(top);
   float s = 0.f, s1 = 0.f;
   for (int i = threadIdx.x; i < segments; i += 64) {
     const float d = p[3 * i] - m;
-    if (d > -INFINITY || p[3 * i + 1] != 0.f) {
-      s += p[3 * i + 1] * exp2_fast(d * k);
-      s1 += p[3 * i + 2] * exp2_fast(d * LOG2E);
-    }
+    s += p[3 * i + 1] * exp2_fast(d * k);
+    s1 += p[3 * i + 2] * exp2_fast(d * LOG2E);
   }
   s = wave_sum(s), s1 = wave_sum(s1);
   if (threadIdx.x != 0) return;

@@ -108,12 +108,13 @@ def distill_statistics(out):
     this rank's share and the caller joins them: with M = max_r row_max_r,
 
         S  = sum_r sum_exp_t_r exp((row_max_r - M) / temperature),   S1 = sum_r sum_exp_r exp(row_max_r - M)      (alpha < 1)
-        D  = sum_r dot_r + mass_local_r (row_max_r - M) / temperature
+        D  = sum_r dot_r + (mass_local_r (row_max_r - M)) / temperature
         P  = sum over the rank that holds the target of (predicted_r + row_max_r - M)
         loss = alpha temperature^2 (entropy - D + mass log S) + (1 - alpha) (log S1 - P)
 
     and each rank's share of the gradient comes from ``distill_bwd`` after M, S and S1 are written over ``row_max``, ``sum_exp_t`` and
-    ``sum_exp``."""
+    ``sum_exp``.  A slice of a row that holds nothing but -inf has the lowest float as its ``row_max`` and sums of 0, so it adds nothing
+    to any of these (the product before the quotient: (row_max_r - M) / temperature may be past the floats)."""
     names = ("loss", "row_max", "sum_exp_t", "sum_exp", "teacher_norm", "mass", "dot", "mass_local", "entropy", "predicted")
     return dict(zip(names, out["stats"].unbind(0)))
 

@@ -623,7 +623,8 @@ int dh_cross_entropy_bwd(const void *src, int64_t ld_src, int from_logits, const
  *   loss = alpha temperature^2 sum p (log p - log q) + (1 - alpha) cross entropy(x, target)
  * alpha < 1 needs targets (int64), alpha = 1 takes none.  An entry listed twice counts twice; a row without entries has no
  * first term.  stats: 10 rows of `pitch` floats:
- *   0 loss, 1 max x = m, 2 S = sum exp((x - m) / temperature), 3 sum exp(x - m) (alpha < 1), 4 l, 5 M = sum p,
+ *   0 loss, 1 max x = m (the lowest float where all x are -inf: sums of 0), 2 S = sum exp((x - m) / temperature),
+ *   3 sum exp(x - m) (alpha < 1), 4 l, 5 M = sum p,
  *   6 D = sum over the entries of this slice p (x - m) / temperature, 7 sum of their p, 8 H = sum p log p,
  *   9 x[target] - m (0 outside the slice)
  * with loss = alpha temperature^2 (H - D + M log S) + (1 - alpha) (log stats[3] - stats[9]).

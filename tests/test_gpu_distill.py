@@ -316,3 +316,59 @@ def test_entries_without_a_weight_on_columns_that_are_switched_off(rows, cols, t
     x[2] = torch.where(x[2] == low, low, x[2] + 500.0)                  # a row far from zero
     out = distill_fwd(inputs, tau, 1.0)
     compare(out, distill_bwd([inputs, out], dout), plain(inputs, tau, 1.0), dout, torch.float32, cols, tau)
+
+
+@pytest.mark.parametrize("rows,cols", [(6, 1200), (1200, 1200), (3, 34000), (2, 70000)])
+@pytest.mark.parametrize("tau,alpha", [(1.0, 1.0), (0.5, 0.4), (2.0, 0.4)])
+@pytest.mark.parametrize("low", [-torch.inf, LOW])
+def test_slices_that_are_switched_off_join(rows, cols, tau, alpha, low):
+    """One rank's whole slice holds nothing but -inf (or the lowest float): what it leaves adds nothing, by the formula as it is written.  The loss of a
+    row that lists a column of -inf there, or has its label there, is infinite.  The joined loss is a sum of the same terms as that of one
+    call, each rounded once more: twice the tolerance of ``compare``."""
+    inputs, dout = case(rows, 2 * cols, 20, torch.float32, alpha, padded=True, tau=tau)
+    inputs["vocab_parallel_logits"][:, :cols] = low
+    inputs["teacher_ids"] = torch.where(inputs["teacher_ids"] >= 0, inputs["teacher_ids"].clamp(min=cols), -1)
+    inputs["teacher_ids"][0, 0] = cols                                   # (row 0 of a padded case lists nothing)
+    if alpha < 1:
+        inputs["target"].clamp_(min=cols)
+    there = []
+    if low == -torch.inf:                                                # the first row lists a column that is switched off, the second has its label there
+        inputs["teacher_ids"][0, 0] = 5
+        there = [0]
+        if alpha < 1:
+            inputs["target"][1] = 7
+            there = [0, 1]
+    want = plain(inputs, tau, alpha)
+    slices = [dict(inputs, vocab_parallel_logits=inputs["vocab_parallel_logits"][:, r * cols:(r + 1) * cols]) for r in range(2)]
+    try:
+        outs = []
+        for rank in range(2):
+            parallel_state.set_tensor_model_parallel(rank, 2)
+            outs.append(distill_fwd(slices[rank], tau, alpha))
+        st = [distill_statistics(o) for o in outs]
+        m = torch.maximum(st[0]["row_max"], st[1]["row_max"])
+        s = sum(o["sum_exp_t"] * torch.exp((o["row_max"] - m) / tau) for o in st)
+        d = sum(o["dot"] + o["mass_local"] * (o["row_max"] - m) / tau for o in st)
+        loss = alpha * tau ** 2 * (st[0]["entropy"] - d + st[0]["mass"] * torch.log(s))
+        s1 = s
+        if alpha < 1:
+            s1 = sum(o["sum_exp"] * torch.exp(o["row_max"] - m) for o in st)
+            mine = [(inputs["target"] >= r * cols) & (inputs["target"] < (r + 1) * cols) for r in range(2)]
+            loss = loss + (1 - alpha) * (torch.log(s1) - sum(torch.where(i, o["predicted"] + o["row_max"] - m, 0.0) for i, o in zip(mine, st)))
+        fine = [r for r in range(rows) if r not in there]
+        assert (loss[there] == torch.inf).all()
+        assert ((loss.double() - want[0]).abs() <= 2 * tolerance(2 * cols, tau) * want[2] + 1e-30)[fine].all()
+        for rank in range(2):
+            parallel_state.set_tensor_model_parallel(rank, 2)
+            for name, joined in (("row_max", m), ("sum_exp_t", s), ("sum_exp", s1)):
+                st[rank][name].copy_(joined)
+            got = distill_bwd([slices[rank], outs[rank]], dout)
+            ref = want[1][:, rank * cols:(rank + 1) * cols] * dout[:, None]
+            assert ((got - ref).abs() <= 2 * tolerance(2 * cols, tau) * want[3][:, rank * cols:(rank + 1) * cols] * dout[:, None]
+                    + ref.abs() * 2.0 ** -24 + 1e-37)[fine].all()
+            assert torch.isfinite(got).all()
+            if rank == 0:                                                # (listed columns there have what is taken off them)
+                got[there] = 0
+                assert (got == 0).all()
+    finally:
+        parallel_state.set_tensor_model_parallel(0, 1)
