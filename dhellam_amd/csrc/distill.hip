@@ -419,7 +419,10 @@ distill_bwd_kernel(const T *logits, int64_t ld, int64_t segment, int segments, T
       at_target = value(to_f(row[c]));
     }
   }
-  if (logits == grad) __syncthreads();
+  if (logits == grad) {                                      // every listed value has arrived before any wavefront writes
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  }
   for (int v = tid; v < nvec; v += U * BT) {
     Vec<T> x[U];
 #pragma unroll
@@ -435,8 +438,9 @@ distill_bwd_kernel(const T *logits, int64_t ld, int64_t segment, int segments, T
       }
   }
   for (int c = nvec * N + tid; c < len; c += BT) out[c] = from_f<T>(value(to_f(row[c])));
-  // the segment's stores are complete, the lists too.  (The barrier by itself waits for LDS only; two stores to one address must not depend on the
-  // order that the memory keeps.  Backward, us, without the wait / with it: 4096 x 128256 in bf16 352 / 356, 4096 x 16032 53.8 / 54.6.)
+  // the segment's stores are complete, the lists too.  (Both barriers of global memory wait for it themselves: __syncthreads() compiles to a wait for
+  // LDS alone, and neither two stores nor a read and a store of one address are to depend on the order that the memory keeps.  Backward, us,
+  // without this wait / with it: 4096 x 128256 in bf16 352 / 356, 4096 x 16032 53.8 / 54.6.)
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   // the label's weight goes with the entry of its column, or alone

@@ -372,3 +372,16 @@ def test_slices_that_are_switched_off_join(rows, cols, tau, alpha, low):
                 assert (got == 0).all()
     finally:
         parallel_state.set_tensor_model_parallel(0, 1)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,cols,k", [(64, 2000, 256), (300, 4001, 1024), (40, 70001, 1024)])
+@pytest.mark.parametrize("tau,alpha", [(1.0, 1.0), (2.0, 0.5)])
+def test_dense_lists_in_place(rows, cols, k, tau, alpha, dtype):
+    """Every third column or so is listed, by wavefronts other than those that write it: over the logits the same bits as beside them."""
+    inputs, dout = case(rows, cols, k, dtype, alpha, tau=tau)
+    inputs["teacher_ids"] = (torch.arange(k, device="cuda") * 3 + torch.arange(rows, device="cuda")[:, None]) % cols
+    out = distill_fwd(inputs, tau, alpha)
+    want = distill_bwd([inputs, out], dout)
+    compare(out, want, plain(inputs, tau, alpha), dout, dtype, cols, tau)
+    assert torch.equal(distill_bwd([inputs, out], dout, grad_out=inputs["vocab_parallel_logits"]), want)
