@@ -280,13 +280,16 @@ route_bwd_kernel(const float *__restrict__ logits, const int32_t *__restrict__ i
         z = lse[t];
         if (mask) on = mask[t] != 0;
       }
+      // the log-sum-exp is one rounded float, off by up to 2^-24 of itself: it serves as the reference, and the row's own sum
+      // (one but for that) makes probabilities of the exponentials, whatever the size of the logits
       float p[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f((x[i] - z) * LOG2E);
-      const float mean = lanes_sum<L>((c[0] * p[0] + c[1] * p[1]) + (c[2] * p[2] + c[3] * p[3]));
+      const float inv = __builtin_amdgcn_rcpf(lanes_sum<L>((p[0] + p[1]) + (p[2] + p[3])));
+      const float mean = lanes_sum<L>((c[0] * p[0] + c[1] * p[1]) + (c[2] * p[2] + c[3] * p[3])) * inv;
       if (on)                                       // (a masked row may hold anything)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) d[i] = p[i] * (ca * (c[i] - mean) + cb * z);
+        for (int i = 0; i < 4; ++i) d[i] = p[i] * inv * (ca * (c[i] - mean) + cb * z);
     }
     if (dgates) {
       float sum = 0.f;

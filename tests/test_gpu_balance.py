@@ -257,3 +257,19 @@ def test_refusals():
                 lambda: route_bwd(logits, idx, gates, dgates.cpu()), lambda: balance_loss_fwd(logits, idx, stream=3)]:
         with pytest.raises(RuntimeError):
             bad()
+
+
+@pytest.mark.parametrize("t,e,k", [(64, 3, 2), (500, 8, 2), (300, 16, 4), (5000, 24, 2), (9000, 60, 6)])
+@pytest.mark.parametrize("offset", [20.0, -100.0, 1000.0, 30000.0])
+def test_the_size_of_the_logits_costs_no_digits(t, e, k, offset):
+    """A softmax does not depend on what all logits of a row have in common.  Probabilities: the argument's difference, product and constant
+    are 2.5 half steps of up to 20, the exponential 2, the sum over 64 and its reciprocal 10, and they come twice (alone and in the
+    mean): 2 (50 + 12) 2^-24 = 7.4e-6 of the terms, below what ``close`` allows."""
+    logits, idx, gates, dgates, mask = router(t, e, k, seed=t, masked=True)
+    logits += offset * torch.linspace(0.5, 1.0, t, device="cuda")[:, None]
+    losses, bal, _ = balance_loss_fwd(logits, idx, mask, A, B)
+    for w in ((1.0, 1.0), (1.0, 0.0), (0.0, 1.0)):
+        want = plain(logits, idx, gates, None, mask, w)
+        close(route_bwd(logits, idx, None, None, bal, torch.tensor(w, device="cuda"))[0], want[3], want[4])
+    close(losses, want[0], want[0].abs())
+    close(bal.prob_sum, want[2], want[2])
