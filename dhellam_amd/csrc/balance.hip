@@ -94,8 +94,9 @@ balance_fwd_kernel(const float *__restrict__ logits, const int32_t *__restrict__
   cnt[w][tid & 63] = 0;
   prob[w][tid & 63] = 0.f;
   __syncthreads();
-  float acc[4] = {0.f, 0.f, 0.f, 0.f}, z = 0.f;
-  int n = 0;
+  // sums of a lane: of up to 64 terms, then those of these, so that none has more than 64 + tokens / 2^20 additions behind one another
+  float acc[4] = {0.f, 0.f, 0.f, 0.f}, z = 0.f, far[4] = {0.f, 0.f, 0.f, 0.f}, far_z = 0.f;
+  int n = 0, terms = 0;
   constexpr int S = (BAL_MAX_K + L - 1) / L;        // choices of a token that a lane counts
   for (int64_t t0 = (int64_t)blockIdx.x * TPB; t0 < tokens; t0 += (int64_t)gridDim.x * TPB) {
     const int64_t t = t0 + tid / L;
@@ -127,7 +128,17 @@ balance_fwd_kernel(const float *__restrict__ logits, const int32_t *__restrict__
         n += 1;
       }
     }
+    if (++terms == 64) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) far[i] += acc[i], acc[i] = 0.f;
+      far_z += z;
+      z = 0.f;
+      terms = 0;
+    }
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc[i] += far[i];
+  z += far_z;
 #pragma unroll
   for (int o = 32; o >= L; o >>= 1)
 #pragma unroll

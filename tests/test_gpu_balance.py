@@ -273,3 +273,17 @@ def test_the_size_of_the_logits_costs_no_digits(t, e, k, offset):
         close(route_bwd(logits, idx, None, None, bal, torch.tensor(w, device="cuda"))[0], want[3], want[4])
     close(losses, want[0], want[0].abs())
     close(bal.prob_sum, want[2], want[2])
+
+
+@pytest.mark.parametrize("e", [41, 63])
+def test_equal_terms_of_many_tokens(e):
+    """2^27 + 5 tokens that all say the same: 8192 terms a lane, whose roundings all go one way.  64 terms behind one another, then 128 sums of
+    them, 2 exchanges, and 16, 16 and 16 partial sums: a half step of the running sum each, which is half the final one on average, 121 2^-24 =
+    7.2e-6, and 2^-23 of a term."""
+    t = (1 << 27) + 5
+    idx = (torch.arange(t, device="cuda") % e).int()[:, None]
+    losses, bal, _ = balance_loss_fwd(torch.zeros(t, e, device="cuda"), idx, None, A, B)
+    assert torch.equal(bal.counts, torch.bincount(idx[:, 0], minlength=e).int()) and bal.tokens.item() == t
+    want = torch.tensor([A, B * torch.log(torch.tensor(float(e), dtype=torch.float64)).item() ** 2], dtype=torch.float64, device="cuda")
+    close(losses, want, want)
+    close(bal.prob_sum, torch.full((e,), t / e, dtype=torch.float64, device="cuda"), t / e)
