@@ -20,6 +20,7 @@
 #include <array>
 #include <map>
 #include <algorithm>
+#include <climits>
 #include <mutex>
 #include <optional>
 #include <tuple>
@@ -347,6 +348,9 @@ std::tuple<Tensor, OptTensor> rope(const Tensor &q, const OptTensor &k, const Te
   return {qo, ko};
 }
 
+// A size for an argument of the C entries that is an int: past its range it is the largest, which they refuse, not what its lower half says.
+int clipped(int64_t n) { return (int)std::min<int64_t>(n, INT_MAX); }
+
 // Rows of heads with any strides, contiguous inside a head; written to only if no two elements share memory.
 void check_heads(const Tensor &t, bool written) {
   PY_ASSERT(t.dim() == 3 && (t.stride(2) == 1 || t.size(2) <= 1), "rotary: expected [tokens, heads, d] with contiguous heads");
@@ -389,7 +393,7 @@ std::tuple<Tensor, OptTensor> rotary(const Tensor &q, const OptTensor &k, const 
   if (k.has_value()) ko = inplace ? *k : at::empty(k->sizes(), k->options());
   launch([&] {
     return dh_rotary(q.data_ptr(), ptr(k), qo.data_ptr(), mptr(ko), (const uint64_t *)steps.data_ptr(), ptr(positions), position_bytes,
-                     tokens, (int)q.size(1), k.has_value() ? (int)k->size(1) : 0, (int)d, (int)rot, q.stride(0), q.stride(1),
+                     tokens, clipped(q.size(1)), k.has_value() ? clipped(k->size(1)) : 0, clipped(d), clipped(rot), q.stride(0), q.stride(1),
                      k.has_value() ? k->stride(0) : 0, k.has_value() ? k->stride(1) : 0, qo.stride(0), qo.stride(1),
                      ko.has_value() ? ko->stride(0) : 0, ko.has_value() ? ko->stride(1) : 0, seq_len, interleaved, backward,
                      (float)factor, type, on.get());
@@ -868,12 +872,12 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> balance_loss_fwd(const Tensor
   int64_t used = 0;
   Tensor lse = part_of(all, used, {t}, logits), prob = part_of(all, used, {e}, logits), losses = part_of(all, used, {2}, logits);
   Tensor counts = part_of(all, used, {e}, idx), n = part_of(all, used, {1}, idx);
-  const int64_t bytes = (int64_t)dh_balance_loss_workspace_bytes(t, (int)e);
+  const int64_t bytes = (int64_t)dh_balance_loss_workspace_bytes(t, clipped(e));
   // of this call alone: a stream's shared scratch would be that of every graph captured on it
   Tensor ws;
   if (bytes) ws = at::empty({bytes}, logits.options().dtype(at::kByte));
   launch([&] {
-    return dh_balance_loss_fwd(logits.data_ptr<float>(), idx.data_ptr<int>(), (const uint8_t *)ptr(mask), t, (int)e, (int)idx.size(1),
+    return dh_balance_loss_fwd(logits.data_ptr<float>(), idx.data_ptr<int>(), (const uint8_t *)ptr(mask), t, clipped(e), clipped(idx.size(1)),
                                (float)balance_coef, (float)z_coef, losses.data_ptr<float>(), counts.data_ptr<int>(),
                                prob.data_ptr<float>(), n.data_ptr<int>(), lse.data_ptr<float>(), bytes ? ws.data_ptr() : nullptr,
                                (size_t)bytes, on.get());
@@ -905,7 +909,7 @@ Tensor route_bwd(const Tensor &logits, const Tensor &idx, const OptTensor &gates
   launch([&] {
     return dh_moe_route_bwd(logits.data_ptr<float>(), idx.data_ptr<int>(), (const float *)ptr(gates), (const float *)ptr(dgates),
                             (const uint8_t *)ptr(mask), (const float *)ptr(lse), (const int32_t *)ptr(counts), (const int32_t *)ptr(n),
-                            (const float *)ptr(dlosses), t, (int)e, (int)idx.size(1), (float)balance_coef, (float)z_coef,
+                            (const float *)ptr(dlosses), t, clipped(e), clipped(idx.size(1)), (float)balance_coef, (float)z_coef,
                             d.data_ptr<float>(), on.get());
   });
   return d;
@@ -1140,7 +1144,7 @@ std::tuple<Tensor, Tensor> distill_fwd(const Tensor &logits, const Tensor &ids, 
   launch([&] {
     return dh_distill_fwd(a.x.data_ptr(), a.rows > 1 ? a.x.stride(0) : a.cols, a.ids.data_ptr(), (int)a.ids.element_size(),
                           a.teacher.data_ptr(), a.teacher_type, (const float *)ptr(lse), (const int64_t *)ptr(a.target), a.rows, a.cols,
-                          (int)a.k, vocab_start, vocab_total, (float)temperature, (float)alpha, a.type, stats.data_ptr<float>(), a.rows,
+                          clipped(a.k), vocab_start, vocab_total, (float)temperature, (float)alpha, a.type, stats.data_ptr<float>(), a.rows,
                           bytes ? ws.data_ptr() : nullptr, (size_t)bytes, on.get());
   });
   const auto shape = logits.sizes().slice(0, logits.dim() - 1);
@@ -1168,7 +1172,7 @@ Tensor distill_bwd(const Tensor &logits, const Tensor &ids, const Tensor &teache
   launch([&] {
     return dh_distill_bwd(a.x.data_ptr(), a.rows > 1 ? a.x.stride(0) : a.cols, a.ids.data_ptr(), (int)a.ids.element_size(),
                           a.teacher.data_ptr(), a.teacher_type, (const int64_t *)ptr(a.target), stats.data_ptr<float>(), a.rows,
-                          d.data_ptr<float>(), a.rows, a.cols, (int)a.k, vocab_start, vocab_total, (float)temperature, (float)alpha,
+                          d.data_ptr<float>(), a.rows, a.cols, clipped(a.k), vocab_start, vocab_total, (float)temperature, (float)alpha,
                           a.type, g.data_ptr(), a.rows > 1 ? g.stride(0) : a.cols, on.get());
   });
   return grad_out.has_value() ? *grad_out : g.view(logits.sizes());

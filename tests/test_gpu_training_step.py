@@ -222,3 +222,22 @@ def test_binding_level_names():
     out, want = C.pydistill_fwd(x, ids, tl, None, target, 2.0, 0.5), loss.distill_fwd(inputs, 2.0, 0.5)
     assert torch.equal(out["loss"], want["loss"])
     assert torch.equal(C.pydistill_bwd(x, ids, tl, target, out, losses.new_ones(9)), loss.distill_bwd([inputs, want], losses.new_ones(9)))
+
+
+def test_sizes_past_an_int_are_refused():
+    """Of tensors without an element, so that nothing that large is held: a size of 2^32 + n is not taken for n."""
+    from dhellam_amd.operators.loss import distill_bwd, distill_fwd
+    from dhellam_amd.operators.moe import balance_loss_fwd, route_bwd
+    from dhellam_amd.operators.rope import rotary_fwd, rotary_table
+    big = 1 << 32
+    empty = lambda *n, dtype=torch.float32: torch.empty(*n, device="cuda", dtype=dtype)
+    t = rotary_table(10000.0, 32, "cuda")
+    idx = empty(0, big + 2, dtype=torch.int32)
+    inputs = {"vocab_parallel_logits": empty(0, 50), "teacher_ids": empty(0, big + 3, dtype=torch.int64), "teacher_logits": empty(0, big + 3)}
+    out = distill_fwd(dict(inputs, teacher_ids=inputs["teacher_ids"][:, :3], teacher_logits=inputs["teacher_logits"][:, :3]))
+    for bad in [lambda: rotary_fwd(empty(0, big + 1, 64), None, t), lambda: rotary_fwd(empty(0, 1, 64), empty(0, big + 1, 64), t),
+                lambda: rotary_fwd(empty(0, 1, big + 64), None, t), lambda: balance_loss_fwd(empty(0, 8), idx),
+                lambda: route_bwd(empty(0, 8), idx, empty(0, big + 2), empty(0, big + 2)), lambda: distill_fwd(inputs),
+                lambda: distill_bwd([inputs, out], empty(0))]:
+        with pytest.raises(RuntimeError):
+            bad()
