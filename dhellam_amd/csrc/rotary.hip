@@ -11,6 +11,8 @@
 // Bound by memory: every element is read and written once.  A lane owns a piece of 16 bytes of the pairs (of both halves, or
 // interleaved), forms its angles once and turns that piece of one or two heads with them.  65536 tokens x 40 heads of 128 in bf16 (1.34 GB):
 // 220 us, 6.1 TB/s; a copy on this card 5.9 TB/s.  Small calls are a launch: 1 token 2.6 us.
+#include <type_traits>
+
 #include "common.h"
 
 namespace dh {
@@ -35,6 +37,14 @@ template <bool NT, int W, typename T> __device__ __forceinline__ void store_piec
   const R v = __builtin_bit_cast(R, x);
   if (NT) __builtin_nontemporal_store(v, reinterpret_cast<R *>(p));
   else *reinterpret_cast<R *>(p) = v;
+}
+
+// The rounding to 16 bits as a step of its own.  The compiler fuses that to fp16 into the sum before it for some elements of a piece and not
+// for others; an element's bits would then depend on where in a piece it lies, so on the number of tokens, on in place or not, and, where
+// pieces overlap, on which lane comes last.
+template <typename T> __device__ __forceinline__ T rounded(float x) {
+  if constexpr (std::is_same_v<T, f16_t>) asm("" : "+v"(x));
+  return from_f<T>(x);
 }
 
 // n / d for n < 2^31 by a product with ceil(2^32 (2^l - d) / d), 2^l the first power of two from d on.
@@ -177,7 +187,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs a) {
 #pragma unroll
       for (int j = 0; j < NP; ++j) {
         const float p = to_f(x[g].v[INTER ? 2 * j : j]), q = to_f(INTER ? x[g].v[2 * j + 1] : y[g].v[j]);
-        const T up = from_f<T>(fmaf(p, cs[j], -(q * sn[j]))), vq = from_f<T>(fmaf(q, cs[j], p * sn[j]));
+        const T up = rounded<T>(fmaf(p, cs[j], -(q * sn[j]))), vq = rounded<T>(fmaf(q, cs[j], p * sn[j]));
         if constexpr (INTER) {
           u.v[2 * j] = up;
           u.v[2 * j + 1] = vq;

@@ -212,3 +212,46 @@ def test_refusals():
         with pytest.raises(RuntimeError):
             bad()
     assert rotary_fwd(q[:0], k[:0], t)[0].shape == (0, 2, 64)
+
+
+@pytest.mark.parametrize("tokens,hq,hk,d,rot,dtype", [
+    (14003, 32, 8, 128, 128, torch.bfloat16), (7001, 31, 10, 256, 128, torch.float16), (7003, 33, 8, 128, 64, torch.float32),      # past the caches
+    (6001, 9, 2, 64, 32, torch.bfloat16), (3001, 7, 4, 192, 64, torch.float16), (3001, 7, 4, 64, 32, torch.float32),               # a rest, in groups of 64 tokens
+    (4001, 7, 4, 80, 20, torch.float16), (9001, 5, 0, 72, 18, torch.bfloat16), (5003, 3, 4, 41, 6, torch.float32)])                # a rest, by single tokens
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_many_tokens(tokens, hq, hk, d, rot, dtype, interleaved):
+    """Enough of them for two heads a lane, odd numbers of heads among them; beside the tensors and over views of a packed projection."""
+    t = rotary_table(10000.0, rot, "cuda", interleaved)
+    at = torch.randint(0, 5000, (tokens,), device="cuda", generator=torch.Generator(device="cuda").manual_seed(2))
+    packed = rand(tokens, (hq + hk + 1) * d, dtype=dtype)
+    views = lambda p: (p[:, :hq * d].unflatten(1, (hq, d)), p[:, hq * d:(hq + hk) * d].unflatten(1, (hk, d)) if hk else None)
+    q, k = views(packed)
+    args = (10000.0, rot, interleaved, None, at)
+    for turn, back in ((rotary_fwd, False), (rotary_bwd, True)):
+        qo, ko, _ = turn(q, k, t, at)
+        check(qo, q, *args, backward=back)
+        if hk:
+            check(ko, k, *args, backward=back)
+        there = packed.clone()
+        a, b, _ = turn(*views(there), t, at, inplace=True)
+        assert torch.equal(a, qo) and (hk == 0 or torch.equal(b, ko))
+        assert torch.equal(there[:, (hq + hk) * d:], packed[:, (hq + hk) * d:])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hq,hk,d,rot", [(7, 4, 80, 20), (8, 1, 128, 128), (6, 2, 64, 40), (12, 4, 96, 48)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_a_token_is_the_same_in_every_call(hq, hk, d, rot, interleaved, dtype):
+    """Alone, among a few and among many, in place and not: the same bits, every time."""
+    t = rotary_table(10000.0, rot, "cuda", interleaved, PARTS)
+    at = torch.arange(9001, device="cuda") * 11
+    q, k = rand(9001, hq, d, dtype=dtype), rand(9001, hk, d, dtype=dtype, seed=1)
+    qo, ko, _ = rotary_fwd(q, k, t, at)
+    for _ in range(3):
+        again = rotary_fwd(q, k, t, at)
+        assert torch.equal(again[0], qo) and torch.equal(again[1], ko)
+    for s in (slice(0, 1), slice(17, 150), slice(8000, 9001)):
+        a, b, _ = rotary_fwd(q[s], k[s], t, at[s])
+        assert torch.equal(a, qo[s]) and torch.equal(b, ko[s])
+    rotary_fwd(q, k, t, at, inplace=True)
+    assert torch.equal(q, qo) and torch.equal(k, ko)
