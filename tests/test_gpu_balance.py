@@ -287,3 +287,10 @@ def test_equal_terms_of_many_tokens(e):
     want = torch.tensor([A, B * torch.log(torch.tensor(float(e), dtype=torch.float64)).item() ** 2], dtype=torch.float64, device="cuda")
     close(losses, want, want)
     close(bal.prob_sum, torch.full((e,), t / e, dtype=torch.float64, device="cuda"), t / e)
+
+
+@pytest.mark.parametrize("t,e,k", [(4097, 1, 1), (5001, 2, 2), (9999, 3, 1), (70003, 4, 4), (2049, 8, 8), (1025, 9, 3), (513, 17, 5), (20001, 24, 2), (3001, 32, 8),
+                                   (257, 33, 8), (30011, 63, 8)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_every_number_of_lanes_in_two_launches(t, e, k, masked):
+    test_losses_counts_and_gradients(t, e, k, masked)

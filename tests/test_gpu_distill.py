@@ -385,3 +385,18 @@ def test_dense_lists_in_place(rows, cols, k, tau, alpha, dtype):
     want = distill_bwd([inputs, out], dout)
     compare(out, want, plain(inputs, tau, alpha), dout, dtype, cols, tau)
     assert torch.equal(distill_bwd([inputs, out], dout, grad_out=inputs["vocab_parallel_logits"]), want)
+
+
+@pytest.mark.parametrize("rows,cols,k,dtype", [(300, 100003, 300, torch.bfloat16), (1500, 100003, 20, torch.float16), (2800, 50257, 64, torch.bfloat16),
+                                               (130, 128256, 1024, torch.float32), (1400, 50257, 8, torch.float32), (7001, 3001, 33, torch.float16)])
+@pytest.mark.parametrize("tau,alpha", [(1.0, 1.0), (2.0, 0.5), (4.0, 0.5), (0.7, 0.5)])
+def test_logits_that_go_past_the_caches(rows, cols, k, dtype, tau, alpha):
+    """More than a part of the last-level cache, with padded lists, repeated columns and the label among them; in place the same bits."""
+    inputs, dout = case(rows, cols, k, dtype, alpha, padded=True, twice=True, tau=tau, teacher=torch.bfloat16)
+    out = distill_fwd(inputs, tau, alpha)
+    d = distill_bwd([inputs, out], dout)
+    for at in range(0, rows, 500):
+        s = slice(at, at + 500)
+        part = {n: (v[s] if v is not None else None) for n, v in inputs.items()}
+        compare({"loss": out["loss"][s]}, d[s], plain(part, tau, alpha), dout[s], dtype, cols, tau)
+    assert torch.equal(distill_bwd([inputs, out], dout, grad_out=inputs["vocab_parallel_logits"]), d)
