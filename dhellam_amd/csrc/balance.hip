@@ -10,7 +10,7 @@
 // stay in registers, then LDS, then one partial sum a workgroup (one of 1024 threads a compute unit) that a second launch adds in order: no
 // atomics on floats, the same result every time.
 //
-// 131072 tokens x 64 experts, k 8: losses 13.9 us (38 MB; 3 of them the second launch), gradient 15.7 us (80 MB, 5.1 TB/s).  Small calls are
+// 131072 tokens x 64 experts, k 8: losses 14.1 us (38 MB; 3 of them the second launch), gradient 15.5 us (80 MB, 5.2 TB/s).  Small calls are
 // launches: 64 tokens x 8 experts 3.9 and 2.9 us.
 #include "common.h"
 
@@ -312,7 +312,7 @@ route_bwd_kernel(const float *__restrict__ logits, const int32_t *__restrict__ i
       bool spread = false;
       if constexpr (L >= 8) {
         // a choice a lane: through a row of LDS, where no expert is chosen twice (each lane finds its own mark there); 131072 tokens x 64
-        // experts, k 8, by exchanges and four comparisons a choice 17.6 us, so 15.7
+        // experts, k 8, by exchanges and four comparisons a choice 17.6 us, so 15.7 (both before the probabilities had a sum of their own)
         const bool chose = (unsigned)e[0] < (unsigned)E;
         float *to = tile[tid / L];
         int32_t *mark = marks[tid / L];

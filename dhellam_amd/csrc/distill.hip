@@ -491,7 +491,9 @@ int64_t segments_of(int64_t rows, int64_t cols, int64_t least, int64_t want) {
 // a segment's length, whole cache lines of any type (4096 x 128256 backward, when it was 398 us: -10)
 int64_t segment_of(int64_t cols, int64_t segments) { return cdiv(cdiv(cols, segments), 64) * 64; }
 // The forward's: one, but for few rows of very many columns, where joining them costs a launch.  us, one workgroup of 1024 threads a row / segments
-// of 4096, bf16: 16 rows of 50257 7.2 / 7.7, of 128256 11.7 / 7.9, 64 of 128256 12.4 / 11.0, 128 12.7 / 13.5, 256 14.0 / 18.7
+// of 4096, bf16: 16 rows of 50257 7.5 / 8.3, of 70000 8.1 / 7.9, of 128256 11.4 / 7.8, of 262144 19.3 / 8.1; 64 rows of 70000 8.1 / 8.4, of 128256
+// 11.4 / 9.7, of 262144 20.1 / 11.7; 99 rows 8.1 / 9.1, 12.2 / 10.5, 20.8 / 15.9; 128 rows 8.1 / 10.7, 12.3 / 11.9, 20.1 / 18.8; 200 rows 8.5 / 11.6,
+// 12.8 / 15.9, 23.1 / 23.6
 int64_t fwd_segment(int64_t rows, int64_t cols) { return segment_of(cols, rows < 100 && cols > 65536 ? segments_of(rows, cols, 4096, 2048) : 1); }
 // Threads of a row's workgroup in the forward.  A wavefront where rows are short, for four of them mostly wait for each other: us, 256 threads / 64,
 // bf16: 2000 x 1000 5.8 / 5.2, 8000 x 1000 14.4 / 8.7, 8000 x 2000 17.2 / 11.2, 8000 x 4001 21.5 / 16.9, but 2000 x 4001 7.3 / 7.9, 512 x 8008 5.3 / 7.3.

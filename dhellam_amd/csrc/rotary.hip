@@ -47,7 +47,8 @@ template <typename T> __device__ __forceinline__ T rounded(float x) {
   return from_f<T>(x);
 }
 
-// n / d for n < 2^31 by a product with ceil(2^32 (2^l - d) / d), 2^l the first power of two from d on.
+// n / d for n < 2^31 by a product with floor(2^32 (2^l - d) / d) + 1, 2^l the first power of two from d on (Granlund and Montgomery, Division
+// by invariant integers using multiplication, 1994).
 struct Divider {
   uint32_t d, m, l;
   explicit Divider(uint32_t by) : d(by < 1 ? 1 : by), m(0), l(0) {
@@ -247,7 +248,8 @@ extern "C" int dh_rotary(const void *q, const void *k, void *q_out, void *k_out,
   const uint64_t lanes = (uint64_t)pieces * (q_slots + k_slots);
   DH_CHECK(lanes < 1u << 22, "hq=%d hk=%d heads of %d are too many", hq, hk, d);
   // where the two parts of a head do not share its memory's 64-byte pieces: us by single tokens / by groups, bf16, 60000 x 40 heads of 64, 32 of
-  // them turned, 160 / 143, 16384 x 40 of 128, 64 turned, 65 / 56; fp16, 60000 x 40 of 80, 20 turned, 250 / 283
+  // them turned, 162 / 138 (pairs 134 / 129), 16384 x 40 of 128, 64 turned, 63 / 61, but 4096 x 40 of 64 9.7 / 11.2; fp16, 60000 x 40 of 80, 20
+  // turned, 196 / 273 (pairs 187 / 278), 30000 x 40 of 96, 48 turned, 125 / 139
   const uint32_t group = rest_pieces && tokens >= 64 && rot * e % 64 == 0 && d * e % 64 == 0 ? 64 : 1, turned_lanes = turned_pieces * (q_slots + k_slots);
   const bool grouped = group > 1;
   RotaryArgs a{{(const char *)q, (char *)q_out, q_token * e, q_head * e, qo_token * e, qo_head * e, hq},

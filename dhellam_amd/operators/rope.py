@@ -62,13 +62,16 @@ def rotary_frequencies(theta: float, dim: int, scaling: Optional[dict] = None):
 
     theta^(-2j / dim), changed by ``scaling`` = {"kind": ..., "factor": s, ...} for contexts s times as long:
 
-    * ``linear``: all divided by s
-    * ``ntk``: theta multiplied by s^(dim / (dim - 2)), so that the slowest pair is divided by s and the fastest stays
+    * ``linear``: all divided by s (position interpolation, Chen et al. 2023)
+    * ``ntk``: theta multiplied by s^(dim / (dim - 2)), so that the slowest pair is divided by s and the fastest stays (the static
+      "NTK-aware" rule)
     * ``parts`` (``original_length``, ``beta_fast`` = 32, ``beta_slow`` = 1, ``attention_factor`` = 0.1 ln s + 1): pairs that turn more
       than ``beta_fast`` times over the original length stay, pairs that turn less than ``beta_slow`` times are divided by s, a line in
-      the pair's index between; cos and sin are multiplied by the attention factor
+      the pair's index between, its ends rounded outwards to pairs; cos and sin are multiplied by the attention factor (YaRN, Peng et al.
+      2023; a configuration's "yarn")
     * ``bands`` (``original_length``, ``low`` = 1, ``high`` = 4): wavelengths below original_length / high stay, above original_length / low
-      they are divided by s, between them a line in original_length / wavelength
+      they are divided by s, between them a line in original_length / wavelength (Llama 3.1's rule; a configuration's "llama3", ``low`` and
+      ``high`` its low and high frequency factors)
     """
     if not (isinstance(dim, int) and dim >= 2 and dim % 2 == 0):
         raise ValueError(f"rotary: the turned part of a head is an even number of elements, not {dim!r}")
