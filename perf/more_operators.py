@@ -8,8 +8,8 @@ plain form in elementary torch operations; with ``own`` true it makes the calls 
 
 The microscaled format, as both sides hold it: a row is cut into blocks of 32, a block has one power of two as its scale and its elements
 in e4m3 (one a byte) or e2m1 (two a byte, the even column in the low half).  Rows are filled up to whole groups of 128 columns with zeros.
-``scales[c, r, i]`` is the exponent code of row r, columns 128 c + 32 i and on: 2^(code - 127), 255 for a block that holds anything not
-finite (its elements are then zeros).  Rows of the scales are filled up to a multiple of four, with zeros as well.
+``scales[c, r // 4, i, r % 4]`` is the exponent code of row r, columns 128 c + 32 i and on: 2^(code - 127), 255 for a block that holds
+anything not finite (its elements are then zeros).  Rows of the scales are filled up to a multiple of four, with zeros as well.
 """
 import math
 
@@ -120,9 +120,14 @@ def _quantise(x, form, rule):
     else:
         c = _e2m1_codes(v).view(rows, kp // 2, 2)
         codes = c[:, :, 0] + 16 * c[:, :, 1]
-    scales = torch.zeros(kp // 128, _up(rows, 4), 4, dtype=torch.uint8, device=x.device)
-    scales[:, :rows] = code.view(rows, kp // 128, 4).transpose(0, 1)
-    return codes, scales
+    scales = torch.zeros(_up(rows, 4), kp // 32, dtype=torch.uint8, device=x.device)
+    scales[:rows] = code
+    return codes, scales.view(-1, 4, kp // 128, 4).permute(2, 0, 3, 1).contiguous()
+
+
+def _by_rows(scales, rows):
+    """The scales' codes as a matrix of a row's blocks."""
+    return scales.permute(1, 3, 0, 2).reshape(4 * scales.shape[1], -1)[:rows]
 
 
 def _values(codes, scales, rows, form, dtype=torch.float32):
@@ -132,7 +137,7 @@ def _values(codes, scales, rows, form, dtype=torch.float32):
     else:
         table = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6, -0.0, -0.5, -1, -1.5, -2, -3, -4, -6], dtype=dtype, device=codes.device)
         v = table[torch.stack([codes & 15, codes >> 4], 2).view(rows, -1).int()]
-    code = scales[:, :rows].transpose(0, 1).reshape(rows, -1).int()
+    code = _by_rows(scales, rows).int()
     bits = torch.where(code == 0, 0x400000, torch.where(code == 255, 0x7FC00000, code << 23)).int()      # 2^-127 is no normal number
     return (v.view(rows, -1, 32) * bits.view(torch.float32).to(dtype).unsqueeze(2)).view(rows, -1)
 
@@ -338,8 +343,9 @@ def _laid_out64(x, rule):
     """Elements and scales as ``run`` gives them."""
     rows = x.shape[0]
     e, scale = _parts64(x, "e4m3", rule)
-    laid = torch.full((_up(x.shape[1], 128) // 128, _up(rows, 4), 4), 2.0 ** -127, dtype=torch.float64, device=x.device)
-    laid[:, :rows] = scale.view(rows, -1, 4).transpose(0, 1)
+    laid = torch.full((_up(x.shape[1], 128) // 128, _up(rows, 4) // 4, 4, 4), 2.0 ** -127, dtype=torch.float64, device=x.device)
+    r = torch.arange(rows, device=x.device)
+    laid[:, r // 4, :, r % 4] = scale.view(rows, -1, 4)
     return [e.view(rows, -1), laid]
 
 
@@ -349,8 +355,9 @@ def _decoded64(pair, rows, form):
     g = torch.tensor(_grid(form), dtype=torch.float64, device=codes.device)
     g = torch.cat([g, g.new_zeros(1), -g, g.new_zeros(1)]) if form == "e4m3" else torch.cat([g, -g])
     c = codes.long() if form == "e4m3" else torch.stack([codes.long() % 16, codes.long() // 16], 2).view(rows, -1)
-    power = _power64(scales[:, :rows].long() - 127)
-    return g[c] * power.permute(1, 0, 2).reshape(rows, -1).repeat_interleave(32, 1)
+    r = torch.arange(rows, device=codes.device)
+    power = _power64(scales[:, r // 4, :, r % 4].long() - 127)
+    return g[c] * power.reshape(rows, -1).repeat_interleave(32, 1)
 
 
 def exact(case, seed):
