@@ -100,6 +100,13 @@ SIGNATURES = {
     "dh_grouped_gemm_nn": (_i32, [_vp] * 4 + [_i32, _i64, _i64, _i64, _i32, _vp, _sz, _vp]),
     "dh_grouped_gemm_tn": (_i32, [_vp] * 4 + [_i32, _i64, _i64, _i64, _i32, _i32, _vp]),
     "dh_grouped_gemm_tn_ws": (_i32, [_vp] * 4 + [_i32, _i64, _i64, _i64, _i32, _i32, _vp, _sz, _vp]),
+    "dh_mx_quantise": (_i32, [_vp, _i64, _i64, _i64, _i32, _i32, _i32] + [_vp] * 5),
+    "dh_rmsnorm_mx": (_i32, [_vp] * 8 + [_i64, _i64, _f32, _i32, _i32, _i32, _vp]),
+    "dh_mx_gemm_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "dh_mx_gemm_nt": (_i32, [_vp, _vp, _i32, _vp, _vp, _i32, _vp] + [_i64] * 4 + [_i32, _i32, _vp, _sz, _vp]),
+    "dh_grad_norm_workspace_bytes": (_sz, [_vp, _i32]),
+    "dh_grad_norm": (_i32, [_vp, _vp, _vp, _i32, _vp, _vp, _sz, _vp]),
+    "dh_grad_clip": (_i32, [_vp] * 5 + [_i32, _vp, C.c_double, C.c_double, _vp, _vp]),
     "dh_grouped_gemm_tn_tiles": (_i32, [_i32, _i64, _i64, _i64, _i32]),
 }
 

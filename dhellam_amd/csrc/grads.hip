@@ -1,0 +1,212 @@
+// What a step does with its gradients before the optimiser: the norm of all of them together and their clipping, over lists of
+// tensors of any number, size and type.
+//
+//   sum_sq = sum over all elements of g^2           norm = |scale| sqrt(sum_sq)
+//   factor = scale min(1, max_norm / (norm + 1e-6)) out = factor g
+//
+// Both passes cut every tensor into pieces of 32768 elements, a workgroup each; a launch takes up to 80 tensors from a table in
+// its arguments.  Squares are added in 64 bits (an fp32 square overflows from 1.8e19 on), a workgroup's sum is written to its own
+// place and one workgroup adds these up in order: the result is the same bits every time.  Bound by memory: 16-byte loads at any alignment.
+#include <cmath>
+
+#include "mx.h"
+
+namespace dh {
+
+constexpr int GRAD_TABLE = 80;
+constexpr int64_t GRAD_PIECE = 32768;
+
+struct GradTable {
+  const void *g[GRAD_TABLE];
+  void *out[GRAD_TABLE];
+  int64_t n[GRAD_TABLE];
+  int first[GRAD_TABLE];             // the tensor's first workgroup in the launch
+  uint8_t type[GRAD_TABLE], out_type[GRAD_TABLE];
+  int count, blocks;
+};
+
+// The tensor that a workgroup belongs to.
+__device__ __forceinline__ int grad_find(const GradTable &t, int block) {
+  int lo = 0, hi = t.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (t.first[mid] <= block) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+template <typename T> __device__ __forceinline__ double grad_piece_sum(const T *g, int64_t n) {
+  double s[2] = {0.0, 0.0};
+#pragma unroll 4
+  for (int i = 0; i < (int)GRAD_PIECE / 2048; ++i) {
+    const int64_t at = (int64_t)i * 2048 + threadIdx.x * 8;
+    float f[8];
+    if (at + 8 <= n) load8(f, g + at);
+    else if (at < n) load8_first(f, g + at, (int)(n - at));
+    else continue;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[j & 1] = fma((double)f[j], (double)f[j], s[j & 1]);
+  }
+  return s[0] + s[1];
+}
+
+__device__ __forceinline__ double wave_sum64(double v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+__global__ void __launch_bounds__(256) grad_norm_kernel(const GradTable t, double *partial) {
+  __shared__ double red[4];
+  const int i = grad_find(t, (int)blockIdx.x);
+  const int64_t at = (int64_t)((int)blockIdx.x - t.first[i]) * GRAD_PIECE, n = t.n[i] - at;
+  double s = 0.0;
+  if (t.type[i] == DH_F32) s = grad_piece_sum(reinterpret_cast<const float *>(t.g[i]) + at, n);
+  else if (t.type[i] == DH_BF16) s = grad_piece_sum(reinterpret_cast<const bf16_t *>(t.g[i]) + at, n);
+  else s = grad_piece_sum(reinterpret_cast<const f16_t *>(t.g[i]) + at, n);
+  s = wave_sum64(s);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) partial[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+}
+
+__global__ void __launch_bounds__(1024) grad_join_kernel(const double *partial, int64_t n, double *sum_sq) {
+  __shared__ double red[16];
+  double s = 0.0;
+  for (int64_t i = threadIdx.x; i < n; i += 1024) s += partial[i];
+  s = wave_sum64(s);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = 0.0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s += red[i];
+    sum_sq[0] = s;
+  }
+}
+
+template <typename T, typename TO> __device__ __forceinline__ void grad_piece_scale(const T *g, TO *out, int64_t n, float factor) {
+#pragma unroll 4
+  for (int i = 0; i < (int)GRAD_PIECE / 2048; ++i) {
+    const int64_t at = (int64_t)i * 2048 + threadIdx.x * 8;
+    float f[8];
+    if (at + 8 <= n) {
+      load8(f, g + at);
+      Loose8<TO> o;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o.v[j] = factor == 0.f ? from_f<TO>(0.f) : from_f<TO>(f[j] * factor);
+      *reinterpret_cast<Loose8<TO> *>(out + at) = o;
+    } else if (at < n) {
+      for (int64_t j = at; j < n; ++j) out[j] = factor == 0.f ? from_f<TO>(0.f) : from_f<TO>(to_f(g[j]) * factor);
+    }
+  }
+}
+
+__global__ void __launch_bounds__(256) grad_clip_kernel(const GradTable t, const double *sum_sq, double max_norm, double scale, float *found) {
+  const double norm = fabs(scale) * sqrt(sum_sq[0]);
+  double factor = scale * fmin(1.0, max_norm / (norm + 1e-6));
+  if (!(norm < INFINITY)) factor = 0.0;
+  if (found && blockIdx.x == 0 && threadIdx.x == 0) {
+    found[0] = (float)norm;
+    found[1] = (float)factor;
+  }
+  if (t.blocks == 0) return;
+  const float f = (float)factor;
+  const int i = grad_find(t, (int)blockIdx.x);
+  const int64_t at = (int64_t)((int)blockIdx.x - t.first[i]) * GRAD_PIECE, n = t.n[i] - at;
+  if (f == 1.f && t.g[i] == t.out[i]) return;              // in place, nothing to change
+#define GRAD_SCALE(T, TO) grad_piece_scale(reinterpret_cast<const T *>(t.g[i]) + at, reinterpret_cast<TO *>(t.out[i]) + at, n, f)
+  if (t.type[i] == DH_F32) GRAD_SCALE(float, float);
+  else if (t.type[i] == DH_BF16) {
+    if (t.out_type[i] == DH_F32) GRAD_SCALE(bf16_t, float);
+    else GRAD_SCALE(bf16_t, bf16_t);
+  } else {
+    if (t.out_type[i] == DH_F32) GRAD_SCALE(f16_t, float);
+    else GRAD_SCALE(f16_t, f16_t);
+  }
+#undef GRAD_SCALE
+}
+
+// Calls fn(table) for the lists in tables of up to GRAD_TABLE tensors that are not empty.
+template <typename F>
+static int grad_tables(const void *const *g, void *const *out, const int64_t *counts, const int *types, const int *out_types, int n, F &&fn) {
+  for (int i = 0; i < n;) {
+    GradTable t{};
+    int64_t blocks = 0;
+    for (; i < n && t.count < GRAD_TABLE; ++i) {
+      DH_CHECK(counts[i] >= 0, "tensor %d: %lld elements", i, (long long)counts[i]);
+      DH_CHECK(types[i] == DH_F32 || types[i] == DH_BF16 || types[i] == DH_F16, "tensor %d: unknown dtype %d", i, types[i]);
+      DH_CHECK(!out || out_types[i] == types[i] || out_types[i] == DH_F32, "tensor %d: results are of its own type or fp32", i);
+      if (counts[i] == 0) continue;
+      DH_CHECK(g[i] && (!out || out[i]), "tensor %d: null pointer", i);
+      const int64_t b = cdiv(counts[i], GRAD_PIECE);
+      DH_CHECK(b < (1ll << 30), "tensor %d is too large", i);
+      if (t.count > 0 && blocks + b >= (1ll << 31)) break;
+      t.g[t.count] = g[i];
+      t.out[t.count] = out ? out[i] : nullptr;
+      t.n[t.count] = counts[i];
+      t.type[t.count] = (uint8_t)types[i];
+      t.out_type[t.count] = (uint8_t)(out ? out_types[i] : 0);
+      t.first[t.count++] = (int)blocks;
+      blocks += b;
+    }
+    t.blocks = (int)blocks;
+    if (t.count > 0)
+      if (const int rc = fn(t)) return rc;
+  }
+  return DH_OK;
+}
+
+}  // namespace dh
+
+extern "C" size_t dh_grad_norm_workspace_bytes(const int64_t *counts, int n) {
+  int64_t blocks = 0;
+  for (int i = 0; i < n; ++i) blocks += counts[i] > 0 ? dh::cdiv(counts[i], dh::GRAD_PIECE) : 0;
+  return (size_t)blocks * 8;
+}
+
+extern "C" int dh_grad_norm(const void *const *grads, const int64_t *counts, const int *dtypes, int n, double *sum_sq, void *workspace,
+                            size_t workspace_bytes, void *stream) {
+  using namespace dh;
+  DH_CHECK(n >= 0 && (n == 0 || (grads && counts && dtypes)) && sum_sq, "bad list");
+  for (int i = 0; i < n; ++i) DH_CHECK(counts[i] >= 0, "tensor %d: %lld elements", i, (long long)counts[i]);
+  const size_t need = dh_grad_norm_workspace_bytes(counts, n);
+  DH_CHECK(need == 0 || (workspace && (uintptr_t)workspace % 8 == 0 && workspace_bytes >= need), "workspace of %zu bytes, %zu are needed", workspace_bytes,
+           need);
+  double *partial = reinterpret_cast<double *>(workspace);
+  int64_t done = 0;
+  const hipStream_t st = (hipStream_t)stream;
+  const int rc = grad_tables(grads, nullptr, counts, dtypes, nullptr, n, [&](const GradTable &t) -> int {
+    hipLaunchKernelGGL(grad_norm_kernel, dim3((unsigned)t.blocks), dim3(256), 0, st, t, partial + done);
+    done += t.blocks;
+    DH_LAUNCH_CHECK();
+    return DH_OK;
+  });
+  if (rc) return rc;
+  hipLaunchKernelGGL(grad_join_kernel, dim3(1), dim3(1024), 0, st, partial, done, sum_sq);
+  DH_LAUNCH_CHECK();
+  return DH_OK;
+}
+
+extern "C" int dh_grad_clip(const void *const *grads, void *const *out, const int64_t *counts, const int *dtypes, const int *out_dtypes, int n,
+                            const double *sum_sq, double max_norm, double scale, float *found, void *stream) {
+  using namespace dh;
+  DH_CHECK(n >= 0 && (n == 0 || (grads && out && counts && dtypes && out_dtypes)) && sum_sq && found, "bad list");
+  DH_CHECK(max_norm >= 0, "max_norm %g", max_norm);
+  DH_CHECK(std::isfinite(scale), "scale %g", scale);
+  const hipStream_t st = (hipStream_t)stream;
+  float *say = found;
+  const int rc = grad_tables(grads, out, counts, dtypes, out_dtypes, n, [&](const GradTable &t) -> int {
+    hipLaunchKernelGGL(grad_clip_kernel, dim3((unsigned)t.blocks), dim3(256), 0, st, t, sum_sq, max_norm, scale, say);
+    say = nullptr;
+    DH_LAUNCH_CHECK();
+    return DH_OK;
+  });
+  if (rc) return rc;
+  if (say) {
+    hipLaunchKernelGGL(grad_clip_kernel, dim3(1), dim3(64), 0, st, GradTable{}, sum_sq, max_norm, scale, say);
+    DH_LAUNCH_CHECK();
+  }
+  return DH_OK;
+}

@@ -1216,6 +1216,172 @@ void zero_all(const std::vector<Tensor> &ts, const OptStream &stream) {
   if (!ptrs.empty()) launch([&] { return dh_zero_many(ptrs.data(), bytes.data(), (int)ptrs.size(), on.get()); });
 }
 
+// ---- microscaled operands -----------------------------------------------------------------------------------------------
+// Codes and scales of a rows x cols matrix in the given format (layout: include/dhellam_hip.h).
+std::pair<Tensor, Tensor> mx_empty(int64_t rows, int64_t cols, int format, const Tensor &like) {
+  const int64_t kp = (cols + 127) / 128 * 128;
+  const auto bytes = like.options().dtype(at::kByte);
+  return {at::empty({rows, format == DH_MX_E4M3 ? kp : kp / 2}, bytes), at::empty({kp / 128, (rows + 3) / 4, 4, 4}, bytes)};
+}
+
+int mx_format(int64_t format) {
+  TORCH_CHECK(format == DH_MX_E4M3 || format == DH_MX_E2M1, "mx: unknown format");
+  return (int)format;
+}
+
+// `along`: 1 rows, 2 columns, 3 both.  -> codes, scales of x, and of its transpose
+std::tuple<OptTensor, OptTensor, OptTensor, OptTensor> mx_quantise(const Tensor &x, int64_t format_, int64_t along, bool cover,
+                                                                   const OptStream &stream) {
+  OnGpu on({&x}, stream);
+  const int format = mx_format(format_), type = dt(x);
+  PY_ASSERT(x.dim() > 0, "mx_quantise: a matrix, or rows with leading dimensions");
+  const int64_t cols = x.size(-1), rows = cols ? x.numel() / cols : x.sizes().slice(0, x.dim() - 1).empty() ? 1 : c10::multiply_integers(x.sizes().slice(0, x.dim() - 1));
+  PY_ASSERT(x.is_contiguous() || (x.dim() == 2 && (x.stride(1) == 1 || cols == 1) && (x.stride(0) >= cols || rows == 1)),
+            "mx_quantise: contiguous, or 2-D with unit inner stride");
+  OptTensor c, s, ct, st;
+  if (along & 1) std::tie(c, s) = mx_empty(rows, cols, format, x);
+  if (along & 2) std::tie(ct, st) = mx_empty(cols, rows, format, x);
+  if (rows == 0 || cols == 0) {      // codes and scales that are all filling
+    for (OptTensor *t : {&c, &s, &ct, &st})
+      if (t->has_value() && (*t)->numel()) (*t)->zero_();
+    return {c, s, ct, st};
+  }
+  launch([&] {
+    return dh_mx_quantise(x.data_ptr(), rows, cols, x.is_contiguous() ? cols : x.stride(0), type, format, cover, mptr(c), mptr(s), mptr(ct), mptr(st),
+                          on.get());
+  });
+  return {c, s, ct, st};
+}
+
+// -> codes, scales, rsigma, sum or None
+std::tuple<Tensor, Tensor, Tensor, OptTensor> rmsnorm_mx(const Tensor &inp, const Tensor &weight, double eps, bool zero_centered,
+                                                         const OptTensor &residual, OptTensor sum_out, const OptTensor &ln_out, bool cover,
+                                                         const OptStream &stream) {
+  OnGpu on({&inp, &weight, opt(residual), opt(sum_out), opt(ln_out)}, stream);
+  const int64_t cols = weight.numel();
+  PY_ASSERT(inp.dim() > 0 && inp.size(-1) == cols, "LayerNorm not possible");
+  PY_ASSERT(inp.is_contiguous() && weight.is_contiguous(), "norm: input and weight must be contiguous");
+  PY_ASSERT(weight.scalar_type() == inp.scalar_type(), "norm: input and weight must be of one type");
+  const auto like = [&](const OptTensor &t) {
+    return !t.has_value() || (t->is_contiguous() && t->numel() == inp.numel() && t->scalar_type() == inp.scalar_type());
+  };
+  PY_ASSERT(like(residual) && like(sum_out) && like(ln_out), "norm: residual, sum_out and ln_out must be contiguous, of the input's size and type");
+  PY_ASSERT(residual.has_value() || !sum_out.has_value(), "norm: sum_out without a residual");
+  PY_ASSERT(!sum_out.has_value() || !ln_out.has_value() || sum_out->data_ptr() != ln_out->data_ptr(), "norm: sum_out and ln_out are one");
+  const int64_t rows = cols ? inp.numel() / cols : 0;
+  const int type = dt(inp);
+  auto [codes, scales] = mx_empty(rows, cols, DH_MX_E4M3, inp);
+  Tensor rsigma = at::empty({rows}, inp.options().dtype(at::kFloat));
+  if (residual.has_value() && !sum_out.has_value()) sum_out = at::empty(residual->sizes(), residual->options());
+  launch([&, &codes = codes, &scales = scales] {
+    return dh_rmsnorm_mx(inp.data_ptr(), ptr(residual), mptr(sum_out), weight.data_ptr(), mptr(ln_out), codes.data_ptr(), scales.data_ptr(),
+                         rsigma.data_ptr<float>(), rows, cols, (float)eps, zero_centered, cover, type, on.get());
+  });
+  return {codes, scales, rsigma, sum_out};
+}
+
+// One operand of mx_gemm_nt: what its codes and scales have to look like for rows x cols.
+void check_mx(const Tensor &codes, const Tensor &scales, int64_t rows, int64_t cols, int format) {
+  const int64_t kp = (cols + 127) / 128 * 128;
+  PY_ASSERT(rows >= 0 && cols >= 0, "mx: negative sizes");
+  PY_ASSERT(codes.scalar_type() == at::kByte && codes.is_contiguous() && codes.dim() == 2 && codes.size(0) == rows &&
+                codes.size(1) == (format == DH_MX_E4M3 ? kp : kp / 2),
+            "mx: codes must be contiguous uint8 [rows, columns rounded up to 128] (e4m3), half as many columns for e2m1");
+  PY_ASSERT(scales.scalar_type() == at::kByte && scales.is_contiguous() && scales.dim() == 4 && scales.size(0) == kp / 128 &&
+                scales.size(1) == (rows + 3) / 4 && scales.size(2) == 4 && scales.size(3) == 4,
+            "mx: scales must be contiguous uint8 [columns / 128, rows / 4, 4, 4]");
+}
+
+Tensor mx_gemm_nt(const Tensor &a, const Tensor &as, int64_t m, int64_t fa_, const Tensor &b, const Tensor &bs, int64_t n, int64_t fb_, int64_t k,
+                  const OptTensor &out, at::ScalarType out_dtype, bool accumulate, const OptStream &stream) {
+  OnGpu on({&a, &as, &b, &bs, opt(out)}, stream);
+  const int fa = mx_format(fa_), fb = mx_format(fb_);
+  check_mx(a, as, m, k, fa);
+  check_mx(b, bs, n, k, fb);
+  PY_ASSERT(out.has_value() || !accumulate, "mx_gemm_nt: nothing to accumulate into");
+  PY_ASSERT(!out.has_value() || (out->dim() == 2 && out->size(0) == m && out->size(1) == n && (out->stride(1) == 1 || n <= 1) && (out->stride(0) >= n || m <= 1)),
+            "mx_gemm_nt: out must be [m, n] with unit inner stride");
+  Tensor c = out.has_value() ? *out : at::empty({m, n}, a.options().dtype(out_dtype));
+  const int type = dt(c);
+  const int64_t bytes = (int64_t)dh_mx_gemm_workspace_bytes(m, n, k);
+  Tensor ws;                           // of this call alone, so that calls and captured graphs that overlap share none
+  if (bytes) ws = at::empty({bytes}, a.options());
+  launch([&] {
+    return dh_mx_gemm_nt(a.data_ptr(), as.data_ptr(), fa, b.data_ptr(), bs.data_ptr(), fb, c.data_ptr(), m, n, k, m > 1 ? c.stride(0) : n, type, accumulate,
+                         bytes ? ws.data_ptr() : nullptr, (size_t)bytes, on.get());
+  });
+  return c;
+}
+
+// ---- gradients of a step -----------------------------------------------------------------------------------------------
+// The lists as the library takes them.
+struct Grads {
+  std::vector<const void *> ptrs;
+  std::vector<int64_t> counts;
+  std::vector<int> types;
+  explicit Grads(const std::vector<Tensor> &ts) {
+    for (const Tensor &t : ts) {
+      TORCH_CHECK(t.is_cuda() && t.device() == ts[0].device(), "dhellam operators need their tensors on one GPU");
+      PY_ASSERT(t.is_non_overlapping_and_dense(), "gradients must fill their memory (contiguous, or a permutation of it)");
+      ptrs.push_back(t.data_ptr());
+      counts.push_back(t.numel());
+      types.push_back(dt(t));
+    }
+  }
+  int n() const { return (int)ptrs.size(); }
+};
+
+Tensor grad_norm(const std::vector<Tensor> &ts, const OptStream &stream) {
+  const Grads g(ts);
+  const Tensor like = ts.empty() ? at::empty({0}, at::TensorOptions().device(at::kCUDA, c10::hip::current_device())) : ts[0];
+  OnGpu on({&like}, stream);
+  Tensor sum = at::empty({1}, like.options().dtype(at::kDouble));
+  const int64_t bytes = (int64_t)dh_grad_norm_workspace_bytes(g.counts.data(), g.n());
+  Tensor ws;                           // of this call alone
+  if (bytes) ws = at::empty({bytes}, like.options().dtype(at::kByte));
+  launch([&] {
+    return dh_grad_norm(g.ptrs.data(), g.counts.data(), g.types.data(), g.n(), sum.data_ptr<double>(), bytes ? ws.data_ptr() : nullptr, (size_t)bytes,
+                        on.get());
+  });
+  return sum;
+}
+
+// -> found fp32 [2]: norm, factor
+Tensor grad_clip(const std::vector<Tensor> &ts, const Tensor &sum, double max_norm, double scale, const std::optional<std::vector<Tensor>> &out_,
+                 const OptStream &stream) {
+  const Grads g(ts);
+  const std::vector<Tensor> &out = out_.has_value() ? *out_ : ts;
+  const Grads o(out);
+  OnGpu on({&sum, ts.empty() ? nullptr : &ts[0], out.empty() ? nullptr : &out[0]}, stream);
+  PY_ASSERT(sum.scalar_type() == at::kDouble && sum.numel() == 1, "clip_grads: sum_sq must be what grad_norm returns");
+  PY_ASSERT(out.size() == ts.size(), "clip_grads: one result per gradient");
+  // [begin, end) of every result, in order of address: two may not meet, nor a result and a gradient that is not its own
+  struct Range { uintptr_t begin, end; };
+  std::vector<Range> ranges;
+  for (size_t i = 0; i < ts.size(); ++i) {
+    PY_ASSERT(out[i].sizes() == ts[i].sizes() && (out[i].strides() == ts[i].strides() || (out[i].is_contiguous() && ts[i].is_contiguous())),
+              "clip_grads: a result must be laid out as its gradient");
+    PY_ASSERT(o.types[i] == g.types[i] || o.types[i] == DH_F32, "clip_grads: a result is of its gradient's type or fp32");
+    if (o.counts[i]) ranges.push_back({(uintptr_t)o.ptrs[i], (uintptr_t)o.ptrs[i] + out[i].nbytes()});
+  }
+  std::sort(ranges.begin(), ranges.end(), [](const Range &a, const Range &b) { return a.begin < b.begin; });
+  for (size_t i = 1; i < ranges.size(); ++i) PY_ASSERT(ranges[i - 1].end <= ranges[i].begin, "clip_grads: two results share memory");
+  for (size_t i = 0; i < ts.size(); ++i) {
+    if (!g.counts[i] || (g.ptrs[i] == o.ptrs[i] && g.types[i] == o.types[i])) continue;
+    const uintptr_t begin = (uintptr_t)g.ptrs[i], end = begin + ts[i].nbytes();
+    auto it = std::upper_bound(ranges.begin(), ranges.end(), begin, [](uintptr_t v, const Range &r) { return v < r.end; });
+    PY_ASSERT(it == ranges.end() || it->begin >= end, "clip_grads: a result shares memory with a gradient that is not its own");
+  }
+  Tensor found = at::empty({2}, sum.options().dtype(at::kFloat));
+  std::vector<void *> outs;
+  for (const void *p : o.ptrs) outs.push_back(const_cast<void *>(p));
+  launch([&] {
+    return dh_grad_clip(g.ptrs.data(), outs.data(), g.counts.data(), g.types.data(), o.types.data(), g.n(), sum.data_ptr<double>(), max_norm, scale,
+                        found.data_ptr<float>(), on.get());
+  });
+  return found;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -1268,4 +1434,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("masked_mean_fwd", &masked_mean_fwd);
   m.def("masked_mean_bwd", &masked_mean_bwd);
   m.def("zero_all", &zero_all);
+  m.def("mx_quantise", &mx_quantise);
+  m.def("rmsnorm_mx", &rmsnorm_mx);
+  m.def("mx_gemm_nt", &mx_gemm_nt);
+  m.def("grad_norm", &grad_norm);
+  m.def("grad_clip", &grad_clip);
 }

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 from .. import _host, _lib
 from ._util import issue
+from .mx import SCALE_RULES, MXTensor, _one_of
 
 
 def pylayernorm_fwd(inp, ln_weight, ln_bias, eps, fwd_sm_margin, zero_centered_gamma, stream, profiling=False,
@@ -25,6 +26,21 @@ def pylayernorm_fwd(inp, ln_weight, ln_bias, eps, fwd_sm_margin, zero_centered_g
     if residual is not None:
         return y, mu, rsigma, ms, total
     return y, mu, rsigma, ms
+
+
+def pyrmsnorm_mx_fwd(inp, ln_weight, eps, zero_centered_gamma, stream=None, profiling=False, residual=None, sum_out=None,
+                     ln_out=None, scale_rule="floor"):
+    """RMSNorm whose result is written in 8 bits with scales (``operators.mx.MXTensor``, e4m3, blocks of 32 along the row), quantised from its
+    fp32 value.  Returns (MXTensor, rsigma, sum, ms); ``residual`` and ``sum_out`` as in ``pylayernorm_fwd`` (sum is None without), the
+    backward is ``pylayernorm_bwd``'s on ``rsigma`` and the row that was normalised.  ``ln_out``: a tensor like the input that receives the result
+    in its own type as well.  ``scale_rule``: see ``operators.mx.mx_quantise``."""
+    if ln_out is not None:
+        _lib.mark_written(ln_out)
+    if sum_out is not None:
+        _lib.mark_written(sum_out)
+    (codes, scales, rsigma, total), ms = issue(_host.rmsnorm_mx, stream, profiling, inp, ln_weight, eps, bool(zero_centered_gamma), residual,
+                                               sum_out, ln_out, _one_of("scale_rule", scale_rule, SCALE_RULES))
+    return MXTensor(codes, scales, codes.shape[0], ln_weight.numel(), "e4m3"), rsigma, total, ms
 
 
 def pylayernorm_bwd(d_ln_out, inp, mu, rsigma, ln_weight, bwd_sm_margin, zero_centered_gamma, stream,

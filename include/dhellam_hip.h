@@ -27,6 +27,7 @@ extern "C" {
 #endif
 
 typedef enum { DH_F32 = 0, DH_BF16 = 1, DH_F16 = 2 } dh_dtype;
+typedef enum { DH_MX_E4M3 = 0, DH_MX_E2M1 = 1 } dh_mx_format;
 
 typedef enum {
   DH_OK = 0,
@@ -39,7 +40,8 @@ typedef enum {
  * dh_norm_bwd and dh_moe_sort take the size of the caller's workspace and
  * check it (1.x trusted the caller); dh_grouped_gemm_nt / _nn take an optional
  * workspace.  2.1: dh_rotary, dh_balance_loss_fwd, dh_moe_route_bwd,
- * dh_distill_fwd and dh_distill_bwd. */
+ * dh_distill_fwd and dh_distill_bwd.  2.2: dh_mx_quantise, dh_rmsnorm_mx,
+ * dh_mx_gemm_nt, dh_grad_norm and dh_grad_clip. */
 int dh_version(void);
 /* Message of the last failing call on this thread ("" if none). */
 const char *dh_last_error(void);
@@ -667,6 +669,51 @@ int dh_masked_mean_fwd(const float *x, const float *mask, int64_t n, float scale
  * backpropagates a gradient of one). */
 int dh_masked_mean_bwd(const float *mask, const float *mask_sum, int64_t n, float scale,
                        float *grad, void *stream);
+
+/* ------------------------------------------------------------------------
+ * Microscaled floating point (the OCP MX formats; no counterpart in the reference): blocks of 32 elements along a row with one
+ * power of two as their scale, elements in e4m3 or e2m1 (dh_mx_format).  A matrix of rows x cols is held as
+ *   codes   [rows][kp] bytes (e4m3) or [rows][kp / 2] (e2m1, the even column in the low half), kp = cols rounded up to 128
+ *   scales  [kp / 128][cells][4][4] bytes, cells = rows / 4 rounded up: the exponent code e (2^(e - 127); 255: NaN) of columns
+ *           128 c + 32 i and on of row r is at [c][r / 4][i][r % 4]
+ * both 16-byte aligned, zeros behind cols and behind the last row.  A block that holds anything not finite gets 255 and zeros.
+ * ---------------------------------------------------------------------- */
+
+/* Quantises x (row stride ldx) along its rows (codes, scales) or along its columns (codes_t, scales_t: the transposed matrix,
+ * cols x rows), or both in one pass; the pair that is not wanted is NULL.  A scale is 2^(floor(log2 m) - 8) for e4m3 and
+ * - 2 for e2m1 with m the block's largest magnitude, so that the largest elements may saturate (448, 6); with `cover` the smallest
+ * power of two at which none does.  Elements are rounded to the nearest, ties to even. */
+int dh_mx_quantise(const void *x, int64_t rows, int64_t cols, int64_t ldx, int dtype, int format,
+                   int cover, void *codes, void *scales, void *codes_t, void *scales_t, void *stream);
+
+/* dh_norm_fwd as RMSNorm (dh_add_norm_fwd with a residual; sum_out may be x or residual) whose result is quantised to e4m3
+ * from its fp32 value.  y (may be NULL): the same result in `dtype` as well.  rsigma fp32 [rows].  cols <= 2^24. */
+int dh_rmsnorm_mx(const void *x, const void *residual, void *sum_out, const void *gamma, void *y,
+                  void *codes, void *scales, float *rsigma, int64_t rows, int64_t cols, float eps,
+                  int zero_centered_gamma, int cover, int dtype, void *stream);
+
+/* c[m, n] (+)= sum over k of a[m, k] b[n, k], both operands in the layout above along k, fp32 sums, c of out_dtype with row
+ * stride ldc; `accumulate` adds to what c holds, with one rounding.  k <= 2^22.  workspace (16-byte aligned, of the call's
+ * own) may be NULL when dh_mx_gemm_workspace_bytes is 0. */
+size_t dh_mx_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k);
+int dh_mx_gemm_nt(const void *a_codes, const void *a_scales, int a_format, const void *b_codes,
+                  const void *b_scales, int b_format, void *c, int64_t m, int64_t n, int64_t k,
+                  int64_t ldc, int out_dtype, int accumulate, void *workspace, size_t workspace_bytes,
+                  void *stream);
+
+/* The norm of many gradients together, and their clipping (no counterpart in the reference, whose optimiser is Megatron's).
+ * grads, counts, dtypes: host arrays of n tensors (any number, any sizes, 0 included).
+ * sum_sq[0] = sum of g^2 over all of them, in 64 bits, the same bits on every call; sums of several ranks add up.
+ * workspace: 8-byte aligned, of the call's own. */
+size_t dh_grad_norm_workspace_bytes(const int64_t *counts, int n);
+int dh_grad_norm(const void *const *grads, const int64_t *counts, const int *dtypes, int n,
+                 double *sum_sq, void *workspace, size_t workspace_bytes, void *stream);
+/* out[i] = factor grads[i] with norm = |scale| sqrt(sum_sq), factor = scale min(1, max_norm / (norm + 1e-6)); where the norm is not
+ * finite the factor is 0 and zeros are written.  found (fp32 [2]): norm, factor.  out[i] is of the gradient's type or fp32, and
+ * grads[i] itself or a place of its own. */
+int dh_grad_clip(const void *const *grads, void *const *out, const int64_t *counts, const int *dtypes,
+                 const int *out_dtypes, int n, const double *sum_sq, double max_norm, double scale,
+                 float *found, void *stream);
 
 #ifdef __cplusplus
 }
