@@ -1303,7 +1303,7 @@ Tensor mx_gemm_nt(const Tensor &a, const Tensor &as, int64_t m, int64_t fa_, con
             "mx_gemm_nt: out must be [m, n] with unit inner stride");
   Tensor c = out.has_value() ? *out : at::empty({m, n}, a.options().dtype(out_dtype));
   const int type = dt(c);
-  const int64_t bytes = (int64_t)dh_mx_gemm_workspace_bytes(m, n, k);
+  const int64_t bytes = (int64_t)dh_mx_gemm_workspace_bytes(m, n, k, fa, fb, type);
   Tensor ws;                           // of this call alone, so that calls and captured graphs that overlap share none
   if (bytes) ws = at::empty({bytes}, a.options());
   launch([&] {

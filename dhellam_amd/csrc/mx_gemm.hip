@@ -13,6 +13,7 @@
 // rounded to 2^-9 (2^-12), far above that.  A result in fp32 is promised to 1e-5 everywhere else in this library, so with an 8-bit
 // operand it is formed from the elements in bf16, which hold them and their scales exactly (mx_wide below).
 #include <algorithm>
+#include <type_traits>
 
 #include "mma.h"
 #include "mx.h"
@@ -89,6 +90,21 @@ template <int BITS> __device__ __forceinline__ MxWide<BITS> mx_wide(const MxFrag
     }
   }
   return o;
+}
+
+// The same instruction as assembly whose sum stays in its registers: with the builtin the compiler moved accumulators about and ran out
+// of registers in mx_w8_kernel.  It does not know these for matrix instructions: what reads a sum waits first.
+template <int FA, int FB, int SELB, int SELA, typename VB, typename VA>
+__device__ __forceinline__ void mx_mma_tied(const VB &b, uint32_t sb, const VA &a, uint32_t sa, floatx4 &c) {
+#ifdef __HIP_DEVICE_COMPILE__                                       // (the host's compiler has no registers for such operands)
+  asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%c5,%c6,0] op_sel_hi:[%c7,%c8,0] cbsz:%c9 blgp:%c10"
+               : "+v"(c)
+               : "v"(b), "v"(a), "v"(sb), "v"(sa), "n"(SELB & 1), "n"(SELA & 1), "n"(SELB >> 1), "n"(SELA >> 1), "n"(FB == 8 ? 0 : 4), "n"(FA == 8 ? 0 : 4));
+#endif
+}
+template <int BITS> __device__ __forceinline__ auto mx_narrow(const int4v *q, int ks) {
+  if constexpr (BITS == 8) return mx_v8i{q[0][0], q[0][1], q[0][2], q[0][3], q[1][0], q[1][1], q[1][2], q[1][3]};
+  else return q[ks];
 }
 
 // c's element: added to if asked, rounded once.
@@ -221,6 +237,260 @@ __global__ void __launch_bounds__(64 * W) mx_direct_kernel(const MxGemmParams p)
   }
 }
 
+// ---- 256 x 256 tiles: eight wavefronts in two alternating groups -------------------------------------------------------------
+// The schedule of grouped_gemm_w8_kernel (grouped_gemm.hip, where its order of reads, waits, copies and barriers is argued): a wavefront has
+// 128 x 64 outputs in four quarters, a quarter of a slice is [reads of fragments, copies | its MFMAs, more reads among them],
+// and the wavefronts 4..7 run one barrier behind the others.  A slice is 128 bytes of a row here too: 256 columns where both operands have
+// 4 bits (two steps of 128, 16 MFMAs of 16 cycles in a quarter), 128 columns otherwise (8 MFMAs of 32 cycles; a 4-bit operand's rows
+// then have 64 bytes).
+//
+// LDS: regions of [128 slots][row bytes] for either half of the tile's rows of a and of b, two stages of them, and the scales in a ring
+// of three.  A slot holds row 64 (s / 64) + 4 (s % 16) + s / 16 % 4 of a's half, row 32 (s / 32) + 2 (s % 16) + s / 16 % 2 of b's, so that
+// the four (two) blocks a lane multiplies are neighbouring rows: their scales are one dword (half of one) of a cell, and a lane's
+// outputs are 8 neighbouring columns.  16-byte chunks are XORed with (slot / 2) % 8, in rows of 64 bytes with (slot / 4) % 4: the 16 lanes of a
+// fragment read hit 16 different chunks of 256 bytes.  Scales come as whole cells, 256 bytes a copy.
+// Scales follow their fragments: those of the half that is read next lie in LDS since the wait two clusters before, and a slot of the
+// ring is written again three slices later, long after its last read.
+// 64 lanes x 4 bytes, as copy_1k
+__device__ __forceinline__ void copy_256(uint32_t lane_off, const int4v &rsrc, uint32_t off, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dword %0, %1, %2 offen lds"
+               :
+               : "v"(lane_off), "s"(rsrc), "s"(off), "s"(dst)
+               : "memory", "m0");
+}
+
+template <int FA, int FB, typename TO>
+__global__ void __launch_bounds__(512) mx_w8_kernel(const MxGemmParams p) {
+  constexpr int KS = FA == 4 && FB == 4 ? 2 : 1;                 // steps of 128 columns in a slice
+  constexpr int RA = KS * MxBytes<FA>::STEP, RB = KS * MxBytes<FB>::STEP;      // bytes of a row in a slice
+  constexpr int NA = RA / 64, NB = RB / 64;                      // copies a wavefront issues for a region; 16-byte reads a fragment takes
+  constexpr uint32_t REGA = 128 * RA, REGB = 128 * RB, OFF_B = 2 * REGA, STAGEB = OFF_B + 2 * REGB;
+  constexpr uint32_t RING = 2 * STAGEB, SLOT = KS * 2048;        // scales of a slice: a's, then b's
+  constexpr int COPIES = KS + 2 * NA + 2 * NB;                   // of a wavefront a slice
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[RING + 3 * SLOT];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = w >> 2, wn = w & 3;
+  const int c = lane & 15, g4 = lane >> 4;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)smem;
+  const uint32_t lda = (uint32_t)p.steps * MxBytes<FA>::STEP, ldb = (uint32_t)p.steps * MxBytes<FB>::STEP;
+
+  // ---- copies: a region is blocks of 1 KB, 8 slots of 128 bytes or 16 of 64; a wavefront takes NA (NB) neighbouring ones
+  uint32_t ca[NA], cb[NB];
+#pragma unroll
+  for (int x = 0; x < NA; ++x) {
+    const int s = NA == 2 ? 8 * (2 * w + x) + (lane >> 3) : 16 * w + (lane >> 2);
+    const int chunk = NA == 2 ? (lane & 7) ^ ((s >> 1) & 7) : (lane & 3) ^ ((s >> 2) & 3);
+    ca[x] = (uint32_t)(64 * (s >> 6) + 4 * (s & 15) + ((s >> 4) & 3)) * lda + (uint32_t)(chunk * 16);
+  }
+#pragma unroll
+  for (int x = 0; x < NB; ++x) {
+    const int s = NB == 2 ? 8 * (2 * w + x) + (lane >> 3) : 16 * w + (lane >> 2);
+    const int chunk = NB == 2 ? (lane & 7) ^ ((s >> 1) & 7) : (lane & 3) ^ ((s >> 2) & 3);
+    cb[x] = (uint32_t)(32 * (s >> 5) + 2 * (s & 15) + ((s >> 4) & 1)) * ldb + (uint32_t)(chunk * 16);
+  }
+  const uint32_t cs = (uint32_t)(lane * 4);
+
+  // ---- fragments and scales
+  const uint32_t fa_lane = (uint32_t)((wm * 64 + c) * RA + (NA == 2 ? (g4 ^ ((c >> 1) & 7)) : (g4 ^ (c >> 2))) * 16);   // chunk 4 + g4: XOR 64; block: + 16 RA
+  const uint32_t fb_lane = (uint32_t)((wn * 32 + c) * RB + (NB == 2 ? (g4 ^ ((c >> 1) & 7)) : (g4 ^ (c >> 2))) * 16);
+  const uint32_t sa_lane = (uint32_t)(wm * 256 + c * 16 + g4 * 4);                              // half: + 512; step: + 1024
+  const uint32_t sb_lane = (uint32_t)(KS * 1024 + wn * 128 + (c >> 1) * 16 + g4 * 4 + 2 * (c & 1));
+  typedef __attribute__((address_space(3))) const int4v *lds_chunk;
+  typedef __attribute__((address_space(3))) const uint32_t *lds_dword;
+  typedef __attribute__((address_space(3))) const uint16_t *lds_half;
+
+  const int pid = gg_xcd_chunk((int)blockIdx.x, p.tiles_m * p.tiles_n), piece = blockIdx.y;
+  int tm, tn;
+  gg_tile_of(pid, p.tiles_m, p.tiles_n, tm, tn);
+  const int nsl = (p.steps + KS - 1) / KS;
+  const int s0 = (int)((int64_t)piece * nsl / p.pieces), cnt = (int)((int64_t)(piece + 1) * nsl / p.pieces) - s0;
+  const int64_t m0 = (int64_t)tm * 256, n0 = (int64_t)tn * 256;
+  // descriptors, cut at the operands' last rows: rows past them read as zeros
+  int4v rsa = raw_rsrc(p.a + m0 * lda, std::min<int64_t>(p.m - m0, 256) * lda), rsb = raw_rsrc(p.b + n0 * ldb, std::min<int64_t>(p.n - n0, 256) * ldb);
+  // (of the scales: a's and b's, where one copy a wavefront does, the one the wavefront copies)
+  const bool sb_first = KS == 1 && w >= 4;
+  int4v rss0 = raw_rsrc(sb_first ? p.bs + n0 * 4 : p.as + m0 * 4, sb_first ? (int64_t)p.steps * p.cells_b * 16 - n0 * 4 : (int64_t)p.steps * p.cells_a * 16 - m0 * 4);
+  int4v rss1 = raw_rsrc(p.bs + n0 * 4, (int64_t)p.steps * p.cells_b * 16 - n0 * 4);
+  const uint32_t gs0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)((sb_first ? p.cells_b : p.cells_a) * 16)), gs1 = (uint32_t)p.cells_b * 16;
+  // they come out of v_readfirstlane, which the copies from assembly have to keep their distance from
+  asm volatile("s_nop 4" : "+s"(rsa), "+s"(rsb), "+s"(rss0), "+s"(rss1));
+
+  // before the copies of slice s (of this piece)
+  auto turn_to = [&](int s) {
+    if (s >= cnt) {
+      rsa[2] = rsb[2] = rss0[2] = rss1[2] = 0;
+    } else if (KS == 2 && (p.steps & 1) && s0 + s == nsl - 1) {
+      // the last step of an odd number: chunks 4..7 are not there
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int ch = (lane & 7) ^ (((8 * (2 * w + x) + (lane >> 3)) >> 1) & 7);
+        if (ch >= 4) ca[x % NA] = cb[x % NB] = 0x80000000u;      // past any descriptor's end
+      }
+    }
+  };
+  auto copy_a = [&](int h, int s, uint32_t stage) {
+#pragma unroll
+    for (int x = 0; x < NA; ++x)
+      copy_1k(ca[x], rsa, (uint32_t)(s0 + s) * RA + (uint32_t)h * 128 * lda, lds0 + stage + (uint32_t)h * REGA + (uint32_t)(NA * w + x) * 1024);
+  };
+  auto copy_b = [&](int h, int s, uint32_t stage) {
+#pragma unroll
+    for (int x = 0; x < NB; ++x)
+      copy_1k(cb[x], rsb, (uint32_t)(s0 + s) * RB + (uint32_t)h * 128 * ldb, lds0 + stage + OFF_B + (uint32_t)h * REGB + (uint32_t)(NB * w + x) * 1024);
+  };
+  auto copy_s = [&](int s, uint32_t slot) {
+    const uint32_t at = lds0 + slot, quarter = (uint32_t)(w & 3) * 256, to = (uint32_t)(w >> 2) * 1024 + quarter;
+    if constexpr (KS == 2) {
+      const uint32_t step = (uint32_t)(2 * (s0 + s) + (w >> 2));
+      copy_256(cs, rss0, step * gs0 + quarter, at + to);
+      copy_256(cs, rss1, step * gs1 + quarter, at + 2048 + to);
+    } else {
+      copy_256(cs, rss0, (uint32_t)(s0 + s) * gs0 + quarter, at + to);
+    }
+  };
+  floatx4 acc[2][2][4][2];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) acc[i >> 4][(i >> 3) & 1][(i >> 1) & 3][i & 1] = floatx4{0.f, 0.f, 0.f, 0.f};
+  int4v fa[2][4][NA], fb[2][2][NB];
+  uint32_t sa[2][KS], sb[2][KS];
+  auto mma_quarter = [&](int qm, int qn, auto rd) {
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int x = 0; x < 8 * KS; ++x) {
+      const int ks = x >> 3, mi = (x >> 1) & 3, nj = x & 1;
+      const auto vb = mx_narrow<FB>(fb[qn][nj], ks);
+      const auto va = mx_narrow<FA>(fa[qm][mi], ks);
+      floatx4 &sum = acc[qm][qn][mi][nj];
+#define MX_SEL(j, i) if (nj == j && mi == i) mx_mma_tied<FA, FB, j, i>(vb, sb[qn][ks], va, sa[qm][ks], sum)
+      MX_SEL(0, 0); MX_SEL(0, 1); MX_SEL(0, 2); MX_SEL(0, 3);
+      MX_SEL(1, 0); MX_SEL(1, 1); MX_SEL(1, 2); MX_SEL(1, 3);
+#undef MX_SEL
+      if (x % KS == KS - 1) {
+        __builtin_amdgcn_sched_barrier(0);
+        rd(x / KS);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    __builtin_amdgcn_s_setprio(0);
+  };
+  auto read_a = [&](int h, uint32_t region, int x0, int x1) {    // reads x0..x1 of the half's 4 NA
+#pragma unroll
+    for (int x = x0; x < x1; ++x)
+      if (x < 4 * NA) fa[h][x & 3][x >> 2] = *(lds_chunk)(region + (fa_lane ^ (uint32_t)((x >> 2) << 6)) + (uint32_t)((x & 3) * 16 * RA));
+  };
+  auto read_b = [&](int h, uint32_t region, uint32_t slot) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int nj = 0; nj < 2; ++nj) fb[h][nj][i] = *(lds_chunk)(region + (fb_lane ^ (uint32_t)(i << 6)) + (uint32_t)(nj * 16 * RB));
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) sb[h][ks] = *(lds_half)(lds0 + slot + sb_lane + (uint32_t)(h * 512 + ks * 1024));
+  };
+  auto read_sa = [&](int h, uint32_t slot) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) sa[h][ks] = *(lds_dword)(lds0 + slot + sa_lane + (uint32_t)(h * 512 + ks * 1024));
+  };
+#define MX_BARRIER()                        \
+  do {                                      \
+    __builtin_amdgcn_sched_barrier(0);      \
+    asm volatile("s_barrier" ::: "memory"); \
+    __builtin_amdgcn_sched_barrier(0);      \
+  } while (0)
+#define MX_READS_DONE() asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory")
+#define MX_WAIT_BARRIER()                                                              \
+  do {                                                                                 \
+    __builtin_amdgcn_sched_barrier(0);                                                 \
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(COPIES) : "memory");         \
+    __builtin_amdgcn_sched_barrier(0);                                                 \
+  } while (0)
+
+  uint32_t r0 = RING, r1 = RING + SLOT, r2 = RING + 2 * SLOT;    // the ring's slots of slices s, s + 1, s + 2
+  turn_to(0);
+  copy_s(0, r0); copy_a(0, 0, 0); copy_b(0, 0, 0); copy_b(1, 0, 0); copy_a(1, 0, 0);
+  turn_to(1);
+  copy_s(1, r1); copy_a(0, 1, STAGEB); copy_b(1, 1, STAGEB); copy_b(0, 1, STAGEB); copy_a(1, 1, STAGEB);
+  MX_WAIT_BARRIER();
+  if (w >= 4) MX_BARRIER();
+  read_a(0, lds0, 0, 8);
+  read_sa(0, r0);
+  read_b(0, lds0 + OFF_B, r0);
+  uint32_t cur = 0;
+  auto slice = [&](auto fc, int s) {
+    constexpr int F = decltype(fc)::value, G = F ^ 1;            // the half of b that is multiplied first (s % 2), and the other
+    const uint32_t nxt = STAGEB - cur, a0 = lds0 + cur, b0 = a0 + OFF_B, na = lds0 + nxt, nb = na + OFF_B;
+    turn_to(s + 2);
+    MX_READS_DONE();
+    read_b(G, b0 + G * REGB, r0);
+    MX_BARRIER();
+    mma_quarter(0, F, [&](int x) { if (x < 3) read_a(1, a0 + REGA, x, x + 1); });
+    MX_BARRIER();
+    MX_READS_DONE();
+    read_a(1, a0 + REGA, 3, 6);
+    read_sa(1, r0);
+    copy_s(s + 2, r2);
+    copy_a(0, s + 2, cur);
+    MX_WAIT_BARRIER();
+    mma_quarter(0, G, [&](int x) { if (x < 2) read_a(1, a0 + REGA, 6 + x, 7 + x); });
+    MX_BARRIER();
+    MX_READS_DONE();
+    read_a(0, na, 0, 3);
+    read_sa(0, r1);
+    copy_b(F, s + 2, cur);
+    MX_WAIT_BARRIER();
+    mma_quarter(1, G, [&](int x) { if (x < 3) read_a(0, na, 3 + x, 4 + x); });
+    MX_BARRIER();
+    MX_READS_DONE();
+    read_b(G, nb + G * REGB, r1);
+    copy_b(G, s + 2, cur);
+    copy_a(1, s + 2, cur);
+    MX_WAIT_BARRIER();
+    mma_quarter(1, F, [&](int x) { if (x < 2) read_a(0, na, 6 + x, 7 + x); });
+    MX_BARRIER();
+    cur = nxt;
+    const uint32_t r = r0;
+    r0 = r1;
+    r1 = r2;
+    r2 = r;
+  };
+  int s = 0;
+#pragma unroll 1
+  for (; s + 1 < cnt; s += 2) {
+    slice(std::integral_constant<int, 0>{}, s);
+    slice(std::integral_constant<int, 1>{}, s + 1);
+  }
+  if (s < cnt) slice(std::integral_constant<int, 0>{}, s);
+  if (w < 4) MX_BARRIER();
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");               // the last copies have landed before the workgroup gives its LDS back
+
+  // the last sums are there: 16 passes of 4 cycles behind the last instruction at most, and nothing reads them before
+  asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) asm volatile("" : "+v"(acc[i >> 4][(i >> 3) & 1][(i >> 1) & 3][i & 1]));
+  // a lane's 8 columns 8 g4 .. of row 4 c + mi of a quarter's 64 rows x 32 columns
+#pragma unroll
+  for (int qm = 0; qm < 2; ++qm)
+#pragma unroll
+    for (int mi = 0; mi < 4; ++mi) {
+      const int64_t row = m0 + 128 * qm + 64 * wm + 4 * c + mi;
+      if (row >= p.m) continue;
+#pragma unroll
+      for (int qn = 0; qn < 2; ++qn) {
+        const int64_t col = n0 + 128 * qn + 32 * wn + 8 * g4;
+        if (col >= p.n) continue;
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = acc[qm][qn][mi][i & 1][i >> 1];
+        if (p.pieces > 1) mx_store<float, 8>(p.ws + ((int64_t)piece * p.m + row) * (4 * p.cells_b) + col, v, 4 * p.cells_b - col, 1, 0);
+        else mx_store<TO, 8>(reinterpret_cast<TO *>(p.c) + row * p.ldc + col, v, p.n - col, p.vec, p.accumulate);
+      }
+    }
+#undef MX_BARRIER
+#undef MX_READS_DONE
+#undef MX_WAIT_BARRIER
+}
+
 // c (+)= the pieces' sums, in order; a thread 4 columns.
 template <typename TO> __global__ void __launch_bounds__(256) mx_join_kernel(const MxGemmParams p) {
   const int64_t groups = p.cells_b, u = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -243,9 +513,16 @@ template <typename TO> __global__ void __launch_bounds__(256) mx_zero_kernel(con
 
 constexpr int MX_MAX_PIECES = 16;
 
-// Which form of mx_direct_kernel a product takes.
+// Which kernel a product takes: mt of 0 is mx_w8_kernel.
 struct MxPlan { int mt, nt, waves, pieces; };
-static MxPlan mx_plan(int64_t m, int64_t n, int64_t steps) {
+static bool mx_wide_needed(int fa, int fb, int out) { return out == DH_F32 && (fa == DH_MX_E4M3 || fb == DH_MX_E4M3); }
+static MxPlan mx_plan(int64_t m, int64_t n, int64_t steps, bool wide) {
+  const int64_t big = cdiv(m, 256) * cdiv(n, 256);
+  if (!wide && m > 128 && n > 128 && big >= 16) {
+    MxPlan q{0, 0, 8, 1};
+    if (big < 256) q.pieces = (int)std::max<int64_t>(1, std::min<int64_t>({256 / big, steps / 4, MX_MAX_PIECES}));
+    return q;
+  }
   MxPlan q{m <= 16 ? 1 : m <= 32 ? 2 : 4, m <= 16 ? 1 : 4, m <= 16 ? 8 : 4, 1};
   const int64_t tiles = cdiv(m, 16 * q.mt) * cdiv(n, 16 * q.nt);
   if (tiles < 256) q.pieces = (int)std::min<int64_t>({512 / std::max<int64_t>(tiles, 1), steps / q.waves, MX_MAX_PIECES});
@@ -254,12 +531,15 @@ static MxPlan mx_plan(int64_t m, int64_t n, int64_t steps) {
 }
 
 template <int FA, int FB, typename TO> static void mx_launch(MxGemmParams p, const MxPlan &q, hipStream_t st) {
-  p.tiles_m = (int)cdiv(p.m, 16 * q.mt);
-  p.tiles_n = (int)cdiv(p.n, 16 * q.nt);
+  constexpr bool WIDE = sizeof(TO) == 4 && (FA == 8 || FB == 8);
+  const int side_m = q.mt ? 16 * q.mt : 256, side_n = q.mt ? 16 * q.nt : 256;
+  p.tiles_m = (int)cdiv(p.m, side_m);
+  p.tiles_n = (int)cdiv(p.n, side_n);
   p.pieces = q.pieces;
   const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), (unsigned)q.pieces), block((unsigned)(64 * q.waves));
-  constexpr bool WIDE = sizeof(TO) == 4 && (FA == 8 || FB == 8);
-  if (q.mt == 1) hipLaunchKernelGGL((mx_direct_kernel<FA, FB, 1, 1, 8, WIDE, TO>), grid, block, 0, st, p);
+  if (q.mt == 0) {
+    if constexpr (!WIDE) hipLaunchKernelGGL((mx_w8_kernel<FA, FB, TO>), grid, block, 0, st, p);
+  } else if (q.mt == 1) hipLaunchKernelGGL((mx_direct_kernel<FA, FB, 1, 1, 8, WIDE, TO>), grid, block, 0, st, p);
   else if (q.mt == 2) hipLaunchKernelGGL((mx_direct_kernel<FA, FB, 2, 4, 4, WIDE, TO>), grid, block, 0, st, p);
   else hipLaunchKernelGGL((mx_direct_kernel<FA, FB, 4, 4, 4, WIDE, TO>), grid, block, 0, st, p);
   if (q.pieces > 1) hipLaunchKernelGGL((mx_join_kernel<TO>), dim3((unsigned)cdiv(p.m * p.cells_b, 256)), dim3(256), 0, st, p);
@@ -275,9 +555,9 @@ static int mx_gemm_sizes(int64_t m, int64_t n, int64_t k) {
   return DH_OK;
 }
 
-extern "C" size_t dh_mx_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k) {
+extern "C" size_t dh_mx_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k, int a_format, int b_format, int out_dtype) {
   if (m <= 0 || n <= 0 || k <= 0 || mx_gemm_sizes(m, n, k) != DH_OK) return 0;
-  const dh::MxPlan q = dh::mx_plan(m, n, dh::cdiv(k, 128));
+  const dh::MxPlan q = dh::mx_plan(m, n, dh::cdiv(k, 128), dh::mx_wide_needed(a_format, b_format, out_dtype));
   return q.pieces > 1 ? (size_t)q.pieces * (size_t)m * (size_t)dh::mx_rows4(n) * 4 : 0;
 }
 
@@ -309,10 +589,11 @@ extern "C" int dh_mx_gemm_nt(const void *a_codes, const void *a_scales, int a_fo
   p.a = (const uint8_t *)a_codes; p.as = (const uint8_t *)a_scales; p.b = (const uint8_t *)b_codes; p.bs = (const uint8_t *)b_scales;
   p.cells_a = mx_rows4(m) / 4; p.cells_b = mx_rows4(n) / 4; p.steps = (int)cdiv(k, 128);
   p.vec = aligned16(c) && ldc * (int64_t)dtype_size(out_dtype) % 16 == 0;
-  const MxPlan q = mx_plan(m, n, p.steps);
+  DH_CHECK(p.steps * std::max(p.cells_a, p.cells_b) * 16 < (1ll << 31), "scales of 2 GiB and more");
+  const MxPlan q = mx_plan(m, n, p.steps, mx_wide_needed(a_format, b_format, out_dtype));
   if (q.pieces > 1) {
-    DH_CHECK(workspace && aligned16(workspace) && workspace_bytes >= dh_mx_gemm_workspace_bytes(m, n, k), "workspace of %zu bytes, %zu are needed",
-             workspace_bytes, dh_mx_gemm_workspace_bytes(m, n, k));
+    const size_t need = dh_mx_gemm_workspace_bytes(m, n, k, a_format, b_format, out_dtype);
+    DH_CHECK(workspace && aligned16(workspace) && workspace_bytes >= need, "workspace of %zu bytes, %zu are needed", workspace_bytes, need);
     p.ws = (float *)workspace;
   }
 #define MX_FORMATS(TO)                                                                  \

@@ -695,7 +695,8 @@ int dh_rmsnorm_mx(const void *x, const void *residual, void *sum_out, const void
 /* c[m, n] (+)= sum over k of a[m, k] b[n, k], both operands in the layout above along k, fp32 sums, c of out_dtype with row
  * stride ldc; `accumulate` adds to what c holds, with one rounding.  k <= 2^22.  workspace (16-byte aligned, of the call's
  * own) may be NULL when dh_mx_gemm_workspace_bytes is 0. */
-size_t dh_mx_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k);
+size_t dh_mx_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k, int a_format, int b_format,
+                                  int out_dtype);
 int dh_mx_gemm_nt(const void *a_codes, const void *a_scales, int a_format, const void *b_codes,
                   const void *b_scales, int b_format, void *c, int64_t m, int64_t n, int64_t k,
                   int64_t ldc, int out_dtype, int accumulate, void *workspace, size_t workspace_bytes,

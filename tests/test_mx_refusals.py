@@ -75,8 +75,9 @@ def test_product_refusals():
     _refused(call(a=None), "null")
     _refused(call(sb=None), "null")
     _refused(call(b=P + 8), "aligned")
-    need = lib.dh_mx_gemm_workspace_bytes(1, 64, 1 << 16)
-    assert need > 0 and lib.dh_mx_gemm_workspace_bytes(0, 8, 8) == 0 and lib.dh_mx_gemm_workspace_bytes(-1, 8, 8) == 0
+    _refused(call(m=1 << 30, k=1 << 12), "2 GiB")
+    need = lib.dh_mx_gemm_workspace_bytes(1, 64, 1 << 16, 0, 1, 1)
+    assert need > 0 and lib.dh_mx_gemm_workspace_bytes(0, 8, 8, 0, 1, 1) == 0 and lib.dh_mx_gemm_workspace_bytes(-1, 8, 8, 0, 1, 1) == 0
     _refused(call(m=1, n=64, k=1 << 16), "workspace")
     _refused(call(m=1, n=64, k=1 << 16, ws=P, wsb=need - 1), "workspace")
     assert call(m=0, c=None) == 0 and call(n=0, c=None, ldc=0) == 0
