@@ -13,6 +13,7 @@
 // rounded to 2^-9 (2^-12), far above that.  A result in fp32 is promised to 1e-5 everywhere else in this library, so with an 8-bit
 // operand it is formed from the elements in bf16, which hold them and their scales exactly (mx_wide below).
 #include <algorithm>
+#include <cstdlib>
 #include <type_traits>
 
 #include "mma.h"
@@ -143,21 +144,31 @@ template <typename TO, int N> __device__ __forceinline__ void mx_store(TO *p, co
 // after the other, and add up through LDS in the order of the wavefronts.  Operand block i of MT (NT) takes the rows MT r + i, so that
 // the scales of a lane's blocks lie side by side.  Where even so there are few workgroups, k is cut into pieces over workgroups as
 // well, and mx_join_kernel adds these in order.
-template <int NB> __device__ __forceinline__ uint32_t mx_scales(const uint8_t *cell_row, int64_t row, int g) {
-  const uint8_t *p = cell_row + (row >> 2) * 16 + g * 4 + (row & 3);
+// Step x of the P that a wavefront takes at a time.  With P of 2 the two steps' eight blocks are dealt out so that a lane's block of step x is
+// block 2 g + x of them: its 4-bit elements of both steps are 32 consecutive bytes, a row's 128.
+template <int BITS, int P, bool WIDE> __device__ __forceinline__ void mx_load(MxFrag<BITS> &f, const uint8_t *row, int g, int x) {
+  if constexpr (BITS == 4) f.q[0] = *reinterpret_cast<const int4v *>(row + (P * g + x) * 16);
+  else
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      // (the instruction's 8-bit lane has the half g % 2 of blocks g / 2 and 2 + g / 2)
+      const int block = WIDE ? P * g + x : P * (2 * i + (g >> 1)) + x, half = WIDE ? i : g & 1;
+      f.q[i] = *reinterpret_cast<const int4v *>(row + block * 32 + half * 16);
+    }
+}
+// The scales of a lane's block of step x, NB rows from `row` on; cells: from the unit's first group of 128 columns on.
+template <int NB, int P> __device__ __forceinline__ uint32_t mx_scales(const uint8_t *s, int64_t cells, int64_t row, int g, int x) {
+  const int block = P * g + x;
+  const uint8_t *p = s + (block >> 2) * cells * 16 + (row >> 2) * 16 + (block & 3) * 4 + (row & 3);
   if constexpr (NB == 4) return *reinterpret_cast<const uint32_t *>(p);
   else if constexpr (NB == 2) return *reinterpret_cast<const uint16_t *>(p);
   else return *p;
 }
 
-template <int BITS, bool WIDE> __device__ __forceinline__ void mx_load(MxFrag<BITS> &f, const uint8_t *row, int g) {
-#pragma unroll
-  for (int i = 0; i < BITS / 4; ++i) f.q[i] = *reinterpret_cast<const int4v *>(row + (WIDE ? 16 * i + 4 * BITS * g : 64 * i + 16 * g));
-}
-
 template <int FA, int FB, int MT, int NT, int W, bool WIDE, typename TO>
 __global__ void __launch_bounds__(64 * W) mx_direct_kernel(const MxGemmParams p) {
   constexpr int TM = 16 * MT, TN = 16 * NT, PITCH = TN + 4;
+  constexpr int P = FB == 4 ? 2 : 1;
   __shared__ __attribute__((aligned(16))) float red[W * TM * PITCH];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int r = lane & 15, g = lane >> 4;
@@ -177,35 +188,52 @@ __global__ void __launch_bounds__(64 * W) mx_direct_kernel(const MxGemmParams p)
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
-  const int s0 = (int)((int64_t)piece * p.steps / p.pieces), s1 = (int)((int64_t)(piece + 1) * p.steps / p.pieces);
-#pragma unroll 2
-  for (int s = s0 + w; s < s1; s += W) {
-    MxFrag<FA> fa[MT];
-    MxFrag<FB> fb[NT];
+  // U steps from s on
+  auto unit = [&](auto u_, int64_t s) {
+    constexpr int U = decltype(u_)::value;
+    MxFrag<FA> fa[U][MT];
+    MxFrag<FB> fb[U][NT];
+    uint32_t sa[U], sb[U];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) mx_load<FB, WIDE>(fb[j], bp[j] + (int64_t)s * MxBytes<FB>::STEP, g);
+    for (int x = 0; x < U; ++x) {
 #pragma unroll
-    for (int i = 0; i < MT; ++i) mx_load<FA, WIDE>(fa[i], ap[i] + (int64_t)s * MxBytes<FA>::STEP, g);
-    const uint32_t sb = mx_scales<NT>(p.bs + (int64_t)s * p.cells_b * 16, srb, g);
-    const uint32_t sa = mx_scales<MT>(p.as + (int64_t)s * p.cells_a * 16, sra, g);
-    if constexpr (WIDE) {
-      MxWide<FB> wb[NT];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) wb[j] = mx_wide<FB>(fb[j], mx_scale_value(sb >> (8 * j) & 0xffu));
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const MxWide<FA> wa = mx_wide<FA>(fa[i], mx_scale_value(sa >> (8 * i) & 0xffu));
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int j = 0; j < NT; ++j) acc[i][j] = Mma<bf16_t>::mma16(wb[j].v[t], wa.v[t], acc[i][j]);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = mx_mma_sel<FA, FB>(j, i, fb[j], sb, fa[i], sa, acc[i][j]);
+      for (int j = 0; j < NT; ++j) mx_load<FB, U, WIDE>(fb[x][j], bp[j] + s * MxBytes<FB>::STEP, g, x);
+      sb[x] = mx_scales<NT, U>(p.bs + s * p.cells_b * 16, p.cells_b, srb, g, x);
     }
+#pragma unroll
+    for (int x = 0; x < U; ++x) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) mx_load<FA, U, WIDE>(fa[x][i], ap[i] + s * MxBytes<FA>::STEP, g, x);
+      sa[x] = mx_scales<MT, U>(p.as + s * p.cells_a * 16, p.cells_a, sra, g, x);
+    }
+#pragma unroll
+    for (int x = 0; x < U; ++x) {
+      if constexpr (WIDE) {
+        MxWide<FB> wb[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) wb[j] = mx_wide<FB>(fb[x][j], mx_scale_value(sb[x] >> (8 * j) & 0xffu));
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const MxWide<FA> wa = mx_wide<FA>(fa[x][i], mx_scale_value(sa[x] >> (8 * i) & 0xffu));
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[i][j] = Mma<bf16_t>::mma16(wb[j].v[e], wa.v[e], acc[i][j]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) acc[i][j] = mx_mma_sel<FA, FB>(j, i, fb[x][j], sb[x], fa[x][i], sa[x], acc[i][j]);
+      }
+    }
+  };
+  // the piece's units, one wavefront after the other; an odd last step is a unit of its own
+  const int units = (p.steps + P - 1) / P;
+  const int u0 = (int)((int64_t)piece * units / p.pieces), u1 = (int)((int64_t)(piece + 1) * units / p.pieces);
+  for (int u = u0 + w; u < u1; u += W) {
+    if (P == 2 && 2 * u + 1 == p.steps) unit(std::integral_constant<int, 1>{}, 2 * u);
+    else unit(std::integral_constant<int, P>{}, (int64_t)P * u);
   }
   // D[row = 4 g + v] of block j is column NT (4 g + v) + j, its column r row MT r + i
   float *mine = red + w * TM * PITCH;
@@ -491,6 +519,188 @@ __global__ void __launch_bounds__(512) mx_w8_kernel(const MxGemmParams p) {
 #undef MX_WAIT_BARRIER
 }
 
+// ---- 128 x 128 tiles: four wavefronts of 64 x 64 outputs, one on a SIMD ------------------------------------------------------
+// For products of fewer than a round of 256 x 256 tiles.  Four stages of LDS; the fragments of slice s + 1 are read among the matrix
+// instructions of slice s, into the other of two sets of registers, and the copies of slice s + 4 go out meanwhile.  One barrier a slice:
+// a wavefront passes it when its reads of slice s are in registers, so the stage of slice s may be written again, and when its own copies
+// of slice s + 1 have landed (those of s + 2 and s + 3 stay in flight), so that slice may be read.
+// Both operands' slots hold row 64 (s / 64) + 4 (s % 16) + s / 16 % 4: four blocks' scales are one dword, and a lane's outputs 16 neighbouring
+// columns of four rows.
+template <int FA, int FB, int STAGES, bool WIDE, typename TO>
+__global__ void __launch_bounds__(256, STAGES == 2 ? 2 : 1) mx_t128_kernel(const MxGemmParams p) {
+  constexpr int KS = FA == 4 && FB == 4 ? 2 : 1;
+  constexpr int RA = KS * MxBytes<FA>::STEP, RB = KS * MxBytes<FB>::STEP, NA = RA / 64, NB = RB / 64;
+  constexpr uint32_t REGA = 128 * RA, REGB = 128 * RB, OFF_S = REGA + REGB, STAGEB = OFF_S + KS * 1024;
+  constexpr int COPIES = KS + 2 * NA + 2 * NB;      // of a wavefront a slice
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[STAGES * STAGEB];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = w >> 1, wn = w & 1;
+  const int c = lane & 15, g4 = lane >> 4;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)smem;
+  const uint32_t lda = (uint32_t)p.steps * MxBytes<FA>::STEP, ldb = (uint32_t)p.steps * MxBytes<FB>::STEP;
+  uint32_t ca[2 * NA], cb[2 * NB];
+#pragma unroll
+  for (int x = 0; x < 2 * NA; ++x) {
+    const int s = NA == 2 ? 8 * (4 * w + x) + (lane >> 3) : 16 * (2 * w + x) + (lane >> 2);
+    const int chunk = NA == 2 ? (lane & 7) ^ ((s >> 1) & 7) : (lane & 3) ^ ((s >> 2) & 3);
+    ca[x] = (uint32_t)(64 * (s >> 6) + 4 * (s & 15) + ((s >> 4) & 3)) * lda + (uint32_t)(chunk * 16);
+  }
+#pragma unroll
+  for (int x = 0; x < 2 * NB; ++x) {
+    const int s = NB == 2 ? 8 * (4 * w + x) + (lane >> 3) : 16 * (2 * w + x) + (lane >> 2);
+    const int chunk = NB == 2 ? (lane & 7) ^ ((s >> 1) & 7) : (lane & 3) ^ ((s >> 2) & 3);
+    cb[x] = (uint32_t)(64 * (s >> 6) + 4 * (s & 15) + ((s >> 4) & 3)) * ldb + (uint32_t)(chunk * 16);
+  }
+  // chunk of a fragment's first 16 bytes, and what leads to its second 16: 4 chunks on, in bf16 (a lane takes block g4) the next one
+  const uint32_t qa = NA == 2 ? (WIDE ? 2 * g4 : g4) ^ ((c >> 1) & 7) : g4 ^ (c >> 2), qb = NB == 2 ? (WIDE ? 2 * g4 : g4) ^ ((c >> 1) & 7) : g4 ^ (c >> 2);
+  constexpr uint32_t SECOND = WIDE ? 16 : 64;
+  const uint32_t fa_lane = (uint32_t)((wm * 64 + c) * RA) + qa * 16;
+  const uint32_t fb_lane = REGA + (uint32_t)((wn * 64 + c) * RB) + qb * 16;
+  // scales of a slice: [step][a's 512 bytes, b's]
+  const uint32_t sa_lane = OFF_S + (uint32_t)(wm * 256 + c * 16 + g4 * 4), sb_lane = OFF_S + (uint32_t)(512 + wn * 256 + c * 16 + g4 * 4);
+  typedef __attribute__((address_space(3))) const int4v *lds_chunk;
+  typedef __attribute__((address_space(3))) const uint32_t *lds_dword;
+
+  const int pid = gg_xcd_chunk((int)blockIdx.x, p.tiles_m * p.tiles_n), piece = blockIdx.y;
+  int tm, tn;
+  gg_tile_of(pid, p.tiles_m, p.tiles_n, tm, tn);
+  const int nsl = (p.steps + KS - 1) / KS;
+  const int s0 = (int)((int64_t)piece * nsl / p.pieces), cnt = (int)((int64_t)(piece + 1) * nsl / p.pieces) - s0;
+  const int64_t m0 = (int64_t)tm * 128, n0 = (int64_t)tn * 128;
+  int4v rsa = raw_rsrc(p.a + m0 * lda, std::min<int64_t>(p.m - m0, 128) * lda), rsb = raw_rsrc(p.b + n0 * ldb, std::min<int64_t>(p.n - n0, 128) * ldb);
+  // a wavefront copies scales of one operand: 256 bytes of a step
+  const bool of_b = w >= 2;
+  int4v rss = raw_rsrc(of_b ? p.bs + n0 * 4 : p.as + m0 * 4, of_b ? (int64_t)p.steps * p.cells_b * 16 - n0 * 4 : (int64_t)p.steps * p.cells_a * 16 - m0 * 4);
+  const uint32_t gs = (uint32_t)__builtin_amdgcn_readfirstlane((int)((of_b ? p.cells_b : p.cells_a) * 16));
+  asm volatile("s_nop 4" : "+s"(rsa), "+s"(rsb), "+s"(rss));
+  auto turn_to = [&](int s) {
+    if (s >= cnt) {
+      rsa[2] = rsb[2] = rss[2] = 0;
+    } else if (KS == 2 && (p.steps & 1) && s0 + s == nsl - 1) {      // chunks 4..7 are not there
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int ch = (lane & 7) ^ (((8 * (4 * w + x) + (lane >> 3)) >> 1) & 7);
+        if (ch >= 4) ca[x % (2 * NA)] = cb[x % (2 * NB)] = 0x80000000u;
+      }
+    }
+  };
+  auto copy = [&](int s, uint32_t stage) {
+    const uint32_t at = lds0 + stage;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+      copy_256((uint32_t)(lane * 4), rss, (uint32_t)(KS * (s0 + s) + ks) * gs + (uint32_t)(w & 1) * 256, at + OFF_S + (uint32_t)(ks * 1024 + w * 256));
+#pragma unroll
+    for (int x = 0; x < 2 * NA; ++x) copy_1k(ca[x], rsa, (uint32_t)(s0 + s) * RA, at + (uint32_t)(2 * NA * w + x) * 1024);
+#pragma unroll
+    for (int x = 0; x < 2 * NB; ++x) copy_1k(cb[x], rsb, (uint32_t)(s0 + s) * RB, at + REGA + (uint32_t)(2 * NB * w + x) * 1024);
+  };
+  floatx4 acc[4][4];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) acc[i >> 2][i & 3] = floatx4{0.f, 0.f, 0.f, 0.f};
+  int4v fa[2][4][NA], fb[2][4][NB];
+  uint32_t sa[2][KS], sb[2][KS];
+  constexpr int READS = 2 * KS + 4 * NA + 4 * NB;
+  auto read = [&](int set, uint32_t at, int x) {                // read x of READS: the scales, then step by step what is multiplied first
+    if (x < KS) sa[set][x] = *(lds_dword)(at + sa_lane + (uint32_t)(x * 1024));
+    else if (x < 2 * KS) sb[set][x - KS] = *(lds_dword)(at + sb_lane + (uint32_t)((x - KS) * 1024));
+    else if (x < 2 * KS + 4 * NB) {
+      const int y = x - 2 * KS;
+      fb[set][y & 3][y >> 2] = *(lds_chunk)(at + (fb_lane ^ (uint32_t)(y >> 2) * SECOND) + (uint32_t)((y & 3) * 16 * RB));
+    } else if (x < READS) {
+      const int y = x - 2 * KS - 4 * NB;
+      fa[set][y & 3][y >> 2] = *(lds_chunk)(at + (fa_lane ^ (uint32_t)(y >> 2) * SECOND) + (uint32_t)((y & 3) * 16 * RA));
+    }
+  };
+  uint32_t stage = 0;                                            // of slice s
+  auto after = [&](uint32_t st) { return st == (STAGES - 1) * STAGEB ? 0u : st + STAGEB; };
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s) {
+    turn_to(s);
+    copy(s, (uint32_t)s * STAGEB);
+  }
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((STAGES - 2) * COPIES) : "memory");
+#pragma unroll
+  for (int x = 0; x < READS; ++x) read(0, lds0, x);
+  turn_to(STAGES - 1);
+  copy(STAGES - 1, (STAGES - 1) * STAGEB);
+  auto slice = [&](auto set_, int s) {
+    constexpr int SET = decltype(set_)::value;
+    const uint32_t next = after(stage);
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((STAGES - 2) * COPIES) : "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    turn_to(s + STAGES);
+    copy(s + STAGES, stage);
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int x = 0; x < READS; ++x) read(SET ^ 1, lds0 + next, x);
+      MxWide<FB> wb[4];
+#pragma unroll
+      for (int nj = 0; nj < 4; ++nj) {
+        MxFrag<FB> f;
+#pragma unroll
+        for (int i = 0; i < NB; ++i) f.q[i] = fb[SET][nj][i];
+        wb[nj] = mx_wide<FB>(f, mx_scale_value(sb[SET][0] >> (8 * nj) & 0xffu));
+      }
+#pragma unroll
+      for (int mi = 0; mi < 4; ++mi) {
+        MxFrag<FA> f;
+#pragma unroll
+        for (int i = 0; i < NA; ++i) f.q[i] = fa[SET][mi][i];
+        const MxWide<FA> wa = mx_wide<FA>(f, mx_scale_value(sa[SET][0] >> (8 * mi) & 0xffu));
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int nj = 0; nj < 4; ++nj) acc[mi][nj] = Mma<bf16_t>::mma16(wb[nj].v[t], wa.v[t], acc[mi][nj]);
+      }
+      stage = next;
+      return;
+    }
+#pragma unroll
+    for (int x = 0; x < 16 * KS; ++x) {
+      const int ks = x >> 4, mi = (x >> 2) & 3, nj = x & 3;
+      const auto vb = mx_narrow<FB>(fb[SET][nj], ks);
+      const auto va = mx_narrow<FA>(fa[SET][mi], ks);
+      floatx4 &sum = acc[mi][nj];
+#define MX_SEL(j, i) if (nj == j && mi == i) mx_mma_tied<FA, FB, j, i>(vb, sb[SET][ks], va, sa[SET][ks], sum)
+      MX_SEL(0, 0); MX_SEL(0, 1); MX_SEL(0, 2); MX_SEL(0, 3);
+      MX_SEL(1, 0); MX_SEL(1, 1); MX_SEL(1, 2); MX_SEL(1, 3);
+      MX_SEL(2, 0); MX_SEL(2, 1); MX_SEL(2, 2); MX_SEL(2, 3);
+      MX_SEL(3, 0); MX_SEL(3, 1); MX_SEL(3, 2); MX_SEL(3, 3);
+#undef MX_SEL
+      __builtin_amdgcn_sched_barrier(0);
+      constexpr int PER = (READS + 16 * KS - 1) / (16 * KS);
+#pragma unroll
+      for (int y = 0; y < PER; ++y) read(SET ^ 1, lds0 + next, PER * x + y);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    stage = next;
+  };
+  int s = 0;
+#pragma unroll 1
+  for (; s + 1 < cnt; s += 2) {
+    slice(std::integral_constant<int, 0>{}, s);
+    slice(std::integral_constant<int, 1>{}, s + 1);
+  }
+  if (s < cnt) slice(std::integral_constant<int, 0>{}, s);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");               // the last copies have landed before the workgroup gives its LDS back
+  asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");             // and the last sums are there
+#pragma unroll
+  for (int i = 0; i < 16; ++i) asm volatile("" : "+v"(acc[i >> 2][i & 3]));
+#pragma unroll
+  for (int mi = 0; mi < 4; ++mi) {
+    const int64_t row = m0 + 64 * wm + 4 * c + mi, col = n0 + 64 * wn + 16 * g4;
+    if (row >= p.m || col >= p.n) continue;
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = acc[mi][i & 3][i >> 2];
+    if (p.pieces > 1) mx_store<float, 16>(p.ws + ((int64_t)piece * p.m + row) * (4 * p.cells_b) + col, v, 4 * p.cells_b - col, 1, 0);
+    else mx_store<TO, 16>(reinterpret_cast<TO *>(p.c) + row * p.ldc + col, v, p.n - col, p.vec, p.accumulate);
+  }
+}
+
 // c (+)= the pieces' sums, in order; a thread 4 columns.
 template <typename TO> __global__ void __launch_bounds__(256) mx_join_kernel(const MxGemmParams p) {
   const int64_t groups = p.cells_b, u = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -513,35 +723,61 @@ template <typename TO> __global__ void __launch_bounds__(256) mx_zero_kernel(con
 
 constexpr int MX_MAX_PIECES = 16;
 
-// Which kernel a product takes: mt of 0 is mx_w8_kernel.
-struct MxPlan { int mt, nt, waves, pieces; };
+// Which kernel a product takes: `side` 256 is mx_w8_kernel, 128 mx_t128_kernel, 0 mx_direct_kernel with mt, nt and waves.
+struct MxPlan { int side, mt, nt, waves, pieces; };
 static bool mx_wide_needed(int fa, int fb, int out) { return out == DH_F32 && (fa == DH_MX_E4M3 || fb == DH_MX_E4M3); }
 static MxPlan mx_plan(int64_t m, int64_t n, int64_t steps, bool wide) {
-  const int64_t big = cdiv(m, 256) * cdiv(n, 256);
-  if (!wide && m > 128 && n > 128 && big >= 16) {
-    MxPlan q{0, 0, 8, 1};
+  static const char *force = getenv("MX_SIDE");
+  const int64_t big = cdiv(m, 256) * cdiv(n, 256), mid = cdiv(m, 128) * cdiv(n, 128);
+  if (force ? atoi(force) == 256 : !wide && m > 128 && n > 128 && big >= 128) {
+    MxPlan q{256, 0, 0, 8, 1};
     if (big < 256) q.pieces = (int)std::max<int64_t>(1, std::min<int64_t>({256 / big, steps / 4, MX_MAX_PIECES}));
     return q;
   }
-  MxPlan q{m <= 16 ? 1 : m <= 32 ? 2 : 4, m <= 16 ? 1 : 4, m <= 16 ? 8 : 4, 1};
+  if (force ? atoi(force) == 128 : m > 64 && n > 64) {
+    MxPlan q{128, 0, 0, 4, 1};
+    if (mid < 256) q.pieces = (int)std::max<int64_t>(1, std::min<int64_t>({256 / mid, steps / 8, MX_MAX_PIECES}));
+    static const char *pc = getenv("MX_PIECES");
+    if (pc) q.pieces = std::max(1, std::min<int>(atoi(pc), steps));
+    return q;
+  }
+  MxPlan q{0, m <= 16 ? 1 : m <= 32 ? 2 : 4, m <= 4 ? 1 : 2, 8, 1};
+  static const char *dd = getenv("MX_DIRECT");
+  if (dd) sscanf(dd, "%d,%d,%d", &q.mt, &q.nt, &q.waves);
   const int64_t tiles = cdiv(m, 16 * q.mt) * cdiv(n, 16 * q.nt);
   if (tiles < 256) q.pieces = (int)std::min<int64_t>({512 / std::max<int64_t>(tiles, 1), steps / q.waves, MX_MAX_PIECES});
   q.pieces = std::max(q.pieces, 1);
+  static const char *pc = getenv("MX_PIECES");
+  if (pc) q.pieces = std::max(1, std::min<int>(atoi(pc), steps));
   return q;
 }
 
 template <int FA, int FB, typename TO> static void mx_launch(MxGemmParams p, const MxPlan &q, hipStream_t st) {
   constexpr bool WIDE = sizeof(TO) == 4 && (FA == 8 || FB == 8);
-  const int side_m = q.mt ? 16 * q.mt : 256, side_n = q.mt ? 16 * q.nt : 256;
+  const int side_m = q.side ? q.side : 16 * q.mt, side_n = q.side ? q.side : 16 * q.nt;
   p.tiles_m = (int)cdiv(p.m, side_m);
   p.tiles_n = (int)cdiv(p.n, side_n);
   p.pieces = q.pieces;
   const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), (unsigned)q.pieces), block((unsigned)(64 * q.waves));
-  if (q.mt == 0) {
-    if constexpr (!WIDE) hipLaunchKernelGGL((mx_w8_kernel<FA, FB, TO>), grid, block, 0, st, p);
-  } else if (q.mt == 1) hipLaunchKernelGGL((mx_direct_kernel<FA, FB, 1, 1, 8, WIDE, TO>), grid, block, 0, st, p);
-  else if (q.mt == 2) hipLaunchKernelGGL((mx_direct_kernel<FA, FB, 2, 4, 4, WIDE, TO>), grid, block, 0, st, p);
-  else hipLaunchKernelGGL((mx_direct_kernel<FA, FB, 4, 4, 4, WIDE, TO>), grid, block, 0, st, p);
+  if (q.side) {
+    if constexpr (!WIDE) {
+      if (q.side == 256) hipLaunchKernelGGL((mx_w8_kernel<FA, FB, TO>), grid, block, 0, st, p);
+    }
+    static const char *stg = getenv("MX_STAGES");
+    if (q.side == 128) {
+      if (WIDE || (stg && atoi(stg) == 2)) hipLaunchKernelGGL((mx_t128_kernel<FA, FB, 2, WIDE, TO>), grid, block, 0, st, p);
+      else if constexpr (!WIDE) hipLaunchKernelGGL((mx_t128_kernel<FA, FB, 4, WIDE, TO>), grid, block, 0, st, p);
+    }
+  }
+#define MX_DIRECT(MT, NT, W) \
+  if (!q.side && q.mt == MT && q.nt == NT && q.waves == W) hipLaunchKernelGGL((mx_direct_kernel<FA, FB, MT, NT, W, WIDE, TO>), grid, block, 0, st, p)
+  MX_DIRECT(1, 1, 8);
+  MX_DIRECT(1, 1, 16);
+  MX_DIRECT(1, 2, 8);
+  MX_DIRECT(2, 2, 8);
+  MX_DIRECT(4, 2, 8);
+  MX_DIRECT(4, 4, 4);
+#undef MX_DIRECT
   if (q.pieces > 1) hipLaunchKernelGGL((mx_join_kernel<TO>), dim3((unsigned)cdiv(p.m * p.cells_b, 256)), dim3(256), 0, st, p);
 }
 
