@@ -103,6 +103,7 @@ SIGNATURES = {
     "dh_mx_quantise": (_i32, [_vp, _i64, _i64, _i64, _i32, _i32, _i32] + [_vp] * 5),
     "dh_rmsnorm_mx": (_i32, [_vp] * 8 + [_i64, _i64, _f32, _i32, _i32, _i32, _vp]),
     "dh_mx_gemm_workspace_bytes": (_sz, [_i64] * 3 + [_i32] * 3),
+    "dh_mx_gemm_path": (_i32, [_i64] * 3 + [_i32] * 3),
     "dh_mx_gemm_nt": (_i32, [_vp, _vp, _i32, _vp, _vp, _i32, _vp] + [_i64] * 4 + [_i32, _i32, _vp, _sz, _vp]),
     "dh_grad_norm_workspace_bytes": (_sz, [_vp, _i32]),
     "dh_grad_norm": (_i32, [_vp, _vp, _vp, _i32, _vp, _vp, _sz, _vp]),

@@ -13,7 +13,6 @@
 // rounded to 2^-9 (2^-12), far above that.  A result in fp32 is promised to 1e-5 everywhere else in this library, so with an 8-bit
 // operand it is formed from the elements in bf16, which hold them and their scales exactly (mx_wide below).
 #include <algorithm>
-#include <cstdlib>
 #include <type_traits>
 
 #include "mma.h"
@@ -519,19 +518,22 @@ __global__ void __launch_bounds__(512) mx_w8_kernel(const MxGemmParams p) {
 #undef MX_WAIT_BARRIER
 }
 
-// ---- 128 x 128 tiles: four wavefronts of 64 x 64 outputs, one on a SIMD ------------------------------------------------------
-// For products of fewer than a round of 256 x 256 tiles.  Four stages of LDS; the fragments of slice s + 1 are read among the matrix
-// instructions of slice s, into the other of two sets of registers, and the copies of slice s + 4 go out meanwhile.  One barrier a slice:
-// a wavefront passes it when its reads of slice s are in registers, so the stage of slice s may be written again, and when its own copies
-// of slice s + 1 have landed (those of s + 2 and s + 3 stay in flight), so that slice may be read.
+// ---- 128 x 128 tiles: four wavefronts of 64 x 64 outputs, two workgroups on a compute unit -------------------------------------
+// For products of too few 256 x 256 tiles, and for fp32 results of 8-bit operands.  Two stages of LDS; the fragments of slice s + 1 are read
+// among the matrix instructions of slice s, into the other of two sets of registers.  One barrier a slice: a wavefront passes it when its
+// reads of slice s are in registers, so the stage of slice s may be written again (by the copies of slice s + 2, which go out next), and when
+// its own copies of slice s + 1 have landed, so that slice may be read.  What a workgroup waits for the other one of the compute unit fills:
+// with four stages and one workgroup 2048 x 4096 x 8192 took 79 us in 8 bits and 58 in 4, with two and two it takes 58 and 40.
+// Bound by LDS: a slice moves 34 KB into it and 72 KB out of it for 512 cycles of matrix instructions a SIMD; 2048 x 4096 x 8192 runs at 2.4
+// (8 bits) and 3.4 PFLOP/s.
 // Both operands' slots hold row 64 (s / 64) + 4 (s % 16) + s / 16 % 4: four blocks' scales are one dword, and a lane's outputs 16 neighbouring
 // columns of four rows.
-template <int FA, int FB, int STAGES, bool WIDE, typename TO>
-__global__ void __launch_bounds__(256, STAGES == 2 ? 2 : 1) mx_t128_kernel(const MxGemmParams p) {
+template <int FA, int FB, bool WIDE, typename TO>
+__global__ void __launch_bounds__(256, 2) mx_t128_kernel(const MxGemmParams p) {
   constexpr int KS = FA == 4 && FB == 4 ? 2 : 1;
   constexpr int RA = KS * MxBytes<FA>::STEP, RB = KS * MxBytes<FB>::STEP, NA = RA / 64, NB = RB / 64;
   constexpr uint32_t REGA = 128 * RA, REGB = 128 * RB, OFF_S = REGA + REGB, STAGEB = OFF_S + KS * 1024;
-  constexpr int COPIES = KS + 2 * NA + 2 * NB;      // of a wavefront a slice
+  constexpr int STAGES = 2, COPIES = KS + 2 * NA + 2 * NB;      // of a wavefront a slice
   __shared__ __attribute__((aligned(1024))) unsigned char smem[STAGES * STAGEB];
 
   const int tid = threadIdx.x, lane = tid & 63;
@@ -685,20 +687,46 @@ __global__ void __launch_bounds__(256, STAGES == 2 ? 2 : 1) mx_t128_kernel(const
     slice(std::integral_constant<int, 1>{}, s + 1);
   }
   if (s < cnt) slice(std::integral_constant<int, 0>{}, s);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");               // the last copies have landed before the workgroup gives its LDS back
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");               // the last copies have landed before LDS is used again,
   asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");             // and the last sums are there
 #pragma unroll
   for (int i = 0; i < 16; ++i) asm volatile("" : "+v"(acc[i >> 2][i & 3]));
+  __syncthreads();
+  // 32 rows of a wavefront's 64 at a time through LDS of its own, so that a store writes whole lines: a lane holds columns 16 g4 + 4 v + nj of
+  // rows 4 c + mi, and stores 16 bytes of a row
+  constexpr int PITCH = 68;
+  float *mine = reinterpret_cast<float *>(smem) + w * 32 * PITCH;
+  auto store = [&](auto *out, int64_t ld, int64_t cols, int vec, int accumulate) {
+    using TS = std::remove_pointer_t<decltype(out)>;
+    constexpr int E = 16 / (int)sizeof(TS), LPR = 64 / E;        // columns of a lane, lanes of a row
 #pragma unroll
-  for (int mi = 0; mi < 4; ++mi) {
-    const int64_t row = m0 + 64 * wm + 4 * c + mi, col = n0 + 64 * wn + 16 * g4;
-    if (row >= p.m || col >= p.n) continue;
-    float v[16];
+    for (int half = 0; half < 2; ++half) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = acc[mi][i & 3][i >> 2];
-    if (p.pieces > 1) mx_store<float, 16>(p.ws + ((int64_t)piece * p.m + row) * (4 * p.cells_b) + col, v, 4 * p.cells_b - col, 1, 0);
-    else mx_store<TO, 16>(reinterpret_cast<TO *>(p.c) + row * p.ldc + col, v, p.n - col, p.vec, p.accumulate);
-  }
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const int mi = 2 * half + i;
+          *reinterpret_cast<floatx4 *>(mine + (2 * c + i) * PITCH + 16 * g4 + 4 * v) = floatx4{acc[mi][0][v], acc[mi][1][v], acc[mi][2][v], acc[mi][3][v]};
+        }
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int it = 0; it < 32 * LPR / 64; ++it) {
+        const int r = it * (64 / LPR) + lane / LPR, e = lane % LPR * E;
+        const int64_t row = m0 + 64 * wm + 4 * (r >> 1) + 2 * half + (r & 1), col = n0 + 64 * wn + e;
+        float v[E];
+#pragma unroll
+        for (int q = 0; q < E / 4; ++q) {
+          const floatx4 x = *reinterpret_cast<const floatx4 *>(mine + r * PITCH + e + 4 * q);
+#pragma unroll
+          for (int y = 0; y < 4; ++y) v[4 * q + y] = x[y];
+        }
+        if (row < p.m && col < cols) mx_store<TS, E>(out + row * ld + col, v, cols - col, vec, accumulate);
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+  };
+  if (p.pieces > 1) store(p.ws + (int64_t)piece * p.m * (4 * p.cells_b), 4 * p.cells_b, 4 * p.cells_b, 1, 0);
+  else store(reinterpret_cast<TO *>(p.c), p.ldc, p.n, p.vec, p.accumulate);
 }
 
 // c (+)= the pieces' sums, in order; a thread 4 columns.
@@ -723,32 +751,49 @@ template <typename TO> __global__ void __launch_bounds__(256) mx_zero_kernel(con
 
 constexpr int MX_MAX_PIECES = 16;
 
-// Which kernel a product takes: `side` 256 is mx_w8_kernel, 128 mx_t128_kernel, 0 mx_direct_kernel with mt, nt and waves.
+// Which kernel a product takes: `side` 256 is mx_w8_kernel, 128 mx_t128_kernel, 0 mx_direct_kernel with mt, nt and waves.  Measured on 1 to
+// 8192 rows, widths of 512 to 8192 and k of 512 to 8192, in us for 8 x 8, 8 x 4 and 4 x 4 bits.
 struct MxPlan { int side, mt, nt, waves, pieces; };
 static bool mx_wide_needed(int fa, int fb, int out) { return out == DH_F32 && (fa == DH_MX_E4M3 || fb == DH_MX_E4M3); }
-static MxPlan mx_plan(int64_t m, int64_t n, int64_t steps, bool wide) {
-  static const char *force = getenv("MX_SIDE");
+static MxPlan mx_plan(int64_t m, int64_t n, int64_t k, int fa, int fb, int out) {
+  const bool wide = mx_wide_needed(fa, fb, out), b4 = fb == DH_MX_E2M1;
+  const int64_t steps = cdiv(k, 128);
   const int64_t big = cdiv(m, 256) * cdiv(n, 256), mid = cdiv(m, 128) * cdiv(n, 128);
-  if (force ? atoi(force) == 256 : !wide && m > 128 && n > 128 && big >= 128) {
-    MxPlan q{256, 0, 0, 8, 1};
-    if (big < 256) q.pieces = (int)std::max<int64_t>(1, std::min<int64_t>({256 / big, steps / 4, MX_MAX_PIECES}));
+  // Tokens of a few sequences.  32 columns a workgroup where that still fills the chip, else 16: 1 x 8192 x 3584 5.0 against 7.0 (8 x 4), 16 x
+  // 7168 x 8192 11.1 against 14.0; but 8-bit weights, whose loads alone keep a compute unit busy, lose at 224 workgroups (13.5 against 17.8).
+  MxPlan q{0, 1, 1, 8, 1};
+  bool direct = m <= 16;
+  if (direct) {
+    if (cdiv(n, 32) >= (b4 ? 224 : 256)) q.nt = 2;
+  } else if (m <= 32 || cdiv(m, 32) * cdiv(n, 32) <= 128) {
+    // 24 x 8192 x 3584 9.4 / 8.1 / 6.5 against 11.3 / 10.7 / 9.5 in tiles of 32 x 64 and pieces of k; 65 x 1280 x 1024 4.7 / 4.5 / 4.4 against 7.6 / 7.1 / 6.6
+    // in tiles of 128
+    direct = true;
+    q.mt = q.nt = 2;
+  } else if (steps <= 32 && cdiv(m, 64) * cdiv(n, 32) <= 256) {
+    // 512 x 512 x 512 5.1 / 5.0 / 4.5 against 6.2 / 6.0 / 5.8 in tiles of 128; past one workgroup a compute unit 1000 x 520 x 1999 13.9 / 15.4 / 9.5 against
+    // 11.3 / 10.4 / 8.8, and at long k 64 x 7168 x 8192 26.7 / 22.9 / 16.5 against 20.0 / 17.1 / 16.4
+    direct = true;
+    q.mt = 4, q.nt = 2;
+  } else if (wide && steps < 32 && mid < 128) {
+    direct = true;                   // 777 x 1001 x 2080 16.1 against 24.7
+    q.mt = q.nt = q.waves = 4;
+  }
+  if (direct) {
+    // k in pieces where few workgroups have long sums: 32 x 1280 x 8192 17.5 / 14.1 / 10.6 whole, 10.0 / 9.3 / 9.1 in up to 4 pieces
+    const int64_t tiles = cdiv(m, 16 * q.mt) * cdiv(n, 16 * q.nt), units = b4 ? (steps + 1) / 2 : steps;
+    if (tiles <= 64) q.pieces = (int)std::max<int64_t>(1, std::min<int64_t>({256 / tiles, units / (2 * q.waves), MX_MAX_PIECES}));
     return q;
   }
-  if (force ? atoi(force) == 128 : m > 64 && n > 64) {
-    MxPlan q{128, 0, 0, 4, 1};
-    if (mid < 256) q.pieces = (int)std::max<int64_t>(1, std::min<int64_t>({256 / mid, steps / 8, MX_MAX_PIECES}));
-    static const char *pc = getenv("MX_PIECES");
-    if (pc) q.pieces = std::max(1, std::min<int>(atoi(pc), steps));
-    return q;
-  }
-  MxPlan q{0, m <= 16 ? 1 : m <= 32 ? 2 : 4, m <= 4 ? 1 : 2, 8, 1};
-  static const char *dd = getenv("MX_DIRECT");
-  if (dd) sscanf(dd, "%d,%d,%d", &q.mt, &q.nt, &q.waves);
-  const int64_t tiles = cdiv(m, 16 * q.mt) * cdiv(n, 16 * q.nt);
-  if (tiles < 256) q.pieces = (int)std::min<int64_t>({512 / std::max<int64_t>(tiles, 1), steps / q.waves, MX_MAX_PIECES});
-  q.pieces = std::max(q.pieces, 1);
-  static const char *pc = getenv("MX_PIECES");
-  if (pc) q.pieces = std::max(1, std::min<int>(atoi(pc), steps));
+  // A round of the chip is 256 tiles of 256 x 256, or 512 of 128 x 128 in 0.6 of its time: 4096 x 7168 x 8192 (2 rounds and 4) 168 / 155 / 115 against
+  // 204 / 176 / 124, 2048 x 4096 x 8192 (half a round and one) 73 / 69 / 59 against 58 / 55 / 40
+  if (!wide && 5 * cdiv(big, 256) <= 3 * cdiv(mid, 512)) return {256, 0, 0, 8, 1};
+  q = {128, 0, 0, 4, 1};
+  // k in pieces, of 8 slices at least, while they have a compute unit each: 128 x 7168 x 8192 42 whole, 23 in four (8 x 8); 777 x 1001 x 2080 13.8 whole, 15.6
+  // in two: the pieces' sums are written and read once more
+  const int64_t slices = fa == DH_MX_E2M1 && b4 ? (steps + 1) / 2 : steps;
+  if (slices >= 24)
+    while (q.pieces < MX_MAX_PIECES && mid * q.pieces * 2 <= 256 && slices >= 16 * q.pieces) q.pieces *= 2;
   return q;
 }
 
@@ -763,20 +808,15 @@ template <int FA, int FB, typename TO> static void mx_launch(MxGemmParams p, con
     if constexpr (!WIDE) {
       if (q.side == 256) hipLaunchKernelGGL((mx_w8_kernel<FA, FB, TO>), grid, block, 0, st, p);
     }
-    static const char *stg = getenv("MX_STAGES");
-    if (q.side == 128) {
-      if (WIDE || (stg && atoi(stg) == 2)) hipLaunchKernelGGL((mx_t128_kernel<FA, FB, 2, WIDE, TO>), grid, block, 0, st, p);
-      else if constexpr (!WIDE) hipLaunchKernelGGL((mx_t128_kernel<FA, FB, 4, WIDE, TO>), grid, block, 0, st, p);
-    }
+    if (q.side == 128) hipLaunchKernelGGL((mx_t128_kernel<FA, FB, WIDE, TO>), grid, block, 0, st, p);
   }
 #define MX_DIRECT(MT, NT, W) \
   if (!q.side && q.mt == MT && q.nt == NT && q.waves == W) hipLaunchKernelGGL((mx_direct_kernel<FA, FB, MT, NT, W, WIDE, TO>), grid, block, 0, st, p)
   MX_DIRECT(1, 1, 8);
-  MX_DIRECT(1, 1, 16);
   MX_DIRECT(1, 2, 8);
   MX_DIRECT(2, 2, 8);
   MX_DIRECT(4, 2, 8);
-  MX_DIRECT(4, 4, 4);
+  if constexpr (WIDE) { MX_DIRECT(4, 4, 4); }
 #undef MX_DIRECT
   if (q.pieces > 1) hipLaunchKernelGGL((mx_join_kernel<TO>), dim3((unsigned)cdiv(p.m * p.cells_b, 256)), dim3(256), 0, st, p);
 }
@@ -793,8 +833,14 @@ static int mx_gemm_sizes(int64_t m, int64_t n, int64_t k) {
 
 extern "C" size_t dh_mx_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k, int a_format, int b_format, int out_dtype) {
   if (m <= 0 || n <= 0 || k <= 0 || mx_gemm_sizes(m, n, k) != DH_OK) return 0;
-  const dh::MxPlan q = dh::mx_plan(m, n, dh::cdiv(k, 128), dh::mx_wide_needed(a_format, b_format, out_dtype));
+  const dh::MxPlan q = dh::mx_plan(m, n, k, a_format, b_format, out_dtype);
   return q.pieces > 1 ? (size_t)q.pieces * (size_t)m * (size_t)dh::mx_rows4(n) * 4 : 0;
+}
+
+extern "C" int dh_mx_gemm_path(int64_t m, int64_t n, int64_t k, int a_format, int b_format, int out_dtype) {
+  if (m <= 0 || n <= 0 || k <= 0 || mx_gemm_sizes(m, n, k) != DH_OK) return 0;
+  const dh::MxPlan q = dh::mx_plan(m, n, k, a_format, b_format, out_dtype);
+  return (q.side ? q.side : 10 * q.mt + q.nt) * 100 + q.pieces;
 }
 
 extern "C" int dh_mx_gemm_nt(const void *a_codes, const void *a_scales, int a_format, const void *b_codes, const void *b_scales, int b_format, void *c,
@@ -826,7 +872,7 @@ extern "C" int dh_mx_gemm_nt(const void *a_codes, const void *a_scales, int a_fo
   p.cells_a = mx_rows4(m) / 4; p.cells_b = mx_rows4(n) / 4; p.steps = (int)cdiv(k, 128);
   p.vec = aligned16(c) && ldc * (int64_t)dtype_size(out_dtype) % 16 == 0;
   DH_CHECK(p.steps * std::max(p.cells_a, p.cells_b) * 16 < (1ll << 31), "scales of 2 GiB and more");
-  const MxPlan q = mx_plan(m, n, p.steps, mx_wide_needed(a_format, b_format, out_dtype));
+  const MxPlan q = mx_plan(m, n, k, a_format, b_format, out_dtype);
   if (q.pieces > 1) {
     const size_t need = dh_mx_gemm_workspace_bytes(m, n, k, a_format, b_format, out_dtype);
     DH_CHECK(workspace && aligned16(workspace) && workspace_bytes >= need, "workspace of %zu bytes, %zu are needed", workspace_bytes, need);

@@ -697,6 +697,9 @@ int dh_rmsnorm_mx(const void *x, const void *residual, void *sum_out, const void
  * own) may be NULL when dh_mx_gemm_workspace_bytes is 0. */
 size_t dh_mx_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k, int a_format, int b_format,
                                   int out_dtype);
+/* Which kernel such a call runs: 100 x (the side of its tiles, 128 or 256; for few outputs 10 x blocks of 16 rows + blocks of 16
+ * columns) + the pieces that k is cut into. */
+int dh_mx_gemm_path(int64_t m, int64_t n, int64_t k, int a_format, int b_format, int out_dtype);
 int dh_mx_gemm_nt(const void *a_codes, const void *a_scales, int a_format, const void *b_codes,
                   const void *b_scales, int b_format, void *c, int64_t m, int64_t n, int64_t k,
                   int64_t ldc, int out_dtype, int accumulate, void *workspace, size_t workspace_bytes,

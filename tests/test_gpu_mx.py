@@ -3,6 +3,7 @@ whose sums are exact, bit for bit as well."""
 import pytest
 import torch
 
+from dhellam_amd import _lib
 from tests import mx_reference as R
 from dhellam_amd.operators.mx import MXTensor, mx_gemm_nt, mx_quantise
 
@@ -103,7 +104,16 @@ def exact_operand(rows, cols, form, seed):
 
 
 PRODUCTS = [(1, 1, 1), (1, 1000, 160), (1, 7168, 8192), (3, 17, 128), (16, 16, 384), (17, 65, 130), (24, 8192, 3584), (33, 100, 4096), (64, 64, 64), (65, 129, 257),
-            (130, 1000, 512), (256, 256, 256), (257, 512, 640), (777, 1001, 2080), (300, 2048, 8192), (1999, 520, 1000), (2048, 2304, 1152), (520, 8200, 384)]
+            (130, 1000, 512), (256, 256, 256), (257, 512, 640), (777, 1001, 2080), (300, 2048, 8192), (1999, 520, 1000), (2048, 2304, 1152), (520, 8200, 384),
+            (32, 1280, 4096), (130, 300, 8192), (2050, 4400, 640), (4100, 2300, 128), (2200, 4111, 1032)]
+
+
+def test_products_reach_every_kernel():
+    path = lambda s, fa, fb, out: _lib.load().dh_mx_gemm_path(*s, FORMS.index(fa), FORMS.index(fb), out)
+    seen = {path(s, fa, fb, out) // 100 for s in PRODUCTS for fa in FORMS for fb in FORMS for out in (0, 1)}
+    assert seen == {11, 12, 22, 42, 44, 128, 256}
+    assert {path(s, "e4m3", "e4m3", out) % 100 > 1 for s in PRODUCTS for out in (0, 1) if path(s, "e4m3", "e4m3", out) // 100 == 128} == {False, True}
+    assert {path(s, "e4m3", "e4m3", 1) % 100 > 1 for s in PRODUCTS if path(s, "e4m3", "e4m3", 1) // 100 < 100} == {False, True}
 
 
 @pytest.mark.parametrize("m,n,k", PRODUCTS)
@@ -125,7 +135,7 @@ def test_product_bits(m, n, k, fa, fb):
         assert torch.equal(out, (want + old).to(dtype))
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 2048, 8192), (100, 520, 1024), (1999, 1001, 520), (2304, 2048, 1024)])
+@pytest.mark.parametrize("m,n,k", [(1, 2048, 8192), (100, 520, 1024), (1999, 1001, 520), (2304, 2048, 1024), (2050, 4400, 1024)])
 @pytest.mark.parametrize("fa,fb", [("e4m3", "e4m3"), ("e4m3", "e2m1"), ("e2m1", "e2m1")])
 def test_product_of_quantised_data(m, n, k, fa, fb):
     """Elements have few bits and scales are powers of two: products are exact.  fp32 results are sums of fp32: should every addition round, each of k
@@ -145,7 +155,7 @@ def test_product_of_quantised_data(m, n, k, fa, fb):
         assert (low - want).norm() <= (half + 2.0 ** -12) * want.norm()
 
 
-@pytest.mark.parametrize("m,n", [(1, 40), (40, 100), (300, 300), (2304, 2048)])
+@pytest.mark.parametrize("m,n", [(1, 40), (40, 100), (300, 300), (2304, 2048), (2050, 4400)])
 @pytest.mark.parametrize("fa,fb", [("e4m3", "e2m1"), ("e2m1", "e2m1"), ("e4m3", "e4m3")])
 def test_product_not_finite_and_extreme_scales(m, n, fa, fb):
     k = 512
@@ -165,7 +175,7 @@ def test_product_not_finite_and_extreme_scales(m, n, fa, fb):
 
 
 def test_product_into_views_leaves_the_rest():
-    for m, n in ((5, 33), (70, 130), (2304, 2050)):
+    for m, n in ((5, 33), (70, 130), (1000, 520), (2304, 2050), (2050, 4401)):
         a, b = exact_operand(m, 384, "e4m3", 9), exact_operand(n, 384, "e2m1", 10)
         want = R.values(a) @ R.values(b).t()
         for dtype in (torch.float32, torch.bfloat16):
@@ -191,7 +201,7 @@ def test_product_of_nothing():
 
 def test_product_twice_the_same_bits_other_streams_and_graphs():
     """Two graphs captured on one stream and calls in between: each product has its own workspace."""
-    cases = [(1, 512, 8192), (40, 640, 4096), (2304, 2048, 1024)]
+    cases = [(1, 512, 8192), (40, 640, 4096), (300, 512, 8192), (2304, 2048, 1024)]
     ops = [(exact_operand(m, k, "e4m3", i), exact_operand(n, k, "e2m1", 20 + i)) for i, (m, n, k) in enumerate(cases)]
     want = [(R.values(a) @ R.values(b).t()).float() for a, b in ops]
     x = matrix(300, 700, torch.bfloat16, 11)
