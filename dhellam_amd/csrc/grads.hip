@@ -36,17 +36,32 @@ __device__ __forceinline__ int grad_find(const GradTable &t, int block) {
   return lo;
 }
 
-template <typename T> __device__ __forceinline__ double grad_piece_sum(const T *g, int64_t n) {
+// N consecutive elements at any address that suits T, 16 bytes or 8; NT: without a place in the caches.
+template <typename T, int N> struct alignas(sizeof(T)) Run { T v[N]; };
+template <bool NT, typename T, int N> __device__ __forceinline__ Run<T, N> grad_load(const T *p) {
+  Run<T, N> x;
+  if constexpr (NT && sizeof(x) == 16) {
+    const dh_u32x4 q = __builtin_nontemporal_load(reinterpret_cast<const typename LooseU4<T>::type *>(p));
+    __builtin_memcpy(&x, &q, 16);
+  } else {
+    x = *reinterpret_cast<const Run<T, N> *>(p);
+  }
+  return x;
+}
+
+template <typename T, bool NT> __device__ __forceinline__ double grad_piece_sum(const T *g, int64_t n) {
+  constexpr int N = 16 / (int)sizeof(T), STEP = 256 * N;
   double s[2] = {0.0, 0.0};
-#pragma unroll 4
-  for (int i = 0; i < (int)GRAD_PIECE / 2048; ++i) {
-    const int64_t at = (int64_t)i * 2048 + threadIdx.x * 8;
-    float f[8];
-    if (at + 8 <= n) load8(f, g + at);
-    else if (at < n) load8_first(f, g + at, (int)(n - at));
-    else continue;
+#pragma unroll 8
+  for (int i = 0; i < (int)GRAD_PIECE / STEP; ++i) {
+    const int64_t at = (int64_t)i * STEP + threadIdx.x * N;
+    if (at + N <= n) {
+      const Run<T, N> x = grad_load<NT, T, N>(g + at);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s[j & 1] = fma((double)f[j], (double)f[j], s[j & 1]);
+      for (int j = 0; j < N; ++j) s[j & 1] = fma((double)to_f(x.v[j]), (double)to_f(x.v[j]), s[j & 1]);
+    } else {
+      for (int64_t j = at; j < n; ++j) s[0] = fma((double)to_f(g[j]), (double)to_f(g[j]), s[0]);
+    }
   }
   return s[0] + s[1];
 }
@@ -57,14 +72,14 @@ __device__ __forceinline__ double wave_sum64(double v) {
   return v;
 }
 
-__global__ void __launch_bounds__(256) grad_norm_kernel(const GradTable t, double *partial) {
+template <bool NT> __global__ void __launch_bounds__(256) grad_norm_kernel(const GradTable t, double *partial) {
   __shared__ double red[4];
   const int i = grad_find(t, (int)blockIdx.x);
   const int64_t at = (int64_t)((int)blockIdx.x - t.first[i]) * GRAD_PIECE, n = t.n[i] - at;
   double s = 0.0;
-  if (t.type[i] == DH_F32) s = grad_piece_sum(reinterpret_cast<const float *>(t.g[i]) + at, n);
-  else if (t.type[i] == DH_BF16) s = grad_piece_sum(reinterpret_cast<const bf16_t *>(t.g[i]) + at, n);
-  else s = grad_piece_sum(reinterpret_cast<const f16_t *>(t.g[i]) + at, n);
+  if (t.type[i] == DH_F32) s = grad_piece_sum<float, NT>(reinterpret_cast<const float *>(t.g[i]) + at, n);
+  else if (t.type[i] == DH_BF16) s = grad_piece_sum<bf16_t, NT>(reinterpret_cast<const bf16_t *>(t.g[i]) + at, n);
+  else s = grad_piece_sum<f16_t, NT>(reinterpret_cast<const f16_t *>(t.g[i]) + at, n);
   s = wave_sum64(s);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
@@ -74,6 +89,7 @@ __global__ void __launch_bounds__(256) grad_norm_kernel(const GradTable t, doubl
 __global__ void __launch_bounds__(1024) grad_join_kernel(const double *partial, int64_t n, double *sum_sq) {
   __shared__ double red[16];
   double s = 0.0;
+#pragma unroll 8
   for (int64_t i = threadIdx.x; i < n; i += 1024) s += partial[i];
   s = wave_sum64(s);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
@@ -86,24 +102,31 @@ __global__ void __launch_bounds__(1024) grad_join_kernel(const double *partial, 
   }
 }
 
-template <typename T, typename TO> __device__ __forceinline__ void grad_piece_scale(const T *g, TO *out, int64_t n, float factor) {
-#pragma unroll 4
-  for (int i = 0; i < (int)GRAD_PIECE / 2048; ++i) {
-    const int64_t at = (int64_t)i * 2048 + threadIdx.x * 8;
-    float f[8];
-    if (at + 8 <= n) {
-      load8(f, g + at);
-      Loose8<TO> o;
+// (a lane stores 16 bytes, so that a wavefront's store is one run of memory: fp32 from 16 bits in pieces of 32 bytes a lane ran at 4.7 TB/s)
+template <typename T, typename TO, bool NT> __device__ __forceinline__ void grad_piece_scale(const T *g, TO *out, int64_t n, float factor) {
+  constexpr int N = 16 / (int)sizeof(TO), STEP = 256 * N;
+#pragma unroll 8
+  for (int i = 0; i < (int)GRAD_PIECE / STEP; ++i) {
+    const int64_t at = (int64_t)i * STEP + threadIdx.x * N;
+    if (at + N <= n) {
+      const Run<T, N> x = grad_load<NT, T, N>(g + at);
+      Run<TO, N> o;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) o.v[j] = factor == 0.f ? from_f<TO>(0.f) : from_f<TO>(f[j] * factor);
-      *reinterpret_cast<Loose8<TO> *>(out + at) = o;
-    } else if (at < n) {
+      for (int j = 0; j < N; ++j) o.v[j] = factor == 0.f ? from_f<TO>(0.f) : from_f<TO>(to_f(x.v[j]) * factor);
+      if constexpr (NT) {
+        dh_u32x4 q;
+        __builtin_memcpy(&q, &o, 16);
+        __builtin_nontemporal_store(q, reinterpret_cast<typename LooseU4<TO>::type *>(out + at));
+      } else {
+        *reinterpret_cast<Run<TO, N> *>(out + at) = o;
+      }
+    } else {
       for (int64_t j = at; j < n; ++j) out[j] = factor == 0.f ? from_f<TO>(0.f) : from_f<TO>(to_f(g[j]) * factor);
     }
   }
 }
 
-__global__ void __launch_bounds__(256) grad_clip_kernel(const GradTable t, const double *sum_sq, double max_norm, double scale, float *found) {
+template <bool NT> __global__ void __launch_bounds__(256) grad_clip_kernel(const GradTable t, const double *sum_sq, double max_norm, double scale, float *found) {
   const double norm = fabs(scale) * sqrt(sum_sq[0]);
   double factor = scale * fmin(1.0, max_norm / (norm + 1e-6));
   if (!(norm < INFINITY)) factor = 0.0;
@@ -116,7 +139,7 @@ __global__ void __launch_bounds__(256) grad_clip_kernel(const GradTable t, const
   const int i = grad_find(t, (int)blockIdx.x);
   const int64_t at = (int64_t)((int)blockIdx.x - t.first[i]) * GRAD_PIECE, n = t.n[i] - at;
   if (f == 1.f && t.g[i] == t.out[i]) return;              // in place, nothing to change
-#define GRAD_SCALE(T, TO) grad_piece_scale(reinterpret_cast<const T *>(t.g[i]) + at, reinterpret_cast<TO *>(t.out[i]) + at, n, f)
+#define GRAD_SCALE(T, TO) grad_piece_scale<T, TO, NT>(reinterpret_cast<const T *>(t.g[i]) + at, reinterpret_cast<TO *>(t.out[i]) + at, n, f)
   if (t.type[i] == DH_F32) GRAD_SCALE(float, float);
   else if (t.type[i] == DH_BF16) {
     if (t.out_type[i] == DH_F32) GRAD_SCALE(bf16_t, float);
@@ -175,10 +198,15 @@ extern "C" int dh_grad_norm(const void *const *grads, const int64_t *counts, con
   DH_CHECK(need == 0 || (workspace && (uintptr_t)workspace % 8 == 0 && workspace_bytes >= need), "workspace of %zu bytes, %zu are needed", workspace_bytes,
            need);
   double *partial = reinterpret_cast<double *>(workspace);
+  // gradients that the last-level cache holds stay there for the clipping: 215 MB in 16 bits to fp32 132 us (165 read past it), 1.1 GB 808 (835)
+  int64_t bytes = 0;
+  for (int i = 0; i < n; ++i) bytes += counts[i] * (int64_t)dtype_size(dtypes[i]);
+  const bool nt = stream_hint(bytes);
   int64_t done = 0;
   const hipStream_t st = (hipStream_t)stream;
   const int rc = grad_tables(grads, nullptr, counts, dtypes, nullptr, n, [&](const GradTable &t) -> int {
-    hipLaunchKernelGGL(grad_norm_kernel, dim3((unsigned)t.blocks), dim3(256), 0, st, t, partial + done);
+    if (nt) hipLaunchKernelGGL((grad_norm_kernel<true>), dim3((unsigned)t.blocks), dim3(256), 0, st, t, partial + done);
+    else hipLaunchKernelGGL((grad_norm_kernel<false>), dim3((unsigned)t.blocks), dim3(256), 0, st, t, partial + done);
     done += t.blocks;
     DH_LAUNCH_CHECK();
     return DH_OK;
@@ -197,15 +225,19 @@ extern "C" int dh_grad_clip(const void *const *grads, void *const *out, const in
   DH_CHECK(std::isfinite(scale), "scale %g", scale);
   const hipStream_t st = (hipStream_t)stream;
   float *say = found;
+  int64_t bytes = 0;
+  for (int i = 0; i < n; ++i) bytes += counts[i] * (int64_t)(dtype_size(dtypes[i]) + dtype_size(out_dtypes[i]));
+  const bool nt = stream_hint(bytes);
   const int rc = grad_tables(grads, out, counts, dtypes, out_dtypes, n, [&](const GradTable &t) -> int {
-    hipLaunchKernelGGL(grad_clip_kernel, dim3((unsigned)t.blocks), dim3(256), 0, st, t, sum_sq, max_norm, scale, say);
+    if (nt) hipLaunchKernelGGL((grad_clip_kernel<true>), dim3((unsigned)t.blocks), dim3(256), 0, st, t, sum_sq, max_norm, scale, say);
+    else hipLaunchKernelGGL((grad_clip_kernel<false>), dim3((unsigned)t.blocks), dim3(256), 0, st, t, sum_sq, max_norm, scale, say);
     say = nullptr;
     DH_LAUNCH_CHECK();
     return DH_OK;
   });
   if (rc) return rc;
   if (say) {
-    hipLaunchKernelGGL(grad_clip_kernel, dim3(1), dim3(64), 0, st, GradTable{}, sum_sq, max_norm, scale, say);
+    hipLaunchKernelGGL((grad_clip_kernel<false>), dim3(1), dim3(64), 0, st, GradTable{}, sum_sq, max_norm, scale, say);
     DH_LAUNCH_CHECK();
   }
   return DH_OK;

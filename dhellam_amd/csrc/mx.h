@@ -74,12 +74,50 @@ __device__ __forceinline__ uint32_t quad_umax(uint32_t v) {
   return v > o ? v : o;
 }
 
+// Largest over the lanes l, l ^ 16, l ^ 32 and l ^ 48, in the vector ALU as well: a swap leaves a lane its own value in one result and the
+// other lane's in the other.  PAIRS: two 16-bit values a lane.
+typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
+template <bool PAIRS> __device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) {
+  if constexpr (PAIRS) return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushort2v, a), __builtin_bit_cast(ushort2v, b)));
+  else return a > b ? a : b;
+}
+template <bool PAIRS> __device__ __forceinline__ uint32_t column_umax(uint32_t v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = umax<PAIRS>(r[0], r[1]);
+  const auto q = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return umax<PAIRS>(q[0], q[1]);
+}
+
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 // 8 values of type T at any address that suits T: 16-byte loads, which the hardware takes at any alignment.
 template <typename T> struct alignas(sizeof(T)) Loose8 { T v[8]; };
-template <typename T> __device__ __forceinline__ void load8(float (&f)[8], const T *p) {
-  const Loose8<T> x = *reinterpret_cast<const Loose8<T> *>(p);
+typedef uint32_t loose2_u32x4 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t loose4_u32x4 __attribute__((ext_vector_type(4), aligned(4)));
+template <typename T> struct LooseU4 { using type = loose4_u32x4; };
+template <> struct LooseU4<bf16_t> { using type = loose2_u32x4; };
+template <> struct LooseU4<f16_t> { using type = loose2_u32x4; };
+template <typename T> __device__ __forceinline__ Loose8<T> load_nt(const T *p) {
+  using V = typename LooseU4<T>::type;
+  Loose8<T> x;
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(x) / 16; ++i) {
+    const dh_u32x4 q = __builtin_nontemporal_load(reinterpret_cast<const V *>(p) + i);
+    __builtin_memcpy(reinterpret_cast<char *>(&x) + 16 * i, &q, 16);
+  }
+  return x;
+}
+template <typename T> __device__ __forceinline__ void store_nt(T *p, const Loose8<T> &x) {
+  using V = typename LooseU4<T>::type;
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(x) / 16; ++i) {
+    dh_u32x4 q;
+    __builtin_memcpy(&q, reinterpret_cast<const char *>(&x) + 16 * i, 16);
+    __builtin_nontemporal_store(q, reinterpret_cast<V *>(p) + i);
+  }
+}
+template <typename T, bool NT = false> __device__ __forceinline__ void load8(float (&f)[8], const T *p) {
+  const Loose8<T> x = NT ? load_nt(p) : *reinterpret_cast<const Loose8<T> *>(p);
 #pragma unroll
   for (int j = 0; j < 8; ++j) f[j] = to_f(x.v[j]);
 }

@@ -21,33 +21,68 @@ struct QuantParams {
   int tiles_c;
 };
 
+// What a lane holds of a row: 8 values, 16-bit ones in pairs as they came.
+template <typename T> struct Held8 {
+  static constexpr bool PAIRS = sizeof(T) == 2;
+  static constexpr int N = PAIRS ? 4 : 8;                  // registers
+  uint32_t v[N];
+  __device__ __forceinline__ void load(const T *p) {
+    const Loose8<T> x = *reinterpret_cast<const Loose8<T> *>(p);
+    __builtin_memcpy(v, &x, sizeof(x));
+  }
+  __device__ __forceinline__ void load_first(const T *p, int n) {
+    T x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = j < n ? p[j] : from_f<T>(0.f);
+    __builtin_memcpy(v, x, sizeof(x));
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = 0;
+  }
+  __device__ __forceinline__ float at(int j) const {
+    if constexpr (!PAIRS) return __uint_as_float(v[j]);
+    else return to_f(__builtin_bit_cast(T, (uint16_t)(v[j >> 1] >> (16 * (j & 1)))));
+  }
+};
+// Magnitudes of a register, and the fp32 bits of the one in its half h.
+template <typename T> __device__ __forceinline__ uint32_t mags(uint32_t v) { return v & (sizeof(T) == 2 ? 0x7fff7fffu : 0x7fffffffu); }
+template <typename T> __device__ __forceinline__ uint32_t mag_bits(uint32_t m, int h) {
+  if constexpr (sizeof(T) == 4) return m;
+  else return __float_as_uint(to_f(__builtin_bit_cast(T, (uint16_t)(m >> (16 * h)))));
+}
+
+// Where 8 rows' codes of a column lie in LDS: column c of 16 units of CB bytes.  The 64 lanes that write at once have c = 8 cg + j (cg of 0..15) and
+// units 4 w + rg (rg of 0..3): slots and units are exchanged by bits of cg, so that they fall on all 64 banks; 16 bytes stay together.
+template <bool E4> __device__ __forceinline__ int mx_tile_at(int c, int unit) {
+  if constexpr (E4) return (c ^ ((c >> 3) & 1)) * 128 + ((unit ^ (((c >> 4) & 7) << 1)) << 3);
+  else return (c ^ ((c >> 3) & 3)) * 64 + ((unit ^ (((c >> 5) & 3) << 2)) << 2);
+}
+
 template <typename T, bool E4, bool ROWS, bool COLS>
 __global__ void __launch_bounds__(256) mx_quantise_kernel(const QuantParams p) {
+  using H = Held8<T>;
+  constexpr bool PAIRS = H::PAIRS;
   constexpr int CB = E4 ? 8 : 4;                           // bytes of 8 codes
-  __shared__ __attribute__((aligned(16))) uint8_t tile[COLS ? 128 * (16 * CB + 16) : 16];
+  __shared__ __attribute__((aligned(16))) uint8_t tile[COLS ? 128 * 16 * CB : 16];
   __shared__ __attribute__((aligned(16))) uint8_t sr[ROWS ? 512 : 16], sc[COLS ? 512 : 16];
-  constexpr int TP = 16 * CB + 16;                         // bytes from one row of the tile to the next
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int rg = lane >> 4, cg = lane & 15;
   const int64_t tr = blockIdx.x / p.tiles_c, tc = blockIdx.x % p.tiles_c;
   const int64_t r0 = tr * 128, c0 = tc * 128;
   const int64_t row0 = r0 + 32 * w + 8 * rg, col0 = c0 + 8 * cg;
   const T *x = reinterpret_cast<const T *>(p.x);
-  float v[8][8];
+  H v[8];
   const int64_t left = p.cols - col0;
-  if (left >= 8) {
+  if (r0 + 128 <= p.rows && c0 + 128 <= p.cols) {          // (of the workgroup: no load waits for a comparison)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (row0 + i < p.rows) load8(v[i], x + (row0 + i) * p.ldx + col0);
-      else
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-    }
+    for (int i = 0; i < 8; ++i) v[i].load(x + (row0 + i) * p.ldx + col0);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const bool in = row0 + i < p.rows && left > 0;
-      load8_first(v[i], in ? x + (row0 + i) * p.ldx + col0 : x, in ? (int)left : 0);
+      if (row0 + i < p.rows && left >= 8) v[i].load(x + (row0 + i) * p.ldx + col0);
+      else if (row0 + i < p.rows && left > 0) v[i].load_first(x + (row0 + i) * p.ldx + col0, (int)left);
+      else v[i].clear();
     }
   }
   if constexpr (ROWS) {
@@ -56,9 +91,13 @@ __global__ void __launch_bounds__(256) mx_quantise_kernel(const QuantParams p) {
     for (int i = 0; i < 8; ++i) {
       uint32_t top = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) { const uint32_t m = magnitude(v[i][j]); top = top > m ? top : m; }
-      const uint32_t code = mx_scale_code<E4>(quad_umax(top), p.cover);
-      const MxPack<E4> o = mx_pack<E4>(v[i], code);
+      for (int j = 0; j < H::N; ++j) top = umax<PAIRS>(top, mags<T>(v[i].v[j]));
+      if constexpr (PAIRS) top = top > (top << 16) ? top >> 16 : top & 0xffffu;      // the larger half, below
+      const uint32_t code = mx_scale_code<E4>(mag_bits<T>(quad_umax(top), 0), p.cover);
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = v[i].at(j);
+      const MxPack<E4> o = mx_pack<E4>(f, code);
       const int r = 32 * w + 8 * rg + i;
       if (r0 + r < p.rows) {
         uint8_t *dst = p.codes + (r0 + r) * (E4 ? kp : kp / 2) + (c0 + 8 * cg) / (E4 ? 1 : 2);
@@ -69,22 +108,23 @@ __global__ void __launch_bounds__(256) mx_quantise_kernel(const QuantParams p) {
     }
   }
   if constexpr (COLS) {
+    uint32_t top[H::N];
+#pragma unroll
+    for (int j = 0; j < H::N; ++j) {
+      top[j] = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top[j] = umax<PAIRS>(top[j], mags<T>(v[i].v[j]));
+      top[j] = column_umax<PAIRS>(top[j]);
+    }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      uint32_t top = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) { const uint32_t m = magnitude(v[i][j]); top = top > m ? top : m; }
-      uint32_t o1 = (uint32_t)__shfl_xor((int)top, 16, 64);
-      top = top > o1 ? top : o1;
-      o1 = (uint32_t)__shfl_xor((int)top, 32, 64);
-      top = top > o1 ? top : o1;
-      const uint32_t code = mx_scale_code<E4>(top, p.cover);
+      const uint32_t code = mx_scale_code<E4>(mag_bits<T>(top[PAIRS ? j >> 1 : j], j & 1), p.cover);
       float col[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) col[i] = v[i][j];
+      for (int i = 0; i < 8; ++i) col[i] = v[i].at(j);
       const MxPack<E4> o = mx_pack<E4>(col, code);
       const int c = 8 * cg + j;
-      uint8_t *dst = tile + c * TP + (4 * w + rg) * CB;
+      uint8_t *dst = tile + mx_tile_at<E4>(c, 4 * w + rg);
       if constexpr (E4) *reinterpret_cast<uint2 *>(dst) = uint2{o.lo, o.hi};
       else *reinterpret_cast<uint32_t *>(dst) = o.lo;
       if (rg == 0) sc[(c >> 2) * 16 + w * 4 + (c & 3)] = (uint8_t)code;
@@ -106,7 +146,8 @@ __global__ void __launch_bounds__(256) mx_quantise_kernel(const QuantParams p) {
     for (int it = 0; it < 128 * LPR / 256; ++it) {
       const int c = (it * 256 + tid) / LPR, b = (it * 256 + tid) % LPR;
       if (c0 + c < p.cols)
-        *reinterpret_cast<dh_u32x4 *>(p.codes_t + (c0 + c) * ldt + tr * (16 * CB) + b * 16) = *reinterpret_cast<const dh_u32x4 *>(tile + c * TP + b * 16);
+        *reinterpret_cast<dh_u32x4 *>(p.codes_t + (c0 + c) * ldt + tr * (16 * CB) + b * 16) =
+            *reinterpret_cast<const dh_u32x4 *>(tile + mx_tile_at<E4>(c, b * (16 / CB)));
     }
   }
 }
@@ -131,85 +172,126 @@ struct NormMxParams {
   float eps, shift;
 };
 
-template <typename T> __device__ __forceinline__ void store8(T *p, const float (&f)[8], int n) {
+// (without NT the accesses keep their lines in the caches; with it, where a call moves more than these hold, they do not displace others)
+template <typename T, bool NT> __device__ __forceinline__ void store8(T *p, const Loose8<T> &o, int n) {
   if (n >= 8) {
-    Loose8<T> o;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) o.v[j] = from_f<T>(f[j]);
-    *reinterpret_cast<Loose8<T> *>(p) = o;
+    if constexpr (NT) store_nt(p, o);
+    else *reinterpret_cast<Loose8<T> *>(p) = o;
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (j < n) p[j] = from_f<T>(f[j]);
+      if (j < n) p[j] = o.v[j];
   }
 }
-
-// x + residual of 8 columns, rounded to T as a separate addition stores it
-template <typename T, bool RES>
-__device__ __forceinline__ void norm_row8(float (&f)[8], const NormMxParams &p, int64_t at, int n) {
-  const T *x = reinterpret_cast<const T *>(p.x) + at;
-  if (n >= 8) load8(f, x);
-  else load8_first(f, n > 0 ? x : reinterpret_cast<const T *>(p.x), n);
-  if constexpr (RES) {
-    if (n > 0) {
-      float r[8];
-      const T *q = reinterpret_cast<const T *>(p.residual) + at;
-      if (n >= 8) load8(r, q);
-      else load8_first(r, q, n);
+template <typename T> __device__ __forceinline__ Loose8<T> rounded8(const float (&f)[8]) {
+  Loose8<T> o;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = to_f(from_f<T>(f[j] + r[j]));
-    }
+  for (int j = 0; j < 8; ++j) o.v[j] = from_f<T>(f[j]);
+  return o;
+}
+// 8 columns of which n exist (WHOLE: all or none), zeros for the others
+template <typename T, bool WHOLE, bool NT> __device__ __forceinline__ Loose8<T> fetch8(const T *p, int n) {
+  Loose8<T> x;
+  if (n >= 8) {
+    x = NT ? load_nt(p) : *reinterpret_cast<const Loose8<T> *>(p);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x.v[j] = from_f<T>(0.f);
+    if (!WHOLE)
+#pragma unroll
+      for (int j = 0; j < 7; ++j)
+        if (j < n) x.v[j] = p[j];
   }
+  return x;
+}
+// x + residual, rounded to T as a separate addition stores it
+template <typename T> __device__ __forceinline__ Loose8<T> sum8(const Loose8<T> &a, const Loose8<T> &b) {
+  Loose8<T> o;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) o.v[j] = from_f<T>(to_f(a.v[j]) + to_f(b.v[j]));
+  return o;
+}
+template <typename T> __device__ __forceinline__ float squares8(const Loose8<T> &a) {
+  float s = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) s += to_f(a.v[j]) * to_f(a.v[j]);
+  return s;
+}
+// The result of 8 columns (n exist) of a row: y, codes; returns the block's scale code (the same in the quad).
+template <typename T> __device__ __forceinline__ uint32_t norm_out8(const NormMxParams &p, const Loose8<T> &x, const Loose8<T> &gamma, float rs, int64_t row, int g,
+                                                                    int64_t kp, bool active) {
+  const int n = p.cols - 8 * g;
+  float y[8];
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    y[j] = to_f(x.v[j]) * rs * (to_f(gamma.v[j]) + p.shift);
+    if (n < 8 && j >= n) y[j] = 0.f;                       // (a row of infinities or NaN makes products of zeros NaN)
+    const uint32_t m = magnitude(y[j]);
+    top = top > m ? top : m;
+  }
+  if (p.y && active && n > 0) store8<T, false>(reinterpret_cast<T *>(p.y) + row * p.cols + 8 * g, rounded8<T>(y), n);
+  const uint32_t code = mx_scale_code<true>(quad_umax(top), p.cover);
+  if (active) {
+    const MxPack<true> o = mx_pack<true>(y, code);
+    *reinterpret_cast<uint2 *>(p.codes + row * kp + 8 * g) = uint2{o.lo, o.hi};
+  }
+  return active ? code : 0u;
 }
 
-template <typename T, int BT, int TPR, int VPT, bool RES>
-__global__ void __launch_bounds__(BT) norm_mx_kernel(const NormMxParams p) {
-  constexpr int RPB = BT / TPR;
-  __shared__ float red[BT / 64];
+// TPR threads a row, ROWS rows a workgroup; gamma stays in registers.  All loads of a row go out before anything waits for one.
+template <typename T, int TPR, int VPT, int ROWS, bool WHOLE, bool RES, bool NT>
+__global__ void __launch_bounds__(TPR *ROWS, VPT == 4 ? 4 : 1) norm_mx_kernel(const NormMxParams p) {
+  constexpr int WPR = TPR / 64;
+  __shared__ float red[2][WPR * ROWS];
   const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
   const int groups = (p.cols + 127) / 128 * 16;
   const int64_t kp = (int64_t)groups * 8, cells = (p.rows + 3) / 4;
   const float inv_cols = 1.0f / (float)p.cols;
-  for (int64_t row0 = (int64_t)blockIdx.x * RPB; row0 < 4 * cells; row0 += (int64_t)gridDim.x * RPB) {
+  const T *x = reinterpret_cast<const T *>(p.x), *res = reinterpret_cast<const T *>(p.residual);
+  Loose8<T> gamma[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int g = lane + i * TPR;
+    gamma[i] = fetch8<T, WHOLE, false>(reinterpret_cast<const T *>(p.gamma) + 8 * g, p.cols - 8 * g);
+  }
+  int turn = 0;
+  for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < 4 * cells; row0 += (int64_t)gridDim.x * ROWS, turn ^= 1) {
     const int64_t row = row0 + sub;
     const bool active = row < p.rows;
-    float v[VPT][8];
+    Loose8<T> held[VPT], add[RES ? VPT : 1];               // the row as it is normalised, in its own type
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int g = lane + i * TPR, n = active ? p.cols - 8 * g : 0;
+      held[i] = fetch8<T, WHOLE, NT>(x + row * p.cols + 8 * g, n);
+      if constexpr (RES) add[i] = fetch8<T, WHOLE, NT>(res + row * p.cols + 8 * g, n);
+    }
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int g = lane + i * TPR;
-      const int n = active ? p.cols - 8 * g : 0;
-      norm_row8<T, RES>(v[i], p, row * p.cols + 8 * g, n);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) s += v[i][j] * v[i][j];
-      if (RES && n > 0) store8(reinterpret_cast<T *>(p.sum_out) + row * p.cols + 8 * g, v[i], n);
+      const int g = lane + i * TPR, n = active ? p.cols - 8 * g : 0;
+      if constexpr (RES) {
+        held[i] = sum8(held[i], add[i]);
+        if (n > 0) store8<T, NT>(reinterpret_cast<T *>(p.sum_out) + row * p.cols + 8 * g, held[i], n);
+      }
+      s += squares8(held[i]);
     }
-    s = TPR == 64 ? wave_sum(s) : block_sum<BT>(s, red);
+    s = wave_sum(s);
+    if constexpr (WPR > 1) {                               // (two sets of sums: the next row's are written before every wavefront has read these)
+      if ((threadIdx.x & 63) == 0) red[turn][threadIdx.x >> 6] = s;
+      __syncthreads();
+      s = 0.f;
+#pragma unroll
+      for (int i = 0; i < WPR; ++i) s += red[turn][sub * WPR + i];
+    }
     const float rs = 1.0f / sqrtf(s * inv_cols + p.eps);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int g = lane + i * TPR;
-      if (g >= groups || row >= 4 * cells) continue;       // (16 lanes at a time: groups is a multiple of 16)
-      const int n = p.cols - 8 * g;
-      float gm[8];
-      const T *gamma = reinterpret_cast<const T *>(p.gamma) + 8 * g;
-      if (n >= 8) load8(gm, gamma);
-      else load8_first(gm, n > 0 ? gamma : reinterpret_cast<const T *>(p.gamma), n);
-      uint32_t top = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[i][j] = n > j && active ? v[i][j] * rs * (gm[j] + p.shift) : 0.f;
-        const uint32_t m = magnitude(v[i][j]);
-        top = top > m ? top : m;
-      }
-      if (p.y && active && n > 0) store8(reinterpret_cast<T *>(p.y) + row * p.cols + 8 * g, v[i], n);
-      const uint32_t code = mx_scale_code<true>(quad_umax(top), p.cover);
-      if (active) {
-        const MxPack<true> o = mx_pack<true>(v[i], code);
-        *reinterpret_cast<uint2 *>(p.codes + row * kp + 8 * g) = uint2{o.lo, o.hi};
-      }
-      if ((lane & 3) == 0)
-        p.scales[((int64_t)(g >> 4) * cells + (row >> 2)) * 16 + ((g >> 2) & 3) * 4 + (row & 3)] = active ? (uint8_t)code : 0;
+      if (g >= groups) continue;                           // (16 lanes at a time: groups is a multiple of 16)
+      const uint32_t code = norm_out8<T>(p, held[i], gamma[i], rs, row, g, kp, active);
+      if ((lane & 3) == 0 && row < 4 * cells)
+        p.scales[((int64_t)(g >> 4) * cells + (row >> 2)) * 16 + ((g >> 2) & 3) * 4 + (row & 3)] = (uint8_t)code;
     }
     if (active && lane == 0) p.rsigma[row] = rs;
   }
@@ -221,60 +303,52 @@ __global__ void __launch_bounds__(1024) norm_mx_long_kernel(const NormMxParams p
   __shared__ float red[16];
   const int groups = (p.cols + 127) / 128 * 16;
   const int64_t kp = (int64_t)groups * 8, cells = (p.rows + 3) / 4;
+  const T *res = reinterpret_cast<const T *>(p.residual);
   for (int64_t row = blockIdx.x; row < 4 * cells; row += gridDim.x) {
     const bool active = row < p.rows;
+    const T *x = reinterpret_cast<const T *>(p.x) + row * p.cols;
     float s = 0.f;
     for (int g = threadIdx.x; active && g < groups; g += 1024) {
-      float v[8];
       const int n = p.cols - 8 * g;
-      norm_row8<T, RES>(v, p, row * p.cols + 8 * g, n);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) s += v[j] * v[j];
-      if (RES && n > 0) store8(reinterpret_cast<T *>(p.sum_out) + row * p.cols + 8 * g, v, n);
+      Loose8<T> v = fetch8<T, false, false>(x + 8 * g, n);
+      if constexpr (RES) {
+        v = sum8(v, fetch8<T, false, false>(res + row * p.cols + 8 * g, n));
+        if (n > 0) store8<T, false>(reinterpret_cast<T *>(p.sum_out) + row * p.cols + 8 * g, v, n);
+      }
+      s += squares8(v);
     }
     s = block_sum<1024>(s, red);
     const float rs = 1.0f / sqrtf(s / (float)p.cols + p.eps);
-    NormMxParams q = p;
-    if (RES) q.x = p.sum_out;                              // a thread reads what it wrote itself
+    if (RES) x = reinterpret_cast<const T *>(p.sum_out) + row * p.cols;      // a thread reads what it wrote itself
     for (int g = threadIdx.x; g < groups; g += 1024) {
-      float v[8], gm[8];
       const int n = p.cols - 8 * g;
-      norm_row8<T, false>(v, q, row * p.cols + 8 * g, active ? n : 0);
-      const T *gamma = reinterpret_cast<const T *>(p.gamma) + 8 * g;
-      if (n >= 8) load8(gm, gamma);
-      else load8_first(gm, n > 0 ? gamma : reinterpret_cast<const T *>(p.gamma), n);
-      uint32_t top = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[j] = n > j && active ? v[j] * rs * (gm[j] + p.shift) : 0.f;
-        const uint32_t m = magnitude(v[j]);
-        top = top > m ? top : m;
-      }
-      if (p.y && active && n > 0) store8(reinterpret_cast<T *>(p.y) + row * p.cols + 8 * g, v, n);
-      const uint32_t code = mx_scale_code<true>(quad_umax(top), p.cover);
-      if (active) {
-        const MxPack<true> o = mx_pack<true>(v, code);
-        *reinterpret_cast<uint2 *>(p.codes + row * kp + 8 * g) = uint2{o.lo, o.hi};
-      }
+      const Loose8<T> v = fetch8<T, false, false>(x + 8 * g, active ? n : 0), gamma = fetch8<T, false, false>(reinterpret_cast<const T *>(p.gamma) + 8 * g, n);
+      const uint32_t code = norm_out8<T>(p, v, gamma, rs, row, g, kp, active);
       if ((threadIdx.x & 3) == 0)
-        p.scales[((int64_t)(g >> 4) * cells + (row >> 2)) * 16 + ((g >> 2) & 3) * 4 + (row & 3)] = active ? (uint8_t)code : 0;
+        p.scales[((int64_t)(g >> 4) * cells + (row >> 2)) * 16 + ((g >> 2) & 3) * 4 + (row & 3)] = (uint8_t)code;
     }
     if (active && threadIdx.x == 0) p.rsigma[row] = rs;
   }
 }
 
-template <typename T, bool RES> static void launch_norm_mx(const NormMxParams &p, hipStream_t st) {
+template <typename T, bool WHOLE, bool RES> static void launch_norm_mx(const NormMxParams &p, hipStream_t st) {
   const int64_t rows4 = mx_rows4(p.rows);
-  const int64_t most = 256 * 16;
-  auto grid = [&](int64_t per) { return dim3((unsigned)std::min(cdiv(rows4, per), most)); };
-#define DH_NORM_MX(BT, TPR, VPT) hipLaunchKernelGGL((norm_mx_kernel<T, BT, TPR, VPT, RES>), grid(BT / TPR), dim3(BT), 0, st, p)
-  if (p.cols <= 512) DH_NORM_MX(256, 64, 1);
-  else if (p.cols <= 1024) DH_NORM_MX(256, 64, 2);
-  else if (p.cols <= 2048) DH_NORM_MX(256, 256, 1);
-  else if (p.cols <= 4096) DH_NORM_MX(256, 256, 2);
-  else if (p.cols <= 8192) DH_NORM_MX(256, 256, 4);
-  else if (p.cols <= 16384) DH_NORM_MX(1024, 1024, 2);
-  else hipLaunchKernelGGL((norm_mx_long_kernel<T, RES>), grid(1), dim3(1024), 0, st, p);
+  const bool nt = stream_hint(p.rows * p.cols * (int64_t)(sizeof(T) * (RES ? 3 : 1) + 1));
+  auto grid = [&](int64_t per, int64_t most) { return dim3((unsigned)std::min(cdiv(rows4, per), most)); };
+#define DH_NORM_MX(TPR, VPT, ROWS)                                                                                                                      \
+  do {                                                                                                                                                \
+    const dim3 g = grid(ROWS, 256 * 8);                                                                                                                 \
+    if (nt) hipLaunchKernelGGL((norm_mx_kernel<T, TPR, VPT, ROWS, WHOLE, RES, true>), g, dim3(TPR * ROWS), 0, st, p);                                    \
+    else hipLaunchKernelGGL((norm_mx_kernel<T, TPR, VPT, ROWS, WHOLE, RES, false>), g, dim3(TPR * ROWS), 0, st, p);                                      \
+  } while (0)
+  if (p.cols <= 512) DH_NORM_MX(64, 1, 4);
+  else if (p.cols <= 1024) DH_NORM_MX(64, 2, 4);
+  else if (p.cols <= 8192 && p.rows <= 256) DH_NORM_MX(1024, 1, 1);
+  else if (p.cols <= 2048) DH_NORM_MX(256, 1, 1);
+  else if (p.cols <= 4096) DH_NORM_MX(256, 2, 1);
+  else if (p.cols <= 8192) DH_NORM_MX(256, 4, 1);
+  else if (p.cols <= 16384) DH_NORM_MX(1024, 2, 1);
+  else hipLaunchKernelGGL((norm_mx_long_kernel<T, RES>), grid(1, 256 * 16), dim3(1024), 0, st, p);
 #undef DH_NORM_MX
 }
 
@@ -310,8 +384,9 @@ extern "C" int dh_rmsnorm_mx(const void *x, const void *residual, void *sum_out,
   DH_CHECK(dh::aligned16(codes) && dh::aligned16(scales), "codes and scales must be 16-byte aligned");
   const dh::NormMxParams p{x, residual, gamma, sum_out, y, (uint8_t *)codes, (uint8_t *)scales, rsigma, rows, (int)cols, cover, eps,
                            zero_centered_gamma ? 1.0f : 0.0f};
-  DH_DISPATCH_DTYPE(dtype, if (residual) dh::launch_norm_mx<T, true>(p, (hipStream_t)stream);
-                    else dh::launch_norm_mx<T, false>(p, (hipStream_t)stream));
+  const hipStream_t st = (hipStream_t)stream;
+  DH_DISPATCH_DTYPE(dtype, if (cols % 8 == 0) { if (residual) dh::launch_norm_mx<T, true, true>(p, st); else dh::launch_norm_mx<T, true, false>(p, st); }
+                    else { if (residual) dh::launch_norm_mx<T, false, true>(p, st); else dh::launch_norm_mx<T, false, false>(p, st); });
   DH_LAUNCH_CHECK();
   return DH_OK;
 }
