@@ -1217,11 +1217,15 @@ void zero_all(const std::vector<Tensor> &ts, const OptStream &stream) {
 }
 
 // ---- microscaled operands -----------------------------------------------------------------------------------------------
-// Codes and scales of a rows x cols matrix in the given format (layout: include/dhellam_hip.h).
+// Codes and scales of a rows x cols matrix in the given format (layout: include/dhellam_hip.h), one allocation for the two.
 std::pair<Tensor, Tensor> mx_empty(int64_t rows, int64_t cols, int format, const Tensor &like) {
-  const int64_t kp = (cols + 127) / 128 * 128;
-  const auto bytes = like.options().dtype(at::kByte);
-  return {at::empty({rows, format == DH_MX_E4M3 ? kp : kp / 2}, bytes), at::empty({kp / 128, (rows + 3) / 4, 4, 4}, bytes)};
+  const int64_t kp = (cols + 127) / 128 * 128, width = format == DH_MX_E4M3 ? kp : kp / 2, cells = (rows + 3) / 4;
+  Tensor codes = at::empty({rows * width + kp / 128 * cells * 16}, like.options().dtype(at::kByte));      // (width is a multiple of 64)
+  Tensor scales = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(codes.storage()), codes.key_set(), codes.dtype());
+  scales.unsafeGetTensorImpl()->set_storage_offset(rows * width);
+  scales.unsafeGetTensorImpl()->set_sizes_contiguous({kp / 128, cells, 4, 4});
+  codes.unsafeGetTensorImpl()->set_sizes_contiguous({rows, width});
+  return {std::move(codes), std::move(scales)};
 }
 
 int mx_format(int64_t format) {
