@@ -102,6 +102,29 @@ __device__ __forceinline__ void mx_mma_tied(const VB &b, uint32_t sb, const VA &
                : "v"(b), "v"(a), "v"(sb), "v"(sa), "n"(SELB & 1), "n"(SELA & 1), "n"(SELB >> 1), "n"(SELA >> 1), "n"(FB == 8 ? 0 : 4), "n"(FA == 8 ? 0 : 4));
 #endif
 }
+// 32 x 32 x 64 of 4 bits, for which this is the faster form: lane l holds block l / 32 (k = 32 (l / 32) and on) of row l % 32; D[row = 8 (v / 4) + 4
+// (l / 32) + v % 4][col = l % 32].  In a loop of nothing else the matrix pipes are busy for 91 to 94 % of the time with it and 53 to 72 % with 16 x
+// 16 x 128 (one to four wavefronts a SIMD), whose instruction takes longer to issue than its 16 cycles; on random data, where the board's power
+// bounds both, 6.5 against 5.9 PFLOP/s.  (With an 8-bit operand it is the other way round: 4.05 against 4.36.)
+template <int SELB, int SELA> __device__ __forceinline__ void mx_mma32_tied(const int4v &b, uint32_t sb, const int4v &a, uint32_t sa, floatx16 &c) {
+#ifdef __HIP_DEVICE_COMPILE__
+  asm volatile("v_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%c5,%c6,0] op_sel_hi:[%c7,%c8,0] cbsz:4 blgp:4"
+               : "+v"(c)
+               : "v"(b), "v"(a), "v"(sb), "v"(sa), "n"(SELB & 1), "n"(SELA & 1), "n"(SELB >> 1), "n"(SELA >> 1));
+#endif
+}
+// The four dwords of a cell are blocks 0..3 of its 128 columns, a row a byte.  Of a lane's two rows y and y + 2: bytes [block][row] of blocks 0, 1
+// and 2, 3.  Of its one row y: the four blocks.
+__device__ __forceinline__ void mx_cell_rows2(uint32_t (&s)[2], const int4v &cell, uint32_t y) {
+  const uint32_t sel = 0x06040200u + y * 0x01010101u;
+  s[0] = __builtin_amdgcn_perm((uint32_t)cell[1], (uint32_t)cell[0], sel);
+  s[1] = __builtin_amdgcn_perm((uint32_t)cell[3], (uint32_t)cell[2], sel);
+}
+__device__ __forceinline__ uint32_t mx_cell_row1(const int4v &cell, uint32_t y) {
+  const uint32_t sel = 0x0400u + y * 0x0101u;
+  const uint32_t lo = __builtin_amdgcn_perm((uint32_t)cell[1], (uint32_t)cell[0], sel), hi = __builtin_amdgcn_perm((uint32_t)cell[3], (uint32_t)cell[2], sel);
+  return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+}
 template <int BITS> __device__ __forceinline__ auto mx_narrow(const int4v *q, int ks) {
   if constexpr (BITS == 8) return mx_v8i{q[0][0], q[0][1], q[0][2], q[0][3], q[1][0], q[1][1], q[1][2], q[1][3]};
   else return q[ks];
@@ -294,12 +317,16 @@ __global__ void __launch_bounds__(512) mx_w8_kernel(const MxGemmParams p) {
   constexpr uint32_t REGA = 128 * RA, REGB = 128 * RB, OFF_B = 2 * REGA, STAGEB = OFF_B + 2 * REGB;
   constexpr uint32_t RING = 2 * STAGEB, SLOT = KS * 2048;        // scales of a slice: a's, then b's
   constexpr int COPIES = KS + 2 * NA + 2 * NB;                   // of a wavefront a slice
+  constexpr bool B32 = KS == 2;                                  // in blocks of 32 x 32 x 64; else 16 x 16 x 128
+  constexpr int SIDE = B32 ? 32 : 16, ABLK = 64 / SIDE, BBLK = 32 / SIDE;      // blocks of a half's 64 rows of a, 32 of b
+  constexpr int APART = B32 ? 4 : NA, BPART = B32 ? 4 : NB;      // 16-byte reads of a block
+  using Acc = std::conditional_t<B32, floatx16, floatx4>;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[RING + 3 * SLOT];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = w >> 2, wn = w & 3;
-  const int c = lane & 15, g4 = lane >> 4;
+  const int c = lane & (SIDE - 1), g4 = lane / SIDE;
   const uint32_t lds0 = (uint32_t)(uintptr_t)smem;
   const uint32_t lda = (uint32_t)p.steps * MxBytes<FA>::STEP, ldb = (uint32_t)p.steps * MxBytes<FB>::STEP;
 
@@ -309,21 +336,24 @@ __global__ void __launch_bounds__(512) mx_w8_kernel(const MxGemmParams p) {
   for (int x = 0; x < NA; ++x) {
     const int s = NA == 2 ? 8 * (2 * w + x) + (lane >> 3) : 16 * w + (lane >> 2);
     const int chunk = NA == 2 ? (lane & 7) ^ ((s >> 1) & 7) : (lane & 3) ^ ((s >> 2) & 3);
-    ca[x] = (uint32_t)(64 * (s >> 6) + 4 * (s & 15) + ((s >> 4) & 3)) * lda + (uint32_t)(chunk * 16);
+    ca[x] = (uint32_t)(64 * (s >> 6) + 4 * (s & 15) + (B32 ? 2 * ((s >> 5) & 1) + ((s >> 4) & 1) : (s >> 4) & 3)) * lda + (uint32_t)(chunk * 16);
   }
 #pragma unroll
   for (int x = 0; x < NB; ++x) {
     const int s = NB == 2 ? 8 * (2 * w + x) + (lane >> 3) : 16 * w + (lane >> 2);
     const int chunk = NB == 2 ? (lane & 7) ^ ((s >> 1) & 7) : (lane & 3) ^ ((s >> 2) & 3);
-    cb[x] = (uint32_t)(32 * (s >> 5) + 2 * (s & 15) + ((s >> 4) & 1)) * ldb + (uint32_t)(chunk * 16);
+    cb[x] = (uint32_t)(32 * (s >> 5) + (B32 ? 4 * (s & 7) + ((s >> 3) & 3) : 2 * (s & 15) + ((s >> 4) & 1))) * ldb + (uint32_t)(chunk * 16);
   }
   const uint32_t cs = (uint32_t)(lane * 4);
 
   // ---- fragments and scales
-  const uint32_t fa_lane = (uint32_t)((wm * 64 + c) * RA + (NA == 2 ? (g4 ^ ((c >> 1) & 7)) : (g4 ^ (c >> 2))) * 16);   // chunk 4 + g4: XOR 64; block: + 16 RA
-  const uint32_t fb_lane = (uint32_t)((wn * 32 + c) * RB + (NB == 2 ? (g4 ^ ((c >> 1) & 7)) : (g4 ^ (c >> 2))) * 16);
-  const uint32_t sa_lane = (uint32_t)(wm * 256 + c * 16 + g4 * 4);                              // half: + 512; step: + 1024
-  const uint32_t sb_lane = (uint32_t)(KS * 1024 + wn * 128 + (c >> 1) * 16 + g4 * 4 + 2 * (c & 1));
+  // chunk of a block's first read; the next: B32 the next chunk (a lane's half is one of the slice's two steps), else 4 chunks on
+  constexpr uint32_t NEXT = B32 ? 16 : 64;
+  const uint32_t qa = NA == 2 ? (B32 ? 4 * g4 : g4) ^ ((c >> 1) & 7) : g4 ^ (c >> 2), qb = NB == 2 ? (B32 ? 4 * g4 : g4) ^ ((c >> 1) & 7) : g4 ^ (c >> 2);
+  const uint32_t fa_lane = (uint32_t)((wm * 64 + c) * RA) + qa * 16, fb_lane = (uint32_t)((wn * 32 + c) * RB) + qb * 16;
+  // half: + 512; 16 x 16: step: + 1024
+  const uint32_t sa_lane = (uint32_t)(wm * 256 + (c & 15) * 16) + (uint32_t)(B32 ? g4 * 1024 : g4 * 4);
+  const uint32_t sb_lane = (uint32_t)(KS * 1024 + wn * 128) + (uint32_t)(B32 ? g4 * 1024 + (c & 7) * 16 : (c >> 1) * 16 + g4 * 4 + 2 * (c & 1));
   typedef __attribute__((address_space(3))) const int4v *lds_chunk;
   typedef __attribute__((address_space(3))) const uint32_t *lds_dword;
   typedef __attribute__((address_space(3))) const uint16_t *lds_half;
@@ -377,48 +407,70 @@ __global__ void __launch_bounds__(512) mx_w8_kernel(const MxGemmParams p) {
       copy_256(cs, rss0, (uint32_t)(s0 + s) * gs0 + quarter, at + to);
     }
   };
-  floatx4 acc[2][2][4][2];
+  Acc acc[2][2][ABLK][BBLK];
 #pragma unroll
-  for (int i = 0; i < 32; ++i) acc[i >> 4][(i >> 3) & 1][(i >> 1) & 3][i & 1] = floatx4{0.f, 0.f, 0.f, 0.f};
-  int4v fa[2][4][NA], fb[2][2][NB];
-  uint32_t sa[2][KS], sb[2][KS];
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int b = 0; b < ABLK; ++b)
+#pragma unroll
+      for (int j = 0; j < BBLK; ++j) acc[i >> 1][i & 1][b][j] = Acc{};
+  int4v fa[2][ABLK][APART], fb[2][BBLK][BPART];
+  // scales as the instructions take them: 16 x 16: [half][step], a byte a block; 32 x 32: a's [half][steps 0, 1 / 2, 3 of 64], b's four steps in one;
+  // a cell just read is taken apart behind the next wait
+  uint32_t sa[2][2], sb[2][KS];
+  int4v cell;
   auto mma_quarter = [&](int qm, int qn, auto rd) {
     __builtin_amdgcn_s_setprio(1);
+    if constexpr (B32) {
 #pragma unroll
-    for (int x = 0; x < 8 * KS; ++x) {
-      const int ks = x >> 3, mi = (x >> 1) & 3, nj = x & 1;
-      const auto vb = mx_narrow<FB>(fb[qn][nj], ks);
-      const auto va = mx_narrow<FA>(fa[qm][mi], ks);
-      floatx4 &sum = acc[qm][qn][mi][nj];
-#define MX_SEL(j, i) if (nj == j && mi == i) mx_mma_tied<FA, FB, j, i>(vb, sb[qn][ks], va, sa[qm][ks], sum)
-      MX_SEL(0, 0); MX_SEL(0, 1); MX_SEL(0, 2); MX_SEL(0, 3);
-      MX_SEL(1, 0); MX_SEL(1, 1); MX_SEL(1, 2); MX_SEL(1, 3);
+      for (int x = 0; x < 8; ++x) {
+        const int t = x >> 1, b = x & 1;
+#define MX_SEL(j, i) if (t == j && b == i) mx_mma32_tied<j, 2 * (j & 1) + i>(fb[qn][0][t], sb[qn][0], fa[qm][b][t], sa[qm][t >> 1], acc[qm][qn][b][0])
+        MX_SEL(0, 0); MX_SEL(0, 1); MX_SEL(1, 0); MX_SEL(1, 1);
+        MX_SEL(2, 0); MX_SEL(2, 1); MX_SEL(3, 0); MX_SEL(3, 1);
 #undef MX_SEL
-      if (x % KS == KS - 1) {
         __builtin_amdgcn_sched_barrier(0);
-        rd(x / KS);
+        rd(x);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const int mi = x >> 1, nj = x & 1;
+        const auto vb = mx_narrow<FB>(fb[qn][nj], 0);
+        const auto va = mx_narrow<FA>(fa[qm][mi], 0);
+        floatx4 &sum = acc[qm][qn][mi][nj];
+#define MX_SEL(j, i) if (nj == j && mi == i) mx_mma_tied<FA, FB, j, i>(vb, sb[qn][0], va, sa[qm][0], sum)
+        MX_SEL(0, 0); MX_SEL(0, 1); MX_SEL(0, 2); MX_SEL(0, 3);
+        MX_SEL(1, 0); MX_SEL(1, 1); MX_SEL(1, 2); MX_SEL(1, 3);
+#undef MX_SEL
+        __builtin_amdgcn_sched_barrier(0);
+        rd(x);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
     __builtin_amdgcn_s_setprio(0);
   };
-  auto read_a = [&](int h, uint32_t region, int x0, int x1) {    // reads x0..x1 of the half's 4 NA
+  auto read_a = [&](int h, uint32_t region, int x0, int x1) {    // reads x0..x1 of the half's ABLK APART
 #pragma unroll
     for (int x = x0; x < x1; ++x)
-      if (x < 4 * NA) fa[h][x & 3][x >> 2] = *(lds_chunk)(region + (fa_lane ^ (uint32_t)((x >> 2) << 6)) + (uint32_t)((x & 3) * 16 * RA));
+      if (x < ABLK * APART)
+        fa[h][x % ABLK][x / ABLK] = *(lds_chunk)(region + (fa_lane ^ (uint32_t)(x / ABLK) * NEXT) + (uint32_t)(x % ABLK * SIDE * RA));
   };
   auto read_b = [&](int h, uint32_t region, uint32_t slot) {
 #pragma unroll
-    for (int i = 0; i < NB; ++i)
+    for (int i = 0; i < BPART; ++i)
 #pragma unroll
-      for (int nj = 0; nj < 2; ++nj) fb[h][nj][i] = *(lds_chunk)(region + (fb_lane ^ (uint32_t)(i << 6)) + (uint32_t)(nj * 16 * RB));
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) sb[h][ks] = *(lds_half)(lds0 + slot + sb_lane + (uint32_t)(h * 512 + ks * 1024));
+      for (int nj = 0; nj < BBLK; ++nj) fb[h][nj][i] = *(lds_chunk)(region + (fb_lane ^ (uint32_t)i * NEXT) + (uint32_t)(nj * SIDE * RB));
+    if constexpr (B32) cell = *(lds_chunk)(lds0 + slot + sb_lane + (uint32_t)(h * 512));
+    else sb[h][0] = *(lds_half)(lds0 + slot + sb_lane + (uint32_t)(h * 512));
   };
   auto read_sa = [&](int h, uint32_t slot) {
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) sa[h][ks] = *(lds_dword)(lds0 + slot + sa_lane + (uint32_t)(h * 512 + ks * 1024));
+    if constexpr (B32) cell = *(lds_chunk)(lds0 + slot + sa_lane + (uint32_t)(h * 512));
+    else sa[h][0] = *(lds_dword)(lds0 + slot + sa_lane + (uint32_t)(h * 512));
   };
+  auto take_sa = [&](int h) { if constexpr (B32) mx_cell_rows2(sa[h], cell, (uint32_t)c >> 4); };
+  auto take_sb = [&](int h) { if constexpr (B32) sb[h][0] = mx_cell_row1(cell, (uint32_t)c >> 3); };
 #define MX_BARRIER()                        \
   do {                                      \
     __builtin_amdgcn_sched_barrier(0);      \
@@ -442,6 +494,7 @@ __global__ void __launch_bounds__(512) mx_w8_kernel(const MxGemmParams p) {
   if (w >= 4) MX_BARRIER();
   read_a(0, lds0, 0, 8);
   read_sa(0, r0);
+  take_sa(0);
   read_b(0, lds0 + OFF_B, r0);
   uint32_t cur = 0;
   auto slice = [&](auto fc, int s) {
@@ -449,11 +502,13 @@ __global__ void __launch_bounds__(512) mx_w8_kernel(const MxGemmParams p) {
     const uint32_t nxt = STAGEB - cur, a0 = lds0 + cur, b0 = a0 + OFF_B, na = lds0 + nxt, nb = na + OFF_B;
     turn_to(s + 2);
     MX_READS_DONE();
+    take_sb(F);
     read_b(G, b0 + G * REGB, r0);
     MX_BARRIER();
     mma_quarter(0, F, [&](int x) { if (x < 3) read_a(1, a0 + REGA, x, x + 1); });
     MX_BARRIER();
     MX_READS_DONE();
+    take_sb(G);
     read_a(1, a0 + REGA, 3, 6);
     read_sa(1, r0);
     copy_s(s + 2, r2);
@@ -462,6 +517,7 @@ __global__ void __launch_bounds__(512) mx_w8_kernel(const MxGemmParams p) {
     mma_quarter(0, G, [&](int x) { if (x < 2) read_a(1, a0 + REGA, 6 + x, 7 + x); });
     MX_BARRIER();
     MX_READS_DONE();
+    take_sa(1);
     read_a(0, na, 0, 3);
     read_sa(0, r1);
     copy_b(F, s + 2, cur);
@@ -469,6 +525,7 @@ __global__ void __launch_bounds__(512) mx_w8_kernel(const MxGemmParams p) {
     mma_quarter(1, G, [&](int x) { if (x < 3) read_a(0, na, 3 + x, 4 + x); });
     MX_BARRIER();
     MX_READS_DONE();
+    take_sa(0);
     read_b(G, nb + G * REGB, r1);
     copy_b(G, s + 2, cur);
     copy_a(1, s + 2, cur);
@@ -494,23 +551,29 @@ __global__ void __launch_bounds__(512) mx_w8_kernel(const MxGemmParams p) {
   // the last sums are there: 16 passes of 4 cycles behind the last instruction at most, and nothing reads them before
   asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
 #pragma unroll
-  for (int i = 0; i < 32; ++i) asm volatile("" : "+v"(acc[i >> 4][(i >> 3) & 1][(i >> 1) & 3][i & 1]));
-  // a lane's 8 columns 8 g4 .. of row 4 c + mi of a quarter's 64 rows x 32 columns
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int b = 0; b < ABLK; ++b)
+#pragma unroll
+      for (int j = 0; j < BBLK; ++j) asm volatile("" : "+v"(acc[i >> 1][i & 1][b][j]));
+  // a lane's columns of a row of a quarter's 64 rows x 32 columns: 16 x 16: 8 g4 .. + 7 of row 4 c + block; 32 x 32: 16 g4 .. + 15 of row 4 (c % 16) +
+  // 2 block + c / 16
+  constexpr int COLS = B32 ? 16 : 8;
 #pragma unroll
   for (int qm = 0; qm < 2; ++qm)
 #pragma unroll
-    for (int mi = 0; mi < 4; ++mi) {
-      const int64_t row = m0 + 128 * qm + 64 * wm + 4 * c + mi;
+    for (int b = 0; b < ABLK; ++b) {
+      const int64_t row = m0 + 128 * qm + 64 * wm + (B32 ? 4 * (c & 15) + 2 * b + (c >> 4) : 4 * c + b);
       if (row >= p.m) continue;
 #pragma unroll
       for (int qn = 0; qn < 2; ++qn) {
-        const int64_t col = n0 + 128 * qn + 32 * wn + 8 * g4;
+        const int64_t col = n0 + 128 * qn + 32 * wn + COLS * g4;
         if (col >= p.n) continue;
-        float v[8];
+        float v[COLS];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = acc[qm][qn][mi][i & 1][i >> 1];
-        if (p.pieces > 1) mx_store<float, 8>(p.ws + ((int64_t)piece * p.m + row) * (4 * p.cells_b) + col, v, 4 * p.cells_b - col, 1, 0);
-        else mx_store<TO, 8>(reinterpret_cast<TO *>(p.c) + row * p.ldc + col, v, p.n - col, p.vec, p.accumulate);
+        for (int i = 0; i < COLS; ++i) v[i] = B32 ? acc[qm][qn][b][0][4 * (i & 3) + (i >> 2)] : acc[qm][qn][b][(i & 1) % BBLK][(i >> 1) & 3];
+        if (p.pieces > 1) mx_store<float, COLS>(p.ws + ((int64_t)piece * p.m + row) * (4 * p.cells_b) + col, v, 4 * p.cells_b - col, 1, 0);
+        else mx_store<TO, COLS>(reinterpret_cast<TO *>(p.c) + row * p.ldc + col, v, p.n - col, p.vec, p.accumulate);
       }
     }
 #undef MX_BARRIER
@@ -533,35 +596,41 @@ __global__ void __launch_bounds__(256, 2) mx_t128_kernel(const MxGemmParams p) {
   constexpr int KS = FA == 4 && FB == 4 ? 2 : 1;
   constexpr int RA = KS * MxBytes<FA>::STEP, RB = KS * MxBytes<FB>::STEP, NA = RA / 64, NB = RB / 64;
   constexpr uint32_t REGA = 128 * RA, REGB = 128 * RB, OFF_S = REGA + REGB, STAGEB = OFF_S + KS * 1024;
+  constexpr bool B32 = KS == 2;                                  // in blocks of 32 x 32 x 64, as in mx_w8_kernel; else 16 x 16 x 128
+  constexpr int SIDE = B32 ? 32 : 16, BLK = 64 / SIDE, APART = B32 ? 4 : NA, BPART = B32 ? 4 : NB;
+  using Acc = std::conditional_t<B32, floatx16, floatx4>;
   constexpr int STAGES = 2, COPIES = KS + 2 * NA + 2 * NB;      // of a wavefront a slice
   __shared__ __attribute__((aligned(1024))) unsigned char smem[STAGES * STAGEB];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = w >> 1, wn = w & 1;
-  const int c = lane & 15, g4 = lane >> 4;
+  const int c = lane & (SIDE - 1), g4 = lane / SIDE;
   const uint32_t lds0 = (uint32_t)(uintptr_t)smem;
   const uint32_t lda = (uint32_t)p.steps * MxBytes<FA>::STEP, ldb = (uint32_t)p.steps * MxBytes<FB>::STEP;
+  auto row_of = [](int s) { return (uint32_t)(64 * (s >> 6) + 4 * (s & 15) + (B32 ? 2 * ((s >> 5) & 1) + ((s >> 4) & 1) : (s >> 4) & 3)); };   // of a slot
   uint32_t ca[2 * NA], cb[2 * NB];
 #pragma unroll
   for (int x = 0; x < 2 * NA; ++x) {
     const int s = NA == 2 ? 8 * (4 * w + x) + (lane >> 3) : 16 * (2 * w + x) + (lane >> 2);
     const int chunk = NA == 2 ? (lane & 7) ^ ((s >> 1) & 7) : (lane & 3) ^ ((s >> 2) & 3);
-    ca[x] = (uint32_t)(64 * (s >> 6) + 4 * (s & 15) + ((s >> 4) & 3)) * lda + (uint32_t)(chunk * 16);
+    ca[x] = row_of(s) * lda + (uint32_t)(chunk * 16);
   }
 #pragma unroll
   for (int x = 0; x < 2 * NB; ++x) {
     const int s = NB == 2 ? 8 * (4 * w + x) + (lane >> 3) : 16 * (2 * w + x) + (lane >> 2);
     const int chunk = NB == 2 ? (lane & 7) ^ ((s >> 1) & 7) : (lane & 3) ^ ((s >> 2) & 3);
-    cb[x] = (uint32_t)(64 * (s >> 6) + 4 * (s & 15) + ((s >> 4) & 3)) * ldb + (uint32_t)(chunk * 16);
+    cb[x] = row_of(s) * ldb + (uint32_t)(chunk * 16);
   }
-  // chunk of a fragment's first 16 bytes, and what leads to its second 16: 4 chunks on, in bf16 (a lane takes block g4) the next one
-  const uint32_t qa = NA == 2 ? (WIDE ? 2 * g4 : g4) ^ ((c >> 1) & 7) : g4 ^ (c >> 2), qb = NB == 2 ? (WIDE ? 2 * g4 : g4) ^ ((c >> 1) & 7) : g4 ^ (c >> 2);
-  constexpr uint32_t SECOND = WIDE ? 16 : 64;
+  // chunk of a block's first read; the next: 32 x 32 and bf16 (a lane takes block g4) the next chunk, else 4 chunks on
+  constexpr uint32_t NEXT = B32 || WIDE ? 16 : 64;
+  const int q0 = B32 ? 4 * g4 : g4;
+  const uint32_t qa = NA == 2 ? (WIDE ? 2 * g4 : q0) ^ ((c >> 1) & 7) : g4 ^ (c >> 2), qb = NB == 2 ? (WIDE ? 2 * g4 : q0) ^ ((c >> 1) & 7) : g4 ^ (c >> 2);
   const uint32_t fa_lane = (uint32_t)((wm * 64 + c) * RA) + qa * 16;
   const uint32_t fb_lane = REGA + (uint32_t)((wn * 64 + c) * RB) + qb * 16;
   // scales of a slice: [step][a's 512 bytes, b's]
-  const uint32_t sa_lane = OFF_S + (uint32_t)(wm * 256 + c * 16 + g4 * 4), sb_lane = OFF_S + (uint32_t)(512 + wn * 256 + c * 16 + g4 * 4);
+  const uint32_t s_lane = OFF_S + (uint32_t)((c & 15) * 16) + (uint32_t)(B32 ? g4 * 1024 : g4 * 4);
+  const uint32_t sa_lane = s_lane + (uint32_t)(wm * 256), sb_lane = s_lane + (uint32_t)(512 + wn * 256);
   typedef __attribute__((address_space(3))) const int4v *lds_chunk;
   typedef __attribute__((address_space(3))) const uint32_t *lds_dword;
 
@@ -598,21 +667,26 @@ __global__ void __launch_bounds__(256, 2) mx_t128_kernel(const MxGemmParams p) {
 #pragma unroll
     for (int x = 0; x < 2 * NB; ++x) copy_1k(cb[x], rsb, (uint32_t)(s0 + s) * RB, at + REGA + (uint32_t)(2 * NB * w + x) * 1024);
   };
-  floatx4 acc[4][4];
+  Acc acc[BLK][BLK];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) acc[i >> 2][i & 3] = floatx4{0.f, 0.f, 0.f, 0.f};
-  int4v fa[2][4][NA], fb[2][4][NB];
-  uint32_t sa[2][KS], sb[2][KS];
-  constexpr int READS = 2 * KS + 4 * NA + 4 * NB;
+  for (int i = 0; i < BLK * BLK; ++i) acc[i / BLK][i % BLK] = Acc{};
+  int4v fa[2][BLK][APART], fb[2][BLK][BPART];
+  uint32_t sa[2], sb[2], na[2], nb[2];                           // this slice's scales, and (16 x 16) the next one's as they come
+  int4v ca_next, cb_next;                                        // (32 x 32) the next one's cells
+  constexpr int READS = 2 + BLK * APART + BLK * BPART;
   auto read = [&](int set, uint32_t at, int x) {                // read x of READS: the scales, then step by step what is multiplied first
-    if (x < KS) sa[set][x] = *(lds_dword)(at + sa_lane + (uint32_t)(x * 1024));
-    else if (x < 2 * KS) sb[set][x - KS] = *(lds_dword)(at + sb_lane + (uint32_t)((x - KS) * 1024));
-    else if (x < 2 * KS + 4 * NB) {
-      const int y = x - 2 * KS;
-      fb[set][y & 3][y >> 2] = *(lds_chunk)(at + (fb_lane ^ (uint32_t)(y >> 2) * SECOND) + (uint32_t)((y & 3) * 16 * RB));
+    if (x == 0) {
+      if constexpr (B32) ca_next = *(lds_chunk)(at + sa_lane);
+      else na[0] = *(lds_dword)(at + sa_lane);
+    } else if (x == 1) {
+      if constexpr (B32) cb_next = *(lds_chunk)(at + sb_lane);
+      else nb[0] = *(lds_dword)(at + sb_lane);
+    } else if (x < 2 + BLK * BPART) {
+      const int y = x - 2;
+      fb[set][y % BLK][y / BLK] = *(lds_chunk)(at + (fb_lane ^ (uint32_t)(y / BLK) * NEXT) + (uint32_t)(y % BLK * SIDE * RB));
     } else if (x < READS) {
-      const int y = x - 2 * KS - 4 * NB;
-      fa[set][y & 3][y >> 2] = *(lds_chunk)(at + (fa_lane ^ (uint32_t)(y >> 2) * SECOND) + (uint32_t)((y & 3) * 16 * RA));
+      const int y = x - 2 - BLK * BPART;
+      fa[set][y % BLK][y / BLK] = *(lds_chunk)(at + (fa_lane ^ (uint32_t)(y / BLK) * NEXT) + (uint32_t)(y % BLK * SIDE * RA));
     }
   };
   uint32_t stage = 0;                                            // of slice s
@@ -633,6 +707,13 @@ __global__ void __launch_bounds__(256, 2) mx_t128_kernel(const MxGemmParams p) {
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((STAGES - 2) * COPIES) : "memory");
     __builtin_amdgcn_sched_barrier(0);
+    if constexpr (B32) {
+      mx_cell_rows2(sa, ca_next, (uint32_t)c >> 4);
+      mx_cell_rows2(sb, cb_next, (uint32_t)c >> 4);
+    } else {
+      sa[0] = na[0];
+      sb[0] = nb[0];
+    }
     turn_to(s + STAGES);
     copy(s + STAGES, stage);
     if constexpr (WIDE) {
@@ -644,14 +725,14 @@ __global__ void __launch_bounds__(256, 2) mx_t128_kernel(const MxGemmParams p) {
         MxFrag<FB> f;
 #pragma unroll
         for (int i = 0; i < NB; ++i) f.q[i] = fb[SET][nj][i];
-        wb[nj] = mx_wide<FB>(f, mx_scale_value(sb[SET][0] >> (8 * nj) & 0xffu));
+        wb[nj] = mx_wide<FB>(f, mx_scale_value(sb[0] >> (8 * nj) & 0xffu));
       }
 #pragma unroll
       for (int mi = 0; mi < 4; ++mi) {
         MxFrag<FA> f;
 #pragma unroll
         for (int i = 0; i < NA; ++i) f.q[i] = fa[SET][mi][i];
-        const MxWide<FA> wa = mx_wide<FA>(f, mx_scale_value(sa[SET][0] >> (8 * mi) & 0xffu));
+        const MxWide<FA> wa = mx_wide<FA>(f, mx_scale_value(sa[0] >> (8 * mi) & 0xffu));
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -661,19 +742,28 @@ __global__ void __launch_bounds__(256, 2) mx_t128_kernel(const MxGemmParams p) {
       return;
     }
 #pragma unroll
-    for (int x = 0; x < 16 * KS; ++x) {
-      const int ks = x >> 4, mi = (x >> 2) & 3, nj = x & 3;
-      const auto vb = mx_narrow<FB>(fb[SET][nj], ks);
-      const auto va = mx_narrow<FA>(fa[SET][mi], ks);
-      floatx4 &sum = acc[mi][nj];
-#define MX_SEL(j, i) if (nj == j && mi == i) mx_mma_tied<FA, FB, j, i>(vb, sb[SET][ks], va, sa[SET][ks], sum)
-      MX_SEL(0, 0); MX_SEL(0, 1); MX_SEL(0, 2); MX_SEL(0, 3);
-      MX_SEL(1, 0); MX_SEL(1, 1); MX_SEL(1, 2); MX_SEL(1, 3);
-      MX_SEL(2, 0); MX_SEL(2, 1); MX_SEL(2, 2); MX_SEL(2, 3);
-      MX_SEL(3, 0); MX_SEL(3, 1); MX_SEL(3, 2); MX_SEL(3, 3);
+    for (int x = 0; x < 16; ++x) {
+      if constexpr (B32) {
+        const int t = x >> 2, bm = (x >> 1) & 1, bn = x & 1;
+#define MX_SEL(j, i, k) if (t == j && bm == i && bn == k) mx_mma32_tied<2 * (j & 1) + k, 2 * (j & 1) + i>(fb[SET][bn][t], sb[t >> 1], fa[SET][bm][t], sa[t >> 1], acc[bm][bn])
+#define MX_SEL4(j) MX_SEL(j, 0, 0); MX_SEL(j, 0, 1); MX_SEL(j, 1, 0); MX_SEL(j, 1, 1)
+        MX_SEL4(0); MX_SEL4(1); MX_SEL4(2); MX_SEL4(3);
+#undef MX_SEL4
 #undef MX_SEL
+      } else {
+        const int mi = x >> 2, nj = x & 3;
+        const auto vb = mx_narrow<FB>(fb[SET][nj], 0);
+        const auto va = mx_narrow<FA>(fa[SET][mi], 0);
+        floatx4 &sum = acc[mi][nj];
+#define MX_SEL(j, i) if (nj == j && mi == i) mx_mma_tied<FA, FB, j, i>(vb, sb[0], va, sa[0], sum)
+        MX_SEL(0, 0); MX_SEL(0, 1); MX_SEL(0, 2); MX_SEL(0, 3);
+        MX_SEL(1, 0); MX_SEL(1, 1); MX_SEL(1, 2); MX_SEL(1, 3);
+        MX_SEL(2, 0); MX_SEL(2, 1); MX_SEL(2, 2); MX_SEL(2, 3);
+        MX_SEL(3, 0); MX_SEL(3, 1); MX_SEL(3, 2); MX_SEL(3, 3);
+#undef MX_SEL
+      }
       __builtin_amdgcn_sched_barrier(0);
-      constexpr int PER = (READS + 16 * KS - 1) / (16 * KS);
+      constexpr int PER = (READS + 15) / 16;
 #pragma unroll
       for (int y = 0; y < PER; ++y) read(SET ^ 1, lds0 + next, PER * x + y);
       __builtin_amdgcn_sched_barrier(0);
@@ -690,7 +780,7 @@ __global__ void __launch_bounds__(256, 2) mx_t128_kernel(const MxGemmParams p) {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");               // the last copies have landed before LDS is used again,
   asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");             // and the last sums are there
 #pragma unroll
-  for (int i = 0; i < 16; ++i) asm volatile("" : "+v"(acc[i >> 2][i & 3]));
+  for (int i = 0; i < BLK * BLK; ++i) asm volatile("" : "+v"(acc[i / BLK][i % BLK]));
   __syncthreads();
   // 32 rows of a wavefront's 64 at a time through LDS of its own, so that a store writes whole lines: a lane holds columns 16 g4 + 4 v + nj of
   // rows 4 c + mi, and stores 16 bytes of a row
@@ -701,13 +791,21 @@ __global__ void __launch_bounds__(256, 2) mx_t128_kernel(const MxGemmParams p) {
     constexpr int E = 16 / (int)sizeof(TS), LPR = 64 / E;        // columns of a lane, lanes of a row
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
+      if constexpr (B32) {
+        // columns 32 x + 16 g4 + 4 v + .. of row 4 (c % 16) + 2 block + c / 16
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 8; ++i)
+          *reinterpret_cast<floatx4 *>(mine + (2 * (c & 15) + (c >> 4)) * PITCH + 32 * (i >> 2) + 16 * g4 + 4 * (i & 3)) =
+              floatx4{acc[half][0][i], acc[half][0][i + 8], acc[half][1][i], acc[half][1][i + 8]};
+      } else {
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const int mi = 2 * half + i;
-          *reinterpret_cast<floatx4 *>(mine + (2 * c + i) * PITCH + 16 * g4 + 4 * v) = floatx4{acc[mi][0][v], acc[mi][1][v], acc[mi][2][v], acc[mi][3][v]};
-        }
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const auto &s = acc[(2 * half + i) % BLK];
+            *reinterpret_cast<floatx4 *>(mine + (2 * c + i) * PITCH + 16 * g4 + 4 * v) = floatx4{s[0][v], s[1 % BLK][v], s[2 % BLK][v], s[3 % BLK][v]};
+          }
+      }
       __builtin_amdgcn_wave_barrier();
 #pragma unroll
       for (int it = 0; it < 32 * LPR / 64; ++it) {
