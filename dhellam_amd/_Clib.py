@@ -21,7 +21,7 @@ __all__ = ["add_tensors", "pygemm", "dense_gemm", "dense_ok", "keep_transposed",
            "pymoe_route_topk", "pymoe_sort", "pymoe_permute", "pymoe_unpermute", "pygrouped_gemm_nt",
            "pygrouped_gemm_nn", "pygrouped_gemm_tn", "pycross_entropy_fwd", "pycross_entropy_bwd",
            "pyembedding_fwd", "pyembedding_bwd", "pyrotary_fwd", "pyrotary_bwd", "pymoe_balance_loss", "pymoe_route_bwd",
-           "pydistill_fwd", "pydistill_bwd"]
+           "pydistill_fwd", "pydistill_bwd", "pymx_quantise", "pymx_gemm_nt", "pyrmsnorm_mx_fwd", "pygrad_norm", "pyclip_grads"]
 
 
 def _timed(profiling: bool, stream, fn):
@@ -661,6 +661,39 @@ def pydistill_bwd(vocab_parallel_logits, teacher_ids, teacher_logits, target, fw
     from .operators.loss import distill_bwd
     return distill_bwd([{"vocab_parallel_logits": vocab_parallel_logits, "teacher_ids": teacher_ids, "teacher_logits": teacher_logits,
                          "target": target}, fwd_out], dout, grad_out)
+
+
+def pymx_quantise(x, format="e4m3", along="rows", scale_rule="floor", profiling=False):
+    """-> [``operators.mx.MXTensor``], two of them (of x, of its transpose) along "both" """
+    from .operators.mx import mx_quantise
+    q, ms = mx_quantise(x, format, along, scale_rule, None, profiling)
+    return _ret(q if along == "both" else (q,), ms, profiling)
+
+
+def pymx_gemm_nt(a, b, out=None, out_dtype=torch.bfloat16, accumulate=False):
+    from .operators.mx import mx_gemm_nt
+    return mx_gemm_nt(a, b, out, out_dtype, accumulate)
+
+
+def pyrmsnorm_mx_fwd(inp, weight, eps, residual=None, profiling=False):
+    """-> [``operators.mx.MXTensor``, rsigma, inp + residual or None]"""
+    from .operators.layernorm import pyrmsnorm_mx_fwd as fwd
+    q, rsigma, total, ms = fwd(inp, weight, eps, False, None, profiling, residual)
+    return _ret((q, rsigma, total), ms, profiling)
+
+
+def pygrad_norm(grads, profiling=False):
+    """-> [sum of squares fp64 [1]]"""
+    from .operators.grads import grad_norm
+    sum_sq, ms = grad_norm(grads, None, profiling)
+    return _ret((sum_sq,), ms, profiling)
+
+
+def pyclip_grads(grads, sum_sq, max_norm, scale=1.0, out=None, profiling=False):
+    """-> [fp32 [2]: norm, factor]"""
+    from .operators.grads import clip_grads
+    found, ms = clip_grads(grads, sum_sq, max_norm, scale, out, None, profiling)
+    return _ret((found,), ms, profiling)
 
 
 def pyembedding_fwd(vocab, token_ids):

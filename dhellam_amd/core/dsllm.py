@@ -42,6 +42,17 @@ def _record(obj, stream) -> None:
             _record(v, stream)
 
 
+def clip_main_grads(parameters, max_norm: float, scale: float = 1.0, out=None) -> torch.Tensor:
+    """Between a step's backward and the optimizer: the global norm of the parameters' ``main_grad`` (times ``scale``, which undoes a
+    loss scale) and their clipping to ``max_norm``, in place or into ``out`` (``operators.grads.clip_grads``).  Returns fp32 [2] on the device:
+    the norm, and the factor that was applied.  Nothing here waits for the GPU."""
+    from ..operators.grads import clip_grads, grad_norm
+    grads = [p.main_grad for p in parameters if getattr(p, "main_grad", None) is not None]
+    if not grads:
+        raise ValueError("no parameter has a main_grad")
+    return clip_grads(grads, grad_norm(grads)[0], max_norm, scale, out)[0]
+
+
 class DSLLMStep:
     def __init__(self, cfg: LayerConfig, num_layers: int, vocab_size: int, seed: int = 0, plan=None,
                  stream1: Optional[torch.cuda.Stream] = None, stream2: Optional[torch.cuda.Stream] = None,
@@ -74,6 +85,10 @@ class DSLLMStep:
     def zero_grads(self) -> None:
         for _, t in self.named_parameters():
             t.main_grad.zero_()
+
+    def clip_grads(self, max_norm: float, scale: float = 1.0, out=None) -> torch.Tensor:
+        """Clips the gradients of a step (or of several) to a global norm, on the current stream; see ``clip_main_grads``."""
+        return clip_main_grads((t for _, t in self.named_parameters()), max_norm, scale, out)
 
     # ---- pieces of a micro-batch --------------------------------------------------------------
     def _exec(self, blocks, fwd_w, bwd_w, x, dy, act_prev, act_new, s1, s2):
