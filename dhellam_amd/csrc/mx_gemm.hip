@@ -59,7 +59,7 @@ __device__ __forceinline__ floatx4 mx_mma_sel(int selb, int sela, const MxFrag<F
 }
 
 // The same 128 columns in four v_mfma_f32_16x16x32_bf16: a lane takes the 32 columns of block g, whose elements times their scale are exact in
-// bf16 unless they lie below its smallest normal number, and every product and its place in the sum are those of fp32.
+// bf16 unless they lie below its smallest normal number (2^-126; all is lost below 2^-133), and products are added in fp32.
 __device__ __forceinline__ float mx_scale_value(uint32_t code) {
   return __uint_as_float(code == 255u ? 0x7fc00000u : code == 0u ? 0x400000u : code << 23);
 }
