@@ -208,6 +208,94 @@ def check_grouped_gemm_order(fn: list) -> int:
     return len(body)
 
 
+def mx_gemm_assembly() -> dict:
+    """The instantiations of ``mx_w8_kernel`` and ``mx_t128_kernel`` as device assembly of ``mx_gemm.hip``, a list of lines each, by their
+    mangled names."""
+    import re
+    import tempfile
+    with tempfile.TemporaryDirectory() as td:
+        out = Path(td) / "mx.s"
+        cmd = [HIPCC, *[f for f in CXXFLAGS if f != "-fPIC"], "--cuda-device-only", "-S", str(CSRC / "mx_gemm.hip"), "-o", str(out)]
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError("hipcc -S failed for mx_gemm.hip:\n" + res.stderr)
+        lines = out.read_text().split("\n")
+    starts = [i for i, l in enumerate(lines) if re.match(r"^_ZN2dh(12mx_w8|14mx_t128)_kernel\w+:", l)]
+    return {lines[a].split(":")[0]: lines[a:next(i for i in range(a, len(lines)) if lines[i].startswith(".Lfunc_end"))] for a in starts}
+
+
+def check_mx_gemm_loops(verbose: bool = False) -> int:
+    """The tiled products of microscaled operands copy to LDS from assembly too, and form their sums in assembly: the generated code of every
+    instantiation is held to the order that the source lays down (``check_mx_gemm_order``).  Returns their number; raises on a violation."""
+    kernels = mx_gemm_assembly()
+    for name, fn in kernels.items():
+        body = check_mx_gemm_order(name, fn)
+        if verbose:
+            print(f"checked {name}: {body} lines", flush=True)
+    return len(kernels)
+
+
+def check_mx_gemm_order(name: str, fn: list) -> int:
+    """One instantiation of ``mx_w8_kernel`` or ``mx_t128_kernel``: two slices in the innermost loop with matrix instructions.  Every copy goes
+    to LDS.  ``mx_w8_kernel``: 16 clusters between barriers, every second one of 8 matrix instructions and no copy, the others beginning with the
+    wait for the wavefront's earlier reads and ending, where they publish copies, with the counted wait.  ``mx_t128_kernel``: a slice ends with
+    the waits for reads and copies and a barrier, and its copies go out behind that.  No scratch accesses in the loop, and behind it the
+    last copies are waited for before LDS is used again or the kernel ends."""
+    import re
+    fa, fb = (int(x) for x in re.search(r"kernelILi(\d)ELi(\d)E", name).groups())
+    eight, wide = "mx_w8" in name, "Lb1E" in name
+    two = fa == 4 and fb == 4
+    rows = lambda bits: 2 if two or bits == 8 else 1                  # 1 KB copies of 64 rows
+    copies = (2 if two else 1) + 2 * rows(fa) + 2 * rows(fb)          # of a wavefront a slice
+    slice_mfmas = 32 if eight else 64 if wide else 16
+    code = [x for x in (l.split(";")[0].strip() for l in fn) if x]
+    labels = {m.group(1): i for i, l in enumerate(code) if (m := re.match(r"^(\.LBB\d+_\d+):", l))}
+    mfmas = lambda part: sum("v_mfma" in x for x in part)
+    is_copy = lambda x: x.startswith("buffer_load")
+
+    def need(ok, what):
+        if not ok:
+            raise RuntimeError(f"{name}: {what}")
+
+    loops = []
+    for i, l in enumerate(code):
+        m = re.match(r"s_c?branch\w* (\.LBB\d+_\d+)", l)
+        if m and m.group(1) in labels and labels[m.group(1)] < i and mfmas(code[labels[m.group(1)] + 1:i]) == 2 * slice_mfmas:
+            loops.append((labels[m.group(1)] + 1, i))
+    need(loops, f"no main loop with {2 * slice_mfmas} matrix instructions")
+    lo, hi = min(loops, key=lambda x: x[1] - x[0])
+    body = [x for x in code[lo:hi] if not x.endswith(":")]
+    need(all(x.endswith("lds") for x in code if is_copy(x)), "a buffer load to registers")
+    need(not any("scratch_" in x for x in body), "scratch accesses in the main loop")
+    need(sum(map(is_copy, body)) == 2 * copies, f"{sum(map(is_copy, body))} copies in the main loop, expected {2 * copies}")
+    at = [i for i, x in enumerate(body) if x.startswith("s_barrier")]
+    if eight:
+        need(len(at) == 16, f"{len(at)} barriers in the main loop, expected 16")
+        clusters = [body[a + 1:b] for a, b in zip([-1] + at, at)]
+        clusters[0] = body[at[-1] + 1:] + clusters[0]
+        for n, cl in enumerate(clusters):
+            need(mfmas(cl) == (8 if n % 2 else 0), f"cluster {n} holds {mfmas(cl)} matrix instructions")
+            dma, waits = [i for i, x in enumerate(cl) if is_copy(x)], [i for i, x in enumerate(cl) if x == "s_waitcnt lgkmcnt(0)"]
+            reads = [i for i, x in enumerate(cl) if x.startswith("ds_read")]
+            if n % 2:
+                need(not dma, f"a copy in cluster {n}, among matrix instructions")
+                continue
+            need(waits and not (reads and reads[0] < waits[0]) and not (dma and dma[0] < waits[0]), f"cluster {n} does not begin with the wait for the earlier reads")
+            need(not dma or f"s_waitcnt vmcnt({copies})" in cl[dma[-1]:], f"cluster {n} publishes copies without the counted wait")
+    else:
+        need(len(at) == 2, f"{len(at)} barriers in the main loop, expected 2")
+        for b in at:
+            need(body[b - 2:b] == ["s_waitcnt lgkmcnt(0)", "s_waitcnt vmcnt(0)"], "a slice ends without the waits for its reads and copies")
+        for part in (body[at[0] + 1:at[1]], body[at[1] + 1:] + body[:at[0]]):
+            need(mfmas(part) == slice_mfmas and sum(map(is_copy, part)) == copies, "a slice's copies or matrix instructions are in another's place")
+    rest = [x for x in code[hi:] if not x.endswith(":")]
+    last = max(i for i, x in enumerate(rest) if "v_mfma" in x)
+    landed = next((i for i in range(last, len(rest)) if rest[i].startswith("s_waitcnt vmcnt(0)")), len(rest))
+    used = next((i for i in range(last, len(rest)) if rest[i].startswith(("ds_", "global_store", "s_endpgm"))), len(rest))
+    need(landed < used, "LDS is used again, or the kernel ends, before the last copies have landed")
+    return len(body)
+
+
 EXT_PKG = ROOT / "dhellam"
 EXT_SUFFIX = sysconfig.get_config_var("EXT_SUFFIX")
 PY_INCLUDE = sysconfig.get_paths()["include"]
@@ -271,6 +359,7 @@ if __name__ == "__main__":
     path = build(verbose="-v" in sys.argv)
     print(path)
     print(f"grouped GEMM main loops checked: {check_grouped_gemm_loops(verbose='-v' in sys.argv)}")
+    print(f"microscaled GEMM main loops checked: {check_mx_gemm_loops(verbose='-v' in sys.argv)}")
     if "--no-ext" not in sys.argv:
         for path in build_extensions(verbose="-v" in sys.argv):
             print(path)
