@@ -130,6 +130,13 @@ template <int BITS> __device__ __forceinline__ auto mx_narrow(const int4v *q, in
   else return q[ks];
 }
 
+// What the chunks of a row in slot s are XORed with, rows of 128 bytes and of 64.  A read of 16 bytes a lane is served 16 lanes at a time, the first 16
+// being lanes 0..3, 12..15, 20..23 and 24..27, the next the rest of the first 32; their chunks have to differ where lanes 0..15 read one chunk of
+// 16 slots and lanes 16..31 its neighbour (16 x 16 x 128), the next but one (mx_wide), or 32 lanes one (32 x 32 x 64).  (slot / 2) % 8 alone costs mx_wide a second
+// pass a read; with slot / 4 % 4 a fifth of LDS's cycles at 4096 x 7168 x 8192 in 8 x 4 bits were conflicts.
+__device__ __forceinline__ int mx_turn8(int s) { return 0x32765410 >> (4 * ((s >> 1) & 7)) & 7; }
+__device__ __forceinline__ int mx_turn4(int s) { return 0x78 >> (2 * ((s >> 2) & 3)) & 3; }
+
 // c's element: added to if asked, rounded once.
 template <typename TO> __device__ __forceinline__ TO mx_out(float v, const TO *old, int accumulate) {
   return from_f<TO>(accumulate ? v + to_f(*old) : v);
@@ -166,6 +173,9 @@ template <typename TO, int N> __device__ __forceinline__ void mx_store(TO *p, co
 // after the other, and add up through LDS in the order of the wavefronts.  Operand block i of MT (NT) takes the rows MT r + i, so that
 // the scales of a lane's blocks lie side by side.  Where even so there are few workgroups, k is cut into pieces over workgroups as
 // well, and mx_join_kernel adds these in order.
+// Bound by the weights' bytes for a few rows: 1 x 7168 x 8192 with 4-bit weights 8 to 9 us for 31 MB (a copy's rate: 6.0), and by launch and the latency
+// of a handful of loads for smaller ones (1 x 1280 x 8192 5 to 6).  Loads of the next step before this step's products did not help where the
+// wavefronts of a compute unit are eight already (1 x 7168 x 8192, 777 x 1001 x 2080), nor did sixteen wavefronts.
 // Step x of the P that a wavefront takes at a time.  With P of 2 the two steps' eight blocks are dealt out so that a lane's block of step x is
 // block 2 g + x of them: its 4-bit elements of both steps are 32 consecutive bytes, a row's 128.
 template <int BITS, int P, bool WIDE> __device__ __forceinline__ void mx_load(MxFrag<BITS> &f, const uint8_t *row, int g, int x) {
@@ -291,16 +301,23 @@ __global__ void __launch_bounds__(64 * W) mx_direct_kernel(const MxGemmParams p)
 // The schedule of grouped_gemm_w8_kernel (grouped_gemm.hip, where its order of reads, waits, copies and barriers is argued): a wavefront has
 // 128 x 64 outputs in four quarters, a quarter of a slice is [reads of fragments, copies | its MFMAs, more reads among them],
 // and the wavefronts 4..7 run one barrier behind the others.  A slice is 128 bytes of a row here too: 256 columns where both operands have
-// 4 bits (two steps of 128, 16 MFMAs of 16 cycles in a quarter), 128 columns otherwise (8 MFMAs of 32 cycles; a 4-bit operand's rows
-// then have 64 bytes).
+// 4 bits (8 MFMAs of 32 x 32 x 64 in a quarter), 128 columns otherwise (8 of 16 x 16 x 128; a 4-bit operand's rows then have 64 bytes).
 //
 // LDS: regions of [128 slots][row bytes] for either half of the tile's rows of a and of b, two stages of them, and the scales in a ring
-// of three.  A slot holds row 64 (s / 64) + 4 (s % 16) + s / 16 % 4 of a's half, row 32 (s / 32) + 2 (s % 16) + s / 16 % 2 of b's, so that
-// the four (two) blocks a lane multiplies are neighbouring rows: their scales are one dword (half of one) of a cell, and a lane's
-// outputs are 8 neighbouring columns.  16-byte chunks are XORed with (slot / 2) % 8, in rows of 64 bytes with (slot / 4) % 4: the 16 lanes of a
-// fragment read hit 16 different chunks of 256 bytes.  Scales come as whole cells, 256 bytes a copy.
+// of three.  Slots are dealt out so that the blocks a lane multiplies are neighbouring rows, whose scales lie in one cell, and a lane's outputs
+// neighbouring columns.  16 x 16: slot s holds row 64 (s / 64) + 4 (s % 16) + s / 16 % 4 of a's half, row 32 (s / 32) + 2 (s % 16) + s / 16 % 2 of
+// b's; the four (two) blocks' scales are read as one dword (half of one).  32 x 32: row 64 (s / 64) + 4 (s % 16) + 2 (s / 32 % 2) + s / 16 % 2 of
+// a's half, row 32 (s / 32) + 4 (s % 8) + s / 8 % 4 of b's; a lane reads a whole cell, [4 blocks of 32][4 rows], and takes its rows' bytes out of
+// it behind the next wait.  16-byte chunks are XORed with mx_turn8 (mx_turn4 in rows of 64 bytes): the lanes of a
+// fragment read that LDS serves at once hit different chunks of 256 bytes.  Scales come as whole cells, 256 bytes a copy.
 // Scales follow their fragments: those of the half that is read next lie in LDS since the wait two clusters before, and a slot of the
 // ring is written again three slices later, long after its last read.
+//
+// Measured, 8192 x 8192 x 8192 to bf16: 8 x 8 bits 370 to 450 us with the board and the data's values (2.4 to 3.0 PFLOP/s), 4 x 4 bits 245 to
+// 290 (3.8 to 4.5; 275 in blocks of 16 x 16 x 128 where these take 264).  Bound by power in 8 bits: the clock falls to 1.76 GHz of 2.4 and the matrix pipes are busy for 78 % of
+// the time; in 4 bits they are busy for half of it at 1.95 GHz.  A tile costs about 10 us beside its slices (first copies, stores of c), which
+// do not overlap with another's: one workgroup fills a compute unit's LDS.  From k of 4096 to 8192 8 x 8 bits run at 3.3 PFLOP/s, 4 x 4 at 5.2.
+// Did not help: c by rows of 512 bytes through LDS (4 us a tile slower), copies a cluster earlier.
 // 64 lanes x 4 bytes, as copy_1k
 __device__ __forceinline__ void copy_256(uint32_t lane_off, const int4v &rsrc, uint32_t off, uint32_t dst) {
   asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dword %0, %1, %2 offen lds"
@@ -335,13 +352,13 @@ __global__ void __launch_bounds__(512) mx_w8_kernel(const MxGemmParams p) {
 #pragma unroll
   for (int x = 0; x < NA; ++x) {
     const int s = NA == 2 ? 8 * (2 * w + x) + (lane >> 3) : 16 * w + (lane >> 2);
-    const int chunk = NA == 2 ? (lane & 7) ^ ((s >> 1) & 7) : (lane & 3) ^ ((s >> 2) & 3);
+    const int chunk = NA == 2 ? (lane & 7) ^ mx_turn8(s) : (lane & 3) ^ mx_turn4(s);
     ca[x] = (uint32_t)(64 * (s >> 6) + 4 * (s & 15) + (B32 ? 2 * ((s >> 5) & 1) + ((s >> 4) & 1) : (s >> 4) & 3)) * lda + (uint32_t)(chunk * 16);
   }
 #pragma unroll
   for (int x = 0; x < NB; ++x) {
     const int s = NB == 2 ? 8 * (2 * w + x) + (lane >> 3) : 16 * w + (lane >> 2);
-    const int chunk = NB == 2 ? (lane & 7) ^ ((s >> 1) & 7) : (lane & 3) ^ ((s >> 2) & 3);
+    const int chunk = NB == 2 ? (lane & 7) ^ mx_turn8(s) : (lane & 3) ^ mx_turn4(s);
     cb[x] = (uint32_t)(32 * (s >> 5) + (B32 ? 4 * (s & 7) + ((s >> 3) & 3) : 2 * (s & 15) + ((s >> 4) & 1))) * ldb + (uint32_t)(chunk * 16);
   }
   const uint32_t cs = (uint32_t)(lane * 4);
@@ -349,7 +366,7 @@ __global__ void __launch_bounds__(512) mx_w8_kernel(const MxGemmParams p) {
   // ---- fragments and scales
   // chunk of a block's first read; the next: B32 the next chunk (a lane's half is one of the slice's two steps), else 4 chunks on
   constexpr uint32_t NEXT = B32 ? 16 : 64;
-  const uint32_t qa = NA == 2 ? (B32 ? 4 * g4 : g4) ^ ((c >> 1) & 7) : g4 ^ (c >> 2), qb = NB == 2 ? (B32 ? 4 * g4 : g4) ^ ((c >> 1) & 7) : g4 ^ (c >> 2);
+  const uint32_t qa = NA == 2 ? (B32 ? 4 * g4 : g4) ^ mx_turn8(c) : g4 ^ mx_turn4(c), qb = NB == 2 ? (B32 ? 4 * g4 : g4) ^ mx_turn8(c) : g4 ^ mx_turn4(c);
   const uint32_t fa_lane = (uint32_t)((wm * 64 + c) * RA) + qa * 16, fb_lane = (uint32_t)((wn * 32 + c) * RB) + qb * 16;
   // half: + 512; 16 x 16: step: + 1024
   const uint32_t sa_lane = (uint32_t)(wm * 256 + (c & 15) * 16) + (uint32_t)(B32 ? g4 * 1024 : g4 * 4);
@@ -382,7 +399,7 @@ __global__ void __launch_bounds__(512) mx_w8_kernel(const MxGemmParams p) {
       // the last step of an odd number: chunks 4..7 are not there
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        const int ch = (lane & 7) ^ (((8 * (2 * w + x) + (lane >> 3)) >> 1) & 7);
+        const int ch = (lane & 7) ^ mx_turn8(8 * (2 * w + x) + (lane >> 3));
         if (ch >= 4) ca[x % NA] = cb[x % NB] = 0x80000000u;      // past any descriptor's end
       }
     }
@@ -588,9 +605,10 @@ __global__ void __launch_bounds__(512) mx_w8_kernel(const MxGemmParams p) {
 // its own copies of slice s + 1 have landed, so that slice may be read.  What a workgroup waits for the other one of the compute unit fills:
 // with four stages and one workgroup 2048 x 4096 x 8192 took 79 us in 8 bits and 58 in 4, with two and two it takes 58 and 40.
 // Bound by LDS: a slice moves 34 KB into it and 72 KB out of it for 512 cycles of matrix instructions a SIMD; 2048 x 4096 x 8192 runs at 2.4
-// (8 bits) and 3.4 PFLOP/s.
-// Both operands' slots hold row 64 (s / 64) + 4 (s % 16) + s / 16 % 4: four blocks' scales are one dword, and a lane's outputs 16 neighbouring
-// columns of four rows.
+// (8 bits) and 3.4 PFLOP/s.  WIDE: by the bf16 matrix instructions, 1024 cycles of a slice a SIMD and workgroup, and the conversions, some 700 of
+// the vector ALU beside them; 8192 x 1024 x 8192 117 us, 1.17 PFLOP/s (a bf16 product of the library's 1.3 to 1.4).
+// Both operands' slots hold row 64 (s / 64) + 4 (s % 16) + s / 16 % 4 in blocks of 16 x 16 (four blocks' scales are one dword), 64 (s / 64) +
+// 4 (s % 16) + 2 (s / 32 % 2) + s / 16 % 2 in blocks of 32 x 32 (scales as cells, taken apart behind the wait, as in mx_w8_kernel).
 template <int FA, int FB, bool WIDE, typename TO>
 __global__ void __launch_bounds__(256, 2) mx_t128_kernel(const MxGemmParams p) {
   constexpr int KS = FA == 4 && FB == 4 ? 2 : 1;
@@ -613,19 +631,19 @@ __global__ void __launch_bounds__(256, 2) mx_t128_kernel(const MxGemmParams p) {
 #pragma unroll
   for (int x = 0; x < 2 * NA; ++x) {
     const int s = NA == 2 ? 8 * (4 * w + x) + (lane >> 3) : 16 * (2 * w + x) + (lane >> 2);
-    const int chunk = NA == 2 ? (lane & 7) ^ ((s >> 1) & 7) : (lane & 3) ^ ((s >> 2) & 3);
+    const int chunk = NA == 2 ? (lane & 7) ^ mx_turn8(s) : (lane & 3) ^ mx_turn4(s);
     ca[x] = row_of(s) * lda + (uint32_t)(chunk * 16);
   }
 #pragma unroll
   for (int x = 0; x < 2 * NB; ++x) {
     const int s = NB == 2 ? 8 * (4 * w + x) + (lane >> 3) : 16 * (2 * w + x) + (lane >> 2);
-    const int chunk = NB == 2 ? (lane & 7) ^ ((s >> 1) & 7) : (lane & 3) ^ ((s >> 2) & 3);
+    const int chunk = NB == 2 ? (lane & 7) ^ mx_turn8(s) : (lane & 3) ^ mx_turn4(s);
     cb[x] = row_of(s) * ldb + (uint32_t)(chunk * 16);
   }
   // chunk of a block's first read; the next: 32 x 32 and bf16 (a lane takes block g4) the next chunk, else 4 chunks on
   constexpr uint32_t NEXT = B32 || WIDE ? 16 : 64;
   const int q0 = B32 ? 4 * g4 : g4;
-  const uint32_t qa = NA == 2 ? (WIDE ? 2 * g4 : q0) ^ ((c >> 1) & 7) : g4 ^ (c >> 2), qb = NB == 2 ? (WIDE ? 2 * g4 : q0) ^ ((c >> 1) & 7) : g4 ^ (c >> 2);
+  const uint32_t qa = NA == 2 ? (WIDE ? 2 * g4 : q0) ^ mx_turn8(c) : g4 ^ mx_turn4(c), qb = NB == 2 ? (WIDE ? 2 * g4 : q0) ^ mx_turn8(c) : g4 ^ mx_turn4(c);
   const uint32_t fa_lane = (uint32_t)((wm * 64 + c) * RA) + qa * 16;
   const uint32_t fb_lane = REGA + (uint32_t)((wn * 64 + c) * RB) + qb * 16;
   // scales of a slice: [step][a's 512 bytes, b's]
@@ -652,7 +670,7 @@ __global__ void __launch_bounds__(256, 2) mx_t128_kernel(const MxGemmParams p) {
     } else if (KS == 2 && (p.steps & 1) && s0 + s == nsl - 1) {      // chunks 4..7 are not there
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        const int ch = (lane & 7) ^ (((8 * (4 * w + x) + (lane >> 3)) >> 1) & 7);
+        const int ch = (lane & 7) ^ mx_turn8(8 * (4 * w + x) + (lane >> 3));
         if (ch >= 4) ca[x % (2 * NA)] = cb[x % (2 * NB)] = 0x80000000u;
       }
     }
@@ -731,7 +749,7 @@ __global__ void __launch_bounds__(256, 2) mx_t128_kernel(const MxGemmParams p) {
 #pragma unroll
         for (int i = 0; i < NA; ++i) f.q[i] = fa[SET][mi][i];
         const MxWide<FA> wa = mx_wide<FA>(f, mx_scale_value(sa[0] >> (8 * mi) & 0xffu));
-        constexpr int PER = (READS + 3) / 4;                     // 8192 x 1024 x 8192: 133 us; with all reads before the conversions 138
+        constexpr int PER = (READS + 3) / 4;                     // with all reads before the conversions 4 % slower
 #pragma unroll
         for (int y = 0; y < PER; ++y) read(SET ^ 1, lds0 + next, PER * mi + y);
 #pragma unroll
@@ -875,8 +893,9 @@ static MxPlan mx_plan(int64_t m, int64_t n, int64_t k, int fa, int fb, int out) 
     direct = true;
     q.mt = 4, q.nt = 2;
   } else if (wide && steps < 32 && mid < 128) {
-    direct = true;                   // 777 x 1001 x 2080 16.1 against 24.7
-    q.mt = q.nt = q.waves = 4;
+    // 777 x 1001 x 2080 14 against 24.7 (15.5 by four wavefronts)
+    direct = true;
+    q.mt = q.nt = 4;
   }
   if (direct) {
     // k in pieces where few workgroups have long sums: 32 x 1280 x 8192 17.5 / 14.1 / 10.6 whole, 10.0 / 9.3 / 9.1 in up to 4 pieces
@@ -915,7 +934,7 @@ template <int FA, int FB, typename TO> static void mx_launch(MxGemmParams p, con
   MX_DIRECT(1, 2, 8);
   MX_DIRECT(2, 2, 8);
   MX_DIRECT(4, 2, 8);
-  if constexpr (WIDE) { MX_DIRECT(4, 4, 4); }
+  if constexpr (WIDE) { MX_DIRECT(4, 4, 8); }
 #undef MX_DIRECT
   if (q.pieces > 1) hipLaunchKernelGGL((mx_join_kernel<TO>), dim3((unsigned)cdiv(p.m * p.cells_b, 256)), dim3(256), 0, st, p);
 }
