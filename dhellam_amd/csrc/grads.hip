@@ -7,6 +7,8 @@
 // Both passes cut every tensor into pieces of 32768 elements, a workgroup each; a launch takes up to 80 tensors from a table in
 // its arguments.  Squares are added in 64 bits (an fp32 square overflows from 1.8e19 on), a workgroup's sum is written to its own
 // place and one workgroup adds these up in order: the result is the same bits every time.  Bound by memory: 16-byte loads at any alignment.
+// 559 M elements in bf16 (1.12 GB) to fp32: norm 155 to 165 us (6.8 to 7.2 TB/s read), the join of 17073 sums 5, clipping 645 (5.2 TB/s read and written, a
+// copy's rate).  Clipping in reverse order, for what the norm's pass left on the chip, gained nothing.
 #include <cmath>
 
 #include "mx.h"
