@@ -910,8 +910,11 @@ static MxPlan mx_plan(int64_t m, int64_t n, int64_t k, int fa, int fb, int out) 
   // k in pieces, of 8 slices at least, while they have a compute unit each: 128 x 7168 x 8192 42 whole, 23 in four (8 x 8); 777 x 1001 x 2080 13.8 whole, 15.6
   // in two: the pieces' sums are written and read once more
   const int64_t slices = fa == DH_MX_E2M1 && b4 ? (steps + 1) / 2 : steps;
+  // Two workgroups on a compute unit where what they save, 0.2 us a slice of a piece, pays for the further pieces' bytes, 3 us a hundred tiles: 2000 x 1024 x
+  // 8192 34.3 in two, 32.9 in four, 300 x 4096 x 8192 29.5 and 25.8; but 2000 x 1024 x 4096 23.6 and 25.6, 512 x 7168 x 4096 24.9 whole and 30.7 in two
+  auto pays = [&] { return mid * q.pieces <= 256 && 8 * slices >= mid * q.pieces * std::max(q.pieces, 2); };
   if (slices >= 24)
-    while (q.pieces < MX_MAX_PIECES && mid * q.pieces * 2 <= 256 && slices >= 16 * q.pieces) q.pieces *= 2;
+    while (q.pieces < MX_MAX_PIECES && slices >= 16 * q.pieces && (mid * q.pieces <= 128 || pays())) q.pieces *= 2;
   return q;
 }
 
