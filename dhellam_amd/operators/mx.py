@@ -52,8 +52,7 @@ def mx_quantise(x, format="e4m3", along="rows", scale_rule="floor", stream=None,
     none does.  Elements are rounded to the nearest, ties to even.  A block that holds anything not finite becomes NaN as a whole."""
     form, way, cover = _one_of("format", format, FORMATS), _one_of("along", along, ALONG), _one_of("scale_rule", scale_rule, SCALE_RULES)
     (c, s, ct, st), ms = issue(_host.mx_quantise, stream, profiling, x, form, way, cover)
-    cols = x.shape[-1]
-    rows = (c.shape[0] if c is not None else x.numel() // cols if cols else 0)
+    rows, cols = x.shape[:-1].numel(), x.shape[-1]
     q = MXTensor(c, s, rows, cols, format) if c is not None else None
     if ct is None:
         return q, ms

@@ -1,5 +1,7 @@
 """Quantisation to microscaled floating point, bit for bit against its definition in 64 bits, and the products of such operands: on numbers
 whose sums are exact, bit for bit as well."""
+import math
+
 import pytest
 import torch
 
@@ -197,6 +199,21 @@ def test_product_of_nothing():
     assert (mx_gemm_nt(none(5, 0, "e4m3"), none(7, 0, "e4m3")) == 0).all()
     out = torch.ones(5, 7, device="cuda")
     assert (mx_gemm_nt(none(5, 0, "e4m3"), none(7, 0, "e4m3"), out=out, accumulate=True) == 1).all()
+
+
+@pytest.mark.parametrize("shape", [(5, 0), (0, 5), (0, 0), (2, 0, 3), (3, 2, 0)])
+@pytest.mark.parametrize("form", ["e4m3", "e2m1"])
+def test_matrices_of_nothing(shape, form):
+    """No rows or no columns: operands of those sizes in either direction, whose products are empty or zero."""
+    x = torch.empty(shape, device="cuda")
+    rows, cols = math.prod(shape[:-1]), shape[-1]
+    (q, qt), _ = mx_quantise(x, form, along="both")
+    for along, m in (("rows", q), ("columns", qt)):
+        alone = mx_quantise(x, form, along=along)[0]
+        assert (alone.rows, alone.cols) == (m.rows, m.cols) == ((rows, cols) if along == "rows" else (cols, rows))
+        assert not m.codes.any() and not m.scales.any()
+        got = mx_gemm_nt(m, mx_quantise(torch.ones(7, m.cols, device="cuda"))[0])
+        assert got.shape == (m.rows, 7) and not got.any()
 
 
 def test_product_twice_the_same_bits_other_streams_and_graphs():
