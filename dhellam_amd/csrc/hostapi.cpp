@@ -1263,7 +1263,7 @@ std::tuple<Tensor, Tensor, Tensor, OptTensor> rmsnorm_mx(const Tensor &inp, cons
                                                          const OptStream &stream) {
   OnGpu on({&inp, &weight, opt(residual), opt(sum_out), opt(ln_out)}, stream);
   const int64_t cols = weight.numel();
-  PY_ASSERT(inp.dim() > 0 && inp.size(-1) == cols, "LayerNorm not possible");
+  PY_ASSERT(inp.dim() > 0 && inp.size(-1) == cols && cols > 0, "LayerNorm not possible");
   PY_ASSERT(inp.is_contiguous() && weight.is_contiguous(), "norm: input and weight must be contiguous");
   PY_ASSERT(weight.scalar_type() == inp.scalar_type(), "norm: input and weight must be of one type");
   const auto like = [&](const OptTensor &t) {

@@ -81,6 +81,8 @@ def test_norm_in_place_not_finite_and_leading_dimensions():
         assert (zero[0].codes & 127 == 0).all() and (zero[0].scales == 0).all()
     empty = pyrmsnorm_mx_fwd(x[:0], gamma, EPS, False)
     assert empty[0].codes.shape[0] == 0 and empty[1].numel() == 0
+    with pytest.raises(AssertionError):
+        pyrmsnorm_mx_fwd(x[:, :0].contiguous(), gamma[:0], EPS, False)
 
 
 def test_norm_captured():
