@@ -11,6 +11,7 @@
 // allocated; a failed argument check raises AssertionError where the Python operator asserted and RuntimeError
 // otherwise; the GIL is released around the library call, as ctypes does.
 #include <torch/extension.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -1217,10 +1218,15 @@ void zero_all(const std::vector<Tensor> &ts, const OptStream &stream) {
 }
 
 // ---- microscaled operands -----------------------------------------------------------------------------------------------
+// at::empty past the dispatcher, which takes half of its time.
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor &like) {
+  return Tensor(at::detail::empty_cuda(sizes, type, like.device(), std::nullopt));
+}
+
 // Codes and scales of a rows x cols matrix in the given format (layout: include/dhellam_hip.h), one allocation for the two.
 std::pair<Tensor, Tensor> mx_empty(int64_t rows, int64_t cols, int format, const Tensor &like) {
   const int64_t kp = (cols + 127) / 128 * 128, width = format == DH_MX_E4M3 ? kp : kp / 2, cells = (rows + 3) / 4;
-  Tensor codes = at::empty({rows * width + kp / 128 * cells * 16}, like.options().dtype(at::kByte));      // (width is a multiple of 64)
+  Tensor codes = fresh({rows * width + kp / 128 * cells * 16}, at::kByte, like);      // (width is a multiple of 64)
   Tensor scales = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(codes.storage()), codes.key_set(), codes.dtype());
   scales.unsafeGetTensorImpl()->set_storage_offset(rows * width);
   scales.unsafeGetTensorImpl()->set_sizes_contiguous({kp / 128, cells, 4, 4});
@@ -1275,8 +1281,8 @@ std::tuple<Tensor, Tensor, Tensor, OptTensor> rmsnorm_mx(const Tensor &inp, cons
   const int64_t rows = cols ? inp.numel() / cols : 0;
   const int type = dt(inp);
   auto [codes, scales] = mx_empty(rows, cols, DH_MX_E4M3, inp);
-  Tensor rsigma = at::empty({rows}, inp.options().dtype(at::kFloat));
-  if (residual.has_value() && !sum_out.has_value()) sum_out = at::empty(residual->sizes(), residual->options());
+  Tensor rsigma = fresh({rows}, at::kFloat, inp);
+  if (residual.has_value() && !sum_out.has_value()) sum_out = fresh(residual->sizes(), residual->scalar_type(), inp);
   launch([&, &codes = codes, &scales = scales] {
     return dh_rmsnorm_mx(inp.data_ptr(), ptr(residual), mptr(sum_out), weight.data_ptr(), mptr(ln_out), codes.data_ptr(), scales.data_ptr(),
                          rsigma.data_ptr<float>(), rows, cols, (float)eps, zero_centered, cover, type, on.get());
@@ -1305,11 +1311,11 @@ Tensor mx_gemm_nt(const Tensor &a, const Tensor &as, int64_t m, int64_t fa_, con
   PY_ASSERT(out.has_value() || !accumulate, "mx_gemm_nt: nothing to accumulate into");
   PY_ASSERT(!out.has_value() || (out->dim() == 2 && out->size(0) == m && out->size(1) == n && (out->stride(1) == 1 || n <= 1) && (out->stride(0) >= n || m <= 1)),
             "mx_gemm_nt: out must be [m, n] with unit inner stride");
-  Tensor c = out.has_value() ? *out : at::empty({m, n}, a.options().dtype(out_dtype));
+  Tensor c = out.has_value() ? *out : fresh({m, n}, out_dtype, a);
   const int type = dt(c);
   const int64_t bytes = (int64_t)dh_mx_gemm_workspace_bytes(m, n, k, fa, fb, type);
   Tensor ws;                           // of this call alone, so that calls and captured graphs that overlap share none
-  if (bytes) ws = at::empty({bytes}, a.options());
+  if (bytes) ws = fresh({bytes}, at::kByte, a);
   launch([&] {
     return dh_mx_gemm_nt(a.data_ptr(), as.data_ptr(), fa, b.data_ptr(), bs.data_ptr(), fb, c.data_ptr(), m, n, k, m > 1 ? c.stride(0) : n, type, accumulate,
                          bytes ? ws.data_ptr() : nullptr, (size_t)bytes, on.get());
@@ -1339,10 +1345,10 @@ Tensor grad_norm(const std::vector<Tensor> &ts, const OptStream &stream) {
   const Grads g(ts);
   const Tensor like = ts.empty() ? at::empty({0}, at::TensorOptions().device(at::kCUDA, c10::hip::current_device())) : ts[0];
   OnGpu on({&like}, stream);
-  Tensor sum = at::empty({1}, like.options().dtype(at::kDouble));
+  Tensor sum = fresh({1}, at::kDouble, like);
   const int64_t bytes = (int64_t)dh_grad_norm_workspace_bytes(g.counts.data(), g.n());
   Tensor ws;                           // of this call alone
-  if (bytes) ws = at::empty({bytes}, like.options().dtype(at::kByte));
+  if (bytes) ws = fresh({bytes}, at::kByte, like);
   launch([&] {
     return dh_grad_norm(g.ptrs.data(), g.counts.data(), g.types.data(), g.n(), sum.data_ptr<double>(), bytes ? ws.data_ptr() : nullptr, (size_t)bytes,
                         on.get());
@@ -1376,7 +1382,7 @@ Tensor grad_clip(const std::vector<Tensor> &ts, const Tensor &sum, double max_no
     auto it = std::upper_bound(ranges.begin(), ranges.end(), begin, [](uintptr_t v, const Range &r) { return v < r.end; });
     PY_ASSERT(it == ranges.end() || it->begin >= end, "clip_grads: a result shares memory with a gradient that is not its own");
   }
-  Tensor found = at::empty({2}, sum.options().dtype(at::kFloat));
+  Tensor found = fresh({2}, at::kFloat, sum);
   std::vector<void *> outs;
   for (const void *p : o.ptrs) outs.push_back(const_cast<void *>(p));
   launch([&] {
