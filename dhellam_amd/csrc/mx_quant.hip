@@ -191,8 +191,8 @@ template <typename T, bool E4> static void launch_quantise(const QuantParams &p,
 // ---- residual addition, RMS norm, 8 bits with scales -----------------------------------------------------------------------
 // A row belongs to TPR threads, a thread holds VPT groups of 8 columns of it (group t + i TPR) from the first load to the last
 // store.  A block of 32 lies in the 4 lanes of a quad, the four blocks of a dword of scales in 16 lanes.
-// Bound by memory: 8192 x 8192 in bf16 with a residual 80 us, 5.9 TB/s (118 with the loads in branches, whose waits come one by one: so whole rows of
-// the commonest widths have a form without).  One row of 8192: 4 us, the launch and two trips to memory.
+// Bound by memory: 8192 x 8192 in bf16 with a residual 88 us, 5.4 TB/s (118 with the loads in branches, whose waits come one by one, and less exact: so whole
+// rows have a form without).  One row of 8192: 4 us, the launch and two trips to memory.
 struct NormMxParams {
   const void *x, *residual, *gamma;
   void *sum_out, *y;
@@ -242,26 +242,91 @@ template <typename T> __device__ __forceinline__ Loose8<T> sum8(const Loose8<T> 
   for (int j = 0; j < 8; ++j) o.v[j] = from_f<T>(to_f(a.v[j]) + to_f(b.v[j]));
   return o;
 }
-template <typename T> __device__ __forceinline__ float squares8(const Loose8<T> &a) {
-  float s = 0.f;
+// The sum of 8 squares.  Sums over lanes are in 64 bits, so that 1/rms is off by some 2^-29 before it is rounded.
+// The sum of 8 squares, in 64 bits as everything up to 1/rms.
+template <typename T> __device__ __forceinline__ double squares8(const Loose8<T> &a) {
+  double s[2] = {0.0, 0.0};
 #pragma unroll
-  for (int j = 0; j < 8; ++j) s += to_f(a.v[j]) * to_f(a.v[j]);
-  return s;
+  for (int j = 0; j < 8; ++j) s[j & 1] = fma((double)to_f(a.v[j]), (double)to_f(a.v[j]), s[j & 1]);
+  return s[0] + s[1];
+}
+template <int CTRL> __device__ __forceinline__ double dpp64(double v) {
+  const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)bits, CTRL, 0xf, 0xf, true);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(bits >> 32), CTRL, 0xf, 0xf, true);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double lane64(double v, int lane) {
+  const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)bits, lane), hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(bits >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// All 64 lanes' sum (a quad's, two quads', a row's of 16, the four rows').
+__device__ __forceinline__ double wave_sum64(double v) {
+  v += dpp64<0xb1>(v);      // lanes l ^ 1
+  v += dpp64<0x4e>(v);      // l ^ 2
+  v += dpp64<0x141>(v);     // 7 - l of the half row
+  v += dpp64<0x140>(v);     // 15 - l of the row
+  return (lane64(v, 0) + lane64(v, 16)) + (lane64(v, 32) + lane64(v, 48));
+}
+// 1 / sqrt(a) to 2^-44: fp32's and one step of Newton's iteration (fp32's alone where that is 0 or not finite).
+__device__ __forceinline__ double rsqrt64(double a) {
+  const float r0 = 1.0f / sqrtf((float)a);
+  const double r = (double)r0;
+  return fabsf(r0) < INFINITY ? fma(r * 0.5, fma(-a * r, r, 1.0), r) : r;
+}
+// What was computed from x before is computed again behind this, not kept: a row and gamma in 32 and in 64 bits do not fit the registers.
+template <typename T> __device__ __forceinline__ void keep_packed(Loose8<T> &x) {
+  uint32_t v[sizeof(x) / 4];
+  __builtin_memcpy(v, &x, sizeof(x));
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(x) / 4); ++i) asm volatile("" : "+v"(v[i]));
+  __builtin_memcpy(&x, v, sizeof(x));
+}
+// v to fp32, rounded to the neighbour whose last bit is set where v lies between two: a rounding to fewer bits behind it gives what it gives for v itself.
+__device__ __forceinline__ float to_odd(double v) {
+  const float f = (float)v;
+  const uint32_t bits = __float_as_uint(f);
+  const double back = (double)f;
+  const bool as_it_is = back == v || (bits & 1) || f == 0.f || !(fabsf(f) < INFINITY);
+  const uint32_t odd = (v > back) == (f > 0.f) ? bits + 1 : bits - 1;
+  return __uint_as_float(as_it_is ? bits : odd);
 }
 // The result of 8 columns (n exist) of a row: y, codes; returns the block's scale code (the same in the quad).
-template <typename T> __device__ __forceinline__ uint32_t norm_out8(const NormMxParams &p, const Loose8<T> &x, const Loose8<T> &gamma, float rs, int64_t row, int g,
+// fp32's y is off by 2^-22 of itself at most: 1/rms rounded, gamma + 1 rounded, two products.  Every place where a scale or an element changes has
+// zeros behind its fourth bit; a y that comes that near to one is formed again in 64 bits, so that codes and scales are those of
+// the exact y (to 2^-43).  One wavefront in 115 has such an element among its 512; without, 1 to 3 elements in 2 million were the neighbour.
+// 8192 x 8192 in bf16 88 us with it and the sums in 64 bits, 80 without; 512 x 8192 12 and 9.7.  All four groups' y before one such test were slower (93).
+template <typename T> __device__ __forceinline__ uint32_t norm_out8(const NormMxParams &p, Loose8<T> x, Loose8<T> gamma, double rs64, int64_t row, int g,
                                                                     int64_t kp, bool active) {
   const int n = p.cols - 8 * g;
+  const float rs = (float)rs64;
+  constexpr uint32_t NEAR = 4;                             // steps of fp32: 2^-22 of y at most
+  keep_packed(x);
+  keep_packed(gamma);
   float y[8];
-  uint32_t top = 0;
+  uint32_t near = ~0u;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     y[j] = to_f(x.v[j]) * rs * (to_f(gamma.v[j]) + p.shift);
     if (n < 8 && j >= n) y[j] = 0.f;                       // (a row of infinities or NaN makes products of zeros NaN)
+    else near = std::min(near, (__float_as_uint(y[j]) + NEAR) << 13);
+  }
+  if (p.y && active && n > 0) store8<T, false>(reinterpret_cast<T *>(p.y) + row * p.cols + 8 * g, rounded8<T>(y), n);
+  if (near <= 2 * NEAR << 13 && active) {
+    keep_packed(x);
+    keep_packed(gamma);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < n && (__float_as_uint(y[j]) + NEAR) << 13 <= 2 * NEAR << 13)
+        y[j] = to_odd((double)to_f(x.v[j]) * rs64 * ((double)to_f(gamma.v[j]) + (double)p.shift));
+  }
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
     const uint32_t m = magnitude(y[j]);
     top = top > m ? top : m;
   }
-  if (p.y && active && n > 0) store8<T, false>(reinterpret_cast<T *>(p.y) + row * p.cols + 8 * g, rounded8<T>(y), n);
   const uint32_t code = mx_scale_code<true>(quad_umax(top), p.cover);
   if (active) {
     const MxPack<true> o = mx_pack<true>(y, code);
@@ -272,13 +337,13 @@ template <typename T> __device__ __forceinline__ uint32_t norm_out8(const NormMx
 
 // TPR threads a row, ROWS rows a workgroup; gamma stays in registers.  All loads of a row go out before anything waits for one.
 template <typename T, int TPR, int VPT, int ROWS, bool WHOLE, bool RES, bool NT>
-__global__ void __launch_bounds__(TPR *ROWS, VPT == 4 ? 4 : 1) norm_mx_kernel(const NormMxParams p) {
+__global__ void __launch_bounds__(TPR *ROWS, VPT == 4 ? (sizeof(T) == 4 ? 3 : 4) : 1) norm_mx_kernel(const NormMxParams p) {
   constexpr int WPR = TPR / 64;
-  __shared__ float red[2][WPR * ROWS];
+  __shared__ double red[2][WPR * ROWS];
   const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
   const int groups = (p.cols + 127) / 128 * 16;
   const int64_t kp = (int64_t)groups * 8, cells = (p.rows + 3) / 4;
-  const float inv_cols = 1.0f / (float)p.cols;
+  const double inv_cols = 1.0 / (double)p.cols;
   const T *x = reinterpret_cast<const T *>(p.x), *res = reinterpret_cast<const T *>(p.residual);
   Loose8<T> gamma[VPT];
 #pragma unroll
@@ -297,7 +362,7 @@ __global__ void __launch_bounds__(TPR *ROWS, VPT == 4 ? 4 : 1) norm_mx_kernel(co
       held[i] = fetch8<T, WHOLE, NT>(x + row * p.cols + 8 * g, n);
       if constexpr (RES) add[i] = fetch8<T, WHOLE, NT>(res + row * p.cols + 8 * g, n);
     }
-    float s = 0.f;
+    double mine = 0.0;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int g = lane + i * TPR, n = active ? p.cols - 8 * g : 0;
@@ -305,17 +370,17 @@ __global__ void __launch_bounds__(TPR *ROWS, VPT == 4 ? 4 : 1) norm_mx_kernel(co
         held[i] = sum8(held[i], add[i]);
         if (n > 0) store8<T, NT>(reinterpret_cast<T *>(p.sum_out) + row * p.cols + 8 * g, held[i], n);
       }
-      s += squares8(held[i]);
+      mine += squares8(held[i]);
     }
-    s = wave_sum(s);
+    double s = wave_sum64(mine);
     if constexpr (WPR > 1) {                               // (two sets of sums: the next row's are written before every wavefront has read these)
       if ((threadIdx.x & 63) == 0) red[turn][threadIdx.x >> 6] = s;
       __syncthreads();
-      s = 0.f;
+      s = 0.0;
 #pragma unroll
       for (int i = 0; i < WPR; ++i) s += red[turn][sub * WPR + i];
     }
-    const float rs = 1.0f / sqrtf(s * inv_cols + p.eps);
+    const double rs = rsqrt64(s * inv_cols + (double)p.eps);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int g = lane + i * TPR;
@@ -324,21 +389,21 @@ __global__ void __launch_bounds__(TPR *ROWS, VPT == 4 ? 4 : 1) norm_mx_kernel(co
       if ((lane & 3) == 0 && row < 4 * cells)
         p.scales[((int64_t)(g >> 4) * cells + (row >> 2)) * 16 + ((g >> 2) & 3) * 4 + (row & 3)] = (uint8_t)code;
     }
-    if (active && lane == 0) p.rsigma[row] = rs;
+    if (active && lane == 0) p.rsigma[row] = (float)rs;
   }
 }
 
 // Rows of any length: one workgroup a row, read once for its statistics and again, from the cache, for its result.
 template <typename T, bool RES>
 __global__ void __launch_bounds__(1024) norm_mx_long_kernel(const NormMxParams p) {
-  __shared__ float red[16];
+  __shared__ double red[16];
   const int groups = (p.cols + 127) / 128 * 16;
   const int64_t kp = (int64_t)groups * 8, cells = (p.rows + 3) / 4;
   const T *res = reinterpret_cast<const T *>(p.residual);
   for (int64_t row = blockIdx.x; row < 4 * cells; row += gridDim.x) {
     const bool active = row < p.rows;
     const T *x = reinterpret_cast<const T *>(p.x) + row * p.cols;
-    float s = 0.f;
+    double s = 0.0;
     for (int g = threadIdx.x; active && g < groups; g += 1024) {
       const int n = p.cols - 8 * g;
       Loose8<T> v = fetch8<T, false, false>(x + 8 * g, n);
@@ -348,8 +413,14 @@ __global__ void __launch_bounds__(1024) norm_mx_long_kernel(const NormMxParams p
       }
       s += squares8(v);
     }
-    s = block_sum<1024>(s, red);
-    const float rs = 1.0f / sqrtf(s / (float)p.cols + p.eps);
+    s = wave_sum64(s);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    s = 0.0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s += red[i];
+    __syncthreads();                                       // (the next row's are written behind these reads)
+    const double rs = rsqrt64(s / (double)p.cols + (double)p.eps);
     if (RES) x = reinterpret_cast<const T *>(p.sum_out) + row * p.cols;      // a thread reads what it wrote itself
     for (int g = threadIdx.x; g < groups; g += 1024) {
       const int n = p.cols - 8 * g;
@@ -358,7 +429,7 @@ __global__ void __launch_bounds__(1024) norm_mx_long_kernel(const NormMxParams p
       if ((threadIdx.x & 3) == 0)
         p.scales[((int64_t)(g >> 4) * cells + (row >> 2)) * 16 + ((g >> 2) & 3) * 4 + (row & 3)] = (uint8_t)code;
     }
-    if (active && threadIdx.x == 0) p.rsigma[row] = rs;
+    if (active && threadIdx.x == 0) p.rsigma[row] = (float)rs;
   }
 }
 

@@ -85,6 +85,31 @@ def test_norm_in_place_not_finite_and_leading_dimensions():
         pyrmsnorm_mx_fwd(x[:, :0].contiguous(), gamma[:0], EPS, False)
 
 
+@pytest.mark.parametrize("rows,cols,dtype", [(1999, 1000, torch.float32), (512, 8192, torch.bfloat16), (128, 16384, torch.float16), (1024, 4096, torch.bfloat16),
+                                             (64, 40000, torch.bfloat16)])
+@pytest.mark.parametrize("centered,rule", [(False, "floor"), (True, "cover")])
+def test_codes_are_those_of_64_bits(rows, cols, dtype, centered, rule):
+    """y is off by 2^-43 of itself, and an element's boundaries lie a 16th of it apart: of 17 million elements in all these cases 3e-5 are expected to differ.
+    (In fp32 throughout it would be some 10; with the squares alone added in fp32, 2.)"""
+    x, _, gamma = inputs(rows, cols, dtype, 71)
+    q = pyrmsnorm_mx_fwd(x, gamma, EPS, centered, scale_rule=rule)[0]
+    held = x.double()
+    eps = torch.tensor(EPS, dtype=torch.float32).double().item()
+    y = held / torch.sqrt(held.square().mean(1, keepdim=True) + eps) * (gamma.double() + (1.0 if centered else 0.0))
+    codes, scales = R.quantise(y, "e4m3", rule)
+    assert torch.equal(q.scales, scales)
+    assert (((q.codes ^ codes) == 0) | (((q.codes | codes) & 127) == 0)).all()      # (zeros of either sign)
+
+
+def test_norm_of_products_past_the_smallest_number():
+    """x rsigma gamma below every fp32 number: zeros, of either sign."""
+    x = torch.randn(8, 256, device="cuda")
+    gamma = torch.full((256,), 1e-38, device="cuda")
+    x[:, ::2] *= 1e-30
+    q = pyrmsnorm_mx_fwd(x, gamma, EPS, False)[0]
+    assert (q.scales != 255).all() and (q.codes[:, :256:2] & 127 == 0).all() and R.values(q).isfinite().all()
+
+
 def test_norm_captured():
     x, r, gamma = inputs(33, 1000, torch.bfloat16, 9)
     stream = torch.cuda.Stream()
