@@ -13,8 +13,8 @@ namespace dh {
 // lanes, and no element goes through LDS before it is rounded.  What a lane holds of a column are 8 neighbouring elements
 // of the transposed result: they are packed in registers and go through LDS as 8 (4) bytes, so that memory gets
 // 128 (64) bytes of a row of the transpose at a time.
-// Bound by memory: 4096 x 7168 in bf16 to e4m3, along both directions 27 to 28 us (119 MB; 23.0 at what a copy of 1 GiB reaches, 5.2 TB/s), along the rows
-// 18.2 (89 MB; 17.1); 4096 x 8192 rows 20.0 (101 MB; 19.5).  A few rows: 4 to 5 us, most of it the launch.  Five or six workgroups on a
+// Bound by memory: 4096 x 7168 in bf16 to e4m3, along both directions 25 to 27 us (119 MB; 23.0 at what a copy of 1 GiB reaches, 5.2 TB/s); 4096 x 8192
+// along the rows 18.5 (101 MB; 19.5).  A few rows: 4 to 5 us, most of it the launch.  Five or six workgroups on a
 // compute unit by fewer registers were slower.
 struct QuantParams {
   const void *x;
