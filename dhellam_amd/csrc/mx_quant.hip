@@ -269,11 +269,14 @@ __device__ __forceinline__ double wave_sum64(double v) {
   v += dpp64<0x140>(v);     // 15 - l of the row
   return (lane64(v, 0) + lane64(v, 16)) + (lane64(v, 32) + lane64(v, 48));
 }
-// 1 / sqrt(a) to 2^-44: fp32's and one step of Newton's iteration (fp32's alone where that is 0 or not finite).
+// 1 / sqrt(a) to 2^-44 for any a of 64 bits: fp32's for a brought to [0.5, 2) by an even power of two, and one step of Newton's iteration
+// (fp32's alone where that is 0, infinite or NaN: a row that holds an infinity has 1/rms = 0).
 __device__ __forceinline__ double rsqrt64(double a) {
-  const float r0 = 1.0f / sqrtf((float)a);
+  const int even = __builtin_amdgcn_frexp_exp(a) & ~1;     // (0 for what is not finite)
+  const double m = ldexp(a, -even);
+  const float r0 = 1.0f / sqrtf((float)m);
   const double r = (double)r0;
-  return fabsf(r0) < INFINITY ? fma(r * 0.5, fma(-a * r, r, 1.0), r) : r;
+  return ldexp(r0 > 0.f && r0 < INFINITY ? fma(r * 0.5, fma(-m * r, r, 1.0), r) : r, -(even >> 1));
 }
 // What was computed from x before is computed again behind this, not kept: a row and gamma in 32 and in 64 bits do not fit the registers.
 template <typename T> __device__ __forceinline__ void keep_packed(Loose8<T> &x) {
@@ -292,13 +295,34 @@ __device__ __forceinline__ float to_odd(double v) {
   const uint32_t odd = (v > back) == (f > 0.f) ? bits + 1 : bits - 1;
   return __uint_as_float(as_it_is ? bits : odd);
 }
+// The magnitude (fp32 bits) past which the largest of a block makes its elements' fp32 arithmetic safe from the smallest numbers: where x / rms or the
+// result is subnormal it is off by more than 2^-22 of itself, but by 2^-150 of the largest |gamma| (or of 1) at most, and it is a zero
+// under a scale of 2^-109 of that.  The larger of the quad's, from the gammas that its threads hold.  (None for a row whose 1/rms may not be normal in fp32.)
+template <typename T> __device__ __forceinline__ float gamma_top(const Loose8<T> &gamma, float shift, float top) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(to_f(gamma.v[j]) + shift));
+  return top;
+}
+__device__ __forceinline__ uint32_t norm_safe_above(float gamma_top) { return __float_as_uint(0x1p-100f * __uint_as_float(quad_umax(magnitude(gamma_top)))); }
+__device__ __forceinline__ uint32_t norm_safe_row(uint32_t safe_above, double rs) { return rs >= 0x1p-100 && rs <= 0x1p100 ? safe_above : ~0u; }
+__device__ __forceinline__ uint32_t top8(const float (&y)[8]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t m = magnitude(y[j]);
+    top = top > m ? top : m;
+  }
+  return quad_umax(top);
+}
 // The result of 8 columns (n exist) of a row: y, codes; returns the block's scale code (the same in the quad).
 // fp32's y is off by 2^-22 of itself at most: 1/rms rounded, gamma + 1 rounded, two products.  Every place where a scale or an element changes has
 // zeros behind its fourth bit; a y that comes that near to one is formed again in 64 bits, so that codes and scales are those of
-// the exact y (to 2^-43).  One wavefront in 115 has such an element among its 512; without, 1 to 3 elements in 2 million were the neighbour.
-// 8192 x 8192 in bf16 88 us with it and the sums in 64 bits, 80 without; 512 x 8192 12 and 9.7.  All four groups' y before one such test were slower (93).
-template <typename T> __device__ __forceinline__ uint32_t norm_out8(const NormMxParams &p, Loose8<T> x, Loose8<T> gamma, double rs64, int64_t row, int g,
-                                                                    int64_t kp, bool active) {
+// the exact y (to 2^-43).  One wavefront in 115 has such an element among its 512 (zeros count as near too, but are not formed again); without, 1 to 3
+// elements in 2 million were the neighbour.  A block that fp32's smallest numbers reach, and a row whose 1/rms they or the largest reach, are formed
+// in 64 bits as a whole (8192 x 8192 86 us back to back, 84 without).  A result past fp32's largest number is not finite.
+// 8192 x 8192 in bf16 88 us with the sums and near elements in 64 bits, 80 without; 512 x 8192 12 and 9.7.  All four groups' y before one such test were slower (93).
+template <typename T> __device__ __forceinline__ uint32_t norm_out8(const NormMxParams &p, Loose8<T> x, Loose8<T> gamma, double rs64, uint32_t safe_above,
+                                                                    int64_t row, int g, int64_t kp, bool active) {
   const int n = p.cols - 8 * g;
   const float rs = (float)rs64;
   constexpr uint32_t NEAR = 4;                             // steps of fp32: 2^-22 of y at most
@@ -312,22 +336,25 @@ template <typename T> __device__ __forceinline__ uint32_t norm_out8(const NormMx
     if (n < 8 && j >= n) y[j] = 0.f;                       // (a row of infinities or NaN makes products of zeros NaN)
     else near = std::min(near, (__float_as_uint(y[j]) + NEAR) << 13);
   }
-  if (p.y && active && n > 0) store8<T, false>(reinterpret_cast<T *>(p.y) + row * p.cols + 8 * g, rounded8<T>(y), n);
   if (near <= 2 * NEAR << 13 && active) {
     keep_packed(x);
     keep_packed(gamma);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (j < n && (__float_as_uint(y[j]) + NEAR) << 13 <= 2 * NEAR << 13)
+      if (j < n && (__float_as_uint(y[j]) + NEAR) << 13 <= 2 * NEAR << 13 && y[j] != 0.f)
         y[j] = to_odd((double)to_f(x.v[j]) * rs64 * ((double)to_f(gamma.v[j]) + (double)p.shift));
   }
-  uint32_t top = 0;
+  uint32_t top = top8(y);
+  if (!(top > safe_above)) {                               // (the same in the quad)
+    keep_packed(x);
+    keep_packed(gamma);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t m = magnitude(y[j]);
-    top = top > m ? top : m;
+    for (int j = 0; j < 8; ++j)
+      if (j < n) y[j] = to_odd((double)to_f(x.v[j]) * rs64 * ((double)to_f(gamma.v[j]) + (double)p.shift));
+    top = top8(y);
   }
-  const uint32_t code = mx_scale_code<true>(quad_umax(top), p.cover);
+  if (p.y && active && n > 0) store8<T, false>(reinterpret_cast<T *>(p.y) + row * p.cols + 8 * g, rounded8<T>(y), n);
+  const uint32_t code = mx_scale_code<true>(top, p.cover);
   if (active) {
     const MxPack<true> o = mx_pack<true>(y, code);
     *reinterpret_cast<uint2 *>(p.codes + row * kp + 8 * g) = uint2{o.lo, o.hi};
@@ -351,6 +378,10 @@ __global__ void __launch_bounds__(TPR *ROWS, VPT == 4 ? (sizeof(T) == 4 ? 3 : 4)
     const int g = lane + i * TPR;
     gamma[i] = fetch8<T, WHOLE, false>(reinterpret_cast<const T *>(p.gamma) + 8 * g, p.cols - 8 * g);
   }
+  float largest = 1.f;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) largest = gamma_top(gamma[i], p.shift, largest);
+  const uint32_t safe_above = norm_safe_above(largest);
   int turn = 0;
   for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < 4 * cells; row0 += (int64_t)gridDim.x * ROWS, turn ^= 1) {
     const int64_t row = row0 + sub;
@@ -381,11 +412,12 @@ __global__ void __launch_bounds__(TPR *ROWS, VPT == 4 ? (sizeof(T) == 4 ? 3 : 4)
       for (int i = 0; i < WPR; ++i) s += red[turn][sub * WPR + i];
     }
     const double rs = rsqrt64(s * inv_cols + (double)p.eps);
+    const uint32_t safe_row = norm_safe_row(safe_above, rs);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int g = lane + i * TPR;
       if (g >= groups) continue;                           // (16 lanes at a time: groups is a multiple of 16)
-      const uint32_t code = norm_out8<T>(p, held[i], gamma[i], rs, row, g, kp, active);
+      const uint32_t code = norm_out8<T>(p, held[i], gamma[i], rs, safe_row, row, g, kp, active);
       if ((lane & 3) == 0 && row < 4 * cells)
         p.scales[((int64_t)(g >> 4) * cells + (row >> 2)) * 16 + ((g >> 2) & 3) * 4 + (row & 3)] = (uint8_t)code;
     }
@@ -400,6 +432,10 @@ __global__ void __launch_bounds__(1024) norm_mx_long_kernel(const NormMxParams p
   const int groups = (p.cols + 127) / 128 * 16;
   const int64_t kp = (int64_t)groups * 8, cells = (p.rows + 3) / 4;
   const T *res = reinterpret_cast<const T *>(p.residual);
+  float largest = 1.f;
+  for (int g = threadIdx.x; g < groups; g += 1024)
+    largest = gamma_top(fetch8<T, false, false>(reinterpret_cast<const T *>(p.gamma) + 8 * g, p.cols - 8 * g), p.shift, largest);
+  const uint32_t safe_above = norm_safe_above(largest);
   for (int64_t row = blockIdx.x; row < 4 * cells; row += gridDim.x) {
     const bool active = row < p.rows;
     const T *x = reinterpret_cast<const T *>(p.x) + row * p.cols;
@@ -421,11 +457,12 @@ __global__ void __launch_bounds__(1024) norm_mx_long_kernel(const NormMxParams p
     for (int i = 0; i < 16; ++i) s += red[i];
     __syncthreads();                                       // (the next row's are written behind these reads)
     const double rs = rsqrt64(s / (double)p.cols + (double)p.eps);
+    const uint32_t safe_row = norm_safe_row(safe_above, rs);
     if (RES) x = reinterpret_cast<const T *>(p.sum_out) + row * p.cols;      // a thread reads what it wrote itself
     for (int g = threadIdx.x; g < groups; g += 1024) {
       const int n = p.cols - 8 * g;
       const Loose8<T> v = fetch8<T, false, false>(x + 8 * g, active ? n : 0), gamma = fetch8<T, false, false>(reinterpret_cast<const T *>(p.gamma) + 8 * g, n);
-      const uint32_t code = norm_out8<T>(p, v, gamma, rs, row, g, kp, active);
+      const uint32_t code = norm_out8<T>(p, v, gamma, rs, safe_row, row, g, kp, active);
       if ((threadIdx.x & 3) == 0)
         p.scales[((int64_t)(g >> 4) * cells + (row >> 2)) * 16 + ((g >> 2) & 3) * 4 + (row & 3)] = (uint8_t)code;
     }

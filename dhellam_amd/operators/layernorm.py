@@ -31,7 +31,8 @@ def pylayernorm_fwd(inp, ln_weight, ln_bias, eps, fwd_sm_margin, zero_centered_g
 def pyrmsnorm_mx_fwd(inp, ln_weight, eps, zero_centered_gamma, stream=None, profiling=False, residual=None, sum_out=None,
                      ln_out=None, scale_rule="floor"):
     """RMSNorm whose result is written in 8 bits with scales (``operators.mx.MXTensor``, e4m3, blocks of 32 along the row): codes
-    and scales of the exact result.  Returns (MXTensor, rsigma, sum, ms); ``residual`` and ``sum_out`` as in ``pylayernorm_fwd`` (sum is None without), the
+    and scales of the exact result, whatever the size of the row's elements.  A row that holds an infinity has rsigma 0, zeros and, in the block of
+    the infinity, NaN.  Returns (MXTensor, rsigma, sum, ms); ``residual`` and ``sum_out`` as in ``pylayernorm_fwd`` (sum is None without), the
     backward is ``pylayernorm_bwd``'s on ``rsigma`` and the row that was normalised.  ``ln_out``: a tensor like the input that receives the result
     in its own type as well.  ``scale_rule``: see ``operators.mx.mx_quantise``."""
     if ln_out is not None:

@@ -687,7 +687,9 @@ int dh_mx_quantise(const void *x, int64_t rows, int64_t cols, int64_t ldx, int d
                    int cover, void *codes, void *scales, void *codes_t, void *scales_t, void *stream);
 
 /* dh_norm_fwd as RMSNorm (dh_add_norm_fwd with a residual; sum_out may be x or residual) whose result is quantised to e4m3:
- * codes and scales are those of the exact result (to 2^-43 of it).  y (may be NULL): the result in `dtype` as well.  rsigma fp32 [rows].  cols <= 2^24. */
+ * codes and scales are those of the exact result (to 2^-43 of it; one past fp32's largest number is not finite) for every row of finite
+ * numbers.  rsigma fp32 [rows]: 1/rms, rounded once; 0 for a row that holds an infinity, which is then zeros but for the infinity's block (NaN).
+ * y (may be NULL): the result in `dtype` as well.  cols <= 2^24. */
 int dh_rmsnorm_mx(const void *x, const void *residual, void *sum_out, const void *gamma, void *y,
                   void *codes, void *scales, float *rsigma, int64_t rows, int64_t cols, float eps,
                   int zero_centered_gamma, int cover, int dtype, void *stream);
