@@ -153,6 +153,18 @@ template <bool NT> __global__ void __launch_bounds__(256) grad_clip_kernel(const
 #undef GRAD_SCALE
 }
 
+// The whole list, before the first table is launched: a call that is refused has changed nothing.
+static int grad_check(const void *const *g, void *const *out, const int64_t *counts, const int *types, const int *out_types, int n) {
+  for (int i = 0; i < n; ++i) {
+    DH_CHECK(counts[i] >= 0, "tensor %d: %lld elements", i, (long long)counts[i]);
+    DH_CHECK(types[i] == DH_F32 || types[i] == DH_BF16 || types[i] == DH_F16, "tensor %d: unknown dtype %d", i, types[i]);
+    DH_CHECK(!out || out_types[i] == types[i] || out_types[i] == DH_F32, "tensor %d: results are of its own type or fp32", i);
+    DH_CHECK(counts[i] == 0 || (g[i] && (!out || out[i])), "tensor %d: null pointer", i);
+    DH_CHECK(counts[i] < GRAD_PIECE << 30, "tensor %d is too large", i);
+  }
+  return DH_OK;
+}
+
 // Calls fn(table) for the lists in tables of up to GRAD_TABLE tensors that are not empty.
 template <typename F>
 static int grad_tables(const void *const *g, void *const *out, const int64_t *counts, const int *types, const int *out_types, int n, F &&fn) {
@@ -160,13 +172,8 @@ static int grad_tables(const void *const *g, void *const *out, const int64_t *co
     GradTable t{};
     int64_t blocks = 0;
     for (; i < n && t.count < GRAD_TABLE; ++i) {
-      DH_CHECK(counts[i] >= 0, "tensor %d: %lld elements", i, (long long)counts[i]);
-      DH_CHECK(types[i] == DH_F32 || types[i] == DH_BF16 || types[i] == DH_F16, "tensor %d: unknown dtype %d", i, types[i]);
-      DH_CHECK(!out || out_types[i] == types[i] || out_types[i] == DH_F32, "tensor %d: results are of its own type or fp32", i);
       if (counts[i] == 0) continue;
-      DH_CHECK(g[i] && (!out || out[i]), "tensor %d: null pointer", i);
       const int64_t b = cdiv(counts[i], GRAD_PIECE);
-      DH_CHECK(b < (1ll << 30), "tensor %d is too large", i);
       if (t.count > 0 && blocks + b >= (1ll << 31)) break;
       t.g[t.count] = g[i];
       t.out[t.count] = out ? out[i] : nullptr;
@@ -195,7 +202,7 @@ extern "C" int dh_grad_norm(const void *const *grads, const int64_t *counts, con
                             size_t workspace_bytes, void *stream) {
   using namespace dh;
   DH_CHECK(n >= 0 && (n == 0 || (grads && counts && dtypes)) && sum_sq, "bad list");
-  for (int i = 0; i < n; ++i) DH_CHECK(counts[i] >= 0, "tensor %d: %lld elements", i, (long long)counts[i]);
+  if (const int rc = grad_check(grads, nullptr, counts, dtypes, nullptr, n)) return rc;
   const size_t need = dh_grad_norm_workspace_bytes(counts, n);
   DH_CHECK(need == 0 || (workspace && (uintptr_t)workspace % 8 == 0 && workspace_bytes >= need), "workspace of %zu bytes, %zu are needed", workspace_bytes,
            need);
@@ -225,6 +232,7 @@ extern "C" int dh_grad_clip(const void *const *grads, void *const *out, const in
   DH_CHECK(n >= 0 && (n == 0 || (grads && out && counts && dtypes && out_dtypes)) && sum_sq && found, "bad list");
   DH_CHECK(max_norm >= 0, "max_norm %g", max_norm);
   DH_CHECK(std::isfinite(scale), "scale %g", scale);
+  if (const int rc = grad_check(grads, out, counts, dtypes, out_dtypes, n)) return rc;
   const hipStream_t st = (hipStream_t)stream;
   float *say = found;
   int64_t bytes = 0;
