@@ -4,6 +4,7 @@
 //   sum_sq = sum over all elements of g^2           norm = |scale| sqrt(sum_sq)
 //   factor = scale min(1, max_norm / (norm + 1e-6)) out = factor g
 //
+// with the norm and the factor in 64 bits; a norm that fp32 cannot hold counts as not finite, and a factor that rounds to 0 in fp32 as 0.
 // Both passes cut every tensor into pieces of 32768 elements, a workgroup each; a launch takes up to 80 tensors from a table in
 // its arguments.  Squares are added in 64 bits (an fp32 square overflows from 1.8e19 on), a workgroup's sum is written to its own
 // place and one workgroup adds these up in order: the result is the same bits every time.  Bound by memory: 16-byte loads at any alignment.
@@ -105,7 +106,7 @@ __global__ void __launch_bounds__(1024) grad_join_kernel(const double *partial, 
 }
 
 // (a lane stores 16 bytes, so that a wavefront's store is one run of memory: fp32 from 16 bits in pieces of 32 bytes a lane ran at 4.7 TB/s)
-template <typename T, typename TO, bool NT> __device__ __forceinline__ void grad_piece_scale(const T *g, TO *out, int64_t n, float factor) {
+template <typename T, typename TO, bool NT> __device__ __forceinline__ void grad_piece_scale(const T *g, TO *out, int64_t n, float factor, float behind) {
   constexpr int N = 16 / (int)sizeof(TO), STEP = 256 * N;
 #pragma unroll 8
   for (int i = 0; i < (int)GRAD_PIECE / STEP; ++i) {
@@ -114,7 +115,7 @@ template <typename T, typename TO, bool NT> __device__ __forceinline__ void grad
       const Run<T, N> x = grad_load<NT, T, N>(g + at);
       Run<TO, N> o;
 #pragma unroll
-      for (int j = 0; j < N; ++j) o.v[j] = factor == 0.f ? from_f<TO>(0.f) : from_f<TO>(to_f(x.v[j]) * factor);
+      for (int j = 0; j < N; ++j) o.v[j] = factor == 0.f ? from_f<TO>(0.f) : from_f<TO>(to_f(x.v[j]) * factor * behind);
       if constexpr (NT) {
         dh_u32x4 q;
         __builtin_memcpy(&q, &o, 16);
@@ -123,7 +124,7 @@ template <typename T, typename TO, bool NT> __device__ __forceinline__ void grad
         *reinterpret_cast<Run<TO, N> *>(out + at) = o;
       }
     } else {
-      for (int64_t j = at; j < n; ++j) out[j] = factor == 0.f ? from_f<TO>(0.f) : from_f<TO>(to_f(g[j]) * factor);
+      for (int64_t j = at; j < n; ++j) out[j] = factor == 0.f ? from_f<TO>(0.f) : from_f<TO>(to_f(g[j]) * factor * behind);
     }
   }
 }
@@ -131,17 +132,18 @@ template <typename T, typename TO, bool NT> __device__ __forceinline__ void grad
 template <bool NT> __global__ void __launch_bounds__(256) grad_clip_kernel(const GradTable t, const double *sum_sq, double max_norm, double scale, float *found) {
   const double norm = fabs(scale) * sqrt(sum_sq[0]);
   double factor = scale * fmin(1.0, max_norm / (norm + 1e-6));
-  if (!(norm < INFINITY)) factor = 0.0;
+  if (!((float)norm < INFINITY) || (float)factor == 0.f) factor = 0.0;
   if (found && blockIdx.x == 0 && threadIdx.x == 0) {
     found[0] = (float)norm;
     found[1] = (float)factor;
   }
   if (t.blocks == 0) return;
-  const float f = (float)factor;
+  // a factor below fp32's normal numbers in two steps, so that it keeps its 24 bits (the second is a power of two)
+  const float behind = fabs(factor) < 0x1p-126 ? 0x1p-64f : 1.f, f = (float)(behind == 1.f ? factor : factor * 0x1p64);
   const int i = grad_find(t, (int)blockIdx.x);
   const int64_t at = (int64_t)((int)blockIdx.x - t.first[i]) * GRAD_PIECE, n = t.n[i] - at;
   if (f == 1.f && t.g[i] == t.out[i]) return;              // in place, nothing to change
-#define GRAD_SCALE(T, TO) grad_piece_scale<T, TO, NT>(reinterpret_cast<const T *>(t.g[i]) + at, reinterpret_cast<TO *>(t.out[i]) + at, n, f)
+#define GRAD_SCALE(T, TO) grad_piece_scale<T, TO, NT>(reinterpret_cast<const T *>(t.g[i]) + at, reinterpret_cast<TO *>(t.out[i]) + at, n, f, behind)
   if (t.type[i] == DH_F32) GRAD_SCALE(float, float);
   else if (t.type[i] == DH_BF16) {
     if (t.out_type[i] == DH_F32) GRAD_SCALE(bf16_t, float);
@@ -231,7 +233,7 @@ extern "C" int dh_grad_clip(const void *const *grads, void *const *out, const in
   using namespace dh;
   DH_CHECK(n >= 0 && (n == 0 || (grads && out && counts && dtypes && out_dtypes)) && sum_sq && found, "bad list");
   DH_CHECK(max_norm >= 0, "max_norm %g", max_norm);
-  DH_CHECK(std::isfinite(scale), "scale %g", scale);
+  DH_CHECK(std::isfinite((float)scale), "scale %g", scale);
   if (const int rc = grad_check(grads, out, counts, dtypes, out_dtypes, n)) return rc;
   const hipStream_t st = (hipStream_t)stream;
   float *say = found;

@@ -19,8 +19,8 @@ def grad_norm(grads, stream=None, profiling=False):
 def clip_grads(grads, sum_sq, max_norm, scale=1.0, out=None, stream=None, profiling=False):
     """out = factor * grads with norm = |scale| sqrt(sum_sq), factor = scale min(1, max_norm / (norm + 1e-6)); in place without ``out``.
     ``scale`` undoes a loss scale on the way; ``max_norm=inf`` clips nothing.  ``out``: a tensor for each gradient, of its layout and its
-    type or fp32 (the optimiser's copies), memory of its own or the gradient itself.  Where the norm is not finite the factor is 0 and zeros are
-    written, whatever the gradients hold: such a step moves no weight.  Returns (found fp32 [2] on the device: norm, factor; ms)."""
+    type or fp32 (the optimiser's copies), memory of its own or the gradient itself.  Where the norm is not finite, or past fp32's
+    largest number, the factor is 0 and zeros are written, whatever the gradients hold: such a step moves no weight.  Returns (found fp32 [2] on the device: norm, factor; ms)."""
     grads = list(grads)
     out = None if out is None else list(out)
     _lib.mark_written(*(grads if out is None else out))

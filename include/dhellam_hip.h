@@ -718,7 +718,8 @@ size_t dh_grad_norm_workspace_bytes(const int64_t *counts, int n);
 int dh_grad_norm(const void *const *grads, const int64_t *counts, const int *dtypes, int n,
                  double *sum_sq, void *workspace, size_t workspace_bytes, void *stream);
 /* out[i] = factor grads[i] with norm = |scale| sqrt(sum_sq), factor = scale min(1, max_norm / (norm + 1e-6)); where the norm is not
- * finite the factor is 0 and zeros are written.  found (fp32 [2]): norm, factor.  out[i] is of the gradient's type or fp32, and
+ * finite, or past fp32's largest number, the factor is 0 and zeros are written, as with a factor below fp32's smallest number.  found (fp32 [2]):
+ * norm, factor.  scale is a number of fp32, finite.  out[i] is of the gradient's type or fp32, and
  * grads[i] itself or a place of its own. */
 int dh_grad_clip(const void *const *grads, void *const *out, const int64_t *counts, const int *dtypes,
                  const int *out_dtypes, int n, const double *sum_sq, double max_norm, double scale,

@@ -41,3 +41,10 @@ def test_results_of_the_clipping(at, what, text):
     g, n, t, o, ot = _lists(at, **{**dict(pointer=P, count=8, dtype=1, out_pointer=P, out_dtype=1), **what})
     assert lib.dh_grad_clip(g, o, n, t, ot, N, P, 1.0, 1.0, P, None) == -1
     assert text in lib.dh_last_error().decode() and f"tensor {at}" in lib.dh_last_error().decode()
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e39, 3.5e38])
+def test_a_scale_past_fp32(scale):
+    lib = _lib_()
+    g, n, t, o, ot = _lists(0, P, 8, 1, P, 1)
+    assert lib.dh_grad_clip(g, o, n, t, ot, N, P, 1.0, scale, P, None) == -1 and "scale" in lib.dh_last_error().decode()
