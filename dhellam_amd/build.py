@@ -226,74 +226,190 @@ def mx_gemm_assembly() -> dict:
 
 def check_mx_gemm_loops(verbose: bool = False) -> int:
     """The tiled products of microscaled operands copy to LDS from assembly too, and form their sums in assembly: the generated code of every
-    instantiation is held to the order that the source lays down (``check_mx_gemm_order``).  Returns their number; raises on a violation."""
+    instantiation is held to the order that the source lays down (``check_mx_gemm_order``) and to the distances that the compiler does not keep
+    for instructions it does not know (``check_mx_gemm_distances``).  Returns their number; raises on a violation."""
     kernels = mx_gemm_assembly()
     for name, fn in kernels.items():
         body = check_mx_gemm_order(name, fn)
+        check_mx_gemm_distances(name, fn)
         if verbose:
             print(f"checked {name}: {body} lines", flush=True)
     return len(kernels)
 
 
-def check_mx_gemm_order(name: str, fn: list) -> int:
-    """One instantiation of ``mx_w8_kernel`` or ``mx_t128_kernel``: two slices in the innermost loop with matrix instructions.  Every copy goes
-    to LDS.  ``mx_w8_kernel``: 16 clusters between barriers, every second one of 8 matrix instructions and no copy, the others beginning with the
-    wait for the wavefront's earlier reads and ending, where they publish copies, with the counted wait.  ``mx_t128_kernel``: a slice ends with
-    the waits for reads and copies and a barrier, and its copies go out behind that.  No scratch accesses in the loop, and behind it the
-    last copies are waited for before LDS is used again or the kernel ends."""
+def _mx_gemm_parts(name: str, fn: list):
+    """The code of an instantiation before, in and behind its main loop (the innermost loop with the matrix instructions of two slices), and what a
+    slice has: its matrix instructions, a wavefront's copies."""
     import re
     fa, fb = (int(x) for x in re.search(r"kernelILi(\d)ELi(\d)E", name).groups())
-    eight, wide = "mx_w8" in name, "Lb1E" in name
     two = fa == 4 and fb == 4
     rows = lambda bits: 2 if two or bits == 8 else 1                  # 1 KB copies of 64 rows
-    copies = (2 if two else 1) + 2 * rows(fa) + 2 * rows(fb)          # of a wavefront a slice
-    slice_mfmas = 32 if eight else 64 if wide else 16
+    copies = (2 if two else 1) + 2 * rows(fa) + 2 * rows(fb)
+    slice_mfmas = 32 if "mx_w8" in name else 64 if "Lb1E" in name else 16
     code = [x for x in (l.split(";")[0].strip() for l in fn) if x]
     labels = {m.group(1): i for i, l in enumerate(code) if (m := re.match(r"^(\.LBB\d+_\d+):", l))}
+    loops = []
+    for i, l in enumerate(code):
+        m = re.match(r"s_c?branch\w* (\.LBB\d+_\d+)", l)
+        if m and m.group(1) in labels and labels[m.group(1)] < i and sum("v_mfma" in x for x in code[labels[m.group(1)] + 1:i]) == 2 * slice_mfmas:
+            loops.append((labels[m.group(1)] + 1, i))
+    if not loops:
+        raise RuntimeError(f"{name}: no main loop with {2 * slice_mfmas} matrix instructions")
+    lo, hi = min(loops, key=lambda x: x[1] - x[0])
+    plain = lambda part: [x for x in part if not x.endswith(":")]
+    return plain(code[:lo]), plain(code[lo:hi]), plain(code[hi:]), slice_mfmas, copies
+
+
+def check_mx_gemm_order(name: str, fn: list) -> int:
+    """One instantiation of ``mx_w8_kernel`` or ``mx_t128_kernel``: the first copies, published before anything is read; two slices in the main loop;
+    and behind it the last slice of an odd number, held to the same.  Every copy goes to LDS.
+    ``mx_w8_kernel``: 8 clusters a slice between barriers, every second one of 8 matrix instructions and no copy, the others beginning with the
+    wait for the wavefront's earlier reads and ending, where they publish copies, with the counted wait.  ``mx_t128_kernel``: a slice begins with
+    the waits for reads and copies and a barrier, and its copies go out behind that.  No scratch accesses in the loop, and behind the last slice the
+    last copies are waited for before LDS is used again or the kernel ends.  Returns the lines of the loop."""
+    first, body, rest, slice_mfmas, copies = _mx_gemm_parts(name, fn)
+    eight = "mx_w8" in name
     mfmas = lambda part: sum("v_mfma" in x for x in part)
-    is_copy = lambda x: x.startswith("buffer_load")
+    copies_of = lambda part: [i for i, x in enumerate(part) if x.startswith("buffer_load")]
+    reads_of = lambda part: [i for i, x in enumerate(part) if x.startswith("ds_read")]
+    barriers = lambda part: [i for i, x in enumerate(part) if x.startswith("s_barrier")]
 
     def need(ok, what):
         if not ok:
             raise RuntimeError(f"{name}: {what}")
 
-    loops = []
-    for i, l in enumerate(code):
-        m = re.match(r"s_c?branch\w* (\.LBB\d+_\d+)", l)
-        if m and m.group(1) in labels and labels[m.group(1)] < i and mfmas(code[labels[m.group(1)] + 1:i]) == 2 * slice_mfmas:
-            loops.append((labels[m.group(1)] + 1, i))
-    need(loops, f"no main loop with {2 * slice_mfmas} matrix instructions")
-    lo, hi = min(loops, key=lambda x: x[1] - x[0])
-    body = [x for x in code[lo:hi] if not x.endswith(":")]
-    need(all(x.endswith("lds") for x in code if is_copy(x)), "a buffer load to registers")
+    def published(part, at):                       # the waits right before a barrier of mx_t128_kernel
+        return part[at - 2:at] == ["s_waitcnt lgkmcnt(0)", "s_waitcnt vmcnt(0)"]
+
+    def check_clusters(clusters, where):
+        dma = 0
+        for n, cl in enumerate(clusters):
+            need(mfmas(cl) == (8 if n % 2 else 0), f"{where}: cluster {n} holds {mfmas(cl)} matrix instructions")
+            need(not any("scratch_" in x for x in cl), f"{where}: scratch accesses in cluster {n}")
+            at, waits, reads = copies_of(cl), [i for i, x in enumerate(cl) if x == "s_waitcnt lgkmcnt(0)"], reads_of(cl)
+            dma += len(at)
+            if n % 2:
+                need(not at, f"{where}: a copy in cluster {n}, among matrix instructions")
+                continue
+            need(waits and not (reads and reads[0] < waits[0]) and not (at and at[0] < waits[0]),
+                 f"{where}: cluster {n} does not begin with the wait for the earlier reads")
+            need(not at or f"s_waitcnt vmcnt({copies})" in cl[at[-1]:], f"{where}: cluster {n} publishes copies without the counted wait")
+        need(dma == len(clusters) // 8 * copies, f"{where}: {dma} copies in {len(clusters) // 8} slices of {copies}")
+
+    need(all(x.endswith("lds") for part in (first, body, rest) for x in part if x.startswith("buffer_load")), "a buffer load to registers")
+    need(mfmas(first) == 0 and mfmas(rest) == slice_mfmas, f"{mfmas(first)} and {mfmas(rest)} matrix instructions before and behind the main loop")
+    # the first two slices' copies
+    dma, reads, at = copies_of(first), reads_of(first), barriers(first)
+    need(len(dma) == 2 * copies, f"{len(dma)} copies before the main loop, expected {2 * copies}")
+    need(at and reads and reads[0] > at[0], "a fragment is read before the first slice is published")
+    if eight:
+        need(len(at) == 2 and at[0] > dma[-1] and f"s_waitcnt vmcnt({copies})" in first[dma[-1]:at[0]] and reads[0] > at[1],
+             "the first slice is not published by the counted wait and a barrier, one more of half of the wavefronts behind it")
+    else:
+        need(len(at) == 1 and dma[copies - 1] < at[0] < dma[copies] and "s_waitcnt vmcnt(0)" in first[dma[copies - 1]:at[0]],
+             "the first slice is not published by the wait for its copies and a barrier")
+    # the main loop
     need(not any("scratch_" in x for x in body), "scratch accesses in the main loop")
-    need(sum(map(is_copy, body)) == 2 * copies, f"{sum(map(is_copy, body))} copies in the main loop, expected {2 * copies}")
-    at = [i for i, x in enumerate(body) if x.startswith("s_barrier")]
+    need(len(copies_of(body)) == 2 * copies, f"{len(copies_of(body))} copies in the main loop, expected {2 * copies}")
+    at = barriers(body)
     if eight:
         need(len(at) == 16, f"{len(at)} barriers in the main loop, expected 16")
         clusters = [body[a + 1:b] for a, b in zip([-1] + at, at)]
         clusters[0] = body[at[-1] + 1:] + clusters[0]
-        for n, cl in enumerate(clusters):
-            need(mfmas(cl) == (8 if n % 2 else 0), f"cluster {n} holds {mfmas(cl)} matrix instructions")
-            dma, waits = [i for i, x in enumerate(cl) if is_copy(x)], [i for i, x in enumerate(cl) if x == "s_waitcnt lgkmcnt(0)"]
-            reads = [i for i, x in enumerate(cl) if x.startswith("ds_read")]
-            if n % 2:
-                need(not dma, f"a copy in cluster {n}, among matrix instructions")
-                continue
-            need(waits and not (reads and reads[0] < waits[0]) and not (dma and dma[0] < waits[0]), f"cluster {n} does not begin with the wait for the earlier reads")
-            need(not dma or f"s_waitcnt vmcnt({copies})" in cl[dma[-1]:], f"cluster {n} publishes copies without the counted wait")
+        check_clusters(clusters, "main loop")
     else:
         need(len(at) == 2, f"{len(at)} barriers in the main loop, expected 2")
-        for b in at:
-            need(body[b - 2:b] == ["s_waitcnt lgkmcnt(0)", "s_waitcnt vmcnt(0)"], "a slice ends without the waits for its reads and copies")
+        need(all(published(body, b) for b in at), "a slice begins without the waits for reads and copies")
         for part in (body[at[0] + 1:at[1]], body[at[1] + 1:] + body[:at[0]]):
-            need(mfmas(part) == slice_mfmas and sum(map(is_copy, part)) == copies, "a slice's copies or matrix instructions are in another's place")
-    rest = [x for x in code[hi:] if not x.endswith(":")]
+            need(mfmas(part) == slice_mfmas and len(copies_of(part)) == copies, "a slice's copies or matrix instructions are in another's place")
+    # the last slice of an odd number
+    at = barriers(rest)
+    if eight:
+        need(len(at) >= 9, f"{len(at)} barriers behind the main loop, expected 9 and more")
+        clusters = [rest[a + 1:b] for a, b in zip([-1] + at, at[:8])]
+        waits = [i for i, x in enumerate(clusters[0]) if x == "s_waitcnt lgkmcnt(0)"]      # (the blocks that the branches over it lead to)
+        need(waits and not reads_of(clusters[0][:waits[-1]]), "last slice: a read before the wait for the earlier ones")
+        clusters[0] = clusters[0][waits[-1]:]
+        check_clusters(clusters, "last slice")
+    else:
+        need(len(at) >= 2 and published(rest, at[0]), "the last slice begins without the waits for reads and copies")
+        part = rest[at[0] + 1:at[1]]
+        need(mfmas(part) == slice_mfmas and len(copies_of(part)) == copies and not reads_of(rest[:at[0]]) and not any("scratch_" in x for x in part),
+             "the last slice's reads, copies or matrix instructions are in another's place")
     last = max(i for i, x in enumerate(rest) if "v_mfma" in x)
     landed = next((i for i in range(last, len(rest)) if rest[i].startswith("s_waitcnt vmcnt(0)")), len(rest))
     used = next((i for i in range(last, len(rest)) if rest[i].startswith(("ds_", "global_store", "s_endpgm"))), len(rest))
     need(landed < used, "LDS is used again, or the kernel ends, before the last copies have landed")
+    need(eight or any(landed < i < used for i in barriers(rest)), "LDS is used again before every wavefront's last copies have landed")
     return len(body)
+
+
+def check_mx_gemm_distances(name: str, fn: list) -> int:
+    """The wait states around instructions from assembly, which the compiler does not insert.  Two between a vector instruction that writes an operand
+    (fragment, scale, sum) of a scaled matrix instruction and that one; 24 (16 passes and what a vector instruction needs behind them, with some to
+    spare) between it and any other access to its sums; five between a vector instruction that writes scalar registers (a lane's read, a comparison)
+    and a copy that takes its descriptor or offset from these.  On every way through the code; an instruction counts as one state, s_nop n as n + 1.
+    Returns the number of instructions that were checked; raises on a violation."""
+    import re
+    two_results = ("v_swap", "v_permlane16_swap", "v_permlane32_swap")
+    scalar_results = ("v_cmp", "v_readlane", "v_readfirstlane", "v_add_co", "v_addc", "v_sub_co", "v_subb", "v_subrev_co", "v_mad_u64", "v_mad_i64", "v_div_scale")
+
+    def registers(operand):
+        out = set()
+        for kind, lo, hi, one in re.findall(r"\b([vas])\[(\d+):(\d+)\]|\b([vas]\d+)\b", operand):
+            out |= {one} if one else {f"{kind}{i}" for i in range(int(lo), int(hi) + 1)}
+        return out
+
+    class Instruction:
+        def __init__(self, line):
+            self.op, _, args = line.partition(" ")
+            # (modifiers name no registers)
+            args = [x.strip() for x in re.split(r",(?![^\[]*\])", args)] if args else []
+            self.uses = [registers(x) for x in args]
+            self.states = int(args[0], 0) + 1 if self.op == "s_nop" else 1
+            vector = self.op.startswith("v_") and not self.op.startswith("v_mfma")
+            self.wrote = set().union(*self.uses[:2 if self.op.startswith(two_results) else 1]) if vector else set()
+            self.wrote_scalars = {r for u in self.uses[:2] for r in u if r[0] == "s"} if self.op.startswith(scalar_results) else set()
+            self.target = args[0] if re.match(r"s_c?branch", self.op) else None
+            self.before, self.behind = [], []
+
+    code, labels = [], {}
+    for line in (l.split(";")[0].strip() for l in fn):
+        if m := re.match(r"^([.\w]+):", line):
+            labels[m.group(1)] = len(code)
+        elif line and not line.startswith("."):
+            code.append(Instruction(line))
+    for i, x in enumerate(code):
+        if x.op not in ("s_branch", "s_endpgm") and i + 1 < len(code):
+            x.behind.append(i + 1)
+        if x.target is not None:
+            x.behind.append(labels[x.target])
+        for j in x.behind:
+            code[j].before.append(i)
+
+    def look(i, states, way, hit, what):
+        left, todo = {}, [(j, states) for j in getattr(code[i], way)]
+        while todo:
+            j, n = todo.pop()
+            if n <= left.get(j, 0):
+                continue
+            left[j] = n
+            if hit(code[j]):
+                raise RuntimeError(f"{name}: {what}: {code[j].op}")
+            todo += [(k, n - code[j].states) for k in getattr(code[j], way)]
+
+    checked = 0
+    for i, x in enumerate(code):
+        if x.op.startswith("v_mfma_scale"):
+            operands, sums = set().union(*x.uses[:6]), x.uses[0]
+            look(i, 2, "before", lambda c: bool(c.wrote & operands), "an operand of a matrix instruction is written within two wait states before it")
+            look(i, 24, "behind", lambda c: not c.op.startswith("v_mfma") and any(sums & u for u in c.uses), "a sum is used too close behind its matrix instruction")
+            checked += 1
+        elif x.op.startswith("buffer_load"):
+            scalars = {r for u in x.uses for r in u if r[0] == "s"}
+            look(i, 5, "before", lambda c: bool(c.wrote_scalars & scalars), "a copy's scalar registers are written within five wait states before it")
+            checked += 1
+    return checked
 
 
 EXT_PKG = ROOT / "dhellam"

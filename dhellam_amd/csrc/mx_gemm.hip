@@ -760,6 +760,10 @@ __global__ void __launch_bounds__(256, 2) mx_t128_kernel(const MxGemmParams p) {
       stage = next;
       return;
     }
+    // two wait states between what put the scales into their registers and the first product: the compiler keeps none for assembly
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 1");
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int x = 0; x < 16; ++x) {
       if constexpr (B32) {
