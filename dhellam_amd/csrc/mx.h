@@ -116,18 +116,6 @@ template <typename T> __device__ __forceinline__ void store_nt(T *p, const Loose
     __builtin_nontemporal_store(q, reinterpret_cast<V *>(p) + i);
   }
 }
-template <typename T, bool NT = false> __device__ __forceinline__ void load8(float (&f)[8], const T *p) {
-  const Loose8<T> x = NT ? load_nt(p) : *reinterpret_cast<const Loose8<T> *>(p);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) f[j] = to_f(x.v[j]);
-}
-// the first n of them, zeros behind
-template <typename T> __device__ __forceinline__ void load8_first(float (&f)[8], const T *p, int n) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j) f[j] = j < n ? to_f(p[j]) : 0.f;
-}
-
-static inline int64_t mx_kp(int64_t cols) { return (cols + 127) / 128 * 128; }
 static inline int64_t mx_rows4(int64_t rows) { return (rows + 3) / 4 * 4; }
 
 }  // namespace dh

@@ -31,7 +31,7 @@ struct MxGemmParams {
   int64_t cells_a, cells_b;           // 16-byte cells of scales in a group of 128 columns
   int steps;                          // k / 128, rounded up
   int accumulate, vec;                // vec: rows of c take 16-byte accesses
-  int tiles_m, tiles_n, pieces;
+  int tiles_m, tiles_n, pieces;       // (of k; one where tiles are of 256 x 256)
 };
 
 template <int BITS> struct MxBytes { static constexpr int STEP = BITS * 16, LANE = BITS * 4; };   // bytes of 128 columns, of a lane's 32
@@ -375,11 +375,10 @@ __global__ void __launch_bounds__(512) mx_w8_kernel(const MxGemmParams p) {
   typedef __attribute__((address_space(3))) const uint32_t *lds_dword;
   typedef __attribute__((address_space(3))) const uint16_t *lds_half;
 
-  const int pid = gg_xcd_chunk((int)blockIdx.x, p.tiles_m * p.tiles_n), piece = blockIdx.y;
+  const int pid = gg_xcd_chunk((int)blockIdx.x, p.tiles_m * p.tiles_n);
   int tm, tn;
   gg_tile_of(pid, p.tiles_m, p.tiles_n, tm, tn);
-  const int nsl = (p.steps + KS - 1) / KS;
-  const int s0 = (int)((int64_t)piece * nsl / p.pieces), cnt = (int)((int64_t)(piece + 1) * nsl / p.pieces) - s0;
+  const int cnt = (p.steps + KS - 1) / KS;                       // slices
   const int64_t m0 = (int64_t)tm * 256, n0 = (int64_t)tn * 256;
   // descriptors, cut at the operands' last rows: rows past them read as zeros
   int4v rsa = raw_rsrc(p.a + m0 * lda, std::min<int64_t>(p.m - m0, 256) * lda), rsb = raw_rsrc(p.b + n0 * ldb, std::min<int64_t>(p.n - n0, 256) * ldb);
@@ -391,11 +390,11 @@ __global__ void __launch_bounds__(512) mx_w8_kernel(const MxGemmParams p) {
   // they come out of v_readfirstlane, which the copies from assembly have to keep their distance from
   asm volatile("s_nop 4" : "+s"(rsa), "+s"(rsb), "+s"(rss0), "+s"(rss1));
 
-  // before the copies of slice s (of this piece)
+  // before the copies of slice s
   auto turn_to = [&](int s) {
     if (s >= cnt) {
       rsa[2] = rsb[2] = rss0[2] = rss1[2] = 0;
-    } else if (KS == 2 && (p.steps & 1) && s0 + s == nsl - 1) {
+    } else if (KS == 2 && (p.steps & 1) && s == cnt - 1) {
       // the last step of an odd number: chunks 4..7 are not there
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
@@ -407,21 +406,21 @@ __global__ void __launch_bounds__(512) mx_w8_kernel(const MxGemmParams p) {
   auto copy_a = [&](int h, int s, uint32_t stage) {
 #pragma unroll
     for (int x = 0; x < NA; ++x)
-      copy_1k(ca[x], rsa, (uint32_t)(s0 + s) * RA + (uint32_t)h * 128 * lda, lds0 + stage + (uint32_t)h * REGA + (uint32_t)(NA * w + x) * 1024);
+      copy_1k(ca[x], rsa, (uint32_t)s * RA + (uint32_t)h * 128 * lda, lds0 + stage + (uint32_t)h * REGA + (uint32_t)(NA * w + x) * 1024);
   };
   auto copy_b = [&](int h, int s, uint32_t stage) {
 #pragma unroll
     for (int x = 0; x < NB; ++x)
-      copy_1k(cb[x], rsb, (uint32_t)(s0 + s) * RB + (uint32_t)h * 128 * ldb, lds0 + stage + OFF_B + (uint32_t)h * REGB + (uint32_t)(NB * w + x) * 1024);
+      copy_1k(cb[x], rsb, (uint32_t)s * RB + (uint32_t)h * 128 * ldb, lds0 + stage + OFF_B + (uint32_t)h * REGB + (uint32_t)(NB * w + x) * 1024);
   };
   auto copy_s = [&](int s, uint32_t slot) {
     const uint32_t at = lds0 + slot, quarter = (uint32_t)(w & 3) * 256, to = (uint32_t)(w >> 2) * 1024 + quarter;
     if constexpr (KS == 2) {
-      const uint32_t step = (uint32_t)(2 * (s0 + s) + (w >> 2));
+      const uint32_t step = (uint32_t)(2 * s + (w >> 2));
       copy_256(cs, rss0, step * gs0 + quarter, at + to);
       copy_256(cs, rss1, step * gs1 + quarter, at + 2048 + to);
     } else {
-      copy_256(cs, rss0, (uint32_t)(s0 + s) * gs0 + quarter, at + to);
+      copy_256(cs, rss0, (uint32_t)s * gs0 + quarter, at + to);
     }
   };
   Acc acc[2][2][ABLK][BBLK];
@@ -589,8 +588,7 @@ __global__ void __launch_bounds__(512) mx_w8_kernel(const MxGemmParams p) {
         float v[COLS];
 #pragma unroll
         for (int i = 0; i < COLS; ++i) v[i] = B32 ? acc[qm][qn][b][0][4 * (i & 3) + (i >> 2)] : acc[qm][qn][b][(i & 1) % BBLK][(i >> 1) & 3];
-        if (p.pieces > 1) mx_store<float, COLS>(p.ws + ((int64_t)piece * p.m + row) * (4 * p.cells_b) + col, v, 4 * p.cells_b - col, 1, 0);
-        else mx_store<TO, COLS>(reinterpret_cast<TO *>(p.c) + row * p.ldc + col, v, p.n - col, p.vec, p.accumulate);
+        mx_store<TO, COLS>(reinterpret_cast<TO *>(p.c) + row * p.ldc + col, v, p.n - col, p.vec, p.accumulate);
       }
     }
 #undef MX_BARRIER
