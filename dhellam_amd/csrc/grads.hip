@@ -162,7 +162,7 @@ static int grad_check(const void *const *g, void *const *out, const int64_t *cou
     DH_CHECK(types[i] == DH_F32 || types[i] == DH_BF16 || types[i] == DH_F16, "tensor %d: unknown dtype %d", i, types[i]);
     DH_CHECK(!out || out_types[i] == types[i] || out_types[i] == DH_F32, "tensor %d: results are of its own type or fp32", i);
     DH_CHECK(counts[i] == 0 || (g[i] && (!out || out[i])), "tensor %d: null pointer", i);
-    DH_CHECK(counts[i] < GRAD_PIECE << 30, "tensor %d is too large", i);
+    DH_CHECK(counts[i] < GRAD_PIECE << 23, "tensor %d is too large", i);
   }
   return DH_OK;
 }
@@ -176,7 +176,7 @@ static int grad_tables(const void *const *g, void *const *out, const int64_t *co
     for (; i < n && t.count < GRAD_TABLE; ++i) {
       if (counts[i] == 0) continue;
       const int64_t b = cdiv(counts[i], GRAD_PIECE);
-      if (t.count > 0 && blocks + b >= (1ll << 31)) break;
+      if (blocks + b >= (1ll << 24)) break;                 // (a launch holds fewer than 2^32 threads; one tensor has half of that at most)
       t.g[t.count] = g[i];
       t.out[t.count] = out ? out[i] : nullptr;
       t.n[t.count] = counts[i];

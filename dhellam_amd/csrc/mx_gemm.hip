@@ -864,8 +864,8 @@ template <typename TO> __global__ void __launch_bounds__(256) mx_join_kernel(con
 
 // c = 0 where there is nothing to sum (k of 0).
 template <typename TO> __global__ void __launch_bounds__(256) mx_zero_kernel(const MxGemmParams p) {
-  const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (u < p.m * p.n) reinterpret_cast<TO *>(p.c)[u / p.n * p.ldc + u % p.n] = from_f<TO>(0.f);
+  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < p.m * p.n; u += (int64_t)gridDim.x * 256)
+    reinterpret_cast<TO *>(p.c)[u / p.n * p.ldc + u % p.n] = from_f<TO>(0.f);
 }
 
 constexpr int MX_MAX_PIECES = 16;
@@ -982,8 +982,7 @@ extern "C" int dh_mx_gemm_nt(const void *a_codes, const void *a_scales, int a_fo
   const hipStream_t st = (hipStream_t)stream;
   if (k == 0) {
     if (!accumulate) {
-      const dim3 grid((unsigned)cdiv(m * n, 256));
-      DH_CHECK(cdiv(m * n, 256) < (1ll << 31), "too large");
+      const dim3 grid((unsigned)std::min<int64_t>(cdiv(m * n, 256), 1 << 20));
       DH_DISPATCH_DTYPE(out_dtype, hipLaunchKernelGGL((mx_zero_kernel<T>), grid, dim3(256), 0, st, p));
       DH_LAUNCH_CHECK();
     }
@@ -996,6 +995,9 @@ extern "C" int dh_mx_gemm_nt(const void *a_codes, const void *a_scales, int a_fo
   p.vec = aligned16(c) && ldc * (int64_t)dtype_size(out_dtype) % 16 == 0;
   DH_CHECK(p.steps * std::max(p.cells_a, p.cells_b) * 16 < (1ll << 31), "scales of 2 GiB and more");
   const MxPlan q = mx_plan(m, n, k, a_format, b_format, out_dtype);
+  // (a launch holds 2^32 - 1 threads a dimension; where k is split there are few tiles and a row's sums are joined by far fewer)
+  const int64_t tiles = cdiv(m, q.side ? q.side : 16 * q.mt) * cdiv(n, q.side ? q.side : 16 * q.nt);
+  DH_CHECK(tiles * 64 * q.waves < (1ll << 32), "%lld tiles are more than a launch takes: m %lld, n %lld", (long long)tiles, (long long)m, (long long)n);
   if (q.pieces > 1) {
     const size_t need = dh_mx_gemm_workspace_bytes(m, n, k, a_format, b_format, out_dtype);
     DH_CHECK(workspace && aligned16(workspace) && workspace_bytes >= need, "workspace of %zu bytes, %zu are needed", workspace_bytes, need);

@@ -500,7 +500,7 @@ extern "C" int dh_mx_quantise(const void *x, int64_t rows, int64_t cols, int64_t
   DH_CHECK(dtype == DH_F32 || dtype == DH_BF16 || dtype == DH_F16, "unknown dtype %d", dtype);
   if (rows == 0 || cols == 0) return DH_OK;
   DH_CHECK(rows < (1ll << 31) && cols < (1ll << 31), "sizes of 2^31 and more: rows %lld, cols %lld", (long long)rows, (long long)cols);
-  DH_CHECK(dh::cdiv(rows, 128) * dh::cdiv(cols, 128) < (1ll << 31), "more than 2^31 tiles");
+  DH_CHECK(dh::cdiv(rows, 128) * dh::cdiv(cols, 128) < (1ll << 24), "more than 2^24 tiles of 128 x 128, which a launch of 256 threads each takes");
   DH_CHECK(x && (codes || codes_t), "null pointer");
   DH_CHECK(!codes == !scales && !codes_t == !scales_t, "codes and scales come in pairs");
   DH_CHECK(ldx >= cols || rows == 1, "row stride %lld of %lld columns", (long long)ldx, (long long)cols);

@@ -682,7 +682,7 @@ int dh_masked_mean_bwd(const float *mask, const float *mask_sum, int64_t n, floa
 /* Quantises x (row stride ldx) along its rows (codes, scales) or along its columns (codes_t, scales_t: the transposed matrix,
  * cols x rows), or both in one pass; the pair that is not wanted is NULL.  A scale is 2^(floor(log2 m) - 8) for e4m3 and
  * - 2 for e2m1 with m the block's largest magnitude, so that the largest elements may saturate (448, 6); with `cover` the smallest
- * power of two at which none does.  Elements are rounded to the nearest, ties to even. */
+ * power of two at which none does.  Elements are rounded to the nearest, ties to even.  Fewer than 2^24 tiles of 128 x 128 elements. */
 int dh_mx_quantise(const void *x, int64_t rows, int64_t cols, int64_t ldx, int dtype, int format,
                    int cover, void *codes, void *scales, void *codes_t, void *scales_t, void *stream);
 
@@ -695,7 +695,8 @@ int dh_rmsnorm_mx(const void *x, const void *residual, void *sum_out, const void
                   int zero_centered_gamma, int cover, int dtype, void *stream);
 
 /* c[m, n] (+)= sum over k of a[m, k] b[n, k], both operands in the layout above along k, fp32 sums, c of out_dtype with row
- * stride ldc; `accumulate` adds to what c holds, with one rounding.  k <= 2^22, scales of an operand below 2 GiB.
+ * stride ldc; `accumulate` adds to what c holds, with one rounding.  k <= 2^22, scales of an operand below 2 GiB, as many
+ * tiles (dh_mx_gemm_path) as a launch of less than 2^32 threads holds, 8 wavefronts a tile (4 where its side is 128).
  * For 16-bit results the matrix instructions drop, of 16 products of 8-bit elements, what lies 2^-13 below the largest (2e-5 of the
  * result on normal data); fp32 results of 8-bit operands are formed from the elements in bf16, to fp32's accuracy (elements times
  * their scale below 2^-126 lose bits, and count as zero below 2^-133).  workspace (16-byte aligned, of the call's
