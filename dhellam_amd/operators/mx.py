@@ -66,9 +66,9 @@ def mx_gemm_nt(a, b, out=None, out_dtype=torch.bfloat16, accumulate=False, strea
     column (of b) NaN.
 
     Sums are held in fp32.  For 16-bit results the matrix instructions add 8-bit products 16 at a time and drop what lies 2^-13 below the
-    largest of them: 2e-5 of the result on normal data, far below its rounding.  fp32 results of 8-bit operands are formed from the elements in
-    bf16 instead, to fp32's own accuracy at a third of the speed (elements times their scale below 2^-126 lose bits there, and count as zero
-    below 2^-133); products of two 4-bit operands are exact either way."""
+    largest of them: 2e-5 of the result on normal data, far below its rounding, but not bounded by the result where large products cancel.  fp32 results
+    of 8-bit operands are formed from the elements in bf16 instead, to fp32's own accuracy at a third of the speed (elements times their scale below
+    2^-126 lose bits there, count as zero below 2^-133 and as infinite from 2^128 on); products of two 4-bit operands are exact either way."""
     if a.cols != b.cols:
         raise RuntimeError(f"mx_gemm_nt: {a.cols} and {b.cols} columns")
     if out is not None:
