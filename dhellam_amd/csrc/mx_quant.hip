@@ -1,6 +1,7 @@
 // Quantisation to microscaled floating point, along the rows of a matrix, along its columns, or both in one pass over it, and the
 // RMS norm (with the residual's addition) that writes its result in 8 bits with scales.  Format and rounding: mx.h.
 #include <algorithm>
+#include <type_traits>
 
 #include "mx.h"
 
@@ -191,7 +192,7 @@ template <typename T, bool E4> static void launch_quantise(const QuantParams &p,
 // ---- residual addition, RMS norm, 8 bits with scales -----------------------------------------------------------------------
 // A row belongs to TPR threads, a thread holds VPT groups of 8 columns of it (group t + i TPR) from the first load to the last
 // store.  A block of 32 lies in the 4 lanes of a quad, the four blocks of a dword of scales in 16 lanes.
-// Bound by memory: 8192 x 8192 in bf16 with a residual 88 us, 5.4 TB/s (118 with the loads in branches, whose waits come one by one, and less exact: so whole
+// Bound by memory: 8192 x 8192 in bf16 with a residual 89 us, 5.3 TB/s (118 with the loads in branches, whose waits come one by one, and less exact: so whole
 // rows have a form without).  One row of 8192: 4 us, the launch and two trips to memory.
 struct NormMxParams {
   const void *x, *residual, *gamma;
@@ -242,7 +243,6 @@ template <typename T> __device__ __forceinline__ Loose8<T> sum8(const Loose8<T> 
   for (int j = 0; j < 8; ++j) o.v[j] = from_f<T>(to_f(a.v[j]) + to_f(b.v[j]));
   return o;
 }
-// The sum of 8 squares.  Sums over lanes are in 64 bits, so that 1/rms is off by some 2^-29 before it is rounded.
 // The sum of 8 squares, in 64 bits as everything up to 1/rms.
 template <typename T> __device__ __forceinline__ double squares8(const Loose8<T> &a) {
   double s[2] = {0.0, 0.0};
@@ -305,24 +305,24 @@ template <typename T> __device__ __forceinline__ float gamma_top(const Loose8<T>
 }
 __device__ __forceinline__ uint32_t norm_safe_above(float gamma_top) { return __float_as_uint(0x1p-100f * __uint_as_float(quad_umax(magnitude(gamma_top)))); }
 __device__ __forceinline__ uint32_t norm_safe_row(uint32_t safe_above, double rs) { return rs >= 0x1p-100 && rs <= 0x1p100 ? safe_above : ~0u; }
-__device__ __forceinline__ uint32_t top8(const float (&y)[8]) {
-  uint32_t top = 0;
+// Not 0 where one of the values is not a zero.
+template <typename T> __device__ __forceinline__ uint32_t any_bits(const Loose8<T> &x) {
+  uint32_t v[sizeof(x) / 4], any = 0;
+  __builtin_memcpy(v, &x, sizeof(x));
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t m = magnitude(y[j]);
-    top = top > m ? top : m;
-  }
-  return quad_umax(top);
+  for (int i = 0; i < (int)(sizeof(x) / 4); ++i) any |= mags<T>(v[i]);
+  return any;
 }
 // The result of 8 columns (n exist) of a row: y, codes; returns the block's scale code (the same in the quad).
 // fp32's y is off by 2^-22 of itself at most: 1/rms rounded, gamma + 1 rounded, two products.  Every place where a scale or an element changes has
 // zeros behind its fourth bit; a y that comes that near to one is formed again in 64 bits, so that codes and scales are those of
 // the exact y (to 2^-43).  One wavefront in 115 has such an element among its 512 (zeros count as near too, but are not formed again); without, 1 to 3
-// elements in 2 million were the neighbour.  A block that fp32's smallest numbers reach, and a row whose 1/rms they or the largest reach, are formed
-// in 64 bits as a whole (8192 x 8192 86 us back to back, 84 without).  A result past fp32's largest number is not finite.
-// 8192 x 8192 in bf16 88 us with the sums and near elements in 64 bits, 80 without; 512 x 8192 12 and 9.7.  All four groups' y before one such test were slower (93).
-template <typename T> __device__ __forceinline__ uint32_t norm_out8(const NormMxParams &p, Loose8<T> x, Loose8<T> gamma, double rs64, uint32_t safe_above,
-                                                                    int64_t row, int g, int64_t kp, bool active) {
+// elements in 2 million were the neighbour.  `lowest`: the least of the largest magnitudes of the blocks so far; where fp32 does not do for
+// a block (norm_safe_row), the row is formed again by the form of EXACT, all in 64 bits.  A result past fp32's largest number is not finite.
+// 8192 x 8192 in bf16 with a residual: 80 us in fp32 throughout, 87 with the sums and near elements in 64 bits, 89 with the range test and the form of
+// EXACT (90 with that test at every block, and 5.5 for one row instead of 4.5); 512 x 8192 15 to 16.  All four groups' y before one test for near ones were slower.
+template <typename T, bool EXACT = false> __device__ __forceinline__ uint32_t norm_out8(const NormMxParams &p, Loose8<T> x, Loose8<T> gamma, double rs64,
+                                                                                        uint32_t &lowest, int64_t row, int g, int64_t kp, bool active) {
   const int n = p.cols - 8 * g;
   const float rs = (float)rs64;
   constexpr uint32_t NEAR = 4;                             // steps of fp32: 2^-22 of y at most
@@ -332,11 +332,12 @@ template <typename T> __device__ __forceinline__ uint32_t norm_out8(const NormMx
   uint32_t near = ~0u;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    y[j] = to_f(x.v[j]) * rs * (to_f(gamma.v[j]) + p.shift);
+    if constexpr (EXACT) y[j] = to_odd((double)to_f(x.v[j]) * rs64 * ((double)to_f(gamma.v[j]) + (double)p.shift));
+    else y[j] = to_f(x.v[j]) * rs * (to_f(gamma.v[j]) + p.shift);
     if (n < 8 && j >= n) y[j] = 0.f;                       // (a row of infinities or NaN makes products of zeros NaN)
     else near = std::min(near, (__float_as_uint(y[j]) + NEAR) << 13);
   }
-  if (near <= 2 * NEAR << 13 && active) {
+  if (!EXACT && near <= 2 * NEAR << 13 && active) {
     keep_packed(x);
     keep_packed(gamma);
 #pragma unroll
@@ -344,16 +345,15 @@ template <typename T> __device__ __forceinline__ uint32_t norm_out8(const NormMx
       if (j < n && (__float_as_uint(y[j]) + NEAR) << 13 <= 2 * NEAR << 13 && y[j] != 0.f)
         y[j] = to_odd((double)to_f(x.v[j]) * rs64 * ((double)to_f(gamma.v[j]) + (double)p.shift));
   }
-  uint32_t top = top8(y);
-  if (!(top > safe_above)) {                               // (the same in the quad)
-    keep_packed(x);
-    keep_packed(gamma);
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < n) y[j] = to_odd((double)to_f(x.v[j]) * rs64 * ((double)to_f(gamma.v[j]) + (double)p.shift));
-    top = top8(y);
-  }
   if (p.y && active && n > 0) store8<T, false>(reinterpret_cast<T *>(p.y) + row * p.cols + 8 * g, rounded8<T>(y), n);
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t m = magnitude(y[j]);
+    top = top > m ? top : m;
+  }
+  top = quad_umax(top);
+  if (!EXACT && 8 * (g & ~3) < p.cols) lowest = std::min(lowest, top);
   const uint32_t code = mx_scale_code<true>(top, p.cover);
   if (active) {
     const MxPack<true> o = mx_pack<true>(y, code);
@@ -378,10 +378,7 @@ __global__ void __launch_bounds__(TPR *ROWS, VPT == 4 ? (sizeof(T) == 4 ? 3 : 4)
     const int g = lane + i * TPR;
     gamma[i] = fetch8<T, WHOLE, false>(reinterpret_cast<const T *>(p.gamma) + 8 * g, p.cols - 8 * g);
   }
-  float largest = 1.f;
-#pragma unroll
-  for (int i = 0; i < VPT; ++i) largest = gamma_top(gamma[i], p.shift, largest);
-  const uint32_t safe_above = norm_safe_above(largest);
+  uint32_t safe_above = 0;
   int turn = 0;
   for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < 4 * cells; row0 += (int64_t)gridDim.x * ROWS, turn ^= 1) {
     const int64_t row = row0 + sub;
@@ -412,14 +409,30 @@ __global__ void __launch_bounds__(TPR *ROWS, VPT == 4 ? (sizeof(T) == 4 ? 3 : 4)
       for (int i = 0; i < WPR; ++i) s += red[turn][sub * WPR + i];
     }
     const double rs = rsqrt64(s * inv_cols + (double)p.eps);
-    const uint32_t safe_row = norm_safe_row(safe_above, rs);
+    if (row0 == (int64_t)blockIdx.x * ROWS) {              // (behind the first row's loads, which do not wait for gamma)
+      float largest = 1.f;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int g = lane + i * TPR;
-      if (g >= groups) continue;                           // (16 lanes at a time: groups is a multiple of 16)
-      const uint32_t code = norm_out8<T>(p, held[i], gamma[i], rs, safe_row, row, g, kp, active);
-      if ((lane & 3) == 0 && row < 4 * cells)
-        p.scales[((int64_t)(g >> 4) * cells + (row >> 2)) * 16 + ((g >> 2) & 3) * 4 + (row & 3)] = (uint8_t)code;
+      for (int i = 0; i < VPT; ++i) largest = gamma_top(gamma[i], p.shift, largest);
+      safe_above = norm_safe_above(largest);
+    }
+    uint32_t lowest = ~0u;
+    auto out = [&](auto exact) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int g = lane + i * TPR;
+        if (g >= groups) continue;                         // (16 lanes at a time: groups is a multiple of 16)
+        const uint32_t code = norm_out8<T, decltype(exact)::value>(p, held[i], gamma[i], rs, lowest, row, g, kp, active);
+        if ((lane & 3) == 0 && row < 4 * cells)
+          p.scales[((int64_t)(g >> 4) * cells + (row >> 2)) * 16 + ((g >> 2) & 3) * 4 + (row & 3)] = (uint8_t)code;
+      }
+    };
+    out(std::false_type{});
+    const uint32_t safe_row = norm_safe_row(safe_above, rs);
+    if (__builtin_expect(active && !(lowest > safe_row), 0)) {      // (the same in the quad)
+      uint32_t any = 0;                                    // (zeros, a masked row's, are what they are)
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) any |= any_bits(held[i]);
+      if (safe_row == ~0u || quad_umax(any)) out(std::true_type{});
     }
     if (active && lane == 0) p.rsigma[row] = (float)rs;
   }
@@ -432,10 +445,6 @@ __global__ void __launch_bounds__(1024) norm_mx_long_kernel(const NormMxParams p
   const int groups = (p.cols + 127) / 128 * 16;
   const int64_t kp = (int64_t)groups * 8, cells = (p.rows + 3) / 4;
   const T *res = reinterpret_cast<const T *>(p.residual);
-  float largest = 1.f;
-  for (int g = threadIdx.x; g < groups; g += 1024)
-    largest = gamma_top(fetch8<T, false, false>(reinterpret_cast<const T *>(p.gamma) + 8 * g, p.cols - 8 * g), p.shift, largest);
-  const uint32_t safe_above = norm_safe_above(largest);
   for (int64_t row = blockIdx.x; row < 4 * cells; row += gridDim.x) {
     const bool active = row < p.rows;
     const T *x = reinterpret_cast<const T *>(p.x) + row * p.cols;
@@ -457,12 +466,13 @@ __global__ void __launch_bounds__(1024) norm_mx_long_kernel(const NormMxParams p
     for (int i = 0; i < 16; ++i) s += red[i];
     __syncthreads();                                       // (the next row's are written behind these reads)
     const double rs = rsqrt64(s / (double)p.cols + (double)p.eps);
-    const uint32_t safe_row = norm_safe_row(safe_above, rs);
     if (RES) x = reinterpret_cast<const T *>(p.sum_out) + row * p.cols;      // a thread reads what it wrote itself
     for (int g = threadIdx.x; g < groups; g += 1024) {
       const int n = p.cols - 8 * g;
       const Loose8<T> v = fetch8<T, false, false>(x + 8 * g, active ? n : 0), gamma = fetch8<T, false, false>(reinterpret_cast<const T *>(p.gamma) + 8 * g, n);
-      const uint32_t code = norm_out8<T>(p, v, gamma, rs, safe_row, row, g, kp, active);
+      uint32_t lowest = ~0u, code = norm_out8<T>(p, v, gamma, rs, lowest, row, g, kp, active);
+      if (__builtin_expect(active && !(lowest > norm_safe_row(norm_safe_above(gamma_top(gamma, p.shift, 1.f)), rs)), 0))
+        code = norm_out8<T, true>(p, v, gamma, rs, lowest, row, g, kp, active);
       if ((threadIdx.x & 3) == 0)
         p.scales[((int64_t)(g >> 4) * cells + (row >> 2)) * 16 + ((g >> 2) & 3) * 4 + (row & 3)] = (uint8_t)code;
     }
