@@ -44,8 +44,9 @@ def _record(obj, stream) -> None:
 
 def clip_main_grads(parameters, max_norm: float, scale: float = 1.0, out=None) -> torch.Tensor:
     """Between a step's backward and the optimizer: the global norm of the parameters' ``main_grad`` (times ``scale``, which undoes a
-    loss scale) and their clipping to ``max_norm``, in place or into ``out`` (``operators.grads.clip_grads``).  Returns fp32 [2] on the device:
-    the norm, and the factor that was applied.  Nothing here waits for the GPU."""
+    loss scale) and their clipping to ``max_norm``, in place or into ``out`` (``operators.grads.clip_grads``).  The parameters are those of the whole
+    model: ranks that hold parts of one call ``grad_norm`` and ``clip_grads`` themselves and add up the sums of squares in between.  Returns fp32 [2]
+    on the device: the norm, and the factor that was applied.  Nothing here waits for the GPU."""
     from ..operators.grads import clip_grads, grad_norm
     grads = [p.main_grad for p in parameters if getattr(p, "main_grad", None) is not None]
     if not grads:

@@ -24,7 +24,7 @@ template <bool E4> __device__ __forceinline__ uint32_t mx_scale_code(uint32_t to
   return top >= 0x7f800000u ? 255u : (uint32_t)e;
 }
 // 2^(127 - code), by which the block's values are multiplied: exact but for what lies far below the smallest element.
-// (A finite block's code is at most 254 - 2, so this is a normal number.  For 255 it is none: the codes are cleared.)
+// (A finite block's code is at most 253, e2m1's under `cover`, so this is a normal number.  For 255 it is none: the codes are cleared.)
 __device__ __forceinline__ float mx_inverse(uint32_t code) { return __uint_as_float((254u - code) << 23); }
 
 // Four consecutive elements, already scaled, to e4m3 (round to nearest even, saturating at 448).

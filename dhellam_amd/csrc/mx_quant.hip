@@ -15,7 +15,8 @@ namespace dh {
 // of the transposed result: they are packed in registers and go through LDS as 8 (4) bytes, so that memory gets
 // 128 (64) bytes of a row of the transpose at a time.
 // Bound by memory: 4096 x 7168 in bf16 to e4m3, along both directions 25 to 27 us (119 MB; 23.0 at what a copy of 1 GiB reaches, 5.2 TB/s); 4096 x 8192
-// along the rows 18.5 (101 MB; 19.5).  A few rows: 4 to 5 us, most of it the launch.  Five or six workgroups on a
+// along the rows 18.5 (101 MB; 19.5).  4096 x 7168 in other forms: bf16 to e2m1 14.8 along the rows (5.0 TB/s) and 20.7 along both (4.3), fp32 to e4m3
+// 22.6 (6.5) and 31.8 (5.6).  A few rows: 4 to 5 us, most of it the launch.  Five or six workgroups on a
 // compute unit by fewer registers were slower.
 struct QuantParams {
   const void *x;
@@ -193,7 +194,8 @@ template <typename T, bool E4> static void launch_quantise(const QuantParams &p,
 // A row belongs to TPR threads, a thread holds VPT groups of 8 columns of it (group t + i TPR) from the first load to the last
 // store.  A block of 32 lies in the 4 lanes of a quad, the four blocks of a dword of scales in 16 lanes.
 // Bound by memory: 8192 x 8192 in bf16 with a residual 89 us, 5.3 TB/s (118 with the loads in branches, whose waits come one by one, and less exact: so whole
-// rows have a form without).  One row of 8192: 4 us, the launch and two trips to memory.
+// rows have a form without), in fp32 180 us (4.9 TB/s).  One row of 8192: 4.5 us, the launch and two trips to memory; 256 rows of 1024 threads 7, 512 and 1024
+// rows of 256 threads 15 and 21, a few rows a compute unit one behind the other.
 struct NormMxParams {
   const void *x, *residual, *gamma;
   void *sum_out, *y;
@@ -438,7 +440,8 @@ __global__ void __launch_bounds__(TPR *ROWS, VPT == 4 ? (sizeof(T) == 4 ? 3 : 4)
   }
 }
 
-// Rows of any length: one workgroup a row, read once for its statistics and again, from the cache, for its result.
+// Rows of any length: one workgroup a row, read once for its statistics and again, from the cache, for its result.  2048 x 20000 in bf16 with a residual
+// 99 us, 2.9 TB/s: a row's two passes wait for one another, and 16 wavefronts of these registers fill a compute unit.
 template <typename T, bool RES>
 __global__ void __launch_bounds__(1024) norm_mx_long_kernel(const NormMxParams p) {
   __shared__ double red[16];

@@ -1,7 +1,7 @@
 """Microscaled floating point: quantisation to 8 and 4 bits with a power of two a block of 32, and products of such operands.
 
 The reference has no low precision; these operators follow its wrapper convention (``stream=None`` means the current stream,
-trailing elapsed-ms return).  A projection Y = X W^T in low precision is three products of the one form ``mx_gemm_nt``, each with
+trailing elapsed-ms return; the product returns its result alone, as ``operators.moe.grouped_gemm_nt`` does).  A projection Y = X W^T in low precision is three products of the one form ``mx_gemm_nt``, each with
 both operands quantised along its reduction:
 
     forward          y  = mx_gemm_nt(x, w)                                        x along its rows, w [out, in] along its rows
@@ -28,7 +28,8 @@ SCALE_RULES = {"floor": False, "cover": True}
 @dataclass
 class MXTensor:
     """A rows x cols matrix in microscaled floating point, blocks of 32 along the columns (the OCP MX formats).  Every row is
-    filled up to whole groups of 128 columns with zeros."""
+    filled up to whole groups of 128 columns with zeros.  ``mx_quantise`` and ``pyrmsnorm_mx_fwd`` make codes and scales as two views of one
+    allocation: what saves a tensor's whole storage, or refuses tensors that share one, wants ``clone()`` of each."""
     codes: torch.Tensor       # uint8 [rows, kp] (e4m3) or [rows, kp / 2] (e2m1: the even column in the low half), kp = cols rounded up to 128
     scales: torch.Tensor      # uint8 [kp / 128, rows / 4 rounded up, 4, 4]: [c, r // 4, i, r % 4] is the exponent code (2^(e - 127), 255: NaN) of
                               # columns 128 c + 32 i and on of row r; zeros for what is not there
