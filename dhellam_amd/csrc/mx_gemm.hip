@@ -34,7 +34,7 @@ struct MxGemmParams {
   int tiles_m, tiles_n, pieces;       // (of k; one where tiles are of 256 x 256)
 };
 
-template <int BITS> struct MxBytes { static constexpr int STEP = BITS * 16, LANE = BITS * 4; };   // bytes of 128 columns, of a lane's 32
+template <int BITS> struct MxBytes { static constexpr int STEP = BITS * 16; };   // bytes of 128 columns
 
 // A lane's share of 128 columns of one row: chunk 0 (and 1) of 16 bytes.
 template <int BITS> struct MxFrag { int4v q[BITS / 4]; };

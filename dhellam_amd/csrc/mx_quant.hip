@@ -96,7 +96,6 @@ __global__ void __launch_bounds__(256) mx_quantise_kernel(const QuantParams p) {
   const int64_t row0 = r0 + 32 * w + 8 * rg, col0 = c0 + 8 * cg;
   const T *x = reinterpret_cast<const T *>(p.x);
   H v[8];
-  const int64_t left = p.cols - col0;
   if (r0 + 128 <= p.rows && c0 + 128 <= p.cols) {          // (of the workgroup: no load waits for a comparison)
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i].load(x + (row0 + i) * p.ldx + col0);
@@ -109,10 +108,10 @@ __global__ void __launch_bounds__(256) mx_quantise_kernel(const QuantParams p) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i].drop(row0 + i < p.rows ? (int)std::min<int64_t>(col0 - at, 8) : 8);
   } else {
+    const int64_t left = p.cols - col0;                    // (fewer than 8)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (row0 + i < p.rows && left >= 8) v[i].load(x + (row0 + i) * p.ldx + col0);
-      else if (row0 + i < p.rows && left > 0) v[i].load_first(x + (row0 + i) * p.ldx + col0, (int)left);
+      if (row0 + i < p.rows && left > 0) v[i].load_first(x + (row0 + i) * p.ldx + col0, (int)left);
       else v[i].clear();
     }
   }
